@@ -54,8 +54,9 @@ MV_API int mv_version(void);
 MV_API const char* mv_last_error(void);
 
 /* Reads (synchronously, on `stream`) the device-side error word of a workspace: 0 = none, 1 = a bounded
- * wait timed out, 2 = an expert id outside [0, E1) was skipped, 3 = a capacity was exceeded. `info` (may be
- * NULL) receives where it was raised. With clear != 0 the word is reset. Host-synchronising; not for use
+ * wait timed out, 2 = an expert id outside [0, E1) was skipped, 3 = a capacity was exceeded, 4 = a page id or
+ * position outside the cache was skipped, 5 = sequence bounds that do not fit the tensors were clamped. `info`
+ * (may be NULL) receives where it was raised. With clear != 0 the word is reset. Host-synchronising; not for use
  * inside stream capture. */
 MV_API int mv_workspace_status(void* workspace, int clear, unsigned int* code, unsigned int* info, void* stream);
 
@@ -282,6 +283,79 @@ MV_API size_t mv_block_decode_workspace_bytes_tc(const mv_block* b, int M);
  * to 32 / 64 / 128 tokens and replays one graph per length (engine.py:716-757, :950-961), where the padded rows
  * also run through the experts; here they are dropped from the expert sort. */
 MV_API int mv_mask_pad_rows(void* ids, int ids_dtype, int N, int NK, const int* n_valid, void* stream);
+
+/* ---- attention over a paged cache and over packed prompts ----
+ *
+ * The attention half of a decoder layer, beside the MoE block above (ming-voice leaves it to its attention
+ * libraries, engine.py:234-282). Common terms:
+ *  - A batch of B sequences is packed: sequence b owns rows [cu_seqlens[b], cu_seqlens[b + 1]) of the token
+ *    tensors (cu_seqlens [B + 1] int32, ascending; a sequence may own no row).
+ *  - Heads are grouped: query head h reads key / value head h / G, G = Hq / Hkv (a whole number, 1..32).
+ *  - Element types: bf16 or f16, one for all tensors of a call. head_dim is 64 or 128, inner stride 1, every row
+ *    and head stride a multiple of 16 bytes, 16-byte aligned pointers. Strides are in elements.
+ *  - All indices (cu_seqlens, lengths, page ids) are read on the device: nothing synchronises the host and a
+ *    captured graph serves every length. What does not fit the tensors is clamped or skipped, never read or
+ *    written out of range, and reported in the workspace's error word (4 or 5).
+ *
+ * Paged cache: k and v [num_pages, page_size, n_kv_heads, head_dim] through strides (page, token, head), so a
+ * [num_pages, n_kv_heads, page_size, head_dim] cache works as well. page_size is a power of two in 8..256.
+ * page_table [B, max_pages] int32 (row stride pt_stride): token s of sequence b lies in page page_table[b, s / page_size]
+ * at slot s % page_size. kv_lens [B] int32 is the length of each sequence in the cache with the call's new tokens
+ * in it: new token i of q_len has position kv_lens[b] - q_len + i. */
+typedef struct mv_paged_kv {
+  void* k;
+  void* v;
+  int dtype; /* MV_BF16 or MV_F16 */
+  int num_pages, page_size, n_kv_heads, head_dim;
+  int pad0;
+  long long k_sp, k_st, k_sh; /* k strides: page, token, head */
+  long long v_sp, v_st, v_sh; /* v strides */
+} mv_paged_kv;
+
+/* Appends the keys and values of T packed new tokens to the cache, rotating the keys (and the queries) by their
+ * positions on the way. k, v [T, n_kv_heads, head_dim] (strides token, head); q / q_out [T, Hq, head_dim] or NULL
+ * (Hq = 0; q_out may be q). The first rot_dim values of a head are rotated in fp32 and rounded once, the rest and
+ * the values are copied: pair i < rot_dim / 2 is (x[i], x[i + rot_dim / 2]), or (x[2i], x[2i + 1]) when interleaved,
+ *   y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin,
+ * with cos_sin [max_pos, rot_dim] f32 (row stride cs_stride): a position's rot_dim / 2 cosines, then its sines.
+ * rot_dim 0 (cos_sin NULL) rotates nothing. positions [T] int32 or NULL replaces the cache position as the row of
+ * cos_sin (the cache slot stays the same). A token whose page id, slot or position is outside the cache, the page
+ * table or cos_sin is skipped (error 4): neither its cache slot nor its q_out row is written. Rows outside every
+ * sequence are left alone. workspace: a zeroed header of mv_attention_workspace_bytes(). */
+MV_API int mv_kv_append(const mv_paged_kv* c, const void* k, long long k_st, long long k_sh, const void* v,
+                        long long v_st, long long v_sh, const void* q, long long q_st, long long q_sh, int Hq,
+                        void* q_out, long long qo_st, long long qo_sh, int T, const int* page_table,
+                        long long pt_stride, int max_pages, const int* cu_seqlens, const int* kv_lens, int B,
+                        const float* cos_sin, long long cs_stride, int max_pos, int rot_dim, int interleaved,
+                        const int* positions, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of packed new tokens over the cache (which holds them already: mv_kv_append first). For row (token i of
+ * sequence b, query head h) over the visible keys j: j <= kv_lens[b] - q_len + i when causal, else j < kv_lens[b]:
+ *   s_j = scale q . k_j,  out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s),  lse = ln sum_j exp(s_j)
+ * q, out [T, Hq, head_dim]; lse [T, Hq] f32 contiguous or NULL. A row without a visible key gives out 0 and
+ * lse -inf. Scores, maxima, sums and outputs are held in fp32; the weights exp(s - max) are rounded to the element
+ * type for their product with v (the tensor cores' operand). Values of masked or unowned slots (of any content,
+ * NaN and infinities included) never reach a result, but for one case: a non-finite value row that some queries of
+ * a sequence see can reach the other queries of that sequence that are computed in the same tile. max_q is the
+ * caller's largest q_len, used to choose a kernel only (a wrong value costs time, not correctness). scale > 0.
+ * Results do not depend on the run: fixed summation order. workspace: mv_attention_workspace_bytes() bytes. */
+MV_API int mv_paged_attention(const mv_paged_kv* c, const void* q, long long q_st, long long q_sh, int Hq, int T,
+                              const int* page_table, long long pt_stride, int max_pages, const int* cu_seqlens,
+                              const int* kv_lens, int B, int max_q, float scale, int causal, void* out,
+                              long long o_st, long long o_sh, float* lse, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* The same over packed prompts that lie in k, v [Tk, Hkv, head_dim] themselves, no cache: sequence b's keys are rows
+ * [cu_seqlens_k[b], cu_seqlens_k[b + 1]) (NULL: cu_seqlens). Causal masks align the ends: token i of q_len sees keys
+ * j <= k_len - q_len + i. */
+MV_API int mv_prompt_attention(const void* q, long long q_st, long long q_sh, const void* k, long long k_st,
+                               long long k_sh, const void* v, long long v_st, long long v_sh, int dtype, int Tq,
+                               int Tk, int Hq, int Hkv, int head_dim, const int* cu_seqlens, const int* cu_seqlens_k,
+                               int B, int max_q, float scale, int causal, void* out, long long o_st, long long o_sh,
+                               float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of the three calls above (any shape; zero-initialised, 256-byte aligned, left as they need it). */
+MV_API size_t mv_attention_workspace_bytes(void);
 
 /* mv_block_decode without a caller workspace: no counterpart in the reference (its Triton launches take
  * torch-allocated buffers). For callers that cannot allocate device memory or keep a workspace -- a C/FFI

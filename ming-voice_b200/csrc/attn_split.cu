@@ -1,0 +1,493 @@
+// Attention of few rows per key head (a decode step, drafted tokens): mma.sync kernel, keys streamed once.
+//
+// Mathematics: out = sum_j 2^(t_j - m) v_j / sum_j 2^(t_j - m), t_j = scale log2(e) q . k_j, with a running maximum m
+// and sum per row: when a key tile raises m, what has been summed is multiplied by 2^(m_old - m_new).
+//
+// Bound: memory. A key row of 2 D values serves the G query heads of its key head (4 G D flops per 4 D bytes), so at
+// G = 4..8 the cache has to stream at HBM speed and the products need a few percent of the tensor pipe. Both
+// products are taken transposed, S^T = K Q^T and O^T = V^T P^T, with the keys (the head's values) in the 16-row
+// operand and the query rows in the 8-column one: 8 rows fill an instruction where the untransposed form would fill
+// half of it. The cost of that is one movmatrix per 8 x 8 block of P.
+//
+// Split: one CTA per SM takes an equal share of all key tiles (attn_common.cuh). A producer warp keeps a ring of
+// key tiles filled by TMA (a box per page and 64 values, 128-byte swizzle); each of the consumer warps takes whole
+// tiles in turn with its own maximum, sum and output in registers, so the warps meet only at the end of a piece.
+// Pieces of an item that ranges cut are joined by the CTA that arrives last, in CTA order.
+#include "attn_common.cuh"
+
+namespace mv {
+namespace attn {
+namespace {
+
+template <int D, int NT>
+struct Cfg {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kBN = D == 128 && NT <= 2 ? 32 : 64;  // keys of a tile
+  static constexpr int kWarps = NT <= 2 ? 8 : 4;             // consumer warps
+  static constexpr int kThreads = 32 * (kWarps + 1);
+  static constexpr int kTile = kBN * D * 2;                   // bytes of a key (or value) tile
+  static constexpr int kStage = 2 * kTile;
+  // a ring slot is always read by the same warp (tile i: slot i % kStages, warp i % kWarps), so a warp never waits
+  // for a slot whose previous copy it has not seen complete
+  static constexpr int kStages = 131072 / kStage;
+  static_assert(kStages % kWarps == 0, "ring slots of one warp");
+  static constexpr int kOS = D + 4;                           // row stride of the merge buffer (no bank conflicts)
+  static constexpr int kMerge = kWarps * kRows * kOS * 4;
+  static constexpr int kPiece = kRows * (D + 2);              // floats of a piece: output, maxima, sums
+  // shared memory: ring | merge | Q fragments | per-warp maxima and sums | row weights | schedule | barriers
+  static constexpr int oMerge = kStages * kStage;
+  static constexpr int oQ = oMerge + kMerge;
+  static constexpr int oM = oQ + (D / 16) * NT * 32 * 8;
+  static constexpr int oL = oM + kWarps * kRows * 4;
+  static constexpr int oPre = oL + kWarps * kRows * 4;
+  static constexpr int oTmp = oPre + (kMaxB + 1) * 8;
+  static constexpr int oBar = oTmp + 32 * 8;
+  static constexpr int oFlag = oBar + 2 * kStages * 8;
+  static constexpr int kSmem = oFlag + 16 + 1024;
+  static_assert(kSmem <= 232448, "shared memory");
+  static_assert(kMaxCtas * kRows * 4 + kRows * 8 <= kMerge, "piece weights share the merge buffer");
+};
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+        "%2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
+    split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Problem p,
+                 int box) {
+  using C = Cfg<D, NT>;
+  constexpr int R = C::kRows, NW = C::kWarps, NS = C::kStages, OS = C::kOS, kBN = C::kBN, MT = kBN / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* sO = reinterpret_cast<float*>(smem + C::oMerge);
+  uint2* sQ = reinterpret_cast<uint2*>(smem + C::oQ);
+  float* sM = reinterpret_cast<float*>(smem + C::oM);
+  float* sL = reinterpret_cast<float*>(smem + C::oL);
+  unsigned long long* pre = reinterpret_cast<unsigned long long*>(smem + C::oPre);
+  unsigned long long* tmp = reinterpret_cast<unsigned long long*>(smem + C::oTmp);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBar);
+  uint64_t* empty = full + NS;
+  volatile int* flag = reinterpret_cast<volatile int*>(smem + C::oFlag);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    fence_mbar_init();
+    tc::prefetch_tmap(&tmK);
+    tc::prefetch_tmap(&tmV);
+  }
+  build_schedule<kBN>(p, pre, tmp);  // its barriers also publish the mbarriers
+  const unsigned long long W = pre[p.B];
+  if (W == 0) return;
+  const Cut cut(W, gridDim.x, p.min_share);
+  Walk<kBN> wk(p, pre, cut.bound(blockIdx.x), cut.bound(blockIdx.x + 1));
+
+  if (warp == NW) {
+    // ---------------------------------------------------------------- producer: lane i issues box i of a tile
+    const int nbox = kBN / box;
+    const int is_v = lane & 1, half = (lane >> 1) % (D / 64), bx = (lane >> 1) / (D / 64);
+    const CUtensorMap* map = is_v ? &tmV : &tmK;
+    int it = 0;
+    bool ok = true;
+    for (; wk.more() && ok; wk.next()) {
+      const int kend = wk.kend();
+      const int i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+      for (int i = wk.first(); i < i1 && ok; ++i, ++it) {
+        const int stage = it % NS;
+        const int j = i * kBN + bx * box;  // first key of the lane's box
+        const bool mine = bx < nbox && j < kend;
+        int page = 0, row = wk.s.k0 + j;
+        if (mine && p.page_table != nullptr) {
+          page = p.page_table[wk.b * p.pt_stride + (j >> p.page_shift)];
+          row = j & ((1 << p.page_shift) - 1);
+          if (page < 0 || page >= p.num_pages) {
+            raise_error(p.ws, kErrBadPage, 0x710u);
+            page = p.num_pages;  // outside the map: reads as zeros
+          }
+        }
+        const int live = min(nbox, (kend - i * kBN + box - 1) / box);
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], ((it / NS) & 1) ^ 1, p.ws, 0x720u));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(live * box * D * 4));
+        __syncwarp();
+        if (mine) {
+          uint8_t* dst = smem + stage * C::kStage + is_v * C::kTile + half * (kBN * 128) + bx * box * 128;
+          tc::tma_load_4d(dst, map, &full[stage], half * 64, row, wk.h, page);
+        }
+      }
+    }
+    // copies in flight land before the CTA exits
+    if (lane == 0)
+      for (int i = 0; i < NS && i < it; ++i)
+        mbar_wait(&full[i], static_cast<uint32_t>(((it - 1 - i) / NS) & 1), p.ws, 0x721u);
+    return;
+  }
+
+  // ------------------------------------------------------------------ consumers
+  const int g = lane >> 2, t4 = lane & 3;
+  const int tid = threadIdx.x;
+  constexpr int NTH = 32 * NW;
+  int it = 0;      // tiles of the CTA so far
+  bool ok = true;  // a wait that ran out: no more tiles, but every barrier is still met
+  for (; wk.more(); wk.next()) {
+    const int kend = wk.kend(), ntok = wk.ntok(), rows = ntok * p.G, first = wk.first();
+    const int i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+    // Q as the 8-column operand's fragments: row n = lane / 4, values 16 ks + 2 (lane % 4) + {0, 1} and + {8, 9}
+    for (int e = tid; e < (D / 16) * NT * 32; e += NTH) {
+      const int l = e & 31, nt = (e >> 5) % NT, ks = (e >> 5) / NT;
+      const int r = nt * 8 + (l >> 2);
+      uint2 v = make_uint2(0u, 0u);
+      if (r < rows) {
+        const uint16_t* src = p.q + (wk.s.q0 + wk.tok0() + r / p.G) * p.q_st + (wk.h * p.G + r % p.G) * p.q_sh +
+                              ks * 16 + (l & 3) * 2;
+        v.x = *reinterpret_cast<const uint32_t*>(src);
+        v.y = *reinterpret_cast<const uint32_t*>(src + 8);
+      }
+      sQ[e] = v;
+    }
+    named_bar(1, NTH);
+
+    // keys seen by the thread's rows (columns of S^T): 8 nt + 2 t4 + {0, 1}
+    int lim[NT][2];
+    int lim_min = kend;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = nt * 8 + t4 * 2 + c;
+        lim[nt][c] = keys_seen(p, wk.s, wk.tok0() + min(r / p.G, ntok - 1) + 1);
+        lim_min = min(lim_min, lim[nt][c]);
+      }
+    float m[NT][2], l[NT][2], o[D / 16][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[j][nt][c] = 0.f;
+    }
+
+    const int base = it - first;  // tile i of the item is the CTA's tile base + i
+    it = base + max(i1, first);
+    const int skip = ((warp - (base + first)) % NW + NW) % NW;
+    for (int i = first + skip; i < i1 && ok; i += NW) {
+      const int cta_tile = base + i, stage = cta_tile % NS;
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], (cta_tile / NS) & 1, p.ws, 0x730u));
+      if (!ok) break;
+      const uint32_t kt = smem_u32(smem + stage * C::kStage), vt = kt + C::kTile;
+      const int nv = min(kBN, kend - i * kBN);  // keys of the tile
+      const int blocks = (nv + 15) / 16;
+      if (nv < blocks * 16) {
+        // rows behind the last key hold anything (an older page's values, NaN): their weights are 0, and 0 * NaN
+        // is not, so the values are cleared
+        constexpr int kVec = D / 8;
+        for (int e = lane; e < (blocks * 16 - nv) * kVec; e += 32) {
+          const int r = nv + e / kVec, c = e % kVec;
+          *reinterpret_cast<uint4*>(smem + stage * C::kStage + C::kTile + (c / 8) * (kBN * 128) + r * 128 +
+                                    (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+      }
+      // S^T = K Q^T
+      float s[MT][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[mt][nt][c] = 0.f;
+      {
+        const int r = (lane & 7) + ((lane >> 3) & 1) * 8, ch = lane >> 4;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint2 qf[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) qf[nt] = sQ[(ks * NT + nt) * 32 + lane];
+          const uint32_t a0 = kt + (ks / 4) * (kBN * 128) + r * 128 + ((((ks & 3) * 2 + ch) ^ (r & 7)) << 4);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            if (mt < blocks) {
+              uint32_t a[4];
+              ldsm4(a, a0 + mt * 16 * 128);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816<BF16>(s[mt][nt], a, qf[nt].x, qf[nt].y);
+            }
+        }
+      }
+      // masks, running maximum, weights
+      const int j0 = i * kBN;
+      const bool masked = j0 + blocks * 16 > lim_min;
+      float tmax[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) tmax[nt][0] = tmax[nt][1] = -INFINITY;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+        if (mt < blocks)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float x = s[mt][nt][c] * p.scale_log2;
+              if (masked && j0 + mt * 16 + g + (c >> 1) * 8 >= lim[nt][c & 1]) x = -INFINITY;
+              s[mt][nt][c] = x;
+              tmax[nt][c & 1] = fmaxf(tmax[nt][c & 1], x);
+            }
+      bool grow = false;
+      float base_m[NT][2], alpha[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = tmax[nt][c];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          const float mn = fmaxf(m[nt][c], x);
+          base_m[nt][c] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every weight is 2^-inf = 0
+          alpha[nt][c] = exp2_approx(m[nt][c] - base_m[nt][c]);
+          grow = grow || mn != m[nt][c];
+          m[nt][c] = mn;
+          l[nt][c] *= alpha[nt][c];
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[j][nt][c] *= alpha[nt][c & 1];
+      }
+      uint32_t pb[MT][NT][2];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+        if (mt < blocks)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float e[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              e[c] = exp2_approx(s[mt][nt][c] - base_m[nt][c & 1]);
+              l[nt][c & 1] += e[c];
+            }
+            // the weights are rounded to the element type here, as operands of the second product
+            pb[mt][nt][0] = transpose8(pack2<BF16>(e[0], e[1]));
+            pb[mt][nt][1] = transpose8(pack2<BF16>(e[2], e[3]));
+          }
+      // O^T += V^T P^T
+      {
+        const int r = (lane & 7) + (lane >> 4) * 8, ch = (lane >> 3) & 1;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          if (mt < blocks) {
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+              uint32_t a[4];
+              const int row = mt * 16 + r;
+              ldsm4_t(a, vt + (j / 4) * (kBN * 128) + row * 128 + ((((j & 3) * 2 + ch) ^ (row & 7)) << 4));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816<BF16>(o[j][nt], a, pb[mt][nt][0], pb[mt][nt][1]);
+            }
+          }
+      }
+      if (nv < blocks * 16) fence_proxy_async_smem();  // this warp's stores before the ring slot's next copy
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+    }
+
+    // sums over the 8 lanes that share a row
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = l[nt][c];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (g == 0) {
+          sM[warp * R + nt * 8 + t4 * 2 + c] = m[nt][c];
+          sL[warp * R + nt * 8 + t4 * 2 + c] = x;
+        }
+      }
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          sO[(warp * R + nt * 8 + t4 * 2 + (c & 1)) * OS + j * 16 + g + (c >> 1) * 8] = o[j][nt][c];
+    named_bar(1, NTH);
+
+    // the warps' parts of a row, joined in warp order: weights 2^(m_w - M); a part without a key has sum 0
+    const bool whole = wk.whole();
+    float* part = p.parts + (blockIdx.x * 2 + (first > 0 ? 0 : 1)) * C::kPiece;
+    constexpr int kVecs = D / 4;
+    for (int e = tid; e < rows * kVecs; e += NTH) {
+      const int r = e / kVecs, d = (e % kVecs) * 4;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+        if (sL[w * R + r] != 0.f) M = fmaxf(M, sM[w * R + r]);
+      float L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float lw = sL[w * R + r];
+        if (lw != 0.f) {
+          const float f = exp2_approx(sM[w * R + r] - M);
+          const float4 v = *reinterpret_cast<const float4*>(sO + (w * R + r) * OS + d);
+          L += f * lw;
+          acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+        }
+      }
+      if (whole) {
+        const int i = r / p.G, h = wk.h * p.G + r % p.G;
+        const bool sees = keys_seen(p, wk.s, wk.tok0() + i + 1) > 0;
+        const long long row = wk.s.q0 + wk.tok0() + i;
+        const float inv = sees ? 1.f / L : 0.f;
+        *reinterpret_cast<uint2*>(p.out + row * p.o_st + h * p.o_sh + d) =
+            make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+        if (p.lse != nullptr && d == 0) p.lse[row * p.Hq + h] = sees ? M * kLn2 + logf(L) : -INFINITY;
+      } else {
+        *reinterpret_cast<float4*>(part + r * D + d) = acc;
+        if (d == 0) {
+          part[R * D + r] = M;
+          part[R * D + R + r] = L;
+        }
+      }
+    }
+    if (!whole) {
+      // the CTA that leaves the item's last missing piece joins them all
+      const unsigned int c0 = cut.cta_of(wk.item_start), c1 = cut.cta_of(wk.item_start + wk.units - 1);
+      const int n = static_cast<int>(c1 - c0) + 1;
+      __threadfence();
+      named_bar(1, NTH);
+      if (tid == 0) {
+        const bool last = atomicAdd(&p.counters[c0], 1u) == static_cast<unsigned int>(n - 1);
+        if (last) p.counters[c0] = 0u;
+        __threadfence();
+        *flag = last;
+      }
+      named_bar(1, NTH);
+      if (*flag) {
+        const float* base_part = p.parts + static_cast<size_t>(c0) * 2 * C::kPiece;
+        // piece i: CTA c0's piece starts the item (its slot 1), every later one starts inside it (slot 0)
+        auto piece = [&](int i) { return base_part + (i == 0 ? C::kPiece : i * 2 * C::kPiece); };
+        float* sW = sO;                      // [rows][n] weights
+        float* sRow = sO + kMaxCtas * R;     // [rows] M, then [rows] L
+        for (int r = warp; r < rows; r += NW) {
+          float M = -INFINITY;
+          for (int i = lane; i < n; i += 32) {
+            const float* pc = piece(i);
+            if (ld_cg_f32(pc + R * D + R + r) != 0.f) M = fmaxf(M, ld_cg_f32(pc + R * D + r));
+          }
+#pragma unroll
+          for (int o2 = 16; o2 > 0; o2 >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o2));
+          float L = 0.f;
+          for (int i = lane; i < n; i += 32) {
+            const float* pc = piece(i);
+            const float lw = ld_cg_f32(pc + R * D + R + r);
+            const float f = lw != 0.f ? exp2_approx(ld_cg_f32(pc + R * D + r) - M) : 0.f;
+            if (lw != 0.f) L += f * lw;
+            sW[r * n + i] = f;
+          }
+          L = warp_sum(L);
+          if (lane == 0) {
+            sRow[r] = M;
+            sRow[R + r] = L;
+          }
+        }
+        named_bar(1, NTH);
+        for (int e = tid; e < rows * kVecs; e += NTH) {
+          const int r = e / kVecs, d = (e % kVecs) * 4;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int i = 0; i < n; ++i) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(i) + r * D + d));
+            const float f = sW[r * n + i];
+            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+          }
+          const int i = r / p.G, h = wk.h * p.G + r % p.G;
+          const bool sees = keys_seen(p, wk.s, wk.tok0() + i + 1) > 0;
+          const long long row = wk.s.q0 + wk.tok0() + i;
+          const float inv = sees ? 1.f / sRow[R + r] : 0.f;
+          *reinterpret_cast<uint2*>(p.out + row * p.o_st + h * p.o_sh + d) =
+              make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+          if (p.lse != nullptr && d == 0) p.lse[row * p.Hq + h] = sees ? sRow[r] * kLn2 + logf(sRow[R + r]) : -INFINITY;
+        }
+      }
+    }
+    named_bar(1, NTH);  // the merge buffer and Q are free again
+  }
+}
+
+template <int D, int NT>
+int launch_split(const Problem& p, const Source& src, bool bf16, int grid, cudaStream_t st) {
+  using C = Cfg<D, NT>;
+  CUtensorMap mk, mv_;
+  const int box = src.box < C::kBN ? src.box : C::kBN;
+  const int rc = make_kv_maps(&mk, &mv_, src, p.Hkv, D, bf16, box);
+  if (rc != MV_OK) return rc;
+  auto fn = bf16 ? split_kernel<D, NT, true> : split_kernel<D, NT, false>;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attention split)");
+  fn<<<grid, C::kThreads, C::kSmem, st>>>(mk, mv_, p, box);
+  return cuda_status(cudaGetLastError(), "attention split launch");
+}
+
+}  // namespace
+
+// The kernel for `rows_hint` rows per (sequence, key head); any number is computed rightly (tiles of tok tokens).
+int run_split(Problem& p, const Source& src, int D, bool bf16, int rows_hint, int grid, cudaStream_t st) {
+  const int nt = rows_hint <= 8 && p.G <= 8 ? 1 : rows_hint <= 16 && p.G <= 16 ? 2 : 4;
+  p.tok = 8 * nt / p.G;
+  p.min_share = 8;
+  if (D == 128) {
+    if (nt == 1) return launch_split<128, 1>(p, src, bf16, grid, st);
+    if (nt == 2) return launch_split<128, 2>(p, src, bf16, grid, st);
+    return launch_split<128, 4>(p, src, bf16, grid, st);
+  }
+  if (nt == 1) return launch_split<64, 1>(p, src, bf16, grid, st);
+  if (nt == 2) return launch_split<64, 2>(p, src, bf16, grid, st);
+  return launch_split<64, 4>(p, src, bf16, grid, st);
+}
+
+}  // namespace attn
+}  // namespace mv

@@ -13,6 +13,8 @@ namespace mv {
 constexpr unsigned int kErrTimeout = 1;     // an mbarrier wait gave up (bounded spin)
 constexpr unsigned int kErrBadExpert = 2;   // an expert id outside [0, E1) was skipped
 constexpr unsigned int kErrOverflow = 3;    // a token capacity was exceeded (skipped)
+constexpr unsigned int kErrBadPage = 4;     // a page id or a position outside the cache (skipped or read as zeros)
+constexpr unsigned int kErrBadSeq = 5;      // sequence bounds or lengths that do not fit the tensors (clamped)
 
 // Wall-clock limit of one bounded wait on the device.
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s

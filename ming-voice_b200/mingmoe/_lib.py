@@ -45,6 +45,13 @@ class Block(C.Structure):
                 ("residual_from_x", I32), ("pad0", I32), ("route_scale", F64), ("next", P)]
 
 
+class PagedKV(C.Structure):
+    """mirror of `mv_paged_kv`"""
+    _fields_ = [("k", P), ("v", P), ("dtype", I32), ("num_pages", I32), ("page_size", I32), ("n_kv_heads", I32),
+                ("head_dim", I32), ("pad0", I32), ("k_sp", I64), ("k_st", I64), ("k_sh", I64), ("v_sp", I64),
+                ("v_st", I64), ("v_sh", I64)]
+
+
 _SIGS = {
     "mv_version": (I32, []),
     "mv_last_error": (C.c_char_p, []),
@@ -76,6 +83,13 @@ _SIGS = {
     "mv_ep_pack": (I32, [P, I64, I32, P, P, I32, I32, P, P]),
     "mv_ep_unpack": (I32, [P, I32, I32, I32, I32, P, P, P]),
     "mv_ep_narrow": (I32, [P, I64, P, P]),
+    "mv_kv_append": (I32, [C.POINTER(PagedKV), P, I64, I64, P, I64, I64, P, I64, I64, I32, P, I64, I64, I32, P, I64,
+                           I32, P, P, I32, P, I64, I32, I32, I32, P, P, SZ, P]),
+    "mv_paged_attention": (I32, [C.POINTER(PagedKV), P, I64, I64, I32, I32, P, I64, I32, P, P, I32, I32, F32, I32, P,
+                                 I64, I64, P, P, SZ, P]),
+    "mv_prompt_attention": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, I32, I32, I32, I32, I32, I32, P, P, I32, I32,
+                                  F32, I32, P, I64, I64, P, P, SZ, P]),
+    "mv_attention_workspace_bytes": (SZ, []),
     "mv_ep_combine": (I32, [P, I64, P, P, I32, P, I32, I32, I32, P, P]),
 }
 
