@@ -290,7 +290,7 @@ MV_API int mv_mask_pad_rows(void* ids, int ids_dtype, int N, int NK, const int* 
  * libraries, engine.py:234-282). Common terms:
  *  - A batch of B sequences is packed: sequence b owns rows [cu_seqlens[b], cu_seqlens[b + 1]) of the token
  *    tensors (cu_seqlens [B + 1] int32, ascending; a sequence may own no row).
- *  - Heads are grouped: query head h reads key / value head h / G, G = Hq / Hkv (a whole number, 1..32).
+ *  - Heads are grouped: query head h reads key / value head h / G, G = Hq / Hkv (a whole number, 1..64).
  *  - Element types: bf16 or f16, one for all tensors of a call. head_dim is 64 or 128, inner stride 1, every row
  *    and head stride a multiple of 16 bytes, 16-byte aligned pointers. Strides are in elements.
  *  - All indices (cu_seqlens, lengths, page ids) are read on the device: nothing synchronises the host and a

@@ -73,18 +73,35 @@ int make_kv_maps(CUtensorMap* mk, CUtensorMap* mv_, const Source& s, int heads, 
   return make_map(mv_, s.v, bf16, d, s.tokens, heads, s.pages, s.v_st, s.v_sh, s.v_sp, box, "v");
 }
 
+int make_q_map(CUtensorMap* m, const Problem& p, int d, bool bf16, int tok) {
+  auto enc = encode_fn();
+  if (enc == nullptr) return fail(MV_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(p.Hq), static_cast<cuuint64_t>(p.T)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.Hq > 1 ? p.q_sh : d) * 2,
+                                 static_cast<cuuint64_t>(p.T > 1 ? p.q_st : d) * 2};
+  const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(p.G), static_cast<cuuint32_t>(tok)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<uint16_t*>(p.q), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MV_ERR_INVALID, "tensor map for q rejected (CUresult %d)", static_cast<int>(r));
+  return MV_OK;
+}
+
 int run_split(Problem& p, const Source& src, int D, bool bf16, int rows_hint, int grid, cudaStream_t st);
+int run_tile(Problem& p, const Source& src, int D, bool bf16, int grid, cudaStream_t st);
 
 namespace {
 
-constexpr size_t kCountersBytes = 1024;                                     // kMaxCtas counters, padded
+constexpr size_t kCountersBytes = 1024 + kMaxCtas * 32;                     // arrival counters, cut items
 constexpr size_t kPartsBytes = size_t(kMaxCtas) * 2 * 256 * (128 + 2) * 4;  // two pieces of 256 rows per CTA
 
 int run(Problem& p, const Source& src, int D, int dtype, int B, const int* cu_q, const int* cu_k, const int* kv_lens,
         int max_q, float scale, void* workspace, size_t workspace_bytes, cudaStream_t st, const char* who) {
   if (!(scale > 0.f) || scale > 3.0e38f) return fail(MV_ERR_INVALID, "%s: scale must be positive and finite", who);
-  if (p.Hq < 1 || p.Hq % p.Hkv != 0 || p.Hq / p.Hkv > 32)
-    return fail(MV_ERR_INVALID, "%s: Hq=%d must be 1..32 times Hkv=%d", who, p.Hq, p.Hkv);
+  if (p.Hq < 1 || p.Hq % p.Hkv != 0 || p.Hq / p.Hkv > 64)
+    return fail(MV_ERR_INVALID, "%s: Hq=%d must be 1..64 times Hkv=%d", who, p.Hq, p.Hkv);
   if (workspace == nullptr || workspace_bytes < mv_attention_workspace_bytes() ||
       (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return fail(MV_ERR_WORKSPACE, "%s: 256-byte aligned workspace of %zu bytes needed", who,
@@ -101,14 +118,15 @@ int run(Problem& p, const Source& src, int D, int dtype, int B, const int* cu_q,
   int rc = MV_OK;
   const long long pt_row = p.pt_stride;
   const int* table = p.page_table;
-  const int rows = max_q > 0 && max_q < 64 ? max_q * p.G : 64;
+  const int rows = max_q > 0 && max_q < 64 ? max_q * p.G : 64 * p.G;
   for (int b0 = 0; b0 < B; b0 += kMaxB) {
     p.B = B - b0 < kMaxB ? B - b0 : kMaxB;
     p.cu_q = cu_q + b0;
     p.cu_k = cu_k == nullptr ? nullptr : cu_k + b0;
     p.kv_lens = kv_lens == nullptr ? nullptr : kv_lens + b0;
     p.page_table = table == nullptr ? nullptr : table + b0 * pt_row;
-    if ((rc = run_split(p, src, D, bf16, rows, grid, st)) != MV_OK) return rc;
+    rc = rows <= 32 ? run_split(p, src, D, bf16, rows, grid, st) : run_tile(p, src, D, bf16, grid, st);
+    if (rc != MV_OK) return rc;
   }
   return MV_OK;
 }

@@ -235,5 +235,8 @@ struct Source {
 // 4-D maps over keys and values [page][head][token][d], 128-byte swizzle, box of 64 values x `box` tokens
 int make_kv_maps(CUtensorMap* mk, CUtensorMap* mv_, const Source& src, int heads, int d, bool bf16, int box);
 
+// 3-D map over queries [token][head][d], 128-byte swizzle, box of 64 values x the G heads of a key head x `tok` tokens
+int make_q_map(CUtensorMap* m, const Problem& p, int d, bool bf16, int tok);
+
 }  // namespace attn
 }  // namespace mv

@@ -1,0 +1,565 @@
+// Attention of many rows per key head (prompts, chunks of new tokens) on the 5th-generation tensor cores.
+//
+// Mathematics: as in attn_split.cu, a running maximum and sum per row over tiles of 128 keys. The maximum that the
+// weights are taken against is raised only when a tile exceeds it by more than 8 (in powers of two): weights then stay
+// below 2^8, nothing overflows, and the accumulator is rarely rescaled; out = sum p v / sum p is the same.
+//
+// Bound: the tensor pipe and the exponential unit together. A 128 x 128 tile of scores takes 2 x 128^2 x D
+// multiply-adds (512 + 512 cycles at D = 128) and 16384 exponentials (1024 cycles at 16 a cycle and SM), so the two
+// have to run side by side.
+//
+// Layout of a CTA (one per SM): a work item is two tiles of 128 rows (row = token * G + head) of one sequence and key
+// head, which share the key and value tiles in shared memory.
+//   warp 0       TMA producer: Q tiles, then K and V tiles in turn into a ring of slots (a box per page and 64 values)
+//   warp 1       MMA issuer: S_t = Q_t K^T and O_t += P_t V, both into TMEM; P_t is the TMEM operand
+//   warps 4..7   softmax of tile 0, warps 8..11 of tile 1: a thread owns a row (a TMEM lane). S -> weights P, written
+//                over S in TMEM; the row's sum and maximum stay in registers; at the end O / sum -> global memory.
+// While one tile's scores are in the softmax, the other tile's products run. The order of issue per tile is
+// PV(j), QK(j + 1): S(j + 1) overwrites P(j) behind the product that reads it.
+// TMEM columns: S_0 | S_1 | O_0 | O_1 (4 x 128 of 512 at D = 128).
+//
+// Split: equal shares of all (item, key tile) units (attn_common.cuh). Pieces of a cut item go to the workspace and
+// combine_kernel joins them in CTA order.
+#include "attn_common.cuh"
+
+namespace mv {
+namespace attn {
+namespace {
+
+constexpr int kBN = 128;        // keys of a tile
+constexpr int kM = 128;         // rows of a tile
+constexpr int kThreads = 384;
+constexpr float kGrow = 8.f;    // growth of the maximum, in powers of two, that is not followed at once
+
+template <int D>
+struct Cfg {
+  static constexpr int kTile = kBN * D * 2;         // bytes of a K or V tile
+  static constexpr int kQ = kM * D * 2;             // bytes of a Q tile
+  static constexpr int kSlots = 131072 / kTile;     // K and V tiles in turn
+  static constexpr int oKV = 2 * kQ;
+  static constexpr int oPre = oKV + kSlots * kTile;
+  static constexpr int oTmp = oPre + (kMaxB + 1) * 8;
+  static constexpr int oBar = oTmp + 32 * 8;
+  static constexpr int kBars = 2 * kSlots + 2 + 6 + 1;
+  static constexpr int oTmem = oBar + kBars * 8;
+  static constexpr int kSmem = oTmem + 16 + 1024;
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+// What combine_kernel needs of a cut item, left by the CTA whose range holds its start.
+struct CutItem {
+  int n;         // pieces (0: none)
+  int row0;      // first token's row
+  int ntok;      // tokens
+  int h;         // key head
+  int first;     // first token that sees a key
+  int pad[3];
+};
+static_assert(sizeof(CutItem) == 32, "");
+
+// D[tmem] (+)= A[tmem] * B[smem], 16-bit operands, fp32 accumulation; issued by one thread.
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Descriptor of V as the MN-major operand (N = head values, contiguous; K = keys): atoms of 8 keys x 64 values
+// (8 x 128 B, 128-byte swizzle). Leading offset (bits 16-29): to the next 64 values; stride offset (32-45): to the
+// next 8 keys, 1024 B.
+__device__ __forceinline__ uint64_t v_desc(uint32_t saddr, uint32_t half_bytes) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(half_bytes >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+
+// kind::f16 instruction descriptor (tc.cuh's fields) for either element type; b_mn: B is MN-major (bit 16).
+__host__ __device__ constexpr uint32_t idesc16(bool bf16, int M, int N, bool b_mn) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// Bounded wait, in line: a call would hold the softmax's registers to the calling convention (setmaxnreg kernels).
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, WsHeader* h, unsigned int info) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      raise_error(h, kErrTimeout, info);
+      return false;
+    }
+  return true;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                const __grid_constant__ CUtensorMap tmV, const Problem p, int box, CutItem* __restrict__ cuts) {
+  using C = Cfg<D>;
+  constexpr int NS = C::kSlots, kHalves = D / 64, kHalfBytes = kBN * 128;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + C::oKV;
+  unsigned long long* pre = reinterpret_cast<unsigned long long*>(smem + C::oPre);
+  unsigned long long* tmp = reinterpret_cast<unsigned long long*>(smem + C::oTmp);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBar);
+  uint64_t* empty = full + NS;
+  uint64_t* q_full = empty + NS;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;  // [2] scores of tile t are in TMEM (and the product before them is complete)
+  uint64_t* p_full = s_full + 2;   // [2] weights of tile t are in TMEM, its accumulator may be added to
+  uint64_t* o_full = p_full + 2;   // [2] the piece's last product of tile t is complete
+  uint64_t* done = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::oTmem);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], kM);
+      mbar_init(&o_full[t], 1);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
+    tc::prefetch_tmap(&tmQ);
+    tc::prefetch_tmap(&tmK);
+    tc::prefetch_tmap(&tmV);
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, 512);
+    tc::tmem_relinquish();
+  }
+  const int half_tok = p.tok / 2;       // tokens of a 128-row tile
+  const int rows_used = half_tok * p.G;
+  if (rows_used < kM) {  // Q rows that no copy writes: any finite values
+    for (int e = threadIdx.x; e < 2 * kHalves * (kM - rows_used) * 8; e += kThreads) {
+      const int c = e & 7, r = rows_used + (e >> 3) % (kM - rows_used), hf = (e >> 3) / (kM - rows_used);
+      *reinterpret_cast<uint4*>(smem + hf * kHalfBytes + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+  }
+  tc::fence_before_sync();
+  build_schedule<kBN>(p, pre, tmp);
+  tc::fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  const unsigned long long W = pre[p.B];
+  const Cut cut(W, gridDim.x, p.min_share);
+  const unsigned long long at = W ? cut.bound(blockIdx.x) : 0, end = W ? cut.bound(blockIdx.x + 1) : 0;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    Walk<kBN> wk(p, pre, at, end);
+    if (warp == 0) {
+      // ---------------------------------------------------------------- TMA producer
+      const int nbox = kBN / box, half = lane % kHalves, bx = lane / kHalves;
+      int it = 0, qn = 0;
+      bool ok = true;
+      for (; wk.more() && ok; wk.next()) {
+        const int kend = wk.kend(), ntok = wk.ntok();
+        const int i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+        if (wk.first() >= i1) continue;
+        const int nt = ntok > half_tok ? 2 : 1;
+        ok = __all_sync(0xffffffffu, wait_bar(q_empty, (qn & 1) ^ 1, p.ws, 0x740u));
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(nt * kHalves * rows_used * 128));
+          for (int t = 0; t < nt; ++t)
+            for (int hf = 0; hf < kHalves; ++hf)
+              tc::tma_load_3d(smem + t * C::kQ + hf * kHalfBytes, &tmQ, q_full, hf * 64, wk.h * p.G,
+                              wk.s.q0 + wk.tok0() + t * half_tok);
+        }
+        ++qn;
+        for (int i = wk.first(); i < i1 && ok; ++i) {
+          const int j = i * kBN + bx * box;
+          const bool mine = bx < nbox && j < kend;
+          int page = 0, row = wk.s.k0 + j;
+          if (mine && p.page_table != nullptr) {
+            page = p.page_table[wk.b * p.pt_stride + (j >> p.page_shift)];
+            row = j & ((1 << p.page_shift) - 1);
+            if (page < 0 || page >= p.num_pages) {
+              raise_error(p.ws, kErrBadPage, 0x711u);
+              page = p.num_pages;  // outside the map: reads as zeros
+            }
+          }
+          const uint32_t bytes = static_cast<uint32_t>(min(nbox, (kend - i * kBN + box - 1) / box) * box * D * 2);
+          for (int kv = 0; kv < 2; ++kv, ++it) {
+            const int slot = it % NS;
+            ok = __all_sync(0xffffffffu, wait_bar(&empty[slot], ((it / NS) & 1) ^ 1, p.ws, 0x741u));
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
+            __syncwarp();
+            if (mine)
+              tc::tma_load_4d(ring + slot * C::kTile + half * kHalfBytes + bx * box * 128, kv ? &tmV : &tmK,
+                              &full[slot], half * 64, row, wk.h, page);
+          }
+        }
+      }
+      // copies in flight land before the CTA exits
+      if (lane == 0) {
+        if (qn > 0) wait_bar(q_full, (qn - 1) & 1, p.ws, 0x742u);
+        for (int i = 0; i < NS && i < it; ++i)
+          wait_bar(&full[i], static_cast<uint32_t>(((it - 1 - i) / NS) & 1), p.ws, 0x743u);
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA issuer (lane 0)
+      constexpr uint32_t id_qk = idesc16(BF16, kM, kBN, false), id_pv = idesc16(BF16, kM, D, true);
+      int it = 0, qn = 0;
+      uint32_t pn[2] = {0, 0};
+      bool ok = true;
+      auto qk = [&](int t, int slot) {
+        if (lane == 0) {
+          const uint32_t qa = smem_u32(smem + t * C::kQ), ka = smem_u32(ring + slot * C::kTile);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks)
+            tc::mma_bf16(tmem + t * 128, tc::sw128_desc(qa + (ks / 4) * kHalfBytes) + 2 * (ks & 3),
+                         tc::sw128_desc(ka + (ks / 4) * kHalfBytes) + 2 * (ks & 3), id_qk, ks != 0);
+          tc::mma_commit(&s_full[t]);
+        }
+      };
+      for (; wk.more() && ok; wk.next()) {
+        const int kend = wk.kend();
+        const int i0 = wk.first(), i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+        if (i0 >= i1) continue;
+        const int nt = wk.ntok() > half_tok ? 2 : 1;
+        ok = wait_bar(q_full, qn & 1, p.ws, 0x750u) && wait_bar(&full[it % NS], (it / NS) & 1, p.ws, 0x751u);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++qn;
+        tc::fence_after_sync();
+        for (int t = 0; t < nt; ++t) qk(t, it % NS);
+        if (lane == 0) {
+          tc::mma_commit(&empty[it % NS]);
+          if (i0 + 1 == i1) tc::mma_commit(q_empty);
+        }
+        ++it;
+        for (int i = i0; i < i1 && ok; ++i) {
+          const bool more = i + 1 < i1;
+          const int vs = it % NS, ks = (it + 1) % NS;
+          ok = wait_bar(&full[vs], (it / NS) & 1, p.ws, 0x752u);
+          if (more) ok = ok && wait_bar(&full[ks], ((it + 1) / NS) & 1, p.ws, 0x753u);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int nv = min(kBN, kend - i * kBN), steps = (nv + 15) / 16;
+          if (nv < steps * 16) {
+            // rows behind the last key hold anything (an older page's values, NaN, another sequence's): their weights
+            // are 0, and 0 * NaN is not, so the values are cleared
+            for (int e = lane; e < (steps * 16 - nv) * kHalves * 8; e += 32) {
+              const int c = e & 7, hf = (e >> 3) % kHalves, r = nv + (e >> 3) / kHalves;
+              *reinterpret_cast<uint4*>(ring + vs * C::kTile + hf * kHalfBytes + r * 128 + c * 16) =
+                  make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          for (int t = 0; t < nt && ok; ++t) {
+            ok = __all_sync(0xffffffffu, wait_bar(&p_full[t], pn[t] & 1, p.ws, 0x754u));
+            if (!ok) break;
+            ++pn[t];
+            tc::fence_after_sync();
+            if (lane == 0) {
+              const uint32_t va = smem_u32(ring + vs * C::kTile);
+              for (int k = 0; k < steps; ++k)
+                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, v_desc(va + k * 2048, kHalfBytes), id_pv,
+                       i > i0 || k > 0);
+              if (!more) tc::mma_commit(&o_full[t]);
+            }
+            if (more) qk(t, ks);
+          }
+          if (!ok) break;
+          if (lane == 0) {
+            tc::mma_commit(&empty[vs]);
+            if (more) tc::mma_commit(&empty[ks]);
+            if (i + 2 == i1) tc::mma_commit(q_empty);
+          }
+          it += more ? 2 : 1;
+        }
+      }
+      // every issued product retires before the TMEM is released
+      if (lane == 0) {
+        tc::mma_commit(done);
+        wait_bar(done, 0u, p.ws, 0x755u);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax: tile t, a thread per row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    Walk<kBN> wk(p, pre, at, end);
+    const int t = warp >= 8, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + 256 + t * 128;
+    uint32_t sn = 0, on = 0;
+    bool ok = true;
+    const int my_tok = t * half_tok + r / p.G, my_head = r % p.G;
+    CutItem mine{};
+    for (; wk.more() && ok; wk.next()) {
+      const int kend = wk.kend(), ntok = wk.ntok(), i0 = wk.first();
+      const int i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+      const bool whole = wk.whole();
+      if (!whole && i0 == 0) {
+        mine.n = static_cast<int>(cut.cta_of(wk.item_start + wk.units - 1) - blockIdx.x) + 1;
+        mine.row0 = wk.s.q0 + wk.tok0();
+        mine.ntok = ntok;
+        mine.h = wk.h;
+        mine.first = p.causal ? max(0, wk.s.nq - wk.s.n - wk.tok0()) : 0;
+      }
+      if (t == 1 && ntok <= half_tok) continue;
+      const bool live = r < rows_used && my_tok < ntok;
+      // keys the row sees; rows that are not there see what the last one does
+      const int lim = keys_seen(p, wk.s, wk.tok0() + min(my_tok, ntok - 1) + 1);
+      const int lim_min = keys_seen(p, wk.s, wk.tok0() + t * half_tok + 1);
+      float m = -INFINITY, l = 0.f;
+      for (int i = i0; i < i1; ++i) {
+        ok = __all_sync(0xffffffffu, wait_bar(&s_full[t], sn & 1, p.ws, 0x760u));
+        if (!ok) break;
+        ++sn;
+        tc::fence_after_sync();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc::tmem_ld32(tS + c * 32, s[c]);
+        tc::tmem_ld_wait();
+        if ((i + 1) * kBN > lim_min) {
+          const int left = lim - i * kBN;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e >= left) s[c][e] = 0xff800000u;  // -inf
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+          for (int e = 1; e < 31; e += 2)
+            mx[c] = max3(mx[c], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+          mx[c] = fmaxf(mx[c], __uint_as_float(s[c][31]));
+        }
+        const float tile_max = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+        const bool grow = tile_max > m && (tile_max - m) * p.scale_log2 > kGrow;  // m = -inf: the difference is inf
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = grow ? exp2_approx((m - tile_max) * p.scale_log2) : 1.f;
+          if (grow) m = tile_max;
+          l *= alpha;
+          if (i > i0) {
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tc::tmem_ld16(tO + c * 16, o);
+              tc::tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st16(tO + c * 16, o);
+            }
+          }
+        }
+        // weights 2^(s scale + base), one fused multiply-add each; the rounding of base is the same for all of a row's
+        // weights and cancels in the quotient, unless it is so large that they overflow: then s - m is taken first
+        float base = m == -INFINITY ? 0.f : -m * p.scale_log2;  // nothing seen yet: every weight is 2^-inf = 0
+        if (__any_sync(0xffffffffu, fabsf(base) > 16777216.f) && fabsf(base) > 16777216.f) {
+          base = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[c][e] = __float_as_uint(__uint_as_float(s[c][e]) - m);
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0 = base, x1 = base;
+            ffma2(x0, x1, __uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1]), p.scale_log2, p.scale_log2);
+            x0 = exp2_approx(x0);
+            x1 = exp2_approx(x1);
+            ffma2(sum[(e & 1) * 2], sum[(e & 1) * 2 + 1], x0, x1, 1.f, 1.f);
+            // the weights are rounded to the element type here, as operands of the second product
+            pk[e] = pack2<BF16>(x0, x1);
+          }
+          tmem_st16(tS + c * 16, pk);
+        }
+        tmem_st_wait();
+        tc::fence_before_sync();
+        mbar_arrive(&p_full[t]);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      }
+      if (!ok) break;
+      const int slot = i0 > 0 ? 0 : 1;
+      float* part = p.parts + (static_cast<size_t>(blockIdx.x) * 2 + slot) * (256 * (128 + 2));
+      const float m2 = m * p.scale_log2;
+      if (i1 > i0) {
+        ok = __all_sync(0xffffffffu, wait_bar(&o_full[t], on & 1, p.ws, 0x761u));
+        if (!ok) break;
+        ++on;
+        tc::fence_after_sync();
+      }
+      const long long row = wk.s.q0 + wk.tok0() + my_tok;
+      const int head = wk.h * p.G + my_head;
+      const bool sees = lim > 0;
+      const float inv = sees ? 1.f / l : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (i1 > i0) {
+          tc::tmem_ld32(tO + c * 32, o);
+          tc::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (!live) continue;
+        if (whole) {
+          uint4* dst = reinterpret_cast<uint4*>(p.out + row * p.o_st + head * p.o_sh + c * 32);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = sees ? pack2<BF16>(__uint_as_float(o[v * 8 + 2 * e]) * inv, __uint_as_float(o[v * 8 + 2 * e + 1]) * inv)
+                          : 0u;
+            dst[v] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+          float4* dst = reinterpret_cast<float4*>(part + (t * kM + r) * D + c * 32);
+#pragma unroll
+          for (int v = 0; v < 8; ++v)
+            dst[v] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]), __uint_as_float(o[4 * v + 2]),
+                                 __uint_as_float(o[4 * v + 3]));
+        }
+      }
+      if (live) {
+        if (whole) {
+          if (p.lse != nullptr) p.lse[row * p.Hq + head] = sees ? m2 * kLn2 + logf(l) : -INFINITY;
+        } else {
+          part[256 * D + t * kM + r] = m2;
+          part[256 * D + 256 + t * kM + r] = l;
+        }
+      }
+      tc::fence_before_sync();  // the accumulator is read before the next item's first product is allowed
+    }
+    if (threadIdx.x == 128) cuts[blockIdx.x] = mine;
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the pieces of the item that starts in CTA blockIdx.x's range and ends in a later one's: rows blockIdx.y * 32 ..
+// + 31 of its 256, weights 2^(m_piece - M), pieces in CTA order.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) combine_kernel(const Problem p, const CutItem* __restrict__ cuts) {
+  __shared__ float sW[32][kMaxCtas + 1];
+  __shared__ float sM[32], sL[32];
+  const CutItem c = cuts[blockIdx.x];
+  if (c.n <= 1) return;
+  const int half_tok = p.tok / 2, rows_used = half_tok * p.G;
+  const int R0 = blockIdx.y * 32;
+  const int t = R0 / kM;
+  if (t * half_tok >= c.ntok) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr size_t kPiece = 256 * (128 + 2);
+  // the first piece is CTA blockIdx.x's last (slot 1), the others are their CTAs' first (slot 0)
+  auto piece = [&](int i) { return p.parts + (static_cast<size_t>(blockIdx.x + i) * 2 + (i == 0)) * kPiece; };
+  auto live = [&](int R) { return R % kM < rows_used && t * half_tok + (R % kM) / p.G < c.ntok; };
+  for (int q = warp; q < 32; q += 8) {
+    const int R = R0 + q;
+    if (!live(R)) continue;
+    float M = -INFINITY;
+    for (int i = lane; i < c.n; i += 32) {
+      const float* pc = piece(i) + 256 * D;
+      if (pc[256 + R] != 0.f) M = fmaxf(M, pc[R]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float L = 0.f;
+    for (int i = lane; i < c.n; i += 32) {
+      const float* pc = piece(i) + 256 * D;
+      const float lw = pc[256 + R];
+      const float f = lw != 0.f ? exp2_approx(pc[R] - M) : 0.f;  // a piece without a visible key counts for nothing
+      if (lw != 0.f) L += f * lw;
+      sW[q][i] = f;
+    }
+    L = warp_sum(L);
+    if (lane == 0) {
+      sM[q] = M;
+      sL[q] = L;
+    }
+  }
+  __syncthreads();
+  constexpr int kVecs = D / 4;
+  for (int e = threadIdx.x; e < 32 * kVecs; e += 256) {
+    const int q = e / kVecs, d = (e % kVecs) * 4, R = R0 + q;
+    if (!live(R)) continue;
+    const int tok = t * half_tok + (R % kM) / p.G, head = c.h * p.G + (R % kM) % p.G;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < c.n; ++i) {
+      const float f = sW[q][i];
+      if (f == 0.f) continue;
+      const float4 v = *reinterpret_cast<const float4*>(piece(i) + R * D + d);
+      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+    }
+    const bool sees = tok >= c.first;
+    const float inv = 1.f / sL[q];
+    const long long row = c.row0 + tok;
+    uint2 w = make_uint2(0u, 0u);
+    if (sees) w = make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(p.out + row * p.o_st + head * p.o_sh + d) = w;
+    if (p.lse != nullptr && d == 0) p.lse[row * p.Hq + head] = sees ? sM[q] * kLn2 + logf(sL[q]) : -INFINITY;
+  }
+}
+
+template <int D, bool BF16>
+int launch_tile(const Problem& p, const Source& src, int grid, CutItem* cuts, cudaStream_t st) {
+  using C = Cfg<D>;
+  CUtensorMap mq, mk, mv_;
+  const int box = src.box < kBN ? src.box : kBN;
+  int rc = make_kv_maps(&mk, &mv_, src, p.Hkv, D, BF16, box);
+  if (rc == MV_OK) rc = make_q_map(&mq, p, D, BF16, p.tok / 2);
+  if (rc != MV_OK) return rc;
+  auto fn = tile_kernel<D, BF16>;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attention tile)");
+  fn<<<grid, kThreads, C::kSmem, st>>>(mq, mk, mv_, p, box, cuts);
+  if ((e = cudaGetLastError()) != cudaSuccess) return cuda_status(e, "attention tile launch");
+  combine_kernel<D, BF16><<<dim3(grid, 8), 256, 0, st>>>(p, cuts);
+  return cuda_status(cudaGetLastError(), "attention combine launch");
+}
+
+}  // namespace
+
+int run_tile(Problem& p, const Source& src, int D, bool bf16, int grid, cudaStream_t st) {
+  p.tok = 2 * (kM / p.G);
+  p.min_share = 4;
+  CutItem* cuts = reinterpret_cast<CutItem*>(p.counters + 256);
+  if (D == 128)
+    return bf16 ? launch_tile<128, true>(p, src, grid, cuts, st) : launch_tile<128, false>(p, src, grid, cuts, st);
+  return bf16 ? launch_tile<64, true>(p, src, grid, cuts, st) : launch_tile<64, false>(p, src, grid, cuts, st);
+}
+
+}  // namespace attn
+}  // namespace mv

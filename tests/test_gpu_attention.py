@@ -185,6 +185,7 @@ PAGED = [  # dtype, d, hq, hkv, page, new, kv
     (FP, 128, 15, 5, 16, [8, 2], [77, 515]),
     (BF, 128, 16, 4, 64, [130, 17, 1], [130, 400, 333]),
     (FP, 64, 28, 4, 32, [65, 256], [300, 256]),
+    (BF, 128, 64, 1, 128, [1, 5], [500, 127]),
 ]
 
 
@@ -365,6 +366,8 @@ PROMPTS = [  # dtype, d, hq, hkv, lens
     (FP, 128, 6, 2, [63, 65]),
     (BF, 128, 20, 1, [33, 150]),
     (FP, 128, 32, 1, [5, 20]),
+    (BF, 64, 80, 2, [33, 150]),
+    (FP, 128, 64, 1, [5, 20]),
 ]
 
 
@@ -488,7 +491,7 @@ def test_refusals(cuda):
     with pytest.raises(ValueError):
         A.paged_attention(q, *args, out=torch.empty(2, 8, 128, dtype=BF, device=dev))
     with pytest.raises(RuntimeError):
-        A.paged_attention(randn((1, 66, 128), BF, dev, 1), *args)  # 33 query heads to a key head
+        A.paged_attention(randn((1, 130, 128), BF, dev, 1), *args)  # 65 query heads to a key head
     with pytest.raises(ValueError):
         A.kv_append(P.cache, k, k[:, :1], P.table, cu, P.lens)
     with pytest.raises(RuntimeError):
