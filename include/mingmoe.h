@@ -318,41 +318,54 @@ typedef struct mv_paged_kv {
  * the values are copied: pair i < rot_dim / 2 is (x[i], x[i + rot_dim / 2]), or (x[2i], x[2i + 1]) when interleaved,
  *   y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin,
  * with cos_sin [max_pos, rot_dim] f32 (row stride cs_stride): a position's rot_dim / 2 cosines, then its sines.
- * rot_dim 0 (cos_sin NULL) rotates nothing. positions [T] int32 or NULL replaces the cache position as the row of
- * cos_sin (the cache slot stays the same). A token whose page id, slot or position is outside the cache, the page
- * table or cos_sin is skipped (error 4): neither its cache slot nor its q_out row is written. Rows outside every
- * sequence are left alone. workspace: a zeroed header of mv_attention_workspace_bytes(). */
-MV_API int mv_kv_append(const mv_paged_kv* c, const void* k, long long k_st, long long k_sh, const void* v,
-                        long long v_st, long long v_sh, const void* q, long long q_st, long long q_sh, int Hq,
-                        void* q_out, long long qo_st, long long qo_sh, int T, const int* page_table,
-                        long long pt_stride, int max_pages, const int* cu_seqlens, const int* kv_lens, int B,
-                        const float* cos_sin, long long cs_stride, int max_pos, int rot_dim, int interleaved,
-                        const int* positions, void* workspace, size_t workspace_bytes, void* stream);
+ * rot_dim 0 (cos_sin NULL) rotates nothing; else a multiple of 16. positions [T] int32 or NULL replaces the cache
+ * position as the row of cos_sin (the cache slot stays the same). A token whose page id, slot or position is outside
+ * the cache, the page table or cos_sin is skipped (error 4): neither its cache slot nor its q_out row is written.
+ * Rows outside every sequence are left alone. workspace: a zeroed header (mv_attention_workspace_bytes() has one). */
+typedef struct mv_kv_append_args {
+  const mv_paged_kv* cache;
+  const void *k, *v, *q;
+  void* q_out;
+  const int *page_table, *cu_seqlens, *kv_lens, *positions;
+  const float* cos_sin;
+  long long k_st, k_sh, v_st, v_sh, q_st, q_sh, qo_st, qo_sh; /* strides: token, head */
+  long long pt_stride, cs_stride;
+  int T, B, Hq, max_pages, max_pos, rot_dim, interleaved, pad0;
+} mv_kv_append_args;
 
-/* Attention of packed new tokens over the cache (which holds them already: mv_kv_append first). For row (token i of
- * sequence b, query head h) over the visible keys j: j <= kv_lens[b] - q_len + i when causal, else j < kv_lens[b]:
+MV_API int mv_kv_append(const mv_kv_append_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of packed new tokens over the cache (mv_paged_attention; it holds the tokens already: mv_kv_append
+ * first), or over packed prompts that lie in k, v [Tk, Hkv, head_dim] themselves (mv_prompt_attention). For row
+ * (token i of sequence b, query head h) over the visible keys j < n, causal: j <= n - q_len + i (n = kv_lens[b], or
+ * the keys cu_seqlens_k[b] .. cu_seqlens_k[b + 1] of a prompt; NULL cu_seqlens_k: cu_seqlens):
  *   s_j = scale q . k_j,  out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s),  lse = ln sum_j exp(s_j)
  * q, out [T, Hq, head_dim]; lse [T, Hq] f32 contiguous or NULL. A row without a visible key gives out 0 and
  * lse -inf. Scores, maxima, sums and outputs are held in fp32; the weights exp(s - max) are rounded to the element
  * type for their product with v (the tensor cores' operand). Values of masked or unowned slots (of any content,
  * NaN and infinities included) never reach a result, but for one case: a non-finite value row that some queries of
  * a sequence see can reach the other queries of that sequence that are computed in the same tile. max_q is the
- * caller's largest q_len, used to choose a kernel only (a wrong value costs time, not correctness). scale > 0.
- * Results do not depend on the run: fixed summation order. workspace: mv_attention_workspace_bytes() bytes. */
-MV_API int mv_paged_attention(const mv_paged_kv* c, const void* q, long long q_st, long long q_sh, int Hq, int T,
-                              const int* page_table, long long pt_stride, int max_pages, const int* cu_seqlens,
-                              const int* kv_lens, int B, int max_q, float scale, int causal, void* out,
-                              long long o_st, long long o_sh, float* lse, void* workspace, size_t workspace_bytes,
-                              void* stream);
+ * caller's largest q_len (0: unknown), used to choose a kernel only: a wrong value costs time, not correctness.
+ * scale > 0. Results do not depend on the run: fixed summation order.
+ * workspace: mv_attention_workspace_bytes() bytes. */
+typedef struct mv_attention_args {
+  const mv_paged_kv* cache; /* paged: the cache; NULL for prompts */
+  const void *q, *k, *v;    /* k, v: prompts only */
+  void* out;
+  float* lse;
+  const int *cu_seqlens, *cu_seqlens_k; /* cu_seqlens_k: prompts only, may be NULL */
+  const int *page_table, *kv_lens;      /* paged only */
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh; /* strides: token, head */
+  long long pt_stride;
+  int T, B, Hq, max_q, causal;
+  int max_pages;                    /* paged */
+  int Tk, Hkv, head_dim, dtype;     /* prompts (paged: the cache's) */
+  float scale;
+  int pad0;
+} mv_attention_args;
 
-/* The same over packed prompts that lie in k, v [Tk, Hkv, head_dim] themselves, no cache: sequence b's keys are rows
- * [cu_seqlens_k[b], cu_seqlens_k[b + 1]) (NULL: cu_seqlens). Causal masks align the ends: token i of q_len sees keys
- * j <= k_len - q_len + i. */
-MV_API int mv_prompt_attention(const void* q, long long q_st, long long q_sh, const void* k, long long k_st,
-                               long long k_sh, const void* v, long long v_st, long long v_sh, int dtype, int Tq,
-                               int Tk, int Hq, int Hkv, int head_dim, const int* cu_seqlens, const int* cu_seqlens_k,
-                               int B, int max_q, float scale, int causal, void* out, long long o_st, long long o_sh,
-                               float* lse, void* workspace, size_t workspace_bytes, void* stream);
+MV_API int mv_paged_attention(const mv_attention_args* a, void* workspace, size_t workspace_bytes, void* stream);
+MV_API int mv_prompt_attention(const mv_attention_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Workspace bytes of the three calls above (any shape; zero-initialised, 256-byte aligned, left as they need it). */
 MV_API size_t mv_attention_workspace_bytes(void);

@@ -97,17 +97,30 @@ namespace {
 constexpr size_t kCountersBytes = 1024 + kMaxCtas * 32;                     // arrival counters, cut items
 constexpr size_t kPartsBytes = size_t(kMaxCtas) * 2 * 256 * (128 + 2) * 4;  // two pieces of 256 rows per CTA
 
-int run(Problem& p, const Source& src, int D, int dtype, int B, const int* cu_q, const int* cu_k, const int* kv_lens,
-        int max_q, float scale, void* workspace, size_t workspace_bytes, cudaStream_t st, const char* who) {
-  if (!(scale > 0.f) || scale > 3.0e38f) return fail(MV_ERR_INVALID, "%s: scale must be positive and finite", who);
-  if (p.Hq < 1 || p.Hq % p.Hkv != 0 || p.Hq / p.Hkv > 64)
-    return fail(MV_ERR_INVALID, "%s: Hq=%d must be 1..64 times Hkv=%d", who, p.Hq, p.Hkv);
+// The shared part of the two entry points: `src` describes the keys, D / dtype / Hkv their heads.
+int run(const mv_attention_args* a, const Source& src, int D, int dtype, int Hkv, void* workspace,
+        size_t workspace_bytes, cudaStream_t st, const char* who) {
+  if (!(a->scale > 0.f) || a->scale > 3.0e38f)
+    return fail(MV_ERR_INVALID, "%s: scale must be positive and finite", who);
+  if (a->Hq < 1 || a->Hq % Hkv != 0 || a->Hq / Hkv > 64)
+    return fail(MV_ERR_INVALID, "%s: Hq=%d must be 1..64 times Hkv=%d", who, a->Hq, Hkv);
+  int rc = check_rows(a->q, a->q_st, a->q_sh, a->Hq, a->T, D, "q", who);
+  if (rc == MV_OK) rc = check_rows(a->out, a->o_st, a->o_sh, a->Hq, a->T, D, "out", who);
+  if (rc != MV_OK) return rc;
   if (workspace == nullptr || workspace_bytes < mv_attention_workspace_bytes() ||
       (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return fail(MV_ERR_WORKSPACE, "%s: 256-byte aligned workspace of %zu bytes needed", who,
                 mv_attention_workspace_bytes());
-  p.G = p.Hq / p.Hkv;
-  p.scale_log2 = scale * kLog2e;
+  const bool paged = a->cache != nullptr;
+  Problem p{};
+  p.q = static_cast<const uint16_t*>(a->q), p.out = static_cast<uint16_t*>(a->out), p.lse = a->lse;
+  p.q_st = a->q_st, p.q_sh = a->q_sh, p.o_st = a->o_st, p.o_sh = a->o_sh;
+  p.T = a->T, p.Tk = a->Tk, p.Hq = a->Hq, p.Hkv = Hkv, p.G = a->Hq / Hkv, p.causal = a->causal != 0;
+  p.scale_log2 = a->scale * kLog2e;
+  if (paged) {
+    p.max_pages = a->max_pages, p.pt_stride = a->pt_stride;
+    p.page_shift = log2_of(src.tokens), p.num_pages = src.pages;
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.ws = reinterpret_cast<WsHeader*>(ws);
   p.counters = reinterpret_cast<unsigned int*>(ws + kWsHeaderBytes);
@@ -115,16 +128,17 @@ int run(Problem& p, const Source& src, int D, int dtype, int B, const int* cu_q,
   const bool bf16 = dtype == MV_BF16;
   int grid = num_sms();
   if (grid > kMaxCtas) grid = kMaxCtas;
-  int rc = MV_OK;
-  const long long pt_row = p.pt_stride;
-  const int* table = p.page_table;
-  const int rows = max_q > 0 && max_q < 64 ? max_q * p.G : 64 * p.G;
-  for (int b0 = 0; b0 < B; b0 += kMaxB) {
-    p.B = B - b0 < kMaxB ? B - b0 : kMaxB;
-    p.cu_q = cu_q + b0;
-    p.cu_k = cu_k == nullptr ? nullptr : cu_k + b0;
-    p.kv_lens = kv_lens == nullptr ? nullptr : kv_lens + b0;
-    p.page_table = table == nullptr ? nullptr : table + b0 * pt_row;
+  const int* cu_k = a->cu_seqlens_k != nullptr ? a->cu_seqlens_k : a->cu_seqlens;
+  const int rows = a->max_q > 0 && a->max_q < 64 ? a->max_q * p.G : 64 * p.G;
+  for (int b0 = 0; b0 < a->B; b0 += kMaxB) {
+    p.B = a->B - b0 < kMaxB ? a->B - b0 : kMaxB;
+    p.cu_q = a->cu_seqlens + b0;
+    if (paged) {
+      p.kv_lens = a->kv_lens + b0;
+      p.page_table = a->page_table + b0 * a->pt_stride;
+    } else {
+      p.cu_k = cu_k + b0;
+    }
     rc = rows <= 32 ? run_split(p, src, D, bf16, rows, grid, st) : run_tile(p, src, D, bf16, grid, st);
     if (rc != MV_OK) return rc;
   }
@@ -140,61 +154,50 @@ using namespace mv::attn;
 
 extern "C" size_t mv_attention_workspace_bytes(void) { return kWsHeaderBytes + kCountersBytes + kPartsBytes; }
 
-extern "C" int mv_paged_attention(const mv_paged_kv* c, const void* q, long long q_st, long long q_sh, int Hq, int T,
-                                  const int* page_table, long long pt_stride, int max_pages, const int* cu_seqlens,
-                                  const int* kv_lens, int B, int max_q, float scale, int causal, void* out,
-                                  long long o_st, long long o_sh, float* lse, void* workspace, size_t workspace_bytes,
-                                  void* stream) {
+extern "C" int mv_paged_attention(const mv_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "mv_paged_attention";
-  int rc = check_cache(c, who);
+  if (a == nullptr) return fail(MV_ERR_INVALID, "%s: null pointer", who);
+  const mv_paged_kv* c = a->cache;
+  const int rc = check_cache(c, who);
   if (rc != MV_OK) return rc;
-  if (T < 0 || B < 0 || max_pages < 0 || max_q < 0)
-    return fail(MV_ERR_INVALID, "%s: bad T=%d / B=%d / max_pages=%d / max_q=%d", who, T, B, max_pages, max_q);
-  if (T == 0 || B == 0) return MV_OK;
-  if (q == nullptr || out == nullptr || cu_seqlens == nullptr || kv_lens == nullptr || page_table == nullptr)
+  if (a->T < 0 || a->B < 0 || a->max_pages < 0 || a->max_q < 0)
+    return fail(MV_ERR_INVALID, "%s: bad T=%d / B=%d / max_pages=%d / max_q=%d", who, a->T, a->B, a->max_pages,
+                a->max_q);
+  if (a->T == 0 || a->B == 0) return MV_OK;
+  if (a->q == nullptr || a->out == nullptr || a->cu_seqlens == nullptr || a->kv_lens == nullptr ||
+      a->page_table == nullptr)
     return fail(MV_ERR_INVALID, "%s: null pointer", who);
-  if (max_pages > 1 && B > 1 && pt_stride < max_pages)
-    return fail(MV_ERR_INVALID, "%s: page table row stride %lld shorter than max_pages=%d", who, pt_stride, max_pages);
-  if ((rc = check_rows(q, q_st, q_sh, Hq, T, c->head_dim, "q", who)) != MV_OK) return rc;
-  if ((rc = check_rows(out, o_st, o_sh, Hq, T, c->head_dim, "out", who)) != MV_OK) return rc;
-  Problem p{};
-  p.q = static_cast<const uint16_t*>(q), p.out = static_cast<uint16_t*>(out), p.lse = lse;
-  p.q_st = q_st, p.q_sh = q_sh, p.o_st = o_st, p.o_sh = o_sh;
-  p.page_table = page_table, p.pt_stride = pt_stride, p.max_pages = max_pages;
-  p.page_shift = log2_of(c->page_size), p.num_pages = c->num_pages;
-  p.T = T, p.Hq = Hq, p.Hkv = c->n_kv_heads, p.causal = causal != 0;
+  if (a->max_pages > 1 && a->B > 1 && a->pt_stride < a->max_pages)
+    return fail(MV_ERR_INVALID, "%s: page table row stride %lld shorter than max_pages=%d", who, a->pt_stride,
+                a->max_pages);
   const Source src{c->k, c->v, c->k_st, c->k_sh, c->k_sp, c->v_st, c->v_sh, c->v_sp, c->page_size, c->num_pages,
                    c->page_size};
-  return run(p, src, c->head_dim, c->dtype, B, cu_seqlens, nullptr, kv_lens, max_q, scale, workspace, workspace_bytes,
+  return run(a, src, c->head_dim, c->dtype, c->n_kv_heads, workspace, workspace_bytes,
              static_cast<cudaStream_t>(stream), who);
 }
 
-extern "C" int mv_prompt_attention(const void* q, long long q_st, long long q_sh, const void* k, long long k_st,
-                                   long long k_sh, const void* v, long long v_st, long long v_sh, int dtype, int Tq,
-                                   int Tk, int Hq, int Hkv, int head_dim, const int* cu_seqlens,
-                                   const int* cu_seqlens_k, int B, int max_q, float scale, int causal, void* out,
-                                   long long o_st, long long o_sh, float* lse, void* workspace,
-                                   size_t workspace_bytes, void* stream) {
+extern "C" int mv_prompt_attention(const mv_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "mv_prompt_attention";
-  if (dtype != MV_BF16 && dtype != MV_F16) return fail(MV_ERR_UNSUPPORTED, "%s: tensors must be bf16 or f16", who);
-  if (head_dim != 64 && head_dim != 128) return fail(MV_ERR_UNSUPPORTED, "%s: head_dim=%d (64 or 128)", who, head_dim);
-  if (Tq < 0 || Tk < 0 || B < 0 || max_q < 0 || Hkv < 1 || Hkv > 4096)
-    return fail(MV_ERR_INVALID, "%s: bad Tq=%d / Tk=%d / B=%d / max_q=%d / Hkv=%d", who, Tq, Tk, B, max_q, Hkv);
-  if (Tq == 0 || B == 0) return MV_OK;
-  if (q == nullptr || out == nullptr || cu_seqlens == nullptr || (Tk > 0 && (k == nullptr || v == nullptr)))
+  if (a == nullptr) return fail(MV_ERR_INVALID, "%s: null pointer", who);
+  const int D = a->head_dim;
+  if (a->cache != nullptr) return fail(MV_ERR_INVALID, "%s: cache must be NULL", who);
+  if (a->dtype != MV_BF16 && a->dtype != MV_F16)
+    return fail(MV_ERR_UNSUPPORTED, "%s: tensors must be bf16 or f16", who);
+  if (D != 64 && D != 128) return fail(MV_ERR_UNSUPPORTED, "%s: head_dim=%d (64 or 128)", who, D);
+  if (a->T < 0 || a->Tk < 0 || a->B < 0 || a->max_q < 0 || a->Hkv < 1 || a->Hkv > 4096)
+    return fail(MV_ERR_INVALID, "%s: bad T=%d / Tk=%d / B=%d / max_q=%d / Hkv=%d", who, a->T, a->Tk, a->B, a->max_q,
+                a->Hkv);
+  if (a->T == 0 || a->B == 0) return MV_OK;
+  if (a->q == nullptr || a->out == nullptr || a->cu_seqlens == nullptr ||
+      (a->Tk > 0 && (a->k == nullptr || a->v == nullptr)))
     return fail(MV_ERR_INVALID, "%s: null pointer", who);
-  int rc = check_rows(q, q_st, q_sh, Hq, Tq, head_dim, "q", who);
-  if (rc == MV_OK) rc = check_rows(out, o_st, o_sh, Hq, Tq, head_dim, "out", who);
-  if (rc == MV_OK && Tk > 0) rc = check_rows(k, k_st, k_sh, Hkv, Tk, head_dim, "k", who);
-  if (rc == MV_OK && Tk > 0) rc = check_rows(v, v_st, v_sh, Hkv, Tk, head_dim, "v", who);
-  if (rc != MV_OK) return rc;
-  Problem p{};
-  p.q = static_cast<const uint16_t*>(q), p.out = static_cast<uint16_t*>(out), p.lse = lse;
-  p.q_st = q_st, p.q_sh = q_sh, p.o_st = o_st, p.o_sh = o_sh;
-  p.T = Tq, p.Tk = Tk, p.Hq = Hq, p.Hkv = Hkv, p.causal = causal != 0;
+  if (a->Tk > 0) {
+    int rc = check_rows(a->k, a->k_st, a->k_sh, a->Hkv, a->Tk, D, "k", who);
+    if (rc == MV_OK) rc = check_rows(a->v, a->v_st, a->v_sh, a->Hkv, a->Tk, D, "v", who);
+    if (rc != MV_OK) return rc;
+  }
   // without a key every row is empty and no copy runs: the maps then stand on one row of q
-  const Source src = Tk > 0 ? Source{k, v, k_st, k_sh, 0, v_st, v_sh, 0, Tk, 1, 64}
-                            : Source{q, q, head_dim, head_dim, 0, head_dim, head_dim, 0, 1, 1, 64};
-  return run(p, src, head_dim, dtype, B, cu_seqlens, cu_seqlens_k != nullptr ? cu_seqlens_k : cu_seqlens, nullptr,
-             max_q, scale, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), who);
+  const Source src = a->Tk > 0 ? Source{a->k, a->v, a->k_st, a->k_sh, 0, a->v_st, a->v_sh, 0, a->Tk, 1, 128}
+                               : Source{a->q, a->q, D, D, 0, D, D, 0, 1, 1, 128};
+  return run(a, src, D, a->dtype, a->Hkv, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), who);
 }

@@ -168,54 +168,53 @@ void launch(const AppendArgs& a, cudaStream_t st) {
 
 using namespace mv;
 
-extern "C" int mv_kv_append(const mv_paged_kv* c, const void* k, long long k_st, long long k_sh, const void* v,
-                            long long v_st, long long v_sh, const void* q, long long q_st, long long q_sh, int Hq,
-                            void* q_out, long long qo_st, long long qo_sh, int T, const int* page_table,
-                            long long pt_stride, int max_pages, const int* cu_seqlens, const int* kv_lens, int B,
-                            const float* cos_sin, long long cs_stride, int max_pos, int rot_dim, int interleaved,
-                            const int* positions, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int mv_kv_append(const mv_kv_append_args* x, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "mv_kv_append";
+  if (x == nullptr) return fail(MV_ERR_INVALID, "%s: null pointer", who);
+  const mv_paged_kv* c = x->cache;
   int rc = attn::check_cache(c, who);
   if (rc != MV_OK) return rc;
-  if (T < 0 || B < 0 || max_pages < 0 || Hq < 0 || Hq > 4096)
-    return fail(MV_ERR_INVALID, "%s: bad T=%d / B=%d / max_pages=%d / Hq=%d", who, T, B, max_pages, Hq);
+  const int T = x->T, B = x->B, Hq = x->Hq, rot = x->rot_dim, D = c->head_dim;
+  if (T < 0 || B < 0 || x->max_pages < 0 || Hq < 0 || Hq > 4096)
+    return fail(MV_ERR_INVALID, "%s: bad T=%d / B=%d / max_pages=%d / Hq=%d", who, T, B, x->max_pages, Hq);
   if (T == 0 || B == 0) return MV_OK;
-  if (k == nullptr || v == nullptr || (Hq > 0 && (q == nullptr || q_out == nullptr)) || cu_seqlens == nullptr ||
-      kv_lens == nullptr || page_table == nullptr)
+  if (x->k == nullptr || x->v == nullptr || (Hq > 0 && (x->q == nullptr || x->q_out == nullptr)) ||
+      x->cu_seqlens == nullptr || x->kv_lens == nullptr || (x->page_table == nullptr && x->max_pages > 0))
     return fail(MV_ERR_INVALID, "%s: null pointer", who);
-  if (rot_dim < 0 || rot_dim > c->head_dim || rot_dim % 16 != 0)
-    return fail(MV_ERR_INVALID, "%s: rot_dim=%d must be a multiple of 16 in 0..%d", who, rot_dim, c->head_dim);
-  if (rot_dim > 0 && (cos_sin == nullptr || max_pos < 1 || cs_stride < rot_dim))
-    return fail(MV_ERR_INVALID, "%s: rot_dim=%d needs a cos_sin table of rows >= rot_dim", who, rot_dim);
-  if (rot_dim > 0 && (!aligned16(cos_sin) || cs_stride % 4 != 0))
+  if (rot < 0 || rot > D || rot % 16 != 0)
+    return fail(MV_ERR_INVALID, "%s: rot_dim=%d must be a multiple of 16 in 0..%d", who, rot, D);
+  if (rot > 0 && (x->cos_sin == nullptr || x->max_pos < 1 || (x->max_pos > 1 && x->cs_stride < rot)))
+    return fail(MV_ERR_INVALID, "%s: rot_dim=%d needs a cos_sin table of rows >= rot_dim", who, rot);
+  if (rot > 0 && (!aligned16(x->cos_sin) || (x->max_pos > 1 && x->cs_stride % 4 != 0)))
     return fail(MV_ERR_ALIGN, "%s: cos_sin rows must be 16-byte aligned", who);
-  if (max_pages > 1 && pt_stride < max_pages && B > 1)
-    return fail(MV_ERR_INVALID, "%s: page table row stride %lld shorter than max_pages=%d", who, pt_stride, max_pages);
-  if ((rc = attn::check_rows(k, k_st, k_sh, c->n_kv_heads, T, c->head_dim, "k", who)) != MV_OK) return rc;
-  if ((rc = attn::check_rows(v, v_st, v_sh, c->n_kv_heads, T, c->head_dim, "v", who)) != MV_OK) return rc;
+  if (x->max_pages > 1 && x->pt_stride < x->max_pages && B > 1)
+    return fail(MV_ERR_INVALID, "%s: page table row stride %lld shorter than max_pages=%d", who, x->pt_stride,
+                x->max_pages);
+  if ((rc = attn::check_rows(x->k, x->k_st, x->k_sh, c->n_kv_heads, T, D, "k", who)) != MV_OK) return rc;
+  if ((rc = attn::check_rows(x->v, x->v_st, x->v_sh, c->n_kv_heads, T, D, "v", who)) != MV_OK) return rc;
   if (Hq > 0) {
-    if ((rc = attn::check_rows(q, q_st, q_sh, Hq, T, c->head_dim, "q", who)) != MV_OK) return rc;
-    if ((rc = attn::check_rows(q_out, qo_st, qo_sh, Hq, T, c->head_dim, "q_out", who)) != MV_OK) return rc;
+    if ((rc = attn::check_rows(x->q, x->q_st, x->q_sh, Hq, T, D, "q", who)) != MV_OK) return rc;
+    if ((rc = attn::check_rows(x->q_out, x->qo_st, x->qo_sh, Hq, T, D, "q_out", who)) != MV_OK) return rc;
   }
   if (workspace == nullptr || workspace_bytes < kWsHeaderBytes)
     return fail(MV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", who, kWsHeaderBytes);
   AppendArgs a{};
-  a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v), a.q = static_cast<const uint16_t*>(q);
-  a.qo = static_cast<uint16_t*>(q_out);
+  a.k = static_cast<const uint16_t*>(x->k), a.v = static_cast<const uint16_t*>(x->v);
+  a.q = static_cast<const uint16_t*>(x->q), a.qo = static_cast<uint16_t*>(x->q_out);
   a.kc = static_cast<uint16_t*>(c->k), a.vc = static_cast<uint16_t*>(c->v);
-  a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
-  a.q_st = q_st, a.q_sh = q_sh, a.qo_st = qo_st, a.qo_sh = qo_sh;
+  a.k_st = x->k_st, a.k_sh = x->k_sh, a.v_st = x->v_st, a.v_sh = x->v_sh;
+  a.q_st = x->q_st, a.q_sh = x->q_sh, a.qo_st = x->qo_st, a.qo_sh = x->qo_sh;
   a.kc_sp = c->k_sp, a.kc_st = c->k_st, a.kc_sh = c->k_sh;
   a.vc_sp = c->v_sp, a.vc_st = c->v_st, a.vc_sh = c->v_sh;
-  a.page_table = page_table, a.cu = cu_seqlens, a.kv_lens = kv_lens, a.positions = positions;
-  a.cos_sin = cos_sin, a.pt_stride = pt_stride, a.cs_stride = cs_stride;
-  a.T = T, a.B = B, a.Hq = Hq, a.Hkv = c->n_kv_heads, a.max_pages = max_pages;
-  a.page_shift = attn::log2_of(c->page_size), a.num_pages = c->num_pages, a.max_pos = max_pos;
-  a.rot = rot_dim, a.interleaved = interleaved != 0;
+  a.page_table = x->page_table, a.cu = x->cu_seqlens, a.kv_lens = x->kv_lens, a.positions = x->positions;
+  a.cos_sin = x->cos_sin, a.pt_stride = x->pt_stride, a.cs_stride = x->cs_stride;
+  a.T = T, a.B = B, a.Hq = Hq, a.Hkv = c->n_kv_heads, a.max_pages = x->max_pages;
+  a.page_shift = attn::log2_of(c->page_size), a.num_pages = c->num_pages, a.max_pos = x->max_pos;
+  a.rot = rot, a.interleaved = x->interleaved != 0;
   a.ws = static_cast<WsHeader*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = c->dtype == MV_BF16;
-  if (c->head_dim == 128)
+  if (D == 128)
     bf ? launch<128, true>(a, st) : launch<128, false>(a, st);
   else
     bf ? launch<64, true>(a, st) : launch<64, false>(a, st);

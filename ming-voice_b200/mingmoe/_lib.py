@@ -52,6 +52,24 @@ class PagedKV(C.Structure):
                 ("v_st", I64), ("v_sh", I64)]
 
 
+class KVAppendArgs(C.Structure):
+    """mirror of `mv_kv_append_args`"""
+    _fields_ = ([(n, P) for n in ("cache", "k", "v", "q", "q_out", "page_table", "cu_seqlens", "kv_lens", "positions",
+                                  "cos_sin")] +
+                [(n, I64) for n in ("k_st", "k_sh", "v_st", "v_sh", "q_st", "q_sh", "qo_st", "qo_sh", "pt_stride",
+                                    "cs_stride")] +
+                [(n, I32) for n in ("T", "B", "Hq", "max_pages", "max_pos", "rot_dim", "interleaved", "pad0")])
+
+
+class AttentionArgs(C.Structure):
+    """mirror of `mv_attention_args`"""
+    _fields_ = ([(n, P) for n in ("cache", "q", "k", "v", "out", "lse", "cu_seqlens", "cu_seqlens_k", "page_table",
+                                  "kv_lens")] +
+                [(n, I64) for n in ("q_st", "q_sh", "k_st", "k_sh", "v_st", "v_sh", "o_st", "o_sh", "pt_stride")] +
+                [(n, I32) for n in ("T", "B", "Hq", "max_q", "causal", "max_pages", "Tk", "Hkv", "head_dim", "dtype")] +
+                [("scale", F32), ("pad0", I32)])
+
+
 _SIGS = {
     "mv_version": (I32, []),
     "mv_last_error": (C.c_char_p, []),
@@ -83,12 +101,9 @@ _SIGS = {
     "mv_ep_pack": (I32, [P, I64, I32, P, P, I32, I32, P, P]),
     "mv_ep_unpack": (I32, [P, I32, I32, I32, I32, P, P, P]),
     "mv_ep_narrow": (I32, [P, I64, P, P]),
-    "mv_kv_append": (I32, [C.POINTER(PagedKV), P, I64, I64, P, I64, I64, P, I64, I64, I32, P, I64, I64, I32, P, I64,
-                           I32, P, P, I32, P, I64, I32, I32, I32, P, P, SZ, P]),
-    "mv_paged_attention": (I32, [C.POINTER(PagedKV), P, I64, I64, I32, I32, P, I64, I32, P, P, I32, I32, F32, I32, P,
-                                 I64, I64, P, P, SZ, P]),
-    "mv_prompt_attention": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, I32, I32, I32, I32, I32, I32, P, P, I32, I32,
-                                  F32, I32, P, I64, I64, P, P, SZ, P]),
+    "mv_kv_append": (I32, [P, P, SZ, P]),
+    "mv_paged_attention": (I32, [P, P, SZ, P]),
+    "mv_prompt_attention": (I32, [P, P, SZ, P]),
     "mv_attention_workspace_bytes": (SZ, []),
     "mv_ep_combine": (I32, [P, I64, P, P, I32, P, I32, I32, I32, P, P]),
 }

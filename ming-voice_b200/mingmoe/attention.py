@@ -13,12 +13,19 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import torch
 
 from . import _lib as L
 
 _DTYPES = (torch.bfloat16, torch.float16)
+
+# The argument structs of the C entry points, packed in one step: a call of a few microseconds is bounded by its host
+# side, where filling a ctypes structure field by field takes several times as long.
+_APPEND = struct.Struct("@10P10q8i")
+_ATTN = struct.Struct("@10P9q10ifi")
+assert _APPEND.size == C.sizeof(L.KVAppendArgs) and _ATTN.size == C.sizeof(L.AttentionArgs)
 
 
 class PagedKV:
@@ -45,7 +52,7 @@ class PagedKV:
         c.k_sp, c.k_st, c.k_sh = k.stride()[:3]
         c.v_sp, c.v_st, c.v_sh = v.stride()[:3]
         self._c = c
-        self._ref = C.byref(c)
+        self._ptr = C.addressof(c)
 
     @classmethod
     def empty(cls, num_pages, page_size, n_kv_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
@@ -53,58 +60,69 @@ class PagedKV:
         return cls(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
 
 
-def _rows(t, name, heads, d, dtype, device):
-    """A [T, heads, d] operand as the kernels take it (copied only where its layout has no 16-byte vectors)."""
-    if t.dim() != 3 or t.shape[2] != d or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [T, {'heads' if heads is None else heads}, {d}], got {tuple(t.shape)}")
+def _rows(t, name, d, dtype, device):
+    """A [T, heads, d] operand as the kernels take it (copied only where its layout has no 16-byte vectors), its
+    shape and its strides."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != d:
+        raise ValueError(f"{name} must be [T, heads, {d}], got {tuple(shape)}")
     if t.dtype != dtype:
         raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
     if t.device != device:
         raise RuntimeError(f"{name} is on {t.device}, expected {device}")
-    st, sh, s1 = t.stride()
+    st, sh, s1 = strides = t.stride()
     if s1 != 1 or (st | sh) & 7 or st < d or sh < d or t.data_ptr() & 15:
         t = t.contiguous()
-    return t
+        strides = t.stride()
+    return t, shape, strides
 
 
-def _out(t, name, like_shape, d, dtype, device):
+def _out(t, name, like, shape, dtype, device):
     if t is None:
-        return torch.empty(like_shape, dtype=dtype, device=device)
-    if t.shape != like_shape or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be {tuple(like_shape)} {dtype} on {device}")
-    if t.stride(2) != 1:
+        t = torch.empty_like(like)
+    elif t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {device}")
+    strides = t.stride()
+    if strides[2] != 1:
         raise ValueError(f"{name} needs a unit inner stride")
-    return t
+    return t, strides
 
 
-def _ints(t, name, shape, device):
+def _ints(t, name, device):
+    """Shape of an int32 index tensor."""
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32")
-    if t.dim() != len(shape) or any(n is not None and a != n for a, n in zip(t.shape, shape)):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
     if t.device != device:
         raise RuntimeError(f"{name} is on {t.device}, expected {device}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+    shape = t.shape
+    if len(shape) == 0 or (t.stride()[-1] != 1 and shape[-1] > 1):
         raise ValueError(f"{name} needs a unit inner stride")
-    return t.data_ptr()
+    return shape
 
 
 def _batch(page_table, cu_seqlens, kv_lens, device):
-    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    lens = _ints(kv_lens, "kv_lens", (None,), device)
-    cu = _ints(cu_seqlens, "cu_seqlens", (B + 1,), device)
-    table = _ints(page_table, "page_table", (B, None), device)
-    return B, cu, lens, table
+    """(sequences, columns and row stride of the page table)"""
+    lens, cu, table = (_ints(kv_lens, "kv_lens", device), _ints(cu_seqlens, "cu_seqlens", device),
+                       _ints(page_table, "page_table", device))
+    B = lens[0]
+    if len(lens) != 1 or len(cu) != 1 or cu[0] != B + 1 or len(table) != 2 or table[0] != B:
+        raise ValueError(f"kv_lens [B], cu_seqlens [B + 1] and page_table [B, max_pages] do not agree: {tuple(lens)}, "
+                         f"{tuple(cu)}, {tuple(table)}")
+    return B, table[1], page_table.stride()[0]
 
 
-def _workspace(device):
-    global _ws_bytes
-    if _ws_bytes == 0:
-        _ws_bytes = L.lib().mv_attention_workspace_bytes()
-    return L.workspace("attention", _ws_bytes, device)
+def _call(fn, args, device, what):
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    ws = _ws.get((device.index, stream))
+    if ws is None:
+        buf = L.workspace("attention", L.lib().mv_attention_workspace_bytes(), device)
+        ws = _ws[(device.index, stream)] = (buf.data_ptr(), buf.numel())
+    rc = fn(args, ws[0], ws[1], stream)
+    if rc:
+        L.check(rc, what)
 
 
-_ws_bytes = 0
+_ws: dict = {}  # (device, stream) -> address and size of the "attention" workspace (its size never changes)
 
 
 def kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, *, q=None, q_out=None, cos_sin=None, positions=None,
@@ -117,40 +135,39 @@ def kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, *, q=None, q_out=Non
     without rotating. rot_dim is a multiple of 16 up to D. Pairs are (i, i + rot_dim / 2), or (2i, 2i + 1) when
     `interleaved`. positions: int32 [T] rows of cos_sin, if not the cache positions. q_out may be q itself."""
     dev, d, dtype = cache.device, cache.head_dim, cache.dtype
-    k = _rows(k, "k", cache.n_kv_heads, d, dtype, dev)
-    v = _rows(v, "v", cache.n_kv_heads, d, dtype, dev)
-    T = k.shape[0]
-    if v.shape[0] != T:
-        raise ValueError("k and v have different numbers of tokens")
-    B, cu, lens, table = _batch(page_table, cu_seqlens, kv_lens, dev)
-    Hq = 0
-    qp = qo = None
+    k, k_shape, ks = _rows(k, "k", d, dtype, dev)
+    v, v_shape, vs = _rows(v, "v", d, dtype, dev)
+    T = k_shape[0]
+    if k_shape[1] != cache.n_kv_heads or v_shape != k_shape:
+        raise ValueError(f"k and v must be [T, {cache.n_kv_heads}, {d}], got {tuple(k_shape)} / {tuple(v_shape)}")
+    B, max_pages, pt_stride = _batch(page_table, cu_seqlens, kv_lens, dev)
+    Hq = qp = qo = 0
     qs = qos = (0, 0)
     if q is not None:
-        q = _rows(q, "q", None, d, dtype, dev)
-        if q.shape[0] != T:
+        q, q_shape, qs = _rows(q, "q", d, dtype, dev)
+        if q_shape[0] != T:
             raise ValueError("q and k have different numbers of tokens")
-        Hq = q.shape[1]
-        q_out = _out(q_out, "q_out", q.shape, d, dtype, dev)
-        qp, qo, qs, qos = q.data_ptr(), q_out.data_ptr(), q.stride(), q_out.stride()
+        Hq = q_shape[1]
+        q_out, qos = _out(q_out, "q_out", q, q_shape, dtype, dev)
+        qp, qo = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
-    cs, cs_stride, max_pos, rot = None, 0, 0, 0
+    cs = cs_stride = max_pos = rot = pos = 0
     if cos_sin is not None:
-        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.device != dev:
+        if cos_sin.dtype != torch.float32 or cos_sin.ndim != 2 or cos_sin.device != dev:
             raise TypeError(f"cos_sin must be fp32 [max_pos, rot_dim] on {dev}")
-        if cos_sin.stride(1) != 1:
+        cs_stride, inner = cos_sin.stride()
+        if inner != 1:
             raise ValueError("cos_sin needs a unit inner stride")
-        cs, cs_stride, (max_pos, rot) = cos_sin.data_ptr(), cos_sin.stride(0), cos_sin.shape
-        if max_pos == 1:
-            cs_stride = rot
-    pos = None if positions is None else _ints(positions, "positions", (T,), dev)
-    ws = _workspace(dev)
-    L.check(L.lib().mv_kv_append(cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                 v.stride(1), qp, qs[0], qs[1], Hq, qo, qos[0], qos[1], T, table,
-                                 page_table.stride(0), page_table.shape[1], cu, lens, B, cs, cs_stride, max_pos, rot,
-                                 interleaved, pos, ws.data_ptr(), ws.numel(),
-                                 torch.cuda.current_stream(dev).cuda_stream), "kv_append")
+        cs, (max_pos, rot) = cos_sin.data_ptr(), cos_sin.shape
+    if positions is not None:
+        if tuple(_ints(positions, "positions", dev)) != (T,):
+            raise ValueError(f"positions must be [{T}]")
+        pos = positions.data_ptr()
+    _call(L.lib().mv_kv_append,
+          _APPEND.pack(cache._ptr, k.data_ptr(), v.data_ptr(), qp, qo, page_table.data_ptr(), cu_seqlens.data_ptr(),
+                       kv_lens.data_ptr(), pos, cs, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], qos[0], qos[1],
+                       pt_stride, cs_stride, T, B, Hq, max_pages, max_pos, rot, bool(interleaved), 0), dev, "kv_append")
     return q_out
 
 
@@ -161,18 +178,16 @@ def paged_attention(q, cache, page_table, cu_seqlens, kv_lens, *, max_q=None, sc
     row that sees no key, whose out is 0). max_q: the largest number of new tokens of a sequence, where the caller
     knows it; it only chooses the kernel. scale defaults to 1 / sqrt(D)."""
     dev, d, dtype = cache.device, cache.head_dim, cache.dtype
-    q = _rows(q, "q", None, d, dtype, dev)
-    T, Hq = q.shape[0], q.shape[1]
-    B, cu, lens, table = _batch(page_table, cu_seqlens, kv_lens, dev)
-    out = _out(out, "out", q.shape, d, dtype, dev)
+    q, shape, qs = _rows(q, "q", d, dtype, dev)
+    T, Hq = shape[0], shape[1]
+    B, max_pages, pt_stride = _batch(page_table, cu_seqlens, kv_lens, dev)
+    out, os_ = _out(out, "out", q, shape, dtype, dev)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    ws = _workspace(dev)
-    L.check(L.lib().mv_paged_attention(cache._ref, q.data_ptr(), q.stride(0), q.stride(1), Hq, T, table,
-                                       page_table.stride(0), page_table.shape[1], cu, lens, B,
-                                       T if max_q is None else max_q, 1.0 / math.sqrt(d) if scale is None else scale,
-                                       causal, out.data_ptr(), out.stride(0), out.stride(1),
-                                       lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(),
-                                       torch.cuda.current_stream(dev).cuda_stream), "paged_attention")
+    _call(L.lib().mv_paged_attention,
+          _ATTN.pack(cache._ptr, q.data_ptr(), 0, 0, out.data_ptr(), lse.data_ptr() if return_lse else 0,
+                     cu_seqlens.data_ptr(), 0, page_table.data_ptr(), kv_lens.data_ptr(), qs[0], qs[1], 0, 0, 0, 0,
+                     os_[0], os_[1], pt_stride, T, B, Hq, T if max_q is None else max_q, bool(causal), max_pages, 0, 0,
+                     0, 0, 1.0 / math.sqrt(d) if scale is None else scale, 0), dev, "paged_attention")
     return (out, lse) if return_lse else out
 
 
@@ -181,37 +196,37 @@ def prompt_attention(q, k, v, cu_seqlens, *, cu_seqlens_k=None, max_q=None, scal
     """Attention over packed prompts: q [Tq, Hq, D], k, v [Tk, Hkv, D], sequence b's queries in rows
     cu_seqlens[b]:cu_seqlens[b + 1] and its keys in the same rows of k and v (or in cu_seqlens_k's). Causal masks
     align the ends: token i of n sees keys j <= n_keys - n + i. Returns as paged_attention."""
-    if q.dim() != 3 or k.dim() != 3:
+    if q.ndim != 3:
         raise ValueError("q, k, v must be [T, heads, D]")
-    L.require_cuda(q)
+    if not q.is_cuda:
+        L.require_cuda(q)
     dev, d, dtype = q.device, q.shape[2], q.dtype
     if dtype not in _DTYPES:
         raise TypeError("prompt_attention: tensors must be bf16 or f16")
-    q = _rows(q, "q", None, d, dtype, dev)
-    k = _rows(k, "k", None, d, dtype, dev)
-    v = _rows(v, "v", k.shape[1], d, dtype, dev)
-    if v.shape[0] != k.shape[0]:
-        raise ValueError("k and v have different numbers of tokens")
-    T, Hq = q.shape[0], q.shape[1]
-    B = cu_seqlens.shape[0] - 1
-    cu = _ints(cu_seqlens, "cu_seqlens", (None,), dev)
-    if B < 0:
-        raise ValueError("cu_seqlens needs at least one entry")
-    cuk = None
+    q, shape, qs = _rows(q, "q", d, dtype, dev)
+    k, k_shape, ks = _rows(k, "k", d, dtype, dev)
+    v, v_shape, vs = _rows(v, "v", d, dtype, dev)
+    if v_shape != k_shape:
+        raise ValueError(f"k and v differ: {tuple(k_shape)} / {tuple(v_shape)}")
+    T, Hq = shape[0], shape[1]
+    cu = _ints(cu_seqlens, "cu_seqlens", dev)
+    B = cu[0] - 1
+    if len(cu) != 1 or B < 0:
+        raise ValueError("cu_seqlens must be [B + 1]")
+    cuk = 0
     if cu_seqlens_k is not None:
-        cuk = _ints(cu_seqlens_k, "cu_seqlens_k", (B + 1,), dev)
-    elif k.shape[0] != T:
+        if _ints(cu_seqlens_k, "cu_seqlens_k", dev) != cu:
+            raise ValueError(f"cu_seqlens_k must be [{B + 1}]")
+        cuk = cu_seqlens_k.data_ptr()
+    elif k_shape[0] != T:
         raise ValueError("q and k have different numbers of tokens: cu_seqlens_k is needed")
-    out = _out(out, "out", q.shape, d, dtype, dev)
+    out, os_ = _out(out, "out", q, shape, dtype, dev)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    ws = _workspace(dev)
-    L.check(L.lib().mv_prompt_attention(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                                        v.data_ptr(), v.stride(0), v.stride(1), L.dt(dtype), T, k.shape[0], Hq,
-                                        k.shape[1], d, cu, cuk, B, T if max_q is None else max_q,
-                                        1.0 / math.sqrt(d) if scale is None else scale, causal, out.data_ptr(),
-                                        out.stride(0), out.stride(1), lse.data_ptr() if return_lse else None,
-                                        ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream),
-            "prompt_attention")
+    _call(L.lib().mv_prompt_attention,
+          _ATTN.pack(0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+                     cu_seqlens.data_ptr(), cuk, 0, 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], 0, T,
+                     B, Hq, T if max_q is None else max_q, bool(causal), 0, k_shape[0], k_shape[1], d, L.dt(dtype),
+                     1.0 / math.sqrt(d) if scale is None else scale, 0), dev, "prompt_attention")
     return (out, lse) if return_lse else out
 
 
