@@ -47,18 +47,18 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 static int make_map(CUtensorMap* m, const void* base, bool bf16, int d, int tokens, int heads, int pages, long long st,
-                    long long sh, long long sp, int box, const char* what) {
+                    long long sh, long long sp, int box, int parts, const char* what) {
   auto enc = encode_fn();
   if (enc == nullptr) return fail(MV_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   // the stride of an axis of one element is never used: a valid one stands in for it
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(tokens),
+  const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(d / 64),
                               static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(pages)};
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(tokens > 1 ? st : d) * 2,
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(tokens > 1 ? st : d) * 2, 128,
                                  static_cast<cuuint64_t>(heads > 1 ? sh : d) * 2,
                                  static_cast<cuuint64_t>(pages > 1 ? sp : d) * 2};
-  const cuuint32_t boxes[4] = {64, static_cast<cuuint32_t>(box), 1, 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+  const cuuint32_t boxes[5] = {64, static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(parts), 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                          const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -67,10 +67,10 @@ static int make_map(CUtensorMap* m, const void* base, bool bf16, int d, int toke
   return MV_OK;
 }
 
-int make_kv_maps(CUtensorMap* mk, CUtensorMap* mv_, const Source& s, int heads, int d, bool bf16, int box) {
-  const int rc = make_map(mk, s.k, bf16, d, s.tokens, heads, s.pages, s.k_st, s.k_sh, s.k_sp, box, "k");
+int make_kv_maps(CUtensorMap* mk, CUtensorMap* mv_, const Source& s, int heads, int d, bool bf16, int box, int parts) {
+  const int rc = make_map(mk, s.k, bf16, d, s.tokens, heads, s.pages, s.k_st, s.k_sh, s.k_sp, box, parts, "k");
   if (rc != MV_OK) return rc;
-  return make_map(mv_, s.v, bf16, d, s.tokens, heads, s.pages, s.v_st, s.v_sh, s.v_sp, box, "v");
+  return make_map(mv_, s.v, bf16, d, s.tokens, heads, s.pages, s.v_st, s.v_sh, s.v_sp, box, parts, "v");
 }
 
 int make_q_map(CUtensorMap* m, const Problem& p, int d, bool bf16, int tok) {

@@ -119,20 +119,32 @@ __device__ __forceinline__ void build_schedule(const Problem& p, unsigned long l
   __syncthreads();
 }
 
-// The CTAs' ranges: [bound(c), bound(c + 1)) of W units over G CTAs (the first `ctas` of the grid have work).
+// a / b: a 64-bit division is a long subroutine, and nearly all counts here fit 32 bits
+__device__ __forceinline__ unsigned long long quot(unsigned long long a, unsigned long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned int>(a) / static_cast<unsigned int>(b);
+  return a / b;
+}
+
+// The CTAs' ranges: [bound(c), bound(c + 1)) of W units over the first `ctas` CTAs of the grid, the first `rest` of
+// them one unit longer.
 struct Cut {
-  unsigned long long W;
-  unsigned int ctas;
-  __device__ __forceinline__ Cut(unsigned long long total, int grid, int min_share) {
-    W = total;
-    const unsigned long long most = (total + min_share - 1) / min_share;
-    ctas = most < static_cast<unsigned long long>(grid) ? static_cast<unsigned int>(most) : grid;
+  unsigned long long share;
+  unsigned int ctas, rest;
+  __device__ __forceinline__ Cut(unsigned long long W, int grid, int min_share) {
+    ctas = static_cast<unsigned int>(min(quot(W + min_share - 1, min_share), static_cast<unsigned long long>(grid)));
     if (ctas == 0) ctas = 1;
+    share = quot(W, ctas);
+    rest = static_cast<unsigned int>(W - share * ctas);
   }
-  __device__ __forceinline__ unsigned long long bound(unsigned int c) const { return W * min(c, ctas) / ctas; }
+  __device__ __forceinline__ unsigned long long bound(unsigned int c) const {
+    c = min(c, ctas);
+    return c * share + min(c, rest);
+  }
   // the CTA whose range holds unit x
   __device__ __forceinline__ unsigned int cta_of(unsigned long long x) const {
-    return static_cast<unsigned int>(((x + 1) * ctas - 1) / W);
+    const unsigned long long long_part = rest * (share + 1);
+    if (x < long_part) return static_cast<unsigned int>(quot(x, share + 1));
+    return rest + static_cast<unsigned int>(quot(x - long_part, share));
   }
 };
 
@@ -156,9 +168,9 @@ struct Walk {
     }
     b = lo;
     s = seq_of(p, b, false);
-    const unsigned long long per_head = (pre[b + 1] - pre[b]) / p.Hkv;
+    const unsigned long long per_head = quot(pre[b + 1] - pre[b], p.Hkv);
     unsigned long long off = at - pre[b];
-    h = static_cast<int>(off / per_head);
+    h = static_cast<int>(quot(off, per_head));
     off -= per_head * h;
     for (t = 0;; ++t) {
       units = item_units<BN>(p, s, t);
@@ -193,6 +205,39 @@ struct Walk {
     }
     units = item_units<BN>(p, s, t);
   }
+};
+
+// Bounded wait, in line: a call would hold the caller's registers to the calling convention.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, WsHeader* h, unsigned int info) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      raise_error(h, kErrTimeout, info);
+      return false;
+    }
+  return true;
+}
+
+// A producer warp's view of the page table: lane x holds the page of box x of the tile at hand, and the next tile's
+// are on their way while this one's copies are issued (a table read between any two tiles would cost an L2 latency
+// each). Packed prompts are one page.
+struct Pages {
+  int ids, next;
+  // lane x: the page of the box that holds keys [j, j + box) of sequence b (j < kend), as read from the table
+  __device__ __forceinline__ static int read(const Problem& p, int b, int j, int kend) {
+    return p.page_table != nullptr && j < kend ? p.page_table[b * p.pt_stride + (j >> p.page_shift)] : 0;
+  }
+  // takes over the ids read ahead. One outside the cache is reported and becomes num_pages, which lies outside the
+  // tensor map and reads as zeros.
+  __device__ __forceinline__ void step(const Problem& p, unsigned int info) {
+    ids = next;
+    if (p.page_table != nullptr && (ids < 0 || ids >= p.num_pages)) {
+      raise_error(p.ws, kErrBadPage, info);
+      ids = p.num_pages;
+    }
+  }
+  __device__ __forceinline__ int of(int box) const { return __shfl_sync(0xffffffffu, ids, box); }
 };
 
 // Value conversions of the element types
@@ -232,8 +277,9 @@ struct Source {
   int tokens, pages, box;
 };
 
-// 4-D maps over keys and values [page][head][token][d], 128-byte swizzle, box of 64 values x `box` tokens
-int make_kv_maps(CUtensorMap* mk, CUtensorMap* mv_, const Source& src, int heads, int d, bool bf16, int box);
+// 5-D maps over keys and values [page][head][64-value part of a head][token][64 values], 128-byte swizzle, box of
+// 64 values x `box` tokens x `parts` parts: in shared memory [part][token][64 values]
+int make_kv_maps(CUtensorMap* mk, CUtensorMap* mv_, const Source& src, int heads, int d, bool bf16, int box, int parts);
 
 // 3-D map over queries [token][head][d], 128-byte swizzle, box of 64 values x the G heads of a key head x `tok` tokens
 int make_q_map(CUtensorMap* m, const Problem& p, int d, bool bf16, int tok);

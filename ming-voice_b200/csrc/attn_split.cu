@@ -9,7 +9,7 @@
 // operand and the query rows in the 8-column one: 8 rows fill an instruction where the untransposed form would fill
 // half of it. The cost of that is one movmatrix per 8 x 8 block of P.
 //
-// Split: one CTA per SM takes an equal share of all key tiles (attn_common.cuh). A producer warp keeps a ring of
+// Split: one CTA per SM takes an equal share of all key tiles (attn_common.cuh). Producer warps keep a ring of
 // key tiles filled by TMA (a box per page and 64 values, 128-byte swizzle); each of the consumer warps takes whole
 // tiles in turn with its own maximum, sum and output in registers, so the warps meet only at the end of a piece.
 // Pieces of an item that ranges cut are joined by the CTA that arrives last, in CTA order.
@@ -24,7 +24,10 @@ struct Cfg {
   static constexpr int kRows = 8 * NT;
   static constexpr int kBN = D == 128 && NT <= 2 ? 32 : 64;  // keys of a tile
   static constexpr int kWarps = NT <= 2 ? 8 : 4;             // consumer warps
-  static constexpr int kThreads = 32 * (kWarps + 1);
+  // producer warps, a tile each in turn: issuing a tile's copies is a chain of some 800 cycles for one warp, which
+  // would hold the ring to 16 KB per 0.43 us (5.6 TB/s over the card, before anything else is in the way)
+  static constexpr int kProd = 4;
+  static constexpr int kThreads = 32 * (kWarps + kProd);
   static constexpr int kTile = kBN * D * 2;                   // bytes of a key (or value) tile
   static constexpr int kStage = 2 * kTile;
   // a ring slot is always read by the same warp (tile i: slot i % kStages, warp i % kWarps), so a warp never waits
@@ -45,7 +48,6 @@ struct Cfg {
   static constexpr int oFlag = oBar + 2 * kStages * 8;
   static constexpr int kSmem = oFlag + 16 + 1024;
   static_assert(kSmem <= 232448, "shared memory");
-  static_assert(kMaxCtas * kRows * 4 + kRows * 8 <= kMerge, "piece weights share the merge buffer");
 };
 
 template <bool BF16>
@@ -84,6 +86,20 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
+// out and lse of values d .. d + 3 of the item's row r from its joined sums
+template <bool BF16, int BN>
+__device__ __forceinline__ void store_row(const Problem& p, const Walk<BN>& wk, int r, int d, const float4& acc, float M,
+                                          float L) {
+  const int i = r / p.G, h = wk.h * p.G + r % p.G;
+  const bool sees = keys_seen(p, wk.s, wk.tok0() + i + 1) > 0;
+  const long long row = wk.s.q0 + wk.tok0() + i;
+  const float inv = 1.f / L;
+  uint2 v = make_uint2(0u, 0u);
+  if (sees) v = make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+  *reinterpret_cast<uint2*>(p.out + row * p.o_st + h * p.o_sh + d) = v;
+  if (p.lse != nullptr && d == 0) p.lse[row * p.Hq + h] = sees ? M * kLn2 + logf(L) : -INFINITY;
+}
+
 template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Problem p,
@@ -103,6 +119,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   volatile int* flag = reinterpret_cast<volatile int*>(smem + C::oFlag);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int box_shift = 31 - __clz(box);
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);
@@ -118,44 +135,43 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   const Cut cut(W, gridDim.x, p.min_share);
   Walk<kBN> wk(p, pre, cut.bound(blockIdx.x), cut.bound(blockIdx.x + 1));
 
-  if (warp == NW) {
-    // ---------------------------------------------------------------- producer: lane i issues box i of a tile
-    const int nbox = kBN / box;
-    const int is_v = lane & 1, half = (lane >> 1) % (D / 64), bx = (lane >> 1) / (D / 64);
-    const CUtensorMap* map = is_v ? &tmV : &tmK;
-    int it = 0;
+  if (warp >= NW) {
+    // ---------------------------------------------------------------- producers: lane 0 issues all copies
+    const int turn = warp - NW;
+    int it = 0, issued = 0;
     bool ok = true;
+    Pages pages;
     for (; wk.more() && ok; wk.next()) {
       const int kend = wk.kend();
-      const int i1 = min(wk.last(), (kend + kBN - 1) / kBN);
-      for (int i = wk.first(); i < i1 && ok; ++i, ++it) {
-        const int stage = it % NS;
-        const int j = i * kBN + bx * box;  // first key of the lane's box
-        const bool mine = bx < nbox && j < kend;
-        int page = 0, row = wk.s.k0 + j;
-        if (mine && p.page_table != nullptr) {
-          page = p.page_table[wk.b * p.pt_stride + (j >> p.page_shift)];
-          row = j & ((1 << p.page_shift) - 1);
-          if (page < 0 || page >= p.num_pages) {
-            raise_error(p.ws, kErrBadPage, 0x710u);
-            page = p.num_pages;  // outside the map: reads as zeros
-          }
-        }
-        const int live = min(nbox, (kend - i * kBN + box - 1) / box);
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], ((it / NS) & 1) ^ 1, p.ws, 0x720u));
+      const int i0 = wk.first(), i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+      const int skip = (turn - it) & (C::kProd - 1);  // tile `it` of the CTA is producer it % kProd's
+      pages.next = Pages::read(p, wk.b, (i0 + skip) * kBN + lane * box, kend);
+      const int base = it - i0;
+      for (int i = i0 + skip; i < i1; i += C::kProd) {
+        const int stage = (base + i) % NS;
+        const int live = min(kBN, kend - i * kBN + box - 1) >> box_shift;  // boxes with a key
+        pages.step(p, 0x710u);
+        pages.next = Pages::read(p, wk.b, (i + C::kProd) * kBN + lane * box, kend);
+        ok = __all_sync(0xffffffffu, wait_bar(&empty[stage], (((base + i) / NS) & 1) ^ 1, p.ws, 0x720u));
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(live * box * D * 4));
-        __syncwarp();
-        if (mine) {
-          uint8_t* dst = smem + stage * C::kStage + is_v * C::kTile + half * (kBN * 128) + bx * box * 128;
-          tc::tma_load_4d(dst, map, &full[stage], half * 64, row, wk.h, page);
+        for (int bx = 0; bx < live; ++bx) {
+          const int j = i * kBN + bx * box, page = pages.of(bx);
+          const int row = p.page_table != nullptr ? j & ((1 << p.page_shift) - 1) : wk.s.k0 + j;
+          if (lane == 0) {
+            uint8_t* dst = smem + stage * C::kStage + bx * box * (2 * D);
+            tc::tma_load_5d(dst, &tmK, &full[stage], 0, row, 0, wk.h, page);
+            tc::tma_load_5d(dst + C::kTile, &tmV, &full[stage], 0, row, 0, wk.h, page);
+          }
         }
+        issued = base + i + 1;
       }
+      it += max(i1 - i0, 0);
     }
-    // copies in flight land before the CTA exits
+    // its last copies land before the CTA exits: tiles issued - 1, issued - 1 - kProd, ..
     if (lane == 0)
-      for (int i = 0; i < NS && i < it; ++i)
-        mbar_wait(&full[i], static_cast<uint32_t>(((it - 1 - i) / NS) & 1), p.ws, 0x721u);
+      for (int i = issued - 1; i >= 0 && i > issued - 1 - NS; i -= C::kProd)
+        wait_bar(&full[i % NS], (i / NS) & 1, p.ws, 0x721u);
     return;
   }
 
@@ -163,6 +179,15 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   const int g = lane >> 2, t4 = lane & 3;
   const int tid = threadIdx.x;
   constexpr int NTH = 32 * NW;
+  // a tile in shared memory is [box of a page][64-value part][key][64 values]
+  const int half_step = box * 128;
+  auto row_at = [&](int r) { return (r >> box_shift) * (box * 2 * D) + (r & (box - 1)) * 128; };
+  int k_row[MT], v_row[MT];  // the rows this lane addresses for the two products
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    k_row[mt] = row_at(mt * 16 + (lane & 7) + ((lane >> 3) & 1) * 8);
+    v_row[mt] = row_at(mt * 16 + (lane & 7) + (lane >> 4) * 8);
+  }
   int it = 0;      // tiles of the CTA so far
   bool ok = true;  // a wait that ran out: no more tiles, but every barrier is still met
   for (; wk.more(); wk.next()) {
@@ -210,7 +235,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     const int skip = ((warp - (base + first)) % NW + NW) % NW;
     for (int i = first + skip; i < i1 && ok; i += NW) {
       const int cta_tile = base + i, stage = cta_tile % NS;
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], (cta_tile / NS) & 1, p.ws, 0x730u));
+      ok = __all_sync(0xffffffffu, wait_bar(&full[stage], (cta_tile / NS) & 1, p.ws, 0x730u));
       if (!ok) break;
       const uint32_t kt = smem_u32(smem + stage * C::kStage), vt = kt + C::kTile;
       const int nv = min(kBN, kend - i * kBN);  // keys of the tile
@@ -221,7 +246,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         constexpr int kVec = D / 8;
         for (int e = lane; e < (blocks * 16 - nv) * kVec; e += 32) {
           const int r = nv + e / kVec, c = e % kVec;
-          *reinterpret_cast<uint4*>(smem + stage * C::kStage + C::kTile + (c / 8) * (kBN * 128) + r * 128 +
+          *reinterpret_cast<uint4*>(smem + stage * C::kStage + C::kTile + row_at(r) + (c / 8) * half_step +
                                     (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
         __syncwarp();
@@ -241,12 +266,12 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
           uint2 qf[NT];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) qf[nt] = sQ[(ks * NT + nt) * 32 + lane];
-          const uint32_t a0 = kt + (ks / 4) * (kBN * 128) + r * 128 + ((((ks & 3) * 2 + ch) ^ (r & 7)) << 4);
+          const uint32_t a0 = kt + (ks / 4) * half_step + ((((ks & 3) * 2 + ch) ^ (r & 7)) << 4);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
             if (mt < blocks) {
               uint32_t a[4];
-              ldsm4(a, a0 + mt * 16 * 128);
+              ldsm4(a, a0 + k_row[mt]);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) mma16816<BF16>(s[mt][nt], a, qf[nt].x, qf[nt].y);
             }
@@ -320,8 +345,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
               uint32_t a[4];
-              const int row = mt * 16 + r;
-              ldsm4_t(a, vt + (j / 4) * (kBN * 128) + row * 128 + ((((j & 3) * 2 + ch) ^ (row & 7)) << 4));
+              ldsm4_t(a, vt + v_row[mt] + (j / 4) * half_step + ((((j & 3) * 2 + ch) ^ (r & 7)) << 4));
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) mma16816<BF16>(o[j][nt], a, pb[mt][nt][0], pb[mt][nt][1]);
             }
@@ -378,13 +402,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         }
       }
       if (whole) {
-        const int i = r / p.G, h = wk.h * p.G + r % p.G;
-        const bool sees = keys_seen(p, wk.s, wk.tok0() + i + 1) > 0;
-        const long long row = wk.s.q0 + wk.tok0() + i;
-        const float inv = sees ? 1.f / L : 0.f;
-        *reinterpret_cast<uint2*>(p.out + row * p.o_st + h * p.o_sh + d) =
-            make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
-        if (p.lse != nullptr && d == 0) p.lse[row * p.Hq + h] = sees ? M * kLn2 + logf(L) : -INFINITY;
+        store_row<BF16>(p, wk, r, d, acc, M, L);
       } else {
         *reinterpret_cast<float4*>(part + r * D + d) = acc;
         if (d == 0) {
@@ -407,50 +425,44 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
       }
       named_bar(1, NTH);
       if (*flag) {
+        // piece 0 is CTA c0's last (slot 1), the others are their CTAs' first (slot 0). kAhead pieces are read at a
+        // time, all their loads in flight together: with one row of many pieces this is a chain of L2 latencies.
+        constexpr int kAhead = NT <= 2 ? 16 : 8;
         const float* base_part = p.parts + static_cast<size_t>(c0) * 2 * C::kPiece;
-        // piece i: CTA c0's piece starts the item (its slot 1), every later one starts inside it (slot 0)
-        auto piece = [&](int i) { return base_part + (i == 0 ? C::kPiece : i * 2 * C::kPiece); };
-        float* sW = sO;                      // [rows][n] weights
-        float* sRow = sO + kMaxCtas * R;     // [rows] M, then [rows] L
-        for (int r = warp; r < rows; r += NW) {
-          float M = -INFINITY;
-          for (int i = lane; i < n; i += 32) {
-            const float* pc = piece(i);
-            if (ld_cg_f32(pc + R * D + R + r) != 0.f) M = fmaxf(M, ld_cg_f32(pc + R * D + r));
-          }
-#pragma unroll
-          for (int o2 = 16; o2 > 0; o2 >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o2));
-          float L = 0.f;
-          for (int i = lane; i < n; i += 32) {
-            const float* pc = piece(i);
-            const float lw = ld_cg_f32(pc + R * D + R + r);
-            const float f = lw != 0.f ? exp2_approx(ld_cg_f32(pc + R * D + r) - M) : 0.f;
-            if (lw != 0.f) L += f * lw;
-            sW[r * n + i] = f;
-          }
-          L = warp_sum(L);
-          if (lane == 0) {
-            sRow[r] = M;
-            sRow[R + r] = L;
-          }
-        }
-        named_bar(1, NTH);
         for (int e = tid; e < rows * kVecs; e += NTH) {
           const int r = e / kVecs, d = (e % kVecs) * 4;
+          float M = -INFINITY, L = 0.f;
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int i = 0; i < n; ++i) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(i) + r * D + d));
-            const float f = sW[r * n + i];
-            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+          for (int i0 = 0; i0 < n; i0 += kAhead) {
+            float pm[kAhead], pl[kAhead];
+            float4 pv[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+              pl[i] = 0.f;
+              if (i0 + i < n) {
+                const float* pc = base_part + (i0 + i == 0 ? C::kPiece : (i0 + i) * 2 * C::kPiece);
+                pm[i] = __ldcg(pc + R * D + r);
+                pl[i] = __ldcg(pc + R * D + R + r);
+                pv[i] = __ldcg(reinterpret_cast<const float4*>(pc + r * D + d));
+              }
+            }
+            float Mn = M;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+              if (pl[i] != 0.f) Mn = fmaxf(Mn, pm[i]);  // a piece without a visible key has sum 0
+            const float a = L != 0.f ? exp2_approx(M - Mn) : 0.f;
+            M = Mn;
+            L *= a;
+            acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+              if (pl[i] != 0.f) {
+                const float f = exp2_approx(pm[i] - M);
+                L += f * pl[i];
+                acc.x += f * pv[i].x, acc.y += f * pv[i].y, acc.z += f * pv[i].z, acc.w += f * pv[i].w;
+              }
           }
-          const int i = r / p.G, h = wk.h * p.G + r % p.G;
-          const bool sees = keys_seen(p, wk.s, wk.tok0() + i + 1) > 0;
-          const long long row = wk.s.q0 + wk.tok0() + i;
-          const float inv = sees ? 1.f / sRow[R + r] : 0.f;
-          *reinterpret_cast<uint2*>(p.out + row * p.o_st + h * p.o_sh + d) =
-              make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
-          if (p.lse != nullptr && d == 0) p.lse[row * p.Hq + h] = sees ? sRow[r] * kLn2 + logf(sRow[R + r]) : -INFINITY;
+          store_row<BF16>(p, wk, r, d, acc, M, L);
         }
       }
     }
@@ -463,7 +475,7 @@ int launch_split(const Problem& p, const Source& src, bool bf16, int grid, cudaS
   using C = Cfg<D, NT>;
   CUtensorMap mk, mv_;
   const int box = src.box < C::kBN ? src.box : C::kBN;
-  const int rc = make_kv_maps(&mk, &mv_, src, p.Hkv, D, bf16, box);
+  const int rc = make_kv_maps(&mk, &mv_, src, p.Hkv, D, bf16, box, D / 64);
   if (rc != MV_OK) return rc;
   auto fn = bf16 ? split_kernel<D, NT, true> : split_kernel<D, NT, false>;
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);

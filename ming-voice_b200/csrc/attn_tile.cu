@@ -10,7 +10,8 @@
 //
 // Layout of a CTA (one per SM): a work item is two tiles of 128 rows (row = token * G + head) of one sequence and key
 // head, which share the key and value tiles in shared memory.
-//   warp 0       TMA producer: Q tiles, then K and V tiles in turn into a ring of slots (a box per page and 64 values)
+//   warps 0,2,3  TMA producers, a K or V tile each in turn, into two rings of slots (a box per page and 64 values);
+//                warp 0 also loads Q
 //   warp 1       MMA issuer: S_t = Q_t K^T and O_t += P_t V, both into TMEM; P_t is the TMEM operand
 //   warps 4..7   softmax of tile 0, warps 8..11 of tile 1: a thread owns a row (a TMEM lane). S -> weights P, written
 //                over S in TMEM; the row's sum and maximum stay in registers; at the end O / sum -> global memory.
@@ -35,12 +36,13 @@ template <int D>
 struct Cfg {
   static constexpr int kTile = kBN * D * 2;         // bytes of a K or V tile
   static constexpr int kQ = kM * D * 2;             // bytes of a Q tile
-  static constexpr int kSlots = 131072 / kTile;     // K and V tiles in turn
-  static constexpr int oKV = 2 * kQ;
-  static constexpr int oPre = oKV + kSlots * kTile;
+  static constexpr int kSlots = 65536 / kTile;      // of each ring
+  static constexpr int oK = 2 * kQ;
+  static constexpr int oV = oK + kSlots * kTile;
+  static constexpr int oPre = oV + kSlots * kTile;
   static constexpr int oTmp = oPre + (kMaxB + 1) * 8;
   static constexpr int oBar = oTmp + 32 * 8;
-  static constexpr int kBars = 2 * kSlots + 2 + 6 + 1;
+  static constexpr int kBars = 4 * kSlots + 2 + 6 + 1;
   static constexpr int oTmem = oBar + kBars * 8;
   static constexpr int kSmem = oTmem + 16 + 1024;
   static_assert(kSmem <= 232448, "shared memory");
@@ -91,18 +93,6 @@ __host__ __device__ constexpr uint32_t idesc16(bool bf16, int M, int N, bool b_m
          (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-// Bounded wait, in line: a call would hold the softmax's registers to the calling convention (setmaxnreg kernels).
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, WsHeader* h, unsigned int info) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity))
-    if (globaltimer_ns() - t0 > kWaitLimitNs) {
-      raise_error(h, kErrTimeout, info);
-      return false;
-    }
-  return true;
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 template <int D, bool BF16>
@@ -113,12 +103,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int NS = C::kSlots, kHalves = D / 64, kHalfBytes = kBN * 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem + C::oKV;
+  uint8_t* kring = smem + C::oK;
+  uint8_t* vring = smem + C::oV;
   unsigned long long* pre = reinterpret_cast<unsigned long long*>(smem + C::oPre);
   unsigned long long* tmp = reinterpret_cast<unsigned long long*>(smem + C::oTmp);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBar);
-  uint64_t* empty = full + NS;
-  uint64_t* q_full = empty + NS;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::oBar);
+  uint64_t* k_empty = k_full + NS;
+  uint64_t* v_full = k_empty + NS;
+  uint64_t* v_empty = v_full + NS;
+  uint64_t* q_full = v_empty + NS;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;  // [2] scores of tile t are in TMEM (and the product before them is complete)
   uint64_t* p_full = s_full + 2;   // [2] weights of tile t are in TMEM, its accumulator may be added to
@@ -129,8 +122,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -169,66 +164,86 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     Walk<kBN> wk(p, pre, at, end);
-    if (warp == 0) {
-      // ---------------------------------------------------------------- TMA producer
-      const int nbox = kBN / box, half = lane % kHalves, bx = lane / kHalves;
-      int it = 0, qn = 0;
+    if (warp != 1) {
+      // ---------------------------------------------------------------- TMA producers: lane 0 issues all copies
+      const int box_shift = 31 - __clz(box);
+      int it = 0, qn = 0;                            // key tiles and items so far
+      int turn = warp == 0 ? 0 : warp - 1;           // copies until this warp's next one: K0, V0, K1, V1, ..
+      uint64_t* last[2] = {nullptr, nullptr};        // what its last K and V copies complete
+      uint32_t last_ph[2] = {0, 0};
       bool ok = true;
+      Pages pages;
       for (; wk.more() && ok; wk.next()) {
         const int kend = wk.kend(), ntok = wk.ntok();
-        const int i1 = min(wk.last(), (kend + kBN - 1) / kBN);
-        if (wk.first() >= i1) continue;
-        const int nt = ntok > half_tok ? 2 : 1;
-        ok = __all_sync(0xffffffffu, wait_bar(q_empty, (qn & 1) ^ 1, p.ws, 0x740u));
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(nt * kHalves * rows_used * 128));
-          for (int t = 0; t < nt; ++t)
-            for (int hf = 0; hf < kHalves; ++hf)
-              tc::tma_load_3d(smem + t * C::kQ + hf * kHalfBytes, &tmQ, q_full, hf * 64, wk.h * p.G,
-                              wk.s.q0 + wk.tok0() + t * half_tok);
-        }
-        ++qn;
-        for (int i = wk.first(); i < i1 && ok; ++i) {
-          const int j = i * kBN + bx * box;
-          const bool mine = bx < nbox && j < kend;
-          int page = 0, row = wk.s.k0 + j;
-          if (mine && p.page_table != nullptr) {
-            page = p.page_table[wk.b * p.pt_stride + (j >> p.page_shift)];
-            row = j & ((1 << p.page_shift) - 1);
-            if (page < 0 || page >= p.num_pages) {
-              raise_error(p.ws, kErrBadPage, 0x711u);
-              page = p.num_pages;  // outside the map: reads as zeros
-            }
+        const int i0 = wk.first(), i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+        if (i0 >= i1) continue;
+        pages.next = Pages::read(p, wk.b, i0 * kBN + lane * box, kend);
+        if (warp == 0) {
+          const int nt = ntok > half_tok ? 2 : 1;
+          ok = __all_sync(0xffffffffu, wait_bar(q_empty, (qn & 1) ^ 1, p.ws, 0x740u));
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(nt * kHalves * rows_used * 128));
+            for (int t = 0; t < nt; ++t)
+              for (int hf = 0; hf < kHalves; ++hf)
+                tc::tma_load_3d(smem + t * C::kQ + hf * kHalfBytes, &tmQ, q_full, hf * 64, wk.h * p.G,
+                                wk.s.q0 + wk.tok0() + t * half_tok);
           }
-          const uint32_t bytes = static_cast<uint32_t>(min(nbox, (kend - i * kBN + box - 1) / box) * box * D * 2);
-          for (int kv = 0; kv < 2; ++kv, ++it) {
-            const int slot = it % NS;
-            ok = __all_sync(0xffffffffu, wait_bar(&empty[slot], ((it / NS) & 1) ^ 1, p.ws, 0x741u));
+          ++qn;
+        }
+        for (int i = i0; i < i1 && ok; ++i, ++it) {
+          const int slot = it % NS;
+          const uint32_t ph = (it / NS) & 1;
+          const int live = min(kBN, kend - i * kBN + box - 1) >> box_shift;  // boxes with a key
+          pages.step(p, 0x711u);
+          pages.next = Pages::read(p, wk.b, (i + 1) * kBN + lane * box, kend);
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            if (turn-- > 0) continue;
+            turn = 2;
+            uint64_t* full = kv ? v_full + slot : k_full + slot;
+            ok = ok && __all_sync(0xffffffffu, wait_bar(kv ? v_empty + slot : k_empty + slot, ph ^ 1, p.ws, 0x741u));
             if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
-            __syncwarp();
-            if (mine)
-              tc::tma_load_4d(ring + slot * C::kTile + half * kHalfBytes + bx * box * 128, kv ? &tmV : &tmK,
-                              &full[slot], half * 64, row, wk.h, page);
+            last[kv] = full;
+            last_ph[kv] = ph;
+            if (lane == 0) mbar_arrive_expect_tx(full, static_cast<uint32_t>(live * box * D * 2));
+            uint8_t* dst = (kv ? vring : kring) + slot * C::kTile;
+            for (int bx = 0; bx < live; ++bx) {
+              const int j = i * kBN + bx * box, page = pages.of(bx);
+              const int row = p.page_table != nullptr ? j & ((1 << p.page_shift) - 1) : wk.s.k0 + j;
+              if (lane == 0)
+#pragma unroll
+                for (int hf = 0; hf < kHalves; ++hf)
+                  tc::tma_load_5d(dst + hf * kHalfBytes + bx * box * 128, kv ? &tmV : &tmK, full, 0, row, hf, wk.h,
+                                  page);
+            }
           }
         }
       }
-      // copies in flight land before the CTA exits
+      // copies in flight land before the CTA exits: the last one into each slot, or after a wait that ran out, this
+      // warp's last ones
       if (lane == 0) {
         if (qn > 0) wait_bar(q_full, (qn - 1) & 1, p.ws, 0x742u);
-        for (int i = 0; i < NS && i < it; ++i)
-          wait_bar(&full[i], static_cast<uint32_t>(((it - 1 - i) / NS) & 1), p.ws, 0x743u);
+        if (ok && warp == 0) {
+          for (int i = 0; i < NS && i < it; ++i) {
+            const uint32_t ph = ((it - 1 - i) / NS) & 1;
+            wait_bar(&k_full[i], ph, p.ws, 0x743u);
+            wait_bar(&v_full[i], ph, p.ws, 0x744u);
+          }
+        } else if (!ok) {
+          for (int kv = 0; kv < 2; ++kv)
+            if (last[kv] != nullptr) wait_bar(last[kv], last_ph[kv], p.ws, 0x745u);
+        }
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA issuer (lane 0)
       constexpr uint32_t id_qk = idesc16(BF16, kM, kBN, false), id_pv = idesc16(BF16, kM, D, true);
-      int it = 0, qn = 0;
+      int kt = 0, vt = 0, qn = 0;  // K, V tiles and items so far
       uint32_t pn[2] = {0, 0};
       bool ok = true;
       auto qk = [&](int t, int slot) {
         if (lane == 0) {
-          const uint32_t qa = smem_u32(smem + t * C::kQ), ka = smem_u32(ring + slot * C::kTile);
+          const uint32_t qa = smem_u32(smem + t * C::kQ), ka = smem_u32(kring + slot * C::kTile);
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
             tc::mma_bf16(tmem + t * 128, tc::sw128_desc(qa + (ks / 4) * kHalfBytes) + 2 * (ks & 3),
@@ -241,22 +256,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int i0 = wk.first(), i1 = min(wk.last(), (kend + kBN - 1) / kBN);
         if (i0 >= i1) continue;
         const int nt = wk.ntok() > half_tok ? 2 : 1;
-        ok = wait_bar(q_full, qn & 1, p.ws, 0x750u) && wait_bar(&full[it % NS], (it / NS) & 1, p.ws, 0x751u);
+        ok = wait_bar(q_full, qn & 1, p.ws, 0x750u) && wait_bar(&k_full[kt % NS], (kt / NS) & 1, p.ws, 0x751u);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ++qn;
         tc::fence_after_sync();
-        for (int t = 0; t < nt; ++t) qk(t, it % NS);
+        for (int t = 0; t < nt; ++t) qk(t, kt % NS);
         if (lane == 0) {
-          tc::mma_commit(&empty[it % NS]);
+          tc::mma_commit(&k_empty[kt % NS]);
           if (i0 + 1 == i1) tc::mma_commit(q_empty);
         }
-        ++it;
-        for (int i = i0; i < i1 && ok; ++i) {
+        ++kt;
+        for (int i = i0; i < i1; ++i, ++vt) {
           const bool more = i + 1 < i1;
-          const int vs = it % NS, ks = (it + 1) % NS;
-          ok = wait_bar(&full[vs], (it / NS) & 1, p.ws, 0x752u);
-          if (more) ok = ok && wait_bar(&full[ks], ((it + 1) / NS) & 1, p.ws, 0x753u);
+          const int vs = vt % NS, ks = kt % NS;
+          ok = wait_bar(&v_full[vs], (vt / NS) & 1, p.ws, 0x752u);
+          if (more) ok = ok && wait_bar(&k_full[ks], (kt / NS) & 1, p.ws, 0x753u);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const int nv = min(kBN, kend - i * kBN), steps = (nv + 15) / 16;
@@ -265,19 +280,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             // are 0, and 0 * NaN is not, so the values are cleared
             for (int e = lane; e < (steps * 16 - nv) * kHalves * 8; e += 32) {
               const int c = e & 7, hf = (e >> 3) % kHalves, r = nv + (e >> 3) / kHalves;
-              *reinterpret_cast<uint4*>(ring + vs * C::kTile + hf * kHalfBytes + r * 128 + c * 16) =
+              *reinterpret_cast<uint4*>(vring + vs * C::kTile + hf * kHalfBytes + r * 128 + c * 16) =
                   make_uint4(0u, 0u, 0u, 0u);
             }
             fence_proxy_async_smem();
             __syncwarp();
           }
-          for (int t = 0; t < nt && ok; ++t) {
+          for (int t = 0; t < nt; ++t) {
             ok = __all_sync(0xffffffffu, wait_bar(&p_full[t], pn[t] & 1, p.ws, 0x754u));
             if (!ok) break;
             ++pn[t];
             tc::fence_after_sync();
             if (lane == 0) {
-              const uint32_t va = smem_u32(ring + vs * C::kTile);
+              const uint32_t va = smem_u32(vring + vs * C::kTile);
               for (int k = 0; k < steps; ++k)
                 mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, v_desc(va + k * 2048, kHalfBytes), id_pv,
                        i > i0 || k > 0);
@@ -287,11 +302,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!ok) break;
           if (lane == 0) {
-            tc::mma_commit(&empty[vs]);
-            if (more) tc::mma_commit(&empty[ks]);
+            tc::mma_commit(&v_empty[vs]);
+            if (more) tc::mma_commit(&k_empty[ks]);
             if (i + 2 == i1) tc::mma_commit(q_empty);
           }
-          it += more ? 2 : 1;
+          kt += more;
         }
       }
       // every issued product retires before the TMEM is released
@@ -538,7 +553,7 @@ int launch_tile(const Problem& p, const Source& src, int grid, CutItem* cuts, cu
   using C = Cfg<D>;
   CUtensorMap mq, mk, mv_;
   const int box = src.box < kBN ? src.box : kBN;
-  int rc = make_kv_maps(&mk, &mv_, src, p.Hkv, D, BF16, box);
+  int rc = make_kv_maps(&mk, &mv_, src, p.Hkv, D, BF16, box, 1);
   if (rc == MV_OK) rc = make_q_map(&mq, p, D, BF16, p.tok / 2);
   if (rc != MV_OK) return rc;
   auto fn = tile_kernel<D, BF16>;
