@@ -40,7 +40,8 @@ struct Problem {
   int B, T, Tk, Hq, Hkv, G;
   int tok;                // tokens of a tile
   int causal;
-  int min_share;          // least units worth a CTA of their own
+  int extra;              // units an item counts besides its key tiles
+  int min_share;          // least units worth a CTA of their own; more than 2 extra
   float scale_log2;       // scale * log2(e): softmax in powers of two
   WsHeader* ws;
   unsigned int* counters;  // [kMaxCtas] arrivals of the split item that starts in a CTA's range (left zeroed)
@@ -78,10 +79,20 @@ __device__ __forceinline__ int keys_seen(const Problem& p, const Seq& s, int end
   return p.causal ? min(s.n, max(s.n - s.nq + end, 0)) : s.n;
 }
 
+// Key tiles of token tile t; at least one, as an item without a visible key still has its rows to write.
 template <int BN>
-__device__ __forceinline__ int item_units(const Problem& p, const Seq& s, int t) {
-  const int kend = keys_seen(p, s, min(s.nq, (t + 1) * p.tok));
-  return max((kend + BN - 1) / BN, 1);  // an item without a visible key still has its rows to write
+__device__ __forceinline__ int item_tiles(const Problem& p, const Seq& s, int t) {
+  return max((keys_seen(p, s, min(s.nq, (t + 1) * p.tok)) + BN - 1) / BN, 1);
+}
+
+// Units of all token tiles of one key head of a sequence; the whole warp with the same s.
+template <int BN>
+__device__ __forceinline__ unsigned long long head_units(const Problem& p, const Seq& s, int tiles) {
+  unsigned long long u = 0;
+  for (int t = threadIdx.x & 31; t < tiles; t += 32) u += item_tiles<BN>(p, s, t) + p.extra;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+  return u;
 }
 
 // Exclusive prefix sums of the sequences' units into pre[0 .. B], by all threads of the CTA; `tmp` [32].
@@ -92,12 +103,21 @@ __device__ __forceinline__ void build_schedule(const Problem& p, unsigned long l
   for (int base = 0; base < p.B; base += nt) {
     const int b = base + tid;
     unsigned long long u = 0;
-    if (b < p.B) {
-      const Seq s = seq_of(p, b, blockIdx.x == 0);
-      const int tiles = (s.nq + p.tok - 1) / p.tok;
-      for (int t = 0; t < tiles; ++t) u += item_units<BN>(p, s, t);
-      u *= p.Hkv;
+    Seq s{0, 0, 0, 0};
+    if (b < p.B) s = seq_of(p, b, blockIdx.x == 0);
+    const int tiles = (s.nq + p.tok - 1) / p.tok;
+    if (tiles <= 4)
+      for (int t = 0; t < tiles; ++t) u += item_tiles<BN>(p, s, t) + p.extra;
+    unsigned int many = __ballot_sync(0xffffffffu, tiles > 4);
+    while (many) {  // long sequences: a warp each
+      const int l = __ffs(many) - 1;
+      many &= many - 1;
+      const Seq o{__shfl_sync(0xffffffffu, s.q0, l), __shfl_sync(0xffffffffu, s.nq, l),
+                  __shfl_sync(0xffffffffu, s.k0, l), __shfl_sync(0xffffffffu, s.n, l)};
+      const unsigned long long v = head_units<BN>(p, o, __shfl_sync(0xffffffffu, tiles, l));
+      if (lane == l) u = v;
     }
+    u *= p.Hkv;
     unsigned long long x = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -113,7 +133,7 @@ __device__ __forceinline__ void build_schedule(const Problem& p, unsigned long l
     }
     if (b < p.B) pre[b] = before + x - u;
     carry = all;
-    __syncthreads();
+    if (base + nt < p.B) __syncthreads();
   }
   if (tid == 0) pre[p.B] = carry;
   __syncthreads();
@@ -125,73 +145,93 @@ __device__ __forceinline__ unsigned long long quot(unsigned long long a, unsigne
   return a / b;
 }
 
-// The CTAs' ranges: [bound(c), bound(c + 1)) of W units over the first `ctas` CTAs of the grid, the first `rest` of
-// them one unit longer.
+// The CTAs' ranges [bound(c), bound(c + 1)) of the W units, before cuts move to nearby ends of items.
 struct Cut {
-  unsigned long long share;
-  unsigned int ctas, rest;
-  __device__ __forceinline__ Cut(unsigned long long W, int grid, int min_share) {
-    ctas = static_cast<unsigned int>(min(quot(W + min_share - 1, min_share), static_cast<unsigned long long>(grid)));
+  unsigned long long W;
+  unsigned int ctas;  // CTAs of the grid that have a range
+  __device__ __forceinline__ Cut(const Problem& p, unsigned long long total, int grid) {
+    W = total;
+    ctas = static_cast<unsigned int>(min(quot(W, p.min_share), static_cast<unsigned long long>(grid)));
+    // one sequence: its heads' items are alike, and so many cuts for each fall on their ends
+    if (p.B == 1 && ctas > p.Hkv) ctas -= ctas % p.Hkv;
     if (ctas == 0) ctas = 1;
-    share = quot(W, ctas);
-    rest = static_cast<unsigned int>(W - share * ctas);
   }
-  __device__ __forceinline__ unsigned long long bound(unsigned int c) const {
-    c = min(c, ctas);
-    return c * share + min(c, rest);
-  }
+  __device__ __forceinline__ unsigned long long bound(unsigned int c) const { return quot(W * min(c, ctas), ctas); }
   // the CTA whose range holds unit x
   __device__ __forceinline__ unsigned int cta_of(unsigned long long x) const {
-    const unsigned long long long_part = rest * (share + 1);
-    if (x < long_part) return static_cast<unsigned int>(quot(x, share + 1));
-    return rest + static_cast<unsigned int>(quot(x - long_part, share));
+    return static_cast<unsigned int>(quot((x + 1) * ctas - 1, W));
   }
 };
 
-// Walks the pieces of a CTA's range. Every role of the CTA walks on its own and sees the same pieces.
+// Walks the pieces of a CTA's range, warp by warp: every warp of the CTA walks on its own and sees the same pieces.
 template <int BN>
 struct Walk {
   const Problem& p;
-  unsigned long long at, end;      // units of the range still to do
-  unsigned long long item_start;   // unit at which the current item starts
-  int b, h, t, units;
+  unsigned long long end;          // end of the range
+  unsigned long long start;        // unit at which the current item starts
+  int b, h, t, tiles;
+  int i0, i1;                      // the piece: key tiles [i0, i1) of the item's `tiles`
+  bool live;
   Seq s;
 
-  __device__ __forceinline__ Walk(const Problem& p_, const unsigned long long* pre, unsigned long long a,
-                                  unsigned long long e)
-      : p(p_), at(a), end(e), b(0), h(0), t(0), units(1) {
-    if (at >= end) return;
-    int lo = 0, hi = p.B - 1;  // the last sequence with pre[b] <= at (it has units: the next one starts behind at)
+  __device__ __forceinline__ Walk(const Problem& p_, const unsigned long long* pre, const Cut& cut, unsigned int c)
+      : p(p_), end(cut.bound(c + 1)), start(cut.bound(c)), b(0), h(0), t(0), tiles(1), i0(0), i1(0) {
+    live = start < end;
+    if (!live) return;
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = p.B - 1;  // the last sequence with pre[b] <= start (it has units: the next starts behind it)
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if (pre[mid] <= at) lo = mid; else hi = mid - 1;
+      if (pre[mid] <= start) lo = mid; else hi = mid - 1;
     }
     b = lo;
     s = seq_of(p, b, false);
     const unsigned long long per_head = quot(pre[b + 1] - pre[b], p.Hkv);
-    unsigned long long off = at - pre[b];
+    unsigned long long off = start - pre[b];
     h = static_cast<int>(quot(off, per_head));
     off -= per_head * h;
-    for (t = 0;; ++t) {
-      units = item_units<BN>(p, s, t);
-      if (off < static_cast<unsigned long long>(units)) break;
-      off -= units;
+    const int n_t = (s.nq + p.tok - 1) / p.tok;
+    for (int t0 = 0; n_t > 1; t0 += 32) {  // 32 token tiles at a time
+      const int u = t0 + lane < n_t ? item_tiles<BN>(p, s, t0 + lane) + p.extra : 0;
+      unsigned long long x = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const unsigned int over = __ballot_sync(0xffffffffu, x > off);
+      if (over) {
+        const int l = __ffs(over) - 1;
+        t = t0 + l;
+        off -= __shfl_sync(0xffffffffu, x, l) - __shfl_sync(0xffffffffu, u, l);
+        break;
+      }
+      off -= __shfl_sync(0xffffffffu, x, 31);
     }
-    item_start = at - off;
+    tiles = item_tiles<BN>(p, s, t);
+    start -= off;
+    // the range's first cut, moved to an end of the item if that is near
+    const int o = static_cast<int>(off);
+    if (o > p.extra && tiles + p.extra - o <= p.extra) {
+      advance();
+    } else {
+      i0 = o <= p.extra ? 0 : o - p.extra;
+      finish();
+    }
   }
-  __device__ __forceinline__ bool more() const { return at < end; }
-  __device__ __forceinline__ int first() const { return static_cast<int>(at - item_start); }
-  __device__ __forceinline__ int last() const {  // one past the piece's last unit
-    return static_cast<int>(min(end - item_start, static_cast<unsigned long long>(units)));
+  // the piece's end: the item's, or the range's where that lies well inside the item
+  __device__ __forceinline__ void finish() {
+    i1 = tiles;
+    if (end < start + tiles + p.extra) {
+      const int o = static_cast<int>(end > start ? end - start : 0);
+      if (o <= p.extra) live = false;  // the cut has moved to the item's start: the next CTA's
+      else if (tiles + p.extra - o > p.extra) i1 = o - p.extra;
+    }
   }
-  __device__ __forceinline__ int tok0() const { return t * p.tok; }
-  __device__ __forceinline__ int ntok() const { return min(p.tok, s.nq - t * p.tok); }
-  __device__ __forceinline__ int kend() const { return keys_seen(p, s, min(s.nq, (t + 1) * p.tok)); }
-  __device__ __forceinline__ bool whole() const { return first() == 0 && last() == units; }
-  __device__ __forceinline__ void next() {
-    at = item_start + last();
-    if (at >= end) return;
-    item_start = at;
+  __device__ __forceinline__ void advance() {
+    start += tiles + p.extra;
+    live = start < end;
+    if (!live) return;
     if ((t + 1) * p.tok < s.nq) {
       ++t;
     } else {
@@ -203,7 +243,28 @@ struct Walk {
         } while (s.nq == 0);
       }
     }
-    units = item_units<BN>(p, s, t);
+    tiles = item_tiles<BN>(p, s, t);
+    i0 = 0;
+    finish();
+  }
+  __device__ __forceinline__ bool more() const { return live; }
+  __device__ __forceinline__ void next() {
+    if (i1 < tiles) live = false;  // cut: the range ends inside this item
+    else advance();
+  }
+  __device__ __forceinline__ bool whole() const { return i0 == 0 && i1 == tiles; }
+  __device__ __forceinline__ int tok0() const { return t * p.tok; }
+  __device__ __forceinline__ int ntok() const { return min(p.tok, s.nq - t * p.tok); }
+  __device__ __forceinline__ int kend() const { return keys_seen(p, s, min(s.nq, (t + 1) * p.tok)); }
+  // the CTAs that hold the first and the last piece of the item
+  __device__ __forceinline__ unsigned int first_cta(const Cut& cut) const {
+    const unsigned int c = cut.cta_of(start);
+    return cut.bound(c + 1) - start <= static_cast<unsigned long long>(p.extra) ? c + 1 : c;
+  }
+  __device__ __forceinline__ unsigned int last_cta(const Cut& cut) const {
+    const unsigned long long e = start + tiles + p.extra;
+    const unsigned int c = cut.cta_of(e - 1);
+    return e - cut.bound(c) <= static_cast<unsigned long long>(p.extra) ? c - 1 : c;
   }
 };
 

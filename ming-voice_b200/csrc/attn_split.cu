@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   build_schedule<kBN>(p, pre, tmp);  // its barriers also publish the mbarriers
   const unsigned long long W = pre[p.B];
   if (W == 0) return;
-  const Cut cut(W, gridDim.x, p.min_share);
-  Walk<kBN> wk(p, pre, cut.bound(blockIdx.x), cut.bound(blockIdx.x + 1));
+  const Cut cut(p, W, gridDim.x);
+  Walk<kBN> wk(p, pre, cut, blockIdx.x);
 
   if (warp >= NW) {
     // ---------------------------------------------------------------- producers: lane 0 issues all copies
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     Pages pages;
     for (; wk.more() && ok; wk.next()) {
       const int kend = wk.kend();
-      const int i0 = wk.first(), i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+      const int i0 = wk.i0, i1 = min(wk.i1, (kend + kBN - 1) / kBN);
       const int skip = (turn - it) & (C::kProd - 1);  // tile `it` of the CTA is producer it % kProd's
       pages.next = Pages::read(p, wk.b, (i0 + skip) * kBN + lane * box, kend);
       const int base = it - i0;
@@ -191,8 +191,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   int it = 0;      // tiles of the CTA so far
   bool ok = true;  // a wait that ran out: no more tiles, but every barrier is still met
   for (; wk.more(); wk.next()) {
-    const int kend = wk.kend(), ntok = wk.ntok(), rows = ntok * p.G, first = wk.first();
-    const int i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+    const int kend = wk.kend(), ntok = wk.ntok(), rows = ntok * p.G, first = wk.i0;
+    const int i1 = min(wk.i1, (kend + kBN - 1) / kBN);
     // Q as the 8-column operand's fragments: row n = lane / 4, values 16 ks + 2 (lane % 4) + {0, 1} and + {8, 9}
     for (int e = tid; e < (D / 16) * NT * 32; e += NTH) {
       const int l = e & 31, nt = (e >> 5) % NT, ks = (e >> 5) / NT;
@@ -413,8 +413,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     }
     if (!whole) {
       // the CTA that leaves the item's last missing piece joins them all
-      const unsigned int c0 = cut.cta_of(wk.item_start), c1 = cut.cta_of(wk.item_start + wk.units - 1);
-      const int n = static_cast<int>(c1 - c0) + 1;
+      const unsigned int c0 = wk.first_cta(cut);
+      const int n = static_cast<int>(wk.last_cta(cut) - c0) + 1;
       __threadfence();
       named_bar(1, NTH);
       if (tid == 0) {
@@ -425,27 +425,32 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
       }
       named_bar(1, NTH);
       if (*flag) {
-        // piece 0 is CTA c0's last (slot 1), the others are their CTAs' first (slot 0). kAhead pieces are read at a
-        // time, all their loads in flight together: with one row of many pieces this is a chain of L2 latencies.
-        constexpr int kAhead = NT <= 2 ? 16 : 8;
+        // piece 0 is CTA c0's last (slot 1), the others are their CTAs' first (slot 0). Many pieces are a chain of L2
+        // latencies: the next kAhead pieces are on their way while kAhead are added.
+        constexpr int kAhead = NT <= 2 ? 8 : 4;
         const float* base_part = p.parts + static_cast<size_t>(c0) * 2 * C::kPiece;
         for (int e = tid; e < rows * kVecs; e += NTH) {
           const int r = e / kVecs, d = (e % kVecs) * 4;
           float M = -INFINITY, L = 0.f;
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int i0 = 0; i0 < n; i0 += kAhead) {
-            float pm[kAhead], pl[kAhead];
-            float4 pv[kAhead];
+          float pm[kAhead], pl[kAhead], nm[kAhead], nl[kAhead];
+          float4 pv[kAhead], nv[kAhead];
+          auto read = [&](int i0, float (&m_)[kAhead], float (&l_)[kAhead], float4 (&v_)[kAhead]) {
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-              pl[i] = 0.f;
-              if (i0 + i < n) {
-                const float* pc = base_part + (i0 + i == 0 ? C::kPiece : (i0 + i) * 2 * C::kPiece);
-                pm[i] = __ldcg(pc + R * D + r);
-                pl[i] = __ldcg(pc + R * D + R + r);
-                pv[i] = __ldcg(reinterpret_cast<const float4*>(pc + r * D + d));
-              }
+              const int k = min(i0 + i, n - 1);
+              const float* pc = base_part + (k == 0 ? C::kPiece : k * 2 * C::kPiece);
+              m_[i] = __ldcg(pc + R * D + r);
+              l_[i] = __ldcg(pc + R * D + R + r);
+              v_[i] = __ldcg(reinterpret_cast<const float4*>(pc + r * D + d));
+              if (i0 + i >= n) l_[i] = 0.f;
             }
+          };
+          read(0, nm, nl, nv);
+          for (int i0 = 0; i0 < n; i0 += kAhead) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) pm[i] = nm[i], pl[i] = nl[i], pv[i] = nv[i];
+            if (i0 + kAhead < n) read(i0 + kAhead, nm, nl, nv);
             float Mn = M;
 #pragma unroll
             for (int i = 0; i < kAhead; ++i)
@@ -490,7 +495,8 @@ int launch_split(const Problem& p, const Source& src, bool bf16, int grid, cudaS
 int run_split(Problem& p, const Source& src, int D, bool bf16, int rows_hint, int grid, cudaStream_t st) {
   const int nt = rows_hint <= 8 && p.G <= 8 ? 1 : rows_hint <= 16 && p.G <= 16 ? 2 : 4;
   p.tok = 8 * nt / p.G;
-  p.min_share = 8;
+  p.extra = 4;
+  p.min_share = 12;
   if (D == 128) {
     if (nt == 1) return launch_split<128, 1>(p, src, bf16, grid, st);
     if (nt == 2) return launch_split<128, 2>(p, src, bf16, grid, st);

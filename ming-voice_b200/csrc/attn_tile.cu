@@ -158,12 +158,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   const unsigned long long W = pre[p.B];
-  const Cut cut(W, gridDim.x, p.min_share);
-  const unsigned long long at = W ? cut.bound(blockIdx.x) : 0, end = W ? cut.bound(blockIdx.x + 1) : 0;
+  const Cut cut(p, W, gridDim.x);
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    Walk<kBN> wk(p, pre, at, end);
+    Walk<kBN> wk(p, pre, cut, blockIdx.x);
     if (warp != 1) {
       // ---------------------------------------------------------------- TMA producers: lane 0 issues all copies
       const int box_shift = 31 - __clz(box);
@@ -175,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Pages pages;
       for (; wk.more() && ok; wk.next()) {
         const int kend = wk.kend(), ntok = wk.ntok();
-        const int i0 = wk.first(), i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+        const int i0 = wk.i0, i1 = min(wk.i1, (kend + kBN - 1) / kBN);
         if (i0 >= i1) continue;
         pages.next = Pages::read(p, wk.b, i0 * kBN + lane * box, kend);
         if (warp == 0) {
@@ -253,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       for (; wk.more() && ok; wk.next()) {
         const int kend = wk.kend();
-        const int i0 = wk.first(), i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+        const int i0 = wk.i0, i1 = min(wk.i1, (kend + kBN - 1) / kBN);
         if (i0 >= i1) continue;
         const int nt = wk.ntok() > half_tok ? 2 : 1;
         ok = wait_bar(q_full, qn & 1, p.ws, 0x750u) && wait_bar(&k_full[kt % NS], (kt / NS) & 1, p.ws, 0x751u);
@@ -319,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ------------------------------------------------------------------ softmax: tile t, a thread per row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    Walk<kBN> wk(p, pre, at, end);
+    Walk<kBN> wk(p, pre, cut, blockIdx.x);
     const int t = warp >= 8, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + 256 + t * 128;
@@ -328,11 +327,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int my_tok = t * half_tok + r / p.G, my_head = r % p.G;
     CutItem mine{};
     for (; wk.more() && ok; wk.next()) {
-      const int kend = wk.kend(), ntok = wk.ntok(), i0 = wk.first();
-      const int i1 = min(wk.last(), (kend + kBN - 1) / kBN);
+      const int kend = wk.kend(), ntok = wk.ntok(), i0 = wk.i0;
+      const int i1 = min(wk.i1, (kend + kBN - 1) / kBN);
       const bool whole = wk.whole();
       if (!whole && i0 == 0) {
-        mine.n = static_cast<int>(cut.cta_of(wk.item_start + wk.units - 1) - blockIdx.x) + 1;
+        mine.n = static_cast<int>(wk.last_cta(cut) - blockIdx.x) + 1;
         mine.row0 = wk.s.q0 + wk.tok0();
         mine.ntok = ntok;
         mine.h = wk.h;
@@ -569,7 +568,8 @@ int launch_tile(const Problem& p, const Source& src, int grid, CutItem* cuts, cu
 
 int run_tile(Problem& p, const Source& src, int D, bool bf16, int grid, cudaStream_t st) {
   p.tok = 2 * (kM / p.G);
-  p.min_share = 4;
+  p.extra = 2;
+  p.min_share = 3;
   CutItem* cuts = reinterpret_cast<CutItem*>(p.counters + 256);
   if (D == 128)
     return bf16 ? launch_tile<128, true>(p, src, grid, cuts, st) : launch_tile<128, false>(p, src, grid, cuts, st);
