@@ -154,11 +154,11 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         pages.next = Pages::read(p, wk.b, (i + C::kProd) * kBN + lane * box, kend);
         ok = __all_sync(0xffffffffu, wait_bar(&empty[stage], (((base + i) / NS) & 1) ^ 1, p.ws, 0x720u));
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(live * box * D * 4));
+        if (tc::elect_one()) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(live * box * D * 4));
         for (int bx = 0; bx < live; ++bx) {
           const int j = i * kBN + bx * box, page = pages.of(bx);
           const int row = p.page_table != nullptr ? j & ((1 << p.page_shift) - 1) : wk.s.k0 + j;
-          if (lane == 0) {
+          if (tc::elect_one()) {
             uint8_t* dst = smem + stage * C::kStage + bx * box * (2 * D);
             tc::tma_load_5d(dst, &tmK, &full[stage], 0, row, 0, wk.h, page);
             tc::tma_load_5d(dst + C::kTile, &tmV, &full[stage], 0, row, 0, wk.h, page);
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
       it += max(i1 - i0, 0);
     }
     // its last copies land before the CTA exits: tiles issued - 1, issued - 1 - kProd, ..
-    if (lane == 0)
+    if (tc::elect_one())
       for (int i = issued - 1; i >= 0 && i > issued - 1 - NS; i -= C::kProd)
         wait_bar(&full[i % NS], (i / NS) & 1, p.ws, 0x721u);
     return;

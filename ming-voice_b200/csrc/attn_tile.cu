@@ -10,8 +10,9 @@
 //
 // Layout of a CTA (one per SM): a work item is two tiles of 128 rows (row = token * G + head) of one sequence and key
 // head, which share the key and value tiles in shared memory.
-//   warps 0,2,3  TMA producers, a K or V tile each in turn, into two rings of slots (a box per page and 64 values);
-//                warp 0 also loads Q
+//   warps 0, 2   TMA producers: Q and K tiles, V tiles, into two rings of slots (a box per page and 64 values). One
+//                warp fills all slots of a ring: its wait for a free slot knows the slot's last use by parity, which
+//                holds only for a warp that has itself issued that use
 //   warp 1       MMA issuer: S_t = Q_t K^T and O_t += P_t V, both into TMEM; P_t is the TMEM operand
 //   warps 4..7   softmax of tile 0, warps 8..11 of tile 1: a thread owns a row (a TMEM lane). S -> weights P, written
 //                over S in TMEM; the row's sum and maximum stay in registers; at the end O / sum -> global memory.
@@ -163,13 +164,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     Walk<kBN> wk(p, pre, cut, blockIdx.x);
-    if (warp != 1) {
+    if (warp == 0 || warp == 2) {
       // ---------------------------------------------------------------- TMA producers: lane 0 issues all copies
+      const bool is_v = warp == 2;
+      const CUtensorMap* map = is_v ? &tmV : &tmK;
+      uint8_t* ring = is_v ? vring : kring;
+      uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
       const int box_shift = 31 - __clz(box);
-      int it = 0, qn = 0;                            // key tiles and items so far
-      int turn = warp == 0 ? 0 : warp - 1;           // copies until this warp's next one: K0, V0, K1, V1, ..
-      uint64_t* last[2] = {nullptr, nullptr};        // what its last K and V copies complete
-      uint32_t last_ph[2] = {0, 0};
+      int it = 0, qn = 0;  // tiles and items so far
       bool ok = true;
       Pages pages;
       for (; wk.more() && ok; wk.next()) {
@@ -177,11 +179,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int i0 = wk.i0, i1 = min(wk.i1, (kend + kBN - 1) / kBN);
         if (i0 >= i1) continue;
         pages.next = Pages::read(p, wk.b, i0 * kBN + lane * box, kend);
-        if (warp == 0) {
+        if (!is_v) {
           const int nt = ntok > half_tok ? 2 : 1;
           ok = __all_sync(0xffffffffu, wait_bar(q_empty, (qn & 1) ^ 1, p.ws, 0x740u));
           if (!ok) break;
-          if (lane == 0) {
+          if (tc::elect_one()) {
             mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(nt * kHalves * rows_used * 128));
             for (int t = 0; t < nt; ++t)
               for (int hf = 0; hf < kHalves; ++hf)
@@ -190,49 +192,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ++qn;
         }
-        for (int i = i0; i < i1 && ok; ++i, ++it) {
+        for (int i = i0; i < i1; ++i, ++it) {
           const int slot = it % NS;
-          const uint32_t ph = (it / NS) & 1;
           const int live = min(kBN, kend - i * kBN + box - 1) >> box_shift;  // boxes with a key
           pages.step(p, 0x711u);
           pages.next = Pages::read(p, wk.b, (i + 1) * kBN + lane * box, kend);
+          ok = __all_sync(0xffffffffu, wait_bar(&empty[slot], ((it / NS) & 1) ^ 1, p.ws, 0x741u));
+          if (!ok) break;
+          if (tc::elect_one()) mbar_arrive_expect_tx(&full[slot], static_cast<uint32_t>(live * box * D * 2));
+          for (int bx = 0; bx < live; ++bx) {
+            const int j = i * kBN + bx * box, page = pages.of(bx);
+            const int row = p.page_table != nullptr ? j & ((1 << p.page_shift) - 1) : wk.s.k0 + j;
+            if (tc::elect_one())
 #pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            if (turn-- > 0) continue;
-            turn = 2;
-            uint64_t* full = kv ? v_full + slot : k_full + slot;
-            ok = ok && __all_sync(0xffffffffu, wait_bar(kv ? v_empty + slot : k_empty + slot, ph ^ 1, p.ws, 0x741u));
-            if (!ok) break;
-            last[kv] = full;
-            last_ph[kv] = ph;
-            if (lane == 0) mbar_arrive_expect_tx(full, static_cast<uint32_t>(live * box * D * 2));
-            uint8_t* dst = (kv ? vring : kring) + slot * C::kTile;
-            for (int bx = 0; bx < live; ++bx) {
-              const int j = i * kBN + bx * box, page = pages.of(bx);
-              const int row = p.page_table != nullptr ? j & ((1 << p.page_shift) - 1) : wk.s.k0 + j;
-              if (lane == 0)
-#pragma unroll
-                for (int hf = 0; hf < kHalves; ++hf)
-                  tc::tma_load_5d(dst + hf * kHalfBytes + bx * box * 128, kv ? &tmV : &tmK, full, 0, row, hf, wk.h,
-                                  page);
-            }
+              for (int hf = 0; hf < kHalves; ++hf)
+                tc::tma_load_5d(ring + slot * C::kTile + hf * kHalfBytes + bx * box * 128, map, &full[slot], 0, row,
+                                hf, wk.h, page);
           }
         }
       }
-      // copies in flight land before the CTA exits: the last one into each slot, or after a wait that ran out, this
-      // warp's last ones
-      if (lane == 0) {
+      // copies in flight land before the CTA exits
+      if (tc::elect_one()) {
         if (qn > 0) wait_bar(q_full, (qn - 1) & 1, p.ws, 0x742u);
-        if (ok && warp == 0) {
-          for (int i = 0; i < NS && i < it; ++i) {
-            const uint32_t ph = ((it - 1 - i) / NS) & 1;
-            wait_bar(&k_full[i], ph, p.ws, 0x743u);
-            wait_bar(&v_full[i], ph, p.ws, 0x744u);
-          }
-        } else if (!ok) {
-          for (int kv = 0; kv < 2; ++kv)
-            if (last[kv] != nullptr) wait_bar(last[kv], last_ph[kv], p.ws, 0x745u);
-        }
+        for (int i = 0; i < NS && i < it; ++i)
+          wait_bar(&full[i], static_cast<uint32_t>(((it - 1 - i) / NS) & 1), p.ws, 0x743u);
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA issuer (lane 0)
@@ -241,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t pn[2] = {0, 0};
       bool ok = true;
       auto qk = [&](int t, int slot) {
-        if (lane == 0) {
+        if (tc::elect_one()) {
           const uint32_t qa = smem_u32(smem + t * C::kQ), ka = smem_u32(kring + slot * C::kTile);
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
@@ -261,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++qn;
         tc::fence_after_sync();
         for (int t = 0; t < nt; ++t) qk(t, kt % NS);
-        if (lane == 0) {
+        if (tc::elect_one()) {
           tc::mma_commit(&k_empty[kt % NS]);
           if (i0 + 1 == i1) tc::mma_commit(q_empty);
         }
@@ -290,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             ++pn[t];
             tc::fence_after_sync();
-            if (lane == 0) {
+            if (tc::elect_one()) {
               const uint32_t va = smem_u32(vring + vs * C::kTile);
               for (int k = 0; k < steps; ++k)
                 mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, v_desc(va + k * 2048, kHalfBytes), id_pv,
@@ -300,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (more) qk(t, ks);
           }
           if (!ok) break;
-          if (lane == 0) {
+          if (tc::elect_one()) {
             tc::mma_commit(&v_empty[vs]);
             if (more) tc::mma_commit(&k_empty[ks]);
             if (i + 2 == i1) tc::mma_commit(q_empty);
@@ -309,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // every issued product retires before the TMEM is released
-      if (lane == 0) {
+      if (tc::elect_one()) {
         tc::mma_commit(done);
         wait_bar(done, 0u, p.ws, 0x755u);
       }
