@@ -13,12 +13,16 @@
 //   warps 0, 2   TMA producers: Q and K tiles, V tiles, into two rings of slots (a box per page and 64 values). One
 //                warp fills all slots of a ring: its wait for a free slot knows the slot's last use by parity, which
 //                holds only for a warp that has itself issued that use
-//   warp 1       MMA issuer: S_t = Q_t K^T and O_t += P_t V, both into TMEM; P_t is the TMEM operand
-//   warps 4..7   softmax of tile 0, warps 8..11 of tile 1: a thread owns a row (a TMEM lane). S -> weights P, written
-//                over S in TMEM; the row's sum and maximum stay in registers; at the end O / sum -> global memory.
-// While one tile's scores are in the softmax, the other tile's products run. The order of issue per tile is
-// PV(j), QK(j + 1): S(j + 1) overwrites P(j) behind the product that reads it.
-// TMEM columns: S_0 | S_1 | O_0 | O_1 (4 x 128 of 512 at D = 128).
+//   warps 1, 3   MMA issuers: S_t = Q_t K^T and O_t += P_t V, both into TMEM; P_t is the TMEM operand. D = 128: warp 1
+//                for both row tiles in turn; D = 64: a warp each
+//   warps 4..7   softmax of tile 0, warps 8..11 of tile 1: a thread owns a row (a TMEM lane). S -> weights P in TMEM;
+//                the row's sum and maximum stay in registers; at the end O / sum -> global memory.
+// D = 128: while one tile's scores are in the softmax, the other tile's products run. TMEM columns: S_0 | S_1 | O_0 | O_1,
+// 128 each; P_t overwrites S_t, so QK(j + 1) follows PV(j), and the one issuer keeps the tiles half a period apart. (An
+// issuer per tile let them fall into step, both in the exponentials and then both waiting: 1155 us instead of 891 for
+// 20000 causal tokens, 16 / 4 heads.)
+// D = 64: the softmax is the bound. S_0 | S_1 (128) | P_0 | P_1 | O_0 | O_1 (64): QK(j + 1) needs only S_t to be in
+// registers, so the softmax finds its next scores ready, and PV(j) starts when half of the weights are there.
 //
 // Split: equal shares of all (item, key tile) units (attn_common.cuh). Pieces of a cut item go to the workspace and
 // combine_kernel joins them in CTA order.
@@ -31,6 +35,7 @@ namespace {
 constexpr int kBN = 128;        // keys of a tile
 constexpr int kM = 128;         // rows of a tile
 constexpr int kThreads = 384;
+constexpr float kHuge = 16777216.f;
 constexpr float kGrow = 8.f;    // growth of the maximum, in powers of two, that is not followed at once
 
 template <int D>
@@ -43,10 +48,18 @@ struct Cfg {
   static constexpr int oPre = oV + kSlots * kTile;
   static constexpr int oTmp = oPre + (kMaxB + 1) * 8;
   static constexpr int oBar = oTmp + 32 * 8;
-  static constexpr int kBars = 4 * kSlots + 2 + 6 + 1;
+  static constexpr int kBars = 4 * kSlots + 2 + 10 + 1;
   static constexpr int oTmem = oBar + kBars * 8;
   static constexpr int kSmem = oTmem + 16 + 1024;
   static_assert(kSmem <= 232448, "shared memory");
+  static constexpr bool kEarly = D == 64;  // P has columns of its own
+  static constexpr int kIssuers = kEarly ? 2 : 1;
+  __device__ __forceinline__ static uint32_t tmem_p(uint32_t base, int t) {
+    return kEarly ? base + 256 + t * 64 : base + t * 128;
+  }
+  __device__ __forceinline__ static uint32_t tmem_o(uint32_t base, int t) {
+    return kEarly ? base + 384 + t * 64 : base + 256 + t * 128;
+  }
 };
 
 // What combine_kernel needs of a cut item, left by the CTA whose range holds its start.
@@ -94,7 +107,53 @@ __host__ __device__ constexpr uint32_t idesc16(bool bf16, int M, int N, bool b_m
          (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// The row's weights 2^(s scale + base) of a tile into TMEM, rounded to the element type there (as operands of the second
+// product); returns their fp32 sum. Bound by the exponential unit: 8 cycles an instruction and scheduler, 1052 for the
+// 128 of a row. (Handing 2 to 8 of 16 pairs to a polynomial of degree 4 or 5 on the FMA pipe gave 1075 to 1219, and
+// longer kernels: the clamp, the rounding and the packed multiplies cost what they relieve.)
+template <typename C, bool BF16>
+__device__ __forceinline__ float weights(const uint32_t (&s)[4][32], float base, float scale, uint32_t tP,
+                                         uint64_t* half_done) {
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float x0 = base, x1 = base;
+      ffma2(x0, x1, __uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1]), scale, scale);
+      x0 = exp2_approx(x0);
+      x1 = exp2_approx(x1);
+      ffma2(sum[(e & 1) * 2], sum[(e & 1) * 2 + 1], x0, x1, 1.f, 1.f);
+      pk[e] = pack2<BF16>(x0, x1);
+    }
+    tmem_st16(tP + c * 16, pk);
+    if (C::kEarly && c == 1) {
+      tmem_st_wait();
+      tc::fence_before_sync();
+      mbar_arrive(half_done);
+    }
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// Key tiles of a piece: [wk.i0, end), of which row tile t sees [wk.i0, end_of[t]).
+struct Tiles {
+  int kend, end, end_of[2];
+  __device__ __forceinline__ Tiles(const Problem& p, const Walk<kBN>& wk, int half_tok) {
+    kend = wk.kend();
+    const int ntok = wk.ntok();
+    end = min(wk.i1, (kend + kBN - 1) / kBN);
+    end_of[0] = min(wk.i1, (keys_seen(p, wk.s, wk.tok0() + min(ntok, half_tok)) + kBN - 1) / kBN);
+    end_of[1] = ntok > half_tok ? end : 0;
+  }
+};
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -114,9 +173,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* v_empty = v_full + NS;
   uint64_t* q_full = v_empty + NS;
   uint64_t* q_empty = q_full + 1;
-  uint64_t* s_full = q_empty + 1;  // [2] scores of tile t are in TMEM (and the product before them is complete)
-  uint64_t* p_full = s_full + 2;   // [2] weights of tile t are in TMEM, its accumulator may be added to
-  uint64_t* o_full = p_full + 2;   // [2] the piece's last product of tile t is complete
+  uint64_t* s_full = q_empty + 1;  // [2] scores of tile t are in TMEM (D = 128: and the product before them is complete)
+  uint64_t* s_free = s_full + 2;   // [2] D = 64: the scores of tile t are in registers
+  uint64_t* p_half = s_free + 2;   // [2] the first half of tile t's weights is in TMEM, its accumulator may be added to
+  uint64_t* p_full = p_half + 2;   // [2] and the second half
+  uint64_t* o_full = p_full + 2;   // [2] tile t's product with V is complete (D = 128: the piece's last one)
   uint64_t* done = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::oTmem);
 
@@ -124,18 +185,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], C::kIssuers);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], C::kIssuers);
     }
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, C::kIssuers);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
+      mbar_init(&s_free[t], kM);
+      mbar_init(&p_half[t], kM);
       mbar_init(&p_full[t], kM);
       mbar_init(&o_full[t], 1);
     }
-    mbar_init(done, 1);
+    mbar_init(done, C::kIssuers);
     fence_mbar_init();
     tc::prefetch_tmap(&tmQ);
     tc::prefetch_tmap(&tmK);
@@ -217,12 +280,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < NS && i < it; ++i)
           wait_bar(&full[i], static_cast<uint32_t>(((it - 1 - i) / NS) & 1), p.ws, 0x743u);
       }
-    } else if (warp == 1) {
-      // ---------------------------------------------------------------- MMA issuer (lane 0)
+    } else if (C::kEarly || warp == 1) {
+      // ---------------------------------------------------------------- MMA issuers (one elected lane)
       constexpr uint32_t id_qk = idesc16(BF16, kM, kBN, false), id_pv = idesc16(BF16, kM, D, true);
       int kt = 0, vt = 0, qn = 0;  // K, V tiles and items so far
-      uint32_t pn[2] = {0, 0};
+      uint32_t pn[2] = {0, 0};     // weights taken
       bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, unsigned int info) {
+        ok = ok && __all_sync(0xffffffffu, wait_bar(bar, parity, p.ws, info));
+        tc::fence_after_sync();
+        return ok;
+      };
+      // this warp's part of a slot's release: behind its products, or at once where it has none
+      auto release = [&](uint64_t* bar, bool used) {
+        if (tc::elect_one()) {
+          if (used) tc::mma_commit(bar);
+          else mbar_arrive(bar);
+        }
+      };
       auto qk = [&](int t, int slot) {
         if (tc::elect_one()) {
           const uint32_t qa = smem_u32(smem + t * C::kQ), ka = smem_u32(kring + slot * C::kTile);
@@ -233,69 +308,110 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::mma_commit(&s_full[t]);
         }
       };
-      for (; wk.more() && ok; wk.next()) {
-        const int kend = wk.kend();
-        const int i0 = wk.i0, i1 = min(wk.i1, (kend + kBN - 1) / kBN);
-        if (i0 >= i1) continue;
-        const int nt = wk.ntok() > half_tok ? 2 : 1;
-        ok = wait_bar(q_full, qn & 1, p.ws, 0x750u) && wait_bar(&k_full[kt % NS], (kt / NS) & 1, p.ws, 0x751u);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        ++qn;
-        tc::fence_after_sync();
-        for (int t = 0; t < nt; ++t) qk(t, kt % NS);
+      // O_t (+)= P_t V over keys [16 k0, 16 k1) of the tile
+      auto pv = [&](int t, int slot, int k0, int k1, bool first) {
         if (tc::elect_one()) {
-          tc::mma_commit(&k_empty[kt % NS]);
-          if (i0 + 1 == i1) tc::mma_commit(q_empty);
+          const uint64_t vd = v_desc(smem_u32(vring + slot * C::kTile), kHalfBytes);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k >= k0 && k < k1)
+              mma_ts(C::tmem_o(tmem, t), C::tmem_p(tmem, t) + k * 8, vd + k * (2048 >> 4), id_pv, !first || k > 0);
         }
-        ++kt;
-        for (int i = i0; i < i1; ++i, ++vt) {
-          const bool more = i + 1 < i1;
-          const int vs = vt % NS, ks = kt % NS;
-          ok = wait_bar(&v_full[vs], (vt / NS) & 1, p.ws, 0x752u);
-          if (more) ok = ok && wait_bar(&k_full[ks], (kt / NS) & 1, p.ws, 0x753u);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int nv = min(kBN, kend - i * kBN), steps = (nv + 15) / 16;
-          if (nv < steps * 16) {
-            // rows behind the last key hold anything (an older page's values, NaN, another sequence's): their weights
-            // are 0, and 0 * NaN is not, so the values are cleared
-            for (int e = lane; e < (steps * 16 - nv) * kHalves * 8; e += 32) {
-              const int c = e & 7, hf = (e >> 3) % kHalves, r = nv + (e >> 3) / kHalves;
-              *reinterpret_cast<uint4*>(vring + vs * C::kTile + hf * kHalfBytes + r * 128 + c * 16) =
-                  make_uint4(0u, 0u, 0u, 0u);
+      };
+      // rows behind the last of a V tile's nv keys hold anything (an older page's values, NaN, another sequence's): their
+      // weights are 0, and 0 * NaN is not, so the values are cleared up to the product's 16 keys (where there are two
+      // issuers, by both: the same zeros)
+      auto clear_tail = [&](int slot, int nv) {
+        const int up = (nv + 15) & ~15;
+        if (nv == up) return;
+        for (int e = lane; e < (up - nv) * kHalves * 8; e += 32) {
+          const int c = e & 7, hf = (e >> 3) % kHalves, r = nv + (e >> 3) / kHalves;
+          *reinterpret_cast<uint4*>(vring + slot * C::kTile + hf * kHalfBytes + r * 128 + c * 16) =
+              make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      };
+      if constexpr (C::kEarly) {
+        // a warp per row tile; QK(j + 1) before PV(j)
+        const int t = warp >> 1;
+        for (; wk.more() && ok; wk.next()) {
+          const Tiles tl(p, wk, half_tok);
+          const int all = tl.end - wk.i0, my = tl.end_of[t] - wk.i0;  // tiles loaded, tiles this row tile sees
+          if (all <= 0) continue;
+          if (!wait(q_full, qn & 1, 0x750u) || !wait(&k_full[kt % NS], (kt / NS) & 1, 0x751u)) break;
+          ++qn;
+          if (my > 0) qk(t, kt % NS);
+          release(&k_empty[kt % NS], my > 0);
+          if (my <= 1) release(q_empty, my > 0);
+          ++kt;
+          for (int i = 0; i < all; ++i, ++vt) {
+            const int vs = vt % NS, ks = kt % NS;
+            if (i + 1 < all) {
+              if (!wait(&k_full[ks], (kt / NS) & 1, 0x752u)) break;
+              if (i + 1 < my) {
+                if (!wait(&s_free[t], pn[t] & 1, 0x753u)) break;
+                qk(t, ks);
+              }
+              release(&k_empty[ks], i + 1 < my);
+              if (i + 2 == my) release(q_empty, true);
+              ++kt;
             }
-            fence_proxy_async_smem();
-            __syncwarp();
+            if (!wait(&v_full[vs], (vt / NS) & 1, 0x754u)) break;
+            if (i < my) {
+              const int nv = min(kBN, tl.kend - (wk.i0 + i) * kBN), k16 = (nv + 15) / 16;
+              clear_tail(vs, nv);
+              if (!wait(&p_half[t], pn[t] & 1, 0x755u)) break;
+              pv(t, vs, 0, min(k16, 4), i == 0);
+              if (!wait(&p_full[t], pn[t] & 1, 0x756u)) break;
+              pv(t, vs, 4, k16, i == 0);
+              ++pn[t];
+              release(&o_full[t], true);
+            }
+            release(&v_empty[vs], i < my);
           }
-          for (int t = 0; t < nt; ++t) {
-            ok = __all_sync(0xffffffffu, wait_bar(&p_full[t], pn[t] & 1, p.ws, 0x754u));
+        }
+      } else {
+        // one warp for both row tiles, which keeps them half a period apart: one in the softmax, one in the products
+        for (; wk.more() && ok; wk.next()) {
+          const Tiles tl(p, wk, half_tok);
+          const int all = tl.end - wk.i0;
+          const int my[2] = {tl.end_of[0] - wk.i0, tl.end_of[1] - wk.i0};
+          if (all <= 0) continue;
+          if (!wait(q_full, qn & 1, 0x750u) || !wait(&k_full[kt % NS], (kt / NS) & 1, 0x751u)) break;
+          ++qn;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (my[t] > 0) qk(t, kt % NS);
+          release(&k_empty[kt % NS], true);
+          if (all == 1) release(q_empty, true);
+          ++kt;
+          for (int i = 0; i < all; ++i, ++vt) {
+            const int vs = vt % NS, ks = kt % NS;
+            const bool more = i + 1 < all;
+            if (!wait(&v_full[vs], (vt / NS) & 1, 0x752u)) break;
+            if (more && !wait(&k_full[ks], (kt / NS) & 1, 0x753u)) break;
+            const int nv = min(kBN, tl.kend - (wk.i0 + i) * kBN);
+            clear_tail(vs, nv);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (i >= my[t] || !wait(&p_full[t], pn[t] & 1, 0x754u)) continue;
+              ++pn[t];
+              pv(t, vs, 0, (nv + 15) / 16, i == 0);
+              if (i + 1 == my[t]) release(&o_full[t], true);
+              if (i + 1 < my[t]) qk(t, ks);
+            }
             if (!ok) break;
-            ++pn[t];
-            tc::fence_after_sync();
-            if (tc::elect_one()) {
-              const uint32_t va = smem_u32(vring + vs * C::kTile);
-              for (int k = 0; k < steps; ++k)
-                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, v_desc(va + k * 2048, kHalfBytes), id_pv,
-                       i > i0 || k > 0);
-              if (!more) tc::mma_commit(&o_full[t]);
-            }
-            if (more) qk(t, ks);
+            release(&v_empty[vs], true);
+            if (more) release(&k_empty[ks], true);
+            if (i + 2 == all) release(q_empty, true);
+            kt += more;
           }
-          if (!ok) break;
-          if (tc::elect_one()) {
-            tc::mma_commit(&v_empty[vs]);
-            if (more) tc::mma_commit(&k_empty[ks]);
-            if (i + 2 == i1) tc::mma_commit(q_empty);
-          }
-          kt += more;
         }
       }
       // every issued product retires before the TMEM is released
-      if (tc::elect_one()) {
-        tc::mma_commit(done);
-        wait_bar(done, 0u, p.ws, 0x755u);
-      }
+      release(done, true);
+      if (warp == 1) wait_bar(done, 0u, p.ws, 0x757u);
       __syncwarp();
     }
   } else {
@@ -304,14 +420,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     Walk<kBN> wk(p, pre, cut, blockIdx.x);
     const int t = warp >= 8, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + 256 + t * 128;
-    uint32_t sn = 0, on = 0;
+    const uint32_t tS = tmem + lanes + t * 128, tP = C::tmem_p(tmem, t) + lanes, tO = C::tmem_o(tmem, t) + lanes;
+    uint32_t sn = 0, on = 0;  // scores taken, products waited for
     bool ok = true;
     const int my_tok = t * half_tok + r / p.G, my_head = r % p.G;
     CutItem mine{};
     for (; wk.more() && ok; wk.next()) {
-      const int kend = wk.kend(), ntok = wk.ntok(), i0 = wk.i0;
-      const int i1 = min(wk.i1, (kend + kBN - 1) / kBN);
+      const Tiles tl(p, wk, half_tok);
+      const int ntok = wk.ntok(), i0 = wk.i0, i1 = tl.end_of[t];
       const bool whole = wk.whole();
       if (!whole && i0 == 0) {
         mine.n = static_cast<int>(wk.last_cta(cut) - blockIdx.x) + 1;
@@ -335,6 +451,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tc::tmem_ld32(tS + c * 32, s[c]);
         tc::tmem_ld_wait();
+        if (C::kEarly) {
+          tc::fence_before_sync();
+          mbar_arrive(&s_free[t]);
+        }
         if ((i + 1) * kBN > lim_min) {
           const int left = lim - i * kBN;
 #pragma unroll
@@ -353,8 +473,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           mx[c] = fmaxf(mx[c], __uint_as_float(s[c][31]));
         }
         const float tile_max = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-        const bool grow = tile_max > m && (tile_max - m) * p.scale_log2 > kGrow;  // m = -inf: the difference is inf
-        if (__any_sync(0xffffffffu, grow)) {
+        const bool grow = (tile_max - m) * p.scale_log2 > kGrow;  // m = -inf: the difference is inf, or NaN if both are
+        // weights 2^(s scale + base), one fused multiply-add each; the rounding of base is the same for all of a row's
+        // weights and cancels in the quotient, unless it is so large that they overflow: then s - m is taken first
+        float base = m == -INFINITY ? 0.f : -m * p.scale_log2;  // nothing seen yet: every weight is 2^-inf = 0
+        if (C::kEarly && i > i0) {  // P_t and O_t are this row tile's again
+          ok = __all_sync(0xffffffffu, wait_bar(&o_full[t], on & 1, p.ws, 0x762u));
+          if (!ok) break;
+          ++on;
+          tc::fence_after_sync();
+        }
+        if (__any_sync(0xffffffffu, grow || fabsf(base) > kHuge)) {
           const float alpha = grow ? exp2_approx((m - tile_max) * p.scale_log2) : 1.f;
           if (grow) m = tile_max;
           l *= alpha;
@@ -369,37 +498,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st16(tO + c * 16, o);
             }
           }
-        }
-        // weights 2^(s scale + base), one fused multiply-add each; the rounding of base is the same for all of a row's
-        // weights and cancels in the quotient, unless it is so large that they overflow: then s - m is taken first
-        float base = m == -INFINITY ? 0.f : -m * p.scale_log2;  // nothing seen yet: every weight is 2^-inf = 0
-        if (__any_sync(0xffffffffu, fabsf(base) > 16777216.f) && fabsf(base) > 16777216.f) {
-          base = 0.f;
+          base = m == -INFINITY ? 0.f : -m * p.scale_log2;
+          if (fabsf(base) > kHuge) {
+            base = 0.f;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) s[c][e] = __float_as_uint(__uint_as_float(s[c][e]) - m);
-        }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x0 = base, x1 = base;
-            ffma2(x0, x1, __uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1]), p.scale_log2, p.scale_log2);
-            x0 = exp2_approx(x0);
-            x1 = exp2_approx(x1);
-            ffma2(sum[(e & 1) * 2], sum[(e & 1) * 2 + 1], x0, x1, 1.f, 1.f);
-            // the weights are rounded to the element type here, as operands of the second product
-            pk[e] = pack2<BF16>(x0, x1);
+              for (int e = 0; e < 32; ++e) s[c][e] = __float_as_uint(__uint_as_float(s[c][e]) - m);
           }
-          tmem_st16(tS + c * 16, pk);
         }
+        l += weights<C, BF16>(s, base, p.scale_log2, tP, &p_half[t]);
         tmem_st_wait();
         tc::fence_before_sync();
         mbar_arrive(&p_full[t]);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
       if (!ok) break;
       const int slot = i0 > 0 ? 0 : 1;
