@@ -85,48 +85,64 @@ __device__ __forceinline__ int item_tiles(const Problem& p, const Seq& s, int t)
   return max((keys_seen(p, s, min(s.nq, (t + 1) * p.tok)) + BN - 1) / BN, 1);
 }
 
-// Units of all token tiles of one key head of a sequence; the whole warp with the same s.
+// sum of floor((a i + b) / m) over 0 <= i < n (a, b >= 0), as a count of lattice points under a line: whole multiples of m
+// are taken out of a and b, then the axes are exchanged, as in Euclid's algorithm.
+__device__ __forceinline__ unsigned int floor_sum(unsigned int n, unsigned int m, unsigned int a, unsigned int b) {
+  unsigned int sum = 0;
+  while (n > 0) {
+    sum += (n * (n - 1) / 2) * (a / m) + n * (b / m);
+    a %= m, b %= m;
+    const unsigned int top = a * n + b;
+    if (top < m) break;
+    n = top / m;
+    b = top % m;
+    const unsigned int t = m;
+    m = a, a = t;
+  }
+  return sum;
+}
+
+// Units of all token tiles of one key head of a sequence.
 template <int BN>
-__device__ __forceinline__ unsigned long long head_units(const Problem& p, const Seq& s, int tiles) {
-  unsigned long long u = 0;
-  for (int t = threadIdx.x & 31; t < tiles; t += 32) u += item_tiles<BN>(p, s, t) + p.extra;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+__device__ __forceinline__ unsigned int head_units(const Problem& p, const Seq& s) {
+  const int tiles = (s.nq + p.tok - 1) / p.tok;
+  if (tiles == 0) return 0;
+  const unsigned int last = item_tiles<BN>(p, s, tiles - 1);
+  if (!p.causal) return tiles * (last + p.extra);
+  // tile t < tiles - 1 sees c + (t + 1) tok keys; the first `ones` of them at most BN
+  const int c = s.n - s.nq;
+  const int ones = min(tiles - 1, max(0, (BN - c) / p.tok));
+  const int rest = tiles - 1 - ones;
+  unsigned int u = last + ones + tiles * p.extra;
+  if (rest > 0) u += floor_sum(rest, BN, p.tok, c + (ones + 1) * p.tok + BN - 1);
   return u;
 }
 
 // Exclusive prefix sums of the sequences' units into pre[0 .. B], by all threads of the CTA; `tmp` [32].
 template <int BN>
-__device__ __forceinline__ void build_schedule(const Problem& p, unsigned long long* pre, unsigned long long* tmp) {
+__device__ __forceinline__ void build_schedule(const Problem& p, unsigned int* pre, unsigned int* tmp) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = (nt + 31) / 32;
-  unsigned long long carry = 0;
+  unsigned int carry = 0;
   for (int base = 0; base < p.B; base += nt) {
     const int b = base + tid;
-    unsigned long long u = 0;
-    Seq s{0, 0, 0, 0};
-    if (b < p.B) s = seq_of(p, b, blockIdx.x == 0);
-    const int tiles = (s.nq + p.tok - 1) / p.tok;
-    if (tiles <= 4)
-      for (int t = 0; t < tiles; ++t) u += item_tiles<BN>(p, s, t) + p.extra;
-    unsigned int many = __ballot_sync(0xffffffffu, tiles > 4);
-    while (many) {  // long sequences: a warp each
-      const int l = __ffs(many) - 1;
-      many &= many - 1;
-      const Seq o{__shfl_sync(0xffffffffu, s.q0, l), __shfl_sync(0xffffffffu, s.nq, l),
-                  __shfl_sync(0xffffffffu, s.k0, l), __shfl_sync(0xffffffffu, s.n, l)};
-      const unsigned long long v = head_units<BN>(p, o, __shfl_sync(0xffffffffu, tiles, l));
-      if (lane == l) u = v;
+    unsigned int u = 0;
+    if (b < p.B) {
+      const Seq s = seq_of(p, b, blockIdx.x == 0);
+      // a sequence whose share of 2^31 units is not enough (a prompt of millions of tokens) is left out and reported
+      const unsigned long long most = static_cast<unsigned long long>((s.nq + p.tok - 1) / p.tok) *
+                                      ((s.n + BN - 1) / BN + 1 + p.extra) * p.Hkv;
+      if (most < (1ull << 31) / p.B) u = head_units<BN>(p, s) * p.Hkv;
+      else if (blockIdx.x == 0) raise_error(p.ws, kErrOverflow, static_cast<unsigned int>(b));
     }
-    u *= p.Hkv;
-    unsigned long long x = u;
+    unsigned int x = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+      const unsigned int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
     if (lane == 31) tmp[warp] = x;
     __syncthreads();
-    unsigned long long before = carry, all = carry;
+    unsigned int before = carry, all = carry;
     for (int w = 0; w < nw; ++w) {
       if (w < warp) before += tmp[w];
       all += tmp[w];
@@ -139,27 +155,29 @@ __device__ __forceinline__ void build_schedule(const Problem& p, unsigned long l
   __syncthreads();
 }
 
-// a / b: a 64-bit division is a long subroutine, and nearly all counts here fit 32 bits
-__device__ __forceinline__ unsigned long long quot(unsigned long long a, unsigned long long b) {
-  if (((a | b) >> 32) == 0) return static_cast<unsigned int>(a) / static_cast<unsigned int>(b);
-  return a / b;
-}
-
-// The CTAs' ranges [bound(c), bound(c + 1)) of the W units, before cuts move to nearby ends of items.
+// The CTAs' ranges [bound(c), bound(c + 1)) of the W units, bound(c) = floor(W c / ctas), before cuts move to nearby ends
+// of items.
 struct Cut {
-  unsigned long long W;
-  unsigned int ctas;  // CTAs of the grid that have a range
-  __device__ __forceinline__ Cut(const Problem& p, unsigned long long total, int grid) {
+  unsigned int W, ctas, share, rest;  // ctas: CTAs of the grid that have a range; W = share ctas + rest
+  __device__ __forceinline__ Cut(const Problem& p, unsigned int total, int grid) {
     W = total;
-    ctas = static_cast<unsigned int>(min(quot(W, p.min_share), static_cast<unsigned long long>(grid)));
+    ctas = min(W / p.min_share, static_cast<unsigned int>(grid));
     // one sequence: its heads' items are alike, and so many cuts for each fall on their ends
     if (p.B == 1 && ctas > p.Hkv) ctas -= ctas % p.Hkv;
     if (ctas == 0) ctas = 1;
+    share = W / ctas;
+    rest = W - share * ctas;
   }
-  __device__ __forceinline__ unsigned long long bound(unsigned int c) const { return quot(W * min(c, ctas), ctas); }
-  // the CTA whose range holds unit x
-  __device__ __forceinline__ unsigned int cta_of(unsigned long long x) const {
-    return static_cast<unsigned int>(quot((x + 1) * ctas - 1, W));
+  __device__ __forceinline__ unsigned int bound(unsigned int c) const {
+    c = min(c, ctas);
+    return c * share + c * rest / ctas;
+  }
+  // the CTA whose range holds unit x: the estimate in floats is off by one at most
+  __device__ __forceinline__ unsigned int cta_of(unsigned int x) const {
+    unsigned int c = min(static_cast<unsigned int>((static_cast<float>(x) + 0.5f) * ctas / W), ctas - 1);
+    if (c > 0 && bound(c) > x) --c;
+    if (bound(c + 1) <= x) ++c;
+    return c;
   }
 };
 
@@ -167,15 +185,16 @@ struct Cut {
 template <int BN>
 struct Walk {
   const Problem& p;
-  unsigned long long end;          // end of the range
-  unsigned long long start;        // unit at which the current item starts
+  const unsigned int* pre;
+  unsigned int end;                // end of the range
+  unsigned int start;              // unit at which the current item starts
   int b, h, t, tiles;
   int i0, i1;                      // the piece: key tiles [i0, i1) of the item's `tiles`
   bool live;
   Seq s;
 
-  __device__ __forceinline__ Walk(const Problem& p_, const unsigned long long* pre, const Cut& cut, unsigned int c)
-      : p(p_), end(cut.bound(c + 1)), start(cut.bound(c)), b(0), h(0), t(0), tiles(1), i0(0), i1(0) {
+  __device__ __forceinline__ Walk(const Problem& p_, const unsigned int* pre_, const Cut& cut, unsigned int c)
+      : p(p_), pre(pre_), end(cut.bound(c + 1)), start(cut.bound(c)), b(0), h(0), t(0), tiles(1), i0(0), i1(0) {
     live = start < end;
     if (!live) return;
     const int lane = threadIdx.x & 31;
@@ -186,17 +205,17 @@ struct Walk {
     }
     b = lo;
     s = seq_of(p, b, false);
-    const unsigned long long per_head = quot(pre[b + 1] - pre[b], p.Hkv);
-    unsigned long long off = start - pre[b];
-    h = static_cast<int>(quot(off, per_head));
+    const unsigned int per_head = (pre[b + 1] - pre[b]) / p.Hkv;
+    unsigned int off = start - pre[b];
+    h = static_cast<int>(off / per_head);
     off -= per_head * h;
     const int n_t = (s.nq + p.tok - 1) / p.tok;
     for (int t0 = 0; n_t > 1; t0 += 32) {  // 32 token tiles at a time
-      const int u = t0 + lane < n_t ? item_tiles<BN>(p, s, t0 + lane) + p.extra : 0;
-      unsigned long long x = u;
+      const unsigned int u = t0 + lane < n_t ? item_tiles<BN>(p, s, t0 + lane) + p.extra : 0;
+      unsigned int x = u;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+        const unsigned int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
       const unsigned int over = __ballot_sync(0xffffffffu, x > off);
@@ -238,9 +257,8 @@ struct Walk {
       t = 0;
       if (++h == p.Hkv) {
         h = 0;
-        do {
-          s = seq_of(p, ++b, false);
-        } while (s.nq == 0);
+        do ++b; while (pre[b + 1] == pre[b]);
+        s = seq_of(p, b, false);
       }
     }
     tiles = item_tiles<BN>(p, s, t);
@@ -259,12 +277,12 @@ struct Walk {
   // the CTAs that hold the first and the last piece of the item
   __device__ __forceinline__ unsigned int first_cta(const Cut& cut) const {
     const unsigned int c = cut.cta_of(start);
-    return cut.bound(c + 1) - start <= static_cast<unsigned long long>(p.extra) ? c + 1 : c;
+    return cut.bound(c + 1) - start <= static_cast<unsigned int>(p.extra) ? c + 1 : c;
   }
   __device__ __forceinline__ unsigned int last_cta(const Cut& cut) const {
-    const unsigned long long e = start + tiles + p.extra;
+    const unsigned int e = start + tiles + p.extra;
     const unsigned int c = cut.cta_of(e - 1);
-    return e - cut.bound(c) <= static_cast<unsigned long long>(p.extra) ? c - 1 : c;
+    return e - cut.bound(c) <= static_cast<unsigned int>(p.extra) ? c - 1 : c;
   }
 };
 
@@ -319,6 +337,23 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
+
+// Launches fn as a programmatic dependent of the stream's previous kernel: its CTAs may start while that one drains, and
+// wait (pdl_wait) before they touch global memory.
+template <typename... P, typename... A>
+int launch_pdl(void (*fn)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, const char* what, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, fn, args...), what);
+}
 
 inline int log2_of(int v) {
   int s = 0;

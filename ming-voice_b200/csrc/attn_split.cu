@@ -43,8 +43,8 @@ struct Cfg {
   static constexpr int oM = oQ + (D / 16) * NT * 32 * 8;
   static constexpr int oL = oM + kWarps * kRows * 4;
   static constexpr int oPre = oL + kWarps * kRows * 4;
-  static constexpr int oTmp = oPre + (kMaxB + 1) * 8;
-  static constexpr int oBar = oTmp + 32 * 8;
+  static constexpr int oTmp = oPre + (kMaxB + 4) * 4;
+  static constexpr int oBar = oTmp + 32 * 4;
   static constexpr int oFlag = oBar + 2 * kStages * 8;
   static constexpr int kSmem = oFlag + 16 + 1024;
   static_assert(kSmem <= 232448, "shared memory");
@@ -112,8 +112,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   uint2* sQ = reinterpret_cast<uint2*>(smem + C::oQ);
   float* sM = reinterpret_cast<float*>(smem + C::oM);
   float* sL = reinterpret_cast<float*>(smem + C::oL);
-  unsigned long long* pre = reinterpret_cast<unsigned long long*>(smem + C::oPre);
-  unsigned long long* tmp = reinterpret_cast<unsigned long long*>(smem + C::oTmp);
+  unsigned int* pre = reinterpret_cast<unsigned int*>(smem + C::oPre);
+  unsigned int* tmp = reinterpret_cast<unsigned int*>(smem + C::oTmp);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBar);
   uint64_t* empty = full + NS;
   volatile int* flag = reinterpret_cast<volatile int*>(smem + C::oFlag);
@@ -129,8 +129,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     tc::prefetch_tmap(&tmK);
     tc::prefetch_tmap(&tmV);
   }
+  pdl_launch_dependents();
+  pdl_wait();
   build_schedule<kBN>(p, pre, tmp);  // its barriers also publish the mbarriers
-  const unsigned long long W = pre[p.B];
+  const unsigned int W = pre[p.B];
   if (W == 0) return;
   const Cut cut(p, W, gridDim.x);
   Walk<kBN> wk(p, pre, cut, blockIdx.x);
@@ -483,10 +485,9 @@ int launch_split(const Problem& p, const Source& src, bool bf16, int grid, cudaS
   const int rc = make_kv_maps(&mk, &mv_, src, p.Hkv, D, bf16, box, D / 64);
   if (rc != MV_OK) return rc;
   auto fn = bf16 ? split_kernel<D, NT, true> : split_kernel<D, NT, false>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attention split)");
-  fn<<<grid, C::kThreads, C::kSmem, st>>>(mk, mv_, p, box);
-  return cuda_status(cudaGetLastError(), "attention split launch");
+  return launch_pdl(fn, dim3(grid), C::kThreads, C::kSmem, st, "attention split launch", mk, mv_, p, box);
 }
 
 }  // namespace

@@ -46,11 +46,13 @@ struct Cfg {
   static constexpr int oK = 2 * kQ;
   static constexpr int oV = oK + kSlots * kTile;
   static constexpr int oPre = oV + kSlots * kTile;
-  static constexpr int oTmp = oPre + (kMaxB + 1) * 8;
-  static constexpr int oBar = oTmp + 32 * 8;
+  static constexpr int oTmp = oPre + (kMaxB + 4) * 4;
+  static constexpr int oBar = oTmp + 32 * 4;
   static constexpr int kBars = 4 * kSlots + 2 + 10 + 1;
   static constexpr int oTmem = oBar + kBars * 8;
-  static constexpr int kSmem = oTmem + 16 + 1024;
+  static constexpr int oOut = (oTmem + 31) / 16 * 16;  // a buffer per softmax warp: 32 rows of 64 B, 80 B apart
+  static constexpr int kOutWarp = 32 * 80;
+  static constexpr int kSmem = oOut + 8 * kOutWarp + 1024;
   static_assert(kSmem <= 232448, "shared memory");
   static constexpr bool kEarly = D == 64;  // P has columns of its own
   static constexpr int kIssuers = kEarly ? 2 : 1;
@@ -165,8 +167,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* kring = smem + C::oK;
   uint8_t* vring = smem + C::oV;
-  unsigned long long* pre = reinterpret_cast<unsigned long long*>(smem + C::oPre);
-  unsigned long long* tmp = reinterpret_cast<unsigned long long*>(smem + C::oTmp);
+  unsigned int* pre = reinterpret_cast<unsigned int*>(smem + C::oPre);
+  unsigned int* tmp = reinterpret_cast<unsigned int*>(smem + C::oTmp);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::oBar);
   uint64_t* k_empty = k_full + NS;
   uint64_t* v_full = k_empty + NS;
@@ -218,10 +220,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_proxy_async_smem();
   }
   tc::fence_before_sync();
+  pdl_launch_dependents();
+  pdl_wait();
   build_schedule<kBN>(p, pre, tmp);
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  const unsigned long long W = pre[p.B];
+  const unsigned int W = pre[p.B];
   const Cut cut(p, W, gridDim.x);
 
   if (warp < 4) {
@@ -526,6 +530,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int head = wk.h * p.G + my_head;
       const bool sees = lim > 0;
       const float inv = sees ? 1.f / l : 0.f;
+      // Output rows go through shared memory 64 B at a time: from registers, a row per lane, every store would touch 32
+      // lines; so it touches 8. Lane x stores 16 B of rows x / 4 + 8 i of the warp's.
+      const long long off = live ? row * p.o_st + head * p.o_sh : -1;
+      uint8_t* buf = smem + C::oOut + (warp - 4) * C::kOutWarp;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -536,9 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0u;
         }
-        if (!live) continue;
         if (whole) {
-          uint4* dst = reinterpret_cast<uint4*>(p.out + row * p.o_st + head * p.o_sh + c * 32);
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             uint32_t w[4];
@@ -546,14 +552,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 4; ++e)
               w[e] = sees ? pack2<BF16>(__uint_as_float(o[v * 8 + 2 * e]) * inv, __uint_as_float(o[v * 8 + 2 * e + 1]) * inv)
                           : 0u;
-            dst[v] = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(buf + lane * 80 + v * 16) = make_uint4(w[0], w[1], w[2], w[3]);
           }
+          __syncwarp();
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int x = v * 8 + (lane >> 2);
+            const long long to = __shfl_sync(0xffffffffu, off, x);
+            const uint4 w = *reinterpret_cast<const uint4*>(buf + x * 80 + (lane & 3) * 16);
+            if (to >= 0) *reinterpret_cast<uint4*>(p.out + to + c * 32 + (lane & 3) * 8) = w;
+          }
+          __syncwarp();
         } else {
-          float4* dst = reinterpret_cast<float4*>(part + (t * kM + r) * D + c * 32);
+          // a piece is [4 values][row]: neighbouring lanes write neighbouring 16 B
+          float4* dst = reinterpret_cast<float4*>(part) + c * 8 * 256 + t * kM + r;
 #pragma unroll
           for (int v = 0; v < 8; ++v)
-            dst[v] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]), __uint_as_float(o[4 * v + 2]),
-                                 __uint_as_float(o[4 * v + 3]));
+            dst[v * 256] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]),
+                                       __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
         }
       }
       if (live) {
@@ -577,68 +593,70 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the pieces of the item that starts in CTA blockIdx.x's range and ends in a later one's: rows blockIdx.y * 32 ..
-// + 31 of its 256, weights 2^(m_piece - M), pieces in CTA order.
+// + 31 of its 256, a lane each, D / 8 values per warp; weights 2^(m_piece - M), pieces in CTA order.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) combine_kernel(const Problem p, const CutItem* __restrict__ cuts) {
-  __shared__ float sW[32][kMaxCtas + 1];
-  __shared__ float sM[32], sL[32];
+  pdl_wait();
   const CutItem c = cuts[blockIdx.x];
   if (c.n <= 1) return;
-  const int half_tok = p.tok / 2, rows_used = half_tok * p.G;
-  const int R0 = blockIdx.y * 32;
-  const int t = R0 / kM;
-  if (t * half_tok >= c.ntok) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int half_tok = p.tok / 2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int R = blockIdx.y * 32 + lane, t = R / kM, r = R % kM;
+  const int tok = t * half_tok + r / p.G;
+  if (r >= half_tok * p.G || tok >= c.ntok) return;
   constexpr size_t kPiece = 256 * (128 + 2);
+  constexpr int kVec = D / 32;                 // float4 per lane
+  constexpr int kAhead = 16 / kVec;            // pieces read at a time
   // the first piece is CTA blockIdx.x's last (slot 1), the others are their CTAs' first (slot 0)
   auto piece = [&](int i) { return p.parts + (static_cast<size_t>(blockIdx.x + i) * 2 + (i == 0)) * kPiece; };
-  auto live = [&](int R) { return R % kM < rows_used && t * half_tok + (R % kM) / p.G < c.ntok; };
-  for (int q = warp; q < 32; q += 8) {
-    const int R = R0 + q;
-    if (!live(R)) continue;
-    float M = -INFINITY;
-    for (int i = lane; i < c.n; i += 32) {
-      const float* pc = piece(i) + 256 * D;
-      if (pc[256 + R] != 0.f) M = fmaxf(M, pc[R]);
-    }
+  float M = -INFINITY, L = 0.f;
+  float4 acc[kVec];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float L = 0.f;
-    for (int i = lane; i < c.n; i += 32) {
-      const float* pc = piece(i) + 256 * D;
-      const float lw = pc[256 + R];
-      const float f = lw != 0.f ? exp2_approx(pc[R] - M) : 0.f;  // a piece without a visible key counts for nothing
-      if (lw != 0.f) L += f * lw;
-      sW[q][i] = f;
+  for (int v = 0; v < kVec; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < c.n; i0 += kAhead) {
+    float pm[kAhead], pl[kAhead];
+    float4 pv[kAhead][kVec];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float* pc = piece(min(i0 + i, c.n - 1));
+      pm[i] = pc[256 * D + R];
+      pl[i] = i0 + i < c.n ? pc[256 * D + 256 + R] : 0.f;
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) pv[i][v] = reinterpret_cast<const float4*>(pc)[(warp * kVec + v) * 256 + R];
     }
-    L = warp_sum(L);
-    if (lane == 0) {
-      sM[q] = M;
-      sL[q] = L;
+    float Mn = M;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (pl[i] != 0.f) Mn = fmaxf(Mn, pm[i]);  // a piece without a visible key counts for nothing
+    const float a = L != 0.f ? exp2_approx(M - Mn) : 0.f;
+    M = Mn;
+    L *= a;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) acc[v].x *= a, acc[v].y *= a, acc[v].z *= a, acc[v].w *= a;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (pl[i] == 0.f) continue;
+      const float f = exp2_approx(pm[i] - M);
+      L += f * pl[i];
+#pragma unroll
+      for (int v = 0; v < kVec; ++v)
+        acc[v].x += f * pv[i][v].x, acc[v].y += f * pv[i][v].y, acc[v].z += f * pv[i][v].z, acc[v].w += f * pv[i][v].w;
     }
   }
-  __syncthreads();
-  constexpr int kVecs = D / 4;
-  for (int e = threadIdx.x; e < 32 * kVecs; e += 256) {
-    const int q = e / kVecs, d = (e % kVecs) * 4, R = R0 + q;
-    if (!live(R)) continue;
-    const int tok = t * half_tok + (R % kM) / p.G, head = c.h * p.G + (R % kM) % p.G;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < c.n; ++i) {
-      const float f = sW[q][i];
-      if (f == 0.f) continue;
-      const float4 v = *reinterpret_cast<const float4*>(piece(i) + R * D + d);
-      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-    }
-    const bool sees = tok >= c.first;
-    const float inv = 1.f / sL[q];
-    const long long row = c.row0 + tok;
-    uint2 w = make_uint2(0u, 0u);
-    if (sees) w = make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
-    *reinterpret_cast<uint2*>(p.out + row * p.o_st + head * p.o_sh + d) = w;
-    if (p.lse != nullptr && d == 0) p.lse[row * p.Hq + head] = sees ? sM[q] * kLn2 + logf(sL[q]) : -INFINITY;
+  const bool sees = tok >= c.first;
+  const float inv = 1.f / L;
+  const long long row = c.row0 + tok;
+  const int head = c.h * p.G + r % p.G;
+  uint16_t* dst = p.out + row * p.o_st + head * p.o_sh + warp * (D / 8);
+#pragma unroll
+  for (int v = 0; v < kVec; v += 2) {
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    if (sees)
+      w = make_uint4(pack2<BF16>(acc[v].x * inv, acc[v].y * inv), pack2<BF16>(acc[v].z * inv, acc[v].w * inv),
+                     pack2<BF16>(acc[v + 1].x * inv, acc[v + 1].y * inv),
+                     pack2<BF16>(acc[v + 1].z * inv, acc[v + 1].w * inv));
+    *reinterpret_cast<uint4*>(dst + v * 4) = w;
   }
+  if (p.lse != nullptr && warp == 0) p.lse[row * p.Hq + head] = sees ? M * kLn2 + logf(L) : -INFINITY;
 }
 
 template <int D, bool BF16>
@@ -650,12 +668,12 @@ int launch_tile(const Problem& p, const Source& src, int grid, CutItem* cuts, cu
   if (rc == MV_OK) rc = make_q_map(&mq, p, D, BF16, p.tok / 2);
   if (rc != MV_OK) return rc;
   auto fn = tile_kernel<D, BF16>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attention tile)");
-  fn<<<grid, kThreads, C::kSmem, st>>>(mq, mk, mv_, p, box, cuts);
-  if ((e = cudaGetLastError()) != cudaSuccess) return cuda_status(e, "attention tile launch");
-  combine_kernel<D, BF16><<<dim3(grid, 8), 256, 0, st>>>(p, cuts);
-  return cuda_status(cudaGetLastError(), "attention combine launch");
+  rc = launch_pdl(fn, dim3(grid), kThreads, C::kSmem, st, "attention tile launch", mq, mk, mv_, p, box, cuts);
+  if (rc != MV_OK) return rc;
+  return launch_pdl(combine_kernel<D, BF16>, dim3(grid, 8), 256, 0, st, "attention combine launch", p,
+                    static_cast<const CutItem*>(cuts));
 }
 
 }  // namespace

@@ -71,6 +71,8 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const AppendArgs a) {
   constexpr int U = D / 16, HL = 32 / U;
   const int lane = threadIdx.x & 31;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 5);
+  pdl_launch_dependents();
+  pdl_wait();
   if (t >= a.T) return;
   const int u = lane % U;
   const int nrot = a.rot / 16;
@@ -157,10 +159,10 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const AppendArgs a) {
 }
 
 template <int D, bool BF16>
-void launch(const AppendArgs& a, cudaStream_t st) {
+int launch(const AppendArgs& a, cudaStream_t st) {
   constexpr int per_warp = 32 / (D / 16) * kBatch;
   const dim3 grid((a.T + 3) / 4, (a.Hq + 2 * a.Hkv + per_warp - 1) / per_warp);
-  kv_append_kernel<D, BF16><<<grid, 128, 0, st>>>(a);
+  return attn::launch_pdl(kv_append_kernel<D, BF16>, grid, 128, 0, st, "mv_kv_append launch", a);
 }
 
 }  // namespace
@@ -214,9 +216,6 @@ extern "C" int mv_kv_append(const mv_kv_append_args* x, void* workspace, size_t 
   a.ws = static_cast<WsHeader*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = c->dtype == MV_BF16;
-  if (D == 128)
-    bf ? launch<128, true>(a, st) : launch<128, false>(a, st);
-  else
-    bf ? launch<64, true>(a, st) : launch<64, false>(a, st);
-  return cuda_status(cudaGetLastError(), "mv_kv_append launch");
+  if (D == 128) return bf ? launch<128, true>(a, st) : launch<128, false>(a, st);
+  return bf ? launch<64, true>(a, st) : launch<64, false>(a, st);
 }
