@@ -94,7 +94,7 @@ int run_tile(Problem& p, const Source& src, int D, bool bf16, int grid, cudaStre
 
 namespace {
 
-constexpr size_t kCountersBytes = 1024 + kMaxCtas * 32;                     // arrival counters, cut items
+constexpr size_t kCutsBytes = (kMaxCtas * sizeof(CutItem) + 255) / 256 * 256;
 constexpr size_t kPartsBytes = size_t(kMaxCtas) * 2 * 256 * (128 + 2) * 4;  // two pieces of 256 rows per CTA
 
 // The shared part of the two entry points: `src` describes the keys, D / dtype / Hkv their heads.
@@ -123,8 +123,8 @@ int run(const mv_attention_args* a, const Source& src, int D, int dtype, int Hkv
   }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.ws = reinterpret_cast<WsHeader*>(ws);
-  p.counters = reinterpret_cast<unsigned int*>(ws + kWsHeaderBytes);
-  p.parts = reinterpret_cast<float*>(ws + kWsHeaderBytes + kCountersBytes);
+  p.cuts = reinterpret_cast<CutItem*>(ws + kWsHeaderBytes);
+  p.parts = reinterpret_cast<float*>(ws + kWsHeaderBytes + kCutsBytes);
   const bool bf16 = dtype == MV_BF16;
   int grid = num_sms();
   if (grid > kMaxCtas) grid = kMaxCtas;
@@ -152,7 +152,7 @@ int run(const mv_attention_args* a, const Source& src, int D, int dtype, int Hkv
 using namespace mv;
 using namespace mv::attn;
 
-extern "C" size_t mv_attention_workspace_bytes(void) { return kWsHeaderBytes + kCountersBytes + kPartsBytes; }
+extern "C" size_t mv_attention_workspace_bytes(void) { return kWsHeaderBytes + kCutsBytes + kPartsBytes; }
 
 extern "C" int mv_paged_attention(const mv_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "mv_paged_attention";
@@ -171,7 +171,7 @@ extern "C" int mv_paged_attention(const mv_attention_args* a, void* workspace, s
     return fail(MV_ERR_INVALID, "%s: page table row stride %lld shorter than max_pages=%d", who, a->pt_stride,
                 a->max_pages);
   const Source src{c->k, c->v, c->k_st, c->k_sh, c->k_sp, c->v_st, c->v_sh, c->v_sp, c->page_size, c->num_pages,
-                   c->page_size};
+                   c->page_size, static_cast<long long>(a->max_pages) * c->page_size};
   return run(a, src, c->head_dim, c->dtype, c->n_kv_heads, workspace, workspace_bytes,
              static_cast<cudaStream_t>(stream), who);
 }
@@ -197,7 +197,7 @@ extern "C" int mv_prompt_attention(const mv_attention_args* a, void* workspace, 
     if (rc != MV_OK) return rc;
   }
   // without a key every row is empty and no copy runs: the maps then stand on one row of q
-  const Source src = a->Tk > 0 ? Source{a->k, a->v, a->k_st, a->k_sh, 0, a->v_st, a->v_sh, 0, a->Tk, 1, 128}
-                               : Source{a->q, a->q, D, D, 0, D, D, 0, 1, 1, 128};
+  const Source src = a->Tk > 0 ? Source{a->k, a->v, a->k_st, a->k_sh, 0, a->v_st, a->v_sh, 0, a->Tk, 1, 128, a->Tk}
+                               : Source{a->q, a->q, D, D, 0, D, D, 0, 1, 1, 128, 0};
   return run(a, src, D, a->dtype, a->Hkv, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), who);
 }

@@ -42,11 +42,23 @@ struct Problem {
   int causal;
   int extra;              // units an item counts besides its key tiles
   int min_share;          // least units worth a CTA of their own; more than 2 extra
+  bool can_cut;           // an item may have more than one tile, so that the joining kernel is needed
   float scale_log2;       // scale * log2(e): softmax in powers of two
   WsHeader* ws;
-  unsigned int* counters;  // [kMaxCtas] arrivals of the split item that starts in a CTA's range (left zeroed)
-  float* parts;            // [kMaxCtas][2] pieces
+  struct CutItem* cuts;  // [kMaxCtas]
+  float* parts;          // [kMaxCtas][2] pieces: slot 1 starts its item, slot 0 starts inside it
 };
+
+// What the joining kernel needs of a cut item, left by the CTA whose range holds its start; written by every CTA.
+struct CutItem {
+  int n;         // pieces: this CTA's and those of the n - 1 next (0: no item is cut behind its start here)
+  int row0;      // first token's row
+  int ntok;      // tokens
+  int h;         // key head
+  int first;     // first token that sees a key
+  int pad[3];
+};
+static_assert(sizeof(CutItem) == 32, "");
 
 struct Seq {
   int q0, nq, k0, n;  // first query row, queries, first key row (packed prompts), keys
@@ -274,10 +286,10 @@ struct Walk {
   __device__ __forceinline__ int tok0() const { return t * p.tok; }
   __device__ __forceinline__ int ntok() const { return min(p.tok, s.nq - t * p.tok); }
   __device__ __forceinline__ int kend() const { return keys_seen(p, s, min(s.nq, (t + 1) * p.tok)); }
-  // the CTAs that hold the first and the last piece of the item
-  __device__ __forceinline__ unsigned int first_cta(const Cut& cut) const {
-    const unsigned int c = cut.cta_of(start);
-    return cut.bound(c + 1) - start <= static_cast<unsigned int>(p.extra) ? c + 1 : c;
+  // of a cut item, seen by CTA c that holds its first piece
+  __device__ __forceinline__ CutItem cut_item(const Cut& cut, unsigned int c) const {
+    return CutItem{static_cast<int>(last_cta(cut) - c) + 1, s.q0 + tok0(), ntok(), h,
+                   p.causal ? max(0, s.nq - s.n - tok0()) : 0, {0, 0, 0}};
   }
   __device__ __forceinline__ unsigned int last_cta(const Cut& cut) const {
     const unsigned int e = start + tiles + p.extra;
@@ -371,6 +383,7 @@ struct Source {
   const void *k, *v;
   long long k_st, k_sh, k_sp, v_st, v_sh, v_sp;
   int tokens, pages, box;
+  long long max_keys;  // no sequence has more
 };
 
 // 5-D maps over keys and values [page][head][64-value part of a head][token][64 values], 128-byte swizzle, box of

@@ -12,7 +12,7 @@
 // Split: one CTA per SM takes an equal share of all key tiles (attn_common.cuh). Producer warps keep a ring of
 // key tiles filled by TMA (a box per page and 64 values, 128-byte swizzle); each of the consumer warps takes whole
 // tiles in turn with its own maximum, sum and output in registers, so the warps meet only at the end of a piece.
-// Pieces of an item that ranges cut are joined by the CTA that arrives last, in CTA order.
+// Pieces of an item that ranges cut go to the workspace and join_kernel joins them in CTA order.
 #include "attn_common.cuh"
 
 namespace mv {
@@ -45,8 +45,7 @@ struct Cfg {
   static constexpr int oPre = oL + kWarps * kRows * 4;
   static constexpr int oTmp = oPre + (kMaxB + 4) * 4;
   static constexpr int oBar = oTmp + 32 * 4;
-  static constexpr int oFlag = oBar + 2 * kStages * 8;
-  static constexpr int kSmem = oFlag + 16 + 1024;
+  static constexpr int kSmem = oBar + 2 * kStages * 8 + 1024;
   static_assert(kSmem <= 232448, "shared memory");
 };
 
@@ -86,18 +85,25 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-// out and lse of values d .. d + 3 of the item's row r from its joined sums
-template <bool BF16, int BN>
-__device__ __forceinline__ void store_row(const Problem& p, const Walk<BN>& wk, int r, int d, const float4& acc, float M,
-                                          float L) {
-  const int i = r / p.G, h = wk.h * p.G + r % p.G;
-  const bool sees = keys_seen(p, wk.s, wk.tok0() + i + 1) > 0;
-  const long long row = wk.s.q0 + wk.tok0() + i;
+// out and lse of values d .. d + 3 of a row from its joined sums
+template <bool BF16>
+__device__ __forceinline__ void store_row(const Problem& p, long long row, int head, int d, bool sees, const float4& acc,
+                                          float M, float L) {
   const float inv = 1.f / L;
   uint2 v = make_uint2(0u, 0u);
   if (sees) v = make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
-  *reinterpret_cast<uint2*>(p.out + row * p.o_st + h * p.o_sh + d) = v;
-  if (p.lse != nullptr && d == 0) p.lse[row * p.Hq + h] = sees ? M * kLn2 + logf(L) : -INFINITY;
+  *reinterpret_cast<uint2*>(p.out + row * p.o_st + head * p.o_sh + d) = v;
+  if (p.lse != nullptr && d == 0) p.lse[row * p.Hq + head] = sees ? M * kLn2 + logf(L) : -INFINITY;
+}
+
+// Joins parts of a row: (M, L, acc) and (m, l, v), weights 2^(m - M); a part without a visible key has sum 0.
+__device__ __forceinline__ void join(float& M, float& L, float4& acc, float m, float l, const float4& v) {
+  if (l == 0.f) return;
+  const float Mn = fmaxf(M, m);
+  const float a = L != 0.f ? exp2_approx(M - Mn) : 0.f, f = exp2_approx(m - Mn);
+  M = Mn;
+  L = L * a + f * l;
+  acc.x = acc.x * a + f * v.x, acc.y = acc.y * a + f * v.y, acc.z = acc.z * a + f * v.z, acc.w = acc.w * a + f * v.w;
 }
 
 template <int D, int NT, bool BF16>
@@ -116,7 +122,6 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   unsigned int* tmp = reinterpret_cast<unsigned int*>(smem + C::oTmp);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::oBar);
   uint64_t* empty = full + NS;
-  volatile int* flag = reinterpret_cast<volatile int*>(smem + C::oFlag);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int box_shift = 31 - __clz(box);
@@ -133,7 +138,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   pdl_wait();
   build_schedule<kBN>(p, pre, tmp);  // its barriers also publish the mbarriers
   const unsigned int W = pre[p.B];
-  if (W == 0) return;
+  if (W == 0) {
+    if (threadIdx.x == 0) p.cuts[blockIdx.x].n = 0;
+    return;
+  }
   const Cut cut(p, W, gridDim.x);
   Walk<kBN> wk(p, pre, cut, blockIdx.x);
 
@@ -192,6 +200,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   }
   int it = 0;      // tiles of the CTA so far
   bool ok = true;  // a wait that ran out: no more tiles, but every barrier is still met
+  CutItem mine{};
   for (; wk.more(); wk.next()) {
     const int kend = wk.kend(), ntok = wk.ntok(), rows = ntok * p.G, first = wk.i0;
     const int i1 = min(wk.i1, (kend + kBN - 1) / kBN);
@@ -404,7 +413,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         }
       }
       if (whole) {
-        store_row<BF16>(p, wk, r, d, acc, M, L);
+        const int i = r / p.G;
+        store_row<BF16>(p, wk.s.q0 + wk.tok0() + i, wk.h * p.G + r % p.G, d, keys_seen(p, wk.s, wk.tok0() + i + 1) > 0,
+                        acc, M, L);
       } else {
         *reinterpret_cast<float4*>(part + r * D + d) = acc;
         if (d == 0) {
@@ -413,81 +424,74 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
         }
       }
     }
-    if (!whole) {
-      // the CTA that leaves the item's last missing piece joins them all
-      const unsigned int c0 = wk.first_cta(cut);
-      const int n = static_cast<int>(wk.last_cta(cut) - c0) + 1;
-      __threadfence();
-      named_bar(1, NTH);
-      if (tid == 0) {
-        const bool last = atomicAdd(&p.counters[c0], 1u) == static_cast<unsigned int>(n - 1);
-        if (last) p.counters[c0] = 0u;
-        __threadfence();
-        *flag = last;
-      }
-      named_bar(1, NTH);
-      if (*flag) {
-        // piece 0 is CTA c0's last (slot 1), the others are their CTAs' first (slot 0). Many pieces are a chain of L2
-        // latencies: the next kAhead pieces are on their way while kAhead are added.
-        constexpr int kAhead = NT <= 2 ? 8 : 4;
-        const float* base_part = p.parts + static_cast<size_t>(c0) * 2 * C::kPiece;
-        for (int e = tid; e < rows * kVecs; e += NTH) {
-          const int r = e / kVecs, d = (e % kVecs) * 4;
-          float M = -INFINITY, L = 0.f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          float pm[kAhead], pl[kAhead], nm[kAhead], nl[kAhead];
-          float4 pv[kAhead], nv[kAhead];
-          auto read = [&](int i0, float (&m_)[kAhead], float (&l_)[kAhead], float4 (&v_)[kAhead]) {
+    if (!whole && first == 0) mine = wk.cut_item(cut, blockIdx.x);
+    named_bar(1, NTH);  // the merge buffer and Q are free again
+  }
+  if (tid == 0) p.cuts[blockIdx.x] = mine;
+}
+
+// Joins the pieces of the item that starts in CTA blockIdx.x's range and ends in a later one's, rows blockIdx.y NT .. + NT - 1.
+// A few rows of many pieces (74 of one long sequence) are a chain of L2 latencies for one CTA (9 us for a single CTA that
+// did it all), so every row has 8 warps: warp w joins pieces w, w + 8, .. in order, then the warps' results are joined.
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(256) join_kernel(const Problem p) {
+  constexpr int R = 8 * NT, kPiece = R * (D + 2), kLanes = D / 4, kAhead = 10;
+  __shared__ float sM[8], sL[8];
+  __shared__ float4 sV[8][kLanes];
+  pdl_wait();
+  const CutItem c = p.cuts[blockIdx.x];
+  if (c.n <= 1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = blockIdx.y * NT; r < blockIdx.y * NT + NT && r < c.ntok * p.G; ++r) {
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = warp; i0 < c.n; i0 += 8 * kAhead) {
+      float m[kAhead], l[kAhead];
+      float4 v[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-              const int k = min(i0 + i, n - 1);
-              const float* pc = base_part + (k == 0 ? C::kPiece : k * 2 * C::kPiece);
-              m_[i] = __ldcg(pc + R * D + r);
-              l_[i] = __ldcg(pc + R * D + R + r);
-              v_[i] = __ldcg(reinterpret_cast<const float4*>(pc + r * D + d));
-              if (i0 + i >= n) l_[i] = 0.f;
-            }
-          };
-          read(0, nm, nl, nv);
-          for (int i0 = 0; i0 < n; i0 += kAhead) {
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) pm[i] = nm[i], pl[i] = nl[i], pv[i] = nv[i];
-            if (i0 + kAhead < n) read(i0 + kAhead, nm, nl, nv);
-            float Mn = M;
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-              if (pl[i] != 0.f) Mn = fmaxf(Mn, pm[i]);  // a piece without a visible key has sum 0
-            const float a = L != 0.f ? exp2_approx(M - Mn) : 0.f;
-            M = Mn;
-            L *= a;
-            acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-              if (pl[i] != 0.f) {
-                const float f = exp2_approx(pm[i] - M);
-                L += f * pl[i];
-                acc.x += f * pv[i].x, acc.y += f * pv[i].y, acc.z += f * pv[i].z, acc.w += f * pv[i].w;
-              }
-          }
-          store_row<BF16>(p, wk, r, d, acc, M, L);
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = i0 + 8 * k;
+        l[k] = 0.f;
+        if (i < c.n) {
+          // the first piece is CTA blockIdx.x's last (slot 1), the others are their CTAs' first (slot 0)
+          const float* pc = p.parts + (static_cast<size_t>(blockIdx.x + i) * 2 + (i == 0)) * kPiece;
+          m[k] = pc[R * D + r];
+          l[k] = pc[R * D + R + r];
+          if (lane < kLanes) v[k] = reinterpret_cast<const float4*>(pc + r * D)[lane];
         }
       }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (i0 + 8 * k < c.n) join(M, L, acc, m[k], l[k], v[k]);
     }
-    named_bar(1, NTH);  // the merge buffer and Q are free again
+    if (lane == 0) sM[warp] = M, sL[warp] = L;
+    if (lane < kLanes) sV[warp][lane] = acc;
+    __syncthreads();
+    if (warp == 0 && lane < kLanes) {
+#pragma unroll
+      for (int w = 1; w < 8; ++w) join(M, L, acc, sM[w], sL[w], sV[w][lane]);
+      const int i = r / p.G;
+      store_row<BF16>(p, c.row0 + i, c.h * p.G + r % p.G, lane * 4, i >= c.first, acc, M, L);
+    }
+    __syncthreads();
   }
 }
 
 template <int D, int NT>
-int launch_split(const Problem& p, const Source& src, bool bf16, int grid, cudaStream_t st) {
+int launch_split(Problem& p, const Source& src, bool bf16, int grid, cudaStream_t st) {
   using C = Cfg<D, NT>;
   CUtensorMap mk, mv_;
   const int box = src.box < C::kBN ? src.box : C::kBN;
+  p.can_cut = src.max_keys > C::kBN;
   const int rc = make_kv_maps(&mk, &mv_, src, p.Hkv, D, bf16, box, D / 64);
   if (rc != MV_OK) return rc;
   auto fn = bf16 ? split_kernel<D, NT, true> : split_kernel<D, NT, false>;
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attention split)");
-  return launch_pdl(fn, dim3(grid), C::kThreads, C::kSmem, st, "attention split launch", mk, mv_, p, box);
+  const int rc2 = launch_pdl(fn, dim3(grid), C::kThreads, C::kSmem, st, "attention split launch", mk, mv_, p, box);
+  if (rc2 != MV_OK || !p.can_cut) return rc2;
+  return launch_pdl(bf16 ? join_kernel<D, NT, true> : join_kernel<D, NT, false>, dim3(grid, 8), 256, 0, st,
+                    "attention join launch", p);
 }
 
 }  // namespace

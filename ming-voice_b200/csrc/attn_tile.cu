@@ -64,17 +64,6 @@ struct Cfg {
   }
 };
 
-// What combine_kernel needs of a cut item, left by the CTA whose range holds its start.
-struct CutItem {
-  int n;         // pieces (0: none)
-  int row0;      // first token's row
-  int ntok;      // tokens
-  int h;         // key head
-  int first;     // first token that sees a key
-  int pad[3];
-};
-static_assert(sizeof(CutItem) == 32, "");
-
 // D[tmem] (+)= A[tmem] * B[smem], 16-bit operands, fp32 accumulation; issued by one thread.
 __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
                                        uint32_t accumulate) {
@@ -160,7 +149,7 @@ struct Tiles {
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, const Problem p, int box, CutItem* __restrict__ cuts) {
+                const __grid_constant__ CUtensorMap tmV, const Problem p, int box) {
   using C = Cfg<D>;
   constexpr int NS = C::kSlots, kHalves = D / 64, kHalfBytes = kBN * 128;
   extern __shared__ uint8_t smem_raw[];
@@ -433,13 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Tiles tl(p, wk, half_tok);
       const int ntok = wk.ntok(), i0 = wk.i0, i1 = tl.end_of[t];
       const bool whole = wk.whole();
-      if (!whole && i0 == 0) {
-        mine.n = static_cast<int>(wk.last_cta(cut) - blockIdx.x) + 1;
-        mine.row0 = wk.s.q0 + wk.tok0();
-        mine.ntok = ntok;
-        mine.h = wk.h;
-        mine.first = p.causal ? max(0, wk.s.nq - wk.s.n - wk.tok0()) : 0;
-      }
+      if (!whole && i0 == 0) mine = wk.cut_item(cut, blockIdx.x);
       if (t == 1 && ntok <= half_tok) continue;
       const bool live = r < rows_used && my_tok < ntok;
       // keys the row sees; rows that are not there see what the last one does
@@ -582,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc::fence_before_sync();  // the accumulator is read before the next item's first product is allowed
     }
-    if (threadIdx.x == 128) cuts[blockIdx.x] = mine;
+    if (threadIdx.x == 128) p.cuts[blockIdx.x] = mine;
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -595,9 +578,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the pieces of the item that starts in CTA blockIdx.x's range and ends in a later one's: rows blockIdx.y * 32 ..
 // + 31 of its 256, a lane each, D / 8 values per warp; weights 2^(m_piece - M), pieces in CTA order.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) combine_kernel(const Problem p, const CutItem* __restrict__ cuts) {
+__global__ void __launch_bounds__(256) combine_kernel(const Problem p) {
   pdl_wait();
-  const CutItem c = cuts[blockIdx.x];
+  const CutItem c = p.cuts[blockIdx.x];
   if (c.n <= 1) return;
   const int half_tok = p.tok / 2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int R = blockIdx.y * 32 + lane, t = R / kM, r = R % kM;
@@ -660,7 +643,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const Problem p, const Cut
 }
 
 template <int D, bool BF16>
-int launch_tile(const Problem& p, const Source& src, int grid, CutItem* cuts, cudaStream_t st) {
+int launch_tile(const Problem& p, const Source& src, int grid, cudaStream_t st) {
   using C = Cfg<D>;
   CUtensorMap mq, mk, mv_;
   const int box = src.box < kBN ? src.box : kBN;
@@ -670,10 +653,9 @@ int launch_tile(const Problem& p, const Source& src, int grid, CutItem* cuts, cu
   auto fn = tile_kernel<D, BF16>;
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attention tile)");
-  rc = launch_pdl(fn, dim3(grid), kThreads, C::kSmem, st, "attention tile launch", mq, mk, mv_, p, box, cuts);
-  if (rc != MV_OK) return rc;
-  return launch_pdl(combine_kernel<D, BF16>, dim3(grid, 8), 256, 0, st, "attention combine launch", p,
-                    static_cast<const CutItem*>(cuts));
+  rc = launch_pdl(fn, dim3(grid), kThreads, C::kSmem, st, "attention tile launch", mq, mk, mv_, p, box);
+  if (rc != MV_OK || !p.can_cut) return rc;
+  return launch_pdl(combine_kernel<D, BF16>, dim3(grid, 8), 256, 0, st, "attention combine launch", p);
 }
 
 }  // namespace
@@ -682,10 +664,10 @@ int run_tile(Problem& p, const Source& src, int D, bool bf16, int grid, cudaStre
   p.tok = 2 * (kM / p.G);
   p.extra = 2;
   p.min_share = 3;
-  CutItem* cuts = reinterpret_cast<CutItem*>(p.counters + 256);
+  p.can_cut = src.max_keys > kBN;
   if (D == 128)
-    return bf16 ? launch_tile<128, true>(p, src, grid, cuts, st) : launch_tile<128, false>(p, src, grid, cuts, st);
-  return bf16 ? launch_tile<64, true>(p, src, grid, cuts, st) : launch_tile<64, false>(p, src, grid, cuts, st);
+    return bf16 ? launch_tile<128, true>(p, src, grid, st) : launch_tile<128, false>(p, src, grid, st);
+  return bf16 ? launch_tile<64, true>(p, src, grid, st) : launch_tile<64, false>(p, src, grid, st);
 }
 
 }  // namespace attn
