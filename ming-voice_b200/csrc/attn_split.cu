@@ -500,8 +500,8 @@ int launch_split(Problem& p, const Source& src, bool bf16, int grid, cudaStream_
 int run_split(Problem& p, const Source& src, int D, bool bf16, int rows_hint, int grid, cudaStream_t st) {
   const int nt = rows_hint <= 8 && p.G <= 8 ? 1 : rows_hint <= 16 && p.G <= 16 ? 2 : 4;
   p.tok = 8 * nt / p.G;
-  p.extra = 4;
-  p.min_share = 12;
+  p.extra = 6;
+  p.min_share = 14;
   if (D == 128) {
     if (nt == 1) return launch_split<128, 1>(p, src, bf16, grid, st);
     if (nt == 2) return launch_split<128, 2>(p, src, bf16, grid, st);

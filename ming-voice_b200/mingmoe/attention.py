@@ -6,6 +6,9 @@ prompts (mv_kv_append, mv_paged_attention, mv_prompt_attention; formulas and rul
     o = paged_attention(q, cache, page_table, cu_seqlens, kv_lens, max_q=1)
 
 Token tensors are packed [T, heads, D] (any row and head stride): sequence b owns rows cu_seqlens[b]:cu_seqlens[b + 1].
+The calls read their arguments in C++ (csrc/attention_host.cpp) where these are as the kernels take them; the Python code
+below it refuses what does not fit and copies what only needs another layout.
+
 Lengths, bounds and page ids are int32 device tensors, read on the device: no call synchronises the host, and a
 captured graph serves whatever lengths its buffers hold at the replay.
 """
@@ -52,7 +55,8 @@ class PagedKV:
         c.k_sp, c.k_st, c.k_sh = k.stride()[:3]
         c.v_sp, c.v_st, c.v_sh = v.stride()[:3]
         self._c = c
-        self._ptr = C.addressof(c)
+        # what every call needs, read in one step
+        self._key = (C.addressof(c), k.device, k.get_device(), k.dtype, self.n_kv_heads, self.head_dim)
 
     @classmethod
     def empty(cls, num_pages, page_size, n_kv_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
@@ -60,50 +64,60 @@ class PagedKV:
         return cls(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
 
 
-def _rows(t, name, d, dtype, device):
-    """A [T, heads, d] operand as the kernels take it (copied only where its layout has no 16-byte vectors), its
-    shape and its strides."""
-    shape = t.shape
-    if len(shape) != 3 or shape[2] != d:
-        raise ValueError(f"{name} must be [T, heads, {d}], got {tuple(shape)}")
+def _fit(t, name, d, dtype, device):
+    """A [T, heads, d] operand that the kernels cannot take as it is: refused, or copied where only its layout has no
+    16-byte vectors."""
+    if t.ndim != 3 or t.shape[2] != d:
+        raise ValueError(f"{name} must be [T, heads, {d}], got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
     if t.device != device:
         raise RuntimeError(f"{name} is on {t.device}, expected {device}")
-    st, sh, s1 = strides = t.stride()
-    if s1 != 1 or (st | sh) & 7 or st < d or sh < d or t.data_ptr() & 15:
-        t = t.contiguous()
-        strides = t.stride()
-    return t, shape, strides
+    return t.contiguous()
 
 
-def _out(t, name, like, shape, dtype, device):
+def _rows(t, name, d, dtype, device, index):
+    """(operand, tokens, heads, token stride, head stride, address)"""
+    p, s = t.data_ptr(), t.stride()
+    if len(s) == 3:
+        st, sh, s1 = s
+        T, H, n = t.shape
+        if (s1 == 1 and n == d and t.dtype is dtype and t.get_device() == index and not (st | sh) & 7 and st >= d
+                and sh >= d and not p & 15):
+            return t, T, H, st, sh, p
+    t = _fit(t, name, d, dtype, device)
+    st, sh, _ = t.stride()
+    return t, t.shape[0], t.shape[1], st, sh, t.data_ptr()
+
+
+def _out(t, name, like, device):
+    """The result buffer: a new one, or the caller's. (buffer, token stride, head stride, address)"""
     if t is None:
         t = torch.empty_like(like)
-    elif t.shape != shape or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {device}")
-    strides = t.stride()
-    if strides[2] != 1:
+    elif t.shape != like.shape or t.dtype != like.dtype or t.device != device:
+        raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype} on {device}")
+    st, sh, s1 = t.stride()
+    if s1 != 1:
         raise ValueError(f"{name} needs a unit inner stride")
-    return t, strides
+    return t, st, sh, t.data_ptr()
 
 
-def _ints(t, name, device):
+def _ints(t, name, device, index):
     """Shape of an int32 index tensor."""
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32")
-    if t.device != device:
+    if t.get_device() != index:
         raise RuntimeError(f"{name} is on {t.device}, expected {device}")
     shape = t.shape
-    if len(shape) == 0 or (t.stride()[-1] != 1 and shape[-1] > 1):
+    if len(shape) == 0 or (shape[-1] > 1 and t.stride()[-1] != 1):
         raise ValueError(f"{name} needs a unit inner stride")
     return shape
 
 
-def _batch(page_table, cu_seqlens, kv_lens, device):
+def _batch(page_table, cu_seqlens, kv_lens, device, index):
     """(sequences, columns and row stride of the page table)"""
-    lens, cu, table = (_ints(kv_lens, "kv_lens", device), _ints(cu_seqlens, "cu_seqlens", device),
-                       _ints(page_table, "page_table", device))
+    lens, cu, table = (_ints(kv_lens, "kv_lens", device, index), _ints(cu_seqlens, "cu_seqlens", device, index),
+                       _ints(page_table, "page_table", device, index))
     B = lens[0]
     if len(lens) != 1 or len(cu) != 1 or cu[0] != B + 1 or len(table) != 2 or table[0] != B:
         raise ValueError(f"kv_lens [B], cu_seqlens [B + 1] and page_table [B, max_pages] do not agree: {tuple(lens)}, "
@@ -111,17 +125,35 @@ def _batch(page_table, cu_seqlens, kv_lens, device):
     return B, table[1], page_table.stride()[0]
 
 
-def _call(fn, args, device, what):
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    ws = _ws.get((device.index, stream))
+def _call(name, args, device, index):
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    ws = _ws.get((index, stream))
     if ws is None:
         buf = L.workspace("attention", L.lib().mv_attention_workspace_bytes(), device)
-        ws = _ws[(device.index, stream)] = (buf.data_ptr(), buf.numel())
-    rc = fn(args, ws[0], ws[1], stream)
+        ws = _ws[(index, stream)] = (buf.data_ptr(), buf.numel())
+        _host().workspace(index, stream, *ws)
+    rc = getattr(L.lib(), name)(args, ws[0], ws[1], stream)
     if rc:
-        L.check(rc, what)
+        L.check(rc, name)
 
 
+def _host():
+    """The C++ host module, bound to the loaded library's entry points."""
+    global _module
+    if _module is None:
+        try:
+            from . import _attention_host as m
+        except ImportError as e:
+            raise ImportError(f"mingmoe/_attention_host.so is missing or does not load ({e}): build it with "
+                              "`python ming-voice_b200/mingmoe/build.py` (or __graft_entry__.build())") from e
+        lib = L.lib()
+        m.bind(*(C.cast(f, C.c_void_p).value for f in (lib.mv_kv_append, lib.mv_paged_attention,
+                                                       lib.mv_prompt_attention)))
+        _module = m
+    return _module
+
+
+_module = None
 _ws: dict = {}  # (device, stream) -> address and size of the "attention" workspace (its size never changes)
 
 
@@ -134,40 +166,42 @@ def kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, *, q=None, q_out=Non
     cos_sin: fp32 [max_pos, rot_dim], a position's rot_dim / 2 cosines then its sines (rotation_table); None copies
     without rotating. rot_dim is a multiple of 16 up to D. Pairs are (i, i + rot_dim / 2), or (2i, 2i + 1) when
     `interleaved`. positions: int32 [T] rows of cos_sin, if not the cache positions. q_out may be q itself."""
-    dev, d, dtype = cache.device, cache.head_dim, cache.dtype
-    k, k_shape, ks = _rows(k, "k", d, dtype, dev)
-    v, v_shape, vs = _rows(v, "v", d, dtype, dev)
-    T = k_shape[0]
-    if k_shape[1] != cache.n_kv_heads or v_shape != k_shape:
-        raise ValueError(f"k and v must be [T, {cache.n_kv_heads}, {d}], got {tuple(k_shape)} / {tuple(v_shape)}")
-    B, max_pages, pt_stride = _batch(page_table, cu_seqlens, kv_lens, dev)
-    Hq = qp = qo = 0
-    qs = qos = (0, 0)
+    r = (_module or _host()).kv_append(cache._key[0], cache._key[2], k, v, page_table, cu_seqlens, kv_lens, q, q_out,
+                                       cos_sin, positions, interleaved)
+    if type(r) is int:
+        L.check(r, "kv_append")
+    if r is not NotImplemented:
+        return r
+    c_ptr, dev, index, dtype, n_kv, d = cache._key
+    k, T, H, k_st, k_sh, kp = _rows(k, "k", d, dtype, dev, index)
+    v, Tv, Hv, v_st, v_sh, vp = _rows(v, "v", d, dtype, dev, index)
+    if H != n_kv or Hv != n_kv or Tv != T:
+        raise ValueError(f"k and v must be [T, {n_kv}, {d}], got {tuple(k.shape)} / {tuple(v.shape)}")
+    B, max_pages, pt_stride = _batch(page_table, cu_seqlens, kv_lens, dev, index)
+    Hq = q_st = q_sh = qp = qo_st = qo_sh = qop = 0
     if q is not None:
-        q, q_shape, qs = _rows(q, "q", d, dtype, dev)
-        if q_shape[0] != T:
+        q, Tq, Hq, q_st, q_sh, qp = _rows(q, "q", d, dtype, dev, index)
+        if Tq != T:
             raise ValueError("q and k have different numbers of tokens")
-        Hq = q_shape[1]
-        q_out, qos = _out(q_out, "q_out", q, q_shape, dtype, dev)
-        qp, qo = q.data_ptr(), q_out.data_ptr()
+        q_out, qo_st, qo_sh, qop = _out(q_out, "q_out", q, dev)
     elif q_out is not None:
         raise ValueError("q_out without q")
     cs = cs_stride = max_pos = rot = pos = 0
     if cos_sin is not None:
-        if cos_sin.dtype != torch.float32 or cos_sin.ndim != 2 or cos_sin.device != dev:
+        if cos_sin.dtype is not torch.float32 or cos_sin.ndim != 2 or cos_sin.get_device() != index:
             raise TypeError(f"cos_sin must be fp32 [max_pos, rot_dim] on {dev}")
         cs_stride, inner = cos_sin.stride()
         if inner != 1:
             raise ValueError("cos_sin needs a unit inner stride")
         cs, (max_pos, rot) = cos_sin.data_ptr(), cos_sin.shape
     if positions is not None:
-        if tuple(_ints(positions, "positions", dev)) != (T,):
+        if tuple(_ints(positions, "positions", dev, index)) != (T,):
             raise ValueError(f"positions must be [{T}]")
         pos = positions.data_ptr()
-    _call(L.lib().mv_kv_append,
-          _APPEND.pack(cache._ptr, k.data_ptr(), v.data_ptr(), qp, qo, page_table.data_ptr(), cu_seqlens.data_ptr(),
-                       kv_lens.data_ptr(), pos, cs, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], qos[0], qos[1],
-                       pt_stride, cs_stride, T, B, Hq, max_pages, max_pos, rot, bool(interleaved), 0), dev, "kv_append")
+    _call("mv_kv_append",
+          _APPEND.pack(c_ptr, kp, vp, qp, qop, page_table.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), pos,
+                       cs, k_st, k_sh, v_st, v_sh, q_st, q_sh, qo_st, qo_sh, pt_stride, cs_stride, T, B, Hq, max_pages,
+                       max_pos, rot, bool(interleaved), 0), dev, index)
     return q_out
 
 
@@ -177,17 +211,22 @@ def paged_attention(q, cache, page_table, cu_seqlens, kv_lens, *, max_q=None, sc
     (kv_append): out [T, Hq, D], and with return_lse also lse [T, Hq] fp32 (ln of the sum of exp scores; -inf for a
     row that sees no key, whose out is 0). max_q: the largest number of new tokens of a sequence, where the caller
     knows it; it only chooses the kernel. scale defaults to 1 / sqrt(D)."""
-    dev, d, dtype = cache.device, cache.head_dim, cache.dtype
-    q, shape, qs = _rows(q, "q", d, dtype, dev)
-    T, Hq = shape[0], shape[1]
-    B, max_pages, pt_stride = _batch(page_table, cu_seqlens, kv_lens, dev)
-    out, os_ = _out(out, "out", q, shape, dtype, dev)
+    r = (_module or _host()).paged_attention(cache._key[0], cache._key[2], q, page_table, cu_seqlens, kv_lens, max_q,
+                                             scale, causal, out, return_lse)
+    if type(r) is int:
+        L.check(r, "paged_attention")
+    if r is not NotImplemented:
+        return r
+    c_ptr, dev, index, dtype, _, d = cache._key
+    q, T, Hq, q_st, q_sh, qp = _rows(q, "q", d, dtype, dev, index)
+    B, max_pages, pt_stride = _batch(page_table, cu_seqlens, kv_lens, dev, index)
+    out, o_st, o_sh, op = _out(out, "out", q, dev)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    _call(L.lib().mv_paged_attention,
-          _ATTN.pack(cache._ptr, q.data_ptr(), 0, 0, out.data_ptr(), lse.data_ptr() if return_lse else 0,
-                     cu_seqlens.data_ptr(), 0, page_table.data_ptr(), kv_lens.data_ptr(), qs[0], qs[1], 0, 0, 0, 0,
-                     os_[0], os_[1], pt_stride, T, B, Hq, T if max_q is None else max_q, bool(causal), max_pages, 0, 0,
-                     0, 0, 1.0 / math.sqrt(d) if scale is None else scale, 0), dev, "paged_attention")
+    _call("mv_paged_attention",
+          _ATTN.pack(c_ptr, qp, 0, 0, op, lse.data_ptr() if return_lse else 0, cu_seqlens.data_ptr(), 0,
+                     page_table.data_ptr(), kv_lens.data_ptr(), q_st, q_sh, 0, 0, 0, 0, o_st, o_sh, pt_stride, T, B, Hq,
+                     T if max_q is None else max_q, bool(causal), max_pages, 0, 0, 0, 0,
+                     1.0 / math.sqrt(d) if scale is None else scale, 0), dev, index)
     return (out, lse) if return_lse else out
 
 
@@ -196,37 +235,41 @@ def prompt_attention(q, k, v, cu_seqlens, *, cu_seqlens_k=None, max_q=None, scal
     """Attention over packed prompts: q [Tq, Hq, D], k, v [Tk, Hkv, D], sequence b's queries in rows
     cu_seqlens[b]:cu_seqlens[b + 1] and its keys in the same rows of k and v (or in cu_seqlens_k's). Causal masks
     align the ends: token i of n sees keys j <= n_keys - n + i. Returns as paged_attention."""
+    r = (_module or _host()).prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, max_q, scale, causal, out, return_lse)
+    if type(r) is int:
+        L.check(r, "prompt_attention")
+    if r is not NotImplemented:
+        return r
+    dtype, index, dev = q.dtype, q.get_device(), q.device
+    if index < 0:
+        L.require_cuda(q)
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise TypeError("prompt_attention: tensors must be bf16 or f16")
     if q.ndim != 3:
         raise ValueError("q, k, v must be [T, heads, D]")
-    if not q.is_cuda:
-        L.require_cuda(q)
-    dev, d, dtype = q.device, q.shape[2], q.dtype
-    if dtype not in _DTYPES:
-        raise TypeError("prompt_attention: tensors must be bf16 or f16")
-    q, shape, qs = _rows(q, "q", d, dtype, dev)
-    k, k_shape, ks = _rows(k, "k", d, dtype, dev)
-    v, v_shape, vs = _rows(v, "v", d, dtype, dev)
-    if v_shape != k_shape:
-        raise ValueError(f"k and v differ: {tuple(k_shape)} / {tuple(v_shape)}")
-    T, Hq = shape[0], shape[1]
-    cu = _ints(cu_seqlens, "cu_seqlens", dev)
+    d = q.shape[2]
+    q, T, Hq, q_st, q_sh, qp = _rows(q, "q", d, dtype, dev, index)
+    k, Tk, Hkv, k_st, k_sh, kp = _rows(k, "k", d, dtype, dev, index)
+    v, Tv, Hv, v_st, v_sh, vp = _rows(v, "v", d, dtype, dev, index)
+    if Tv != Tk or Hv != Hkv:
+        raise ValueError(f"k and v differ: {tuple(k.shape)} / {tuple(v.shape)}")
+    cu = _ints(cu_seqlens, "cu_seqlens", dev, index)
     B = cu[0] - 1
     if len(cu) != 1 or B < 0:
         raise ValueError("cu_seqlens must be [B + 1]")
     cuk = 0
     if cu_seqlens_k is not None:
-        if _ints(cu_seqlens_k, "cu_seqlens_k", dev) != cu:
+        if _ints(cu_seqlens_k, "cu_seqlens_k", dev, index) != cu:
             raise ValueError(f"cu_seqlens_k must be [{B + 1}]")
         cuk = cu_seqlens_k.data_ptr()
-    elif k_shape[0] != T:
+    elif Tk != T:
         raise ValueError("q and k have different numbers of tokens: cu_seqlens_k is needed")
-    out, os_ = _out(out, "out", q, shape, dtype, dev)
+    out, o_st, o_sh, op = _out(out, "out", q, dev)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    _call(L.lib().mv_prompt_attention,
-          _ATTN.pack(0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
-                     cu_seqlens.data_ptr(), cuk, 0, 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], 0, T,
-                     B, Hq, T if max_q is None else max_q, bool(causal), 0, k_shape[0], k_shape[1], d, L.dt(dtype),
-                     1.0 / math.sqrt(d) if scale is None else scale, 0), dev, "prompt_attention")
+    _call("mv_prompt_attention",
+          _ATTN.pack(0, qp, kp, vp, op, lse.data_ptr() if return_lse else 0, cu_seqlens.data_ptr(), cuk, 0, 0, q_st, q_sh,
+                     k_st, k_sh, v_st, v_sh, o_st, o_sh, 0, T, B, Hq, T if max_q is None else max_q, bool(causal), 0, Tk,
+                     Hkv, d, L.dt(dtype), 1.0 / math.sqrt(d) if scale is None else scale, 0), dev, index)
     return (out, lse) if return_lse else out
 
 

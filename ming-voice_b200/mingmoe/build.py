@@ -4,7 +4,8 @@
 
 Each translation unit compiles to an object under `mingmoe/_build/` (skipped when up to date), then they
 link into `mingmoe/libmingmoe.so` next to this file. The CUDA runtime is linked statically, so the library
-depends only on the driver.
+depends only on the driver. `csrc/attention_host.cpp`, the host side of the attention calls, becomes the Python module
+`mingmoe/_attention_host.so` beside it (g++, torch's headers; no device code).
 """
 from __future__ import annotations
 
@@ -83,5 +84,35 @@ def build(verbose: bool = False, force: bool = False, ptxas_v: bool = False, out
     return OUT
 
 
+HOST_SRC = os.path.join(CSRC, "attention_host.cpp")
+HOST_OUT = os.path.join(HERE, "_attention_host.so")
+
+
+def build_host(verbose: bool = False, force: bool = False) -> str:
+    """The Python module `_attention_host`."""
+    newest = max(os.path.getmtime(p) for p in [HOST_SRC, *glob.glob(os.path.join(INCLUDE, "*.h"))])
+    if os.path.exists(HOST_OUT) and os.path.getmtime(HOST_OUT) >= newest and not force:
+        return HOST_OUT
+    import sysconfig
+
+    import torch
+    tdir = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    inc = [os.path.join(tdir, "include"), os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(cuda, "include"), INCLUDE]
+    tmp = HOST_OUT + ".tmp"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in inc], HOST_SRC, "-o",
+           tmp, f"-L{os.path.join(tdir, 'lib')}", "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {HOST_SRC}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, HOST_OUT)
+    return HOST_OUT
+
+
 if __name__ == "__main__":
+    print(build_host(verbose="-v" in sys.argv, force="--force" in sys.argv))
     print(build(verbose="-v" in sys.argv, force="--force" in sys.argv, ptxas_v="--ptxas" in sys.argv))
