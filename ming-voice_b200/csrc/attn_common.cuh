@@ -155,7 +155,8 @@ __device__ __forceinline__ void build_schedule(const Problem& p, unsigned int* p
     if (lane == 31) tmp[warp] = x;
     __syncthreads();
     unsigned int before = carry, all = carry;
-    for (int w = 0; w < nw; ++w) {
+    const int used = min(nw, (p.B - base + 31) / 32);  // warps that hold a sequence
+    for (int w = 0; w < used; ++w) {
       if (w < warp) before += tmp[w];
       all += tmp[w];
     }

@@ -8,6 +8,10 @@
 // multiply-adds (512 + 512 cycles at D = 128) and 16384 exponentials (1024 cycles at 16 a cycle and SM), so the two
 // have to run side by side.
 //
+// Measured on a B200: 20000 causal tokens in 2 prompts, 16 / 4 heads of 128, bf16: 850 us (1232 TFLOP/s, 73 % of the measured
+// burst; 1006 us in a long loop, where power is the bound); 2043 new tokens over 45000 cached 210 us (1082); 9999 tokens, all
+// pairs, 16 / 16 heads of 64, f16: 190 us (606; the exponential unit is busy 75 % of the time).
+//
 // Layout of a CTA (one per SM): a work item is two tiles of 128 rows (row = token * G + head) of one sequence and key
 // head, which share the key and value tiles in shared memory.
 //   warps 0, 2   TMA producers: Q and K tiles, V tiles, into two rings of slots (a box per page and 64 values). One
