@@ -346,7 +346,9 @@ MV_API int mv_kv_append(const mv_kv_append_args* a, void* workspace, size_t work
  * NaN and infinities included) never reach a result, but for one case: a non-finite value row that some queries of
  * a sequence see can reach the other queries of that sequence that are computed in the same tile. max_q is the
  * caller's largest q_len (0: unknown), used to choose a kernel only: a wrong value costs time, not correctness.
- * scale > 0. Results do not depend on the run: fixed summation order.
+ * scale > 0. Results do not depend on the run: fixed summation order. A sequence whose work does not fit its share of
+ * the 32-bit schedule (2^31 / min(B, 1024) key tiles over all token tiles and key heads: a prompt of millions of tokens)
+ * is left out and reported (error 3).
  * workspace: mv_attention_workspace_bytes() bytes. */
 typedef struct mv_attention_args {
   const mv_paged_kv* cache; /* paged: the cache; NULL for prompts */
@@ -367,7 +369,8 @@ typedef struct mv_attention_args {
 MV_API int mv_paged_attention(const mv_attention_args* a, void* workspace, size_t workspace_bytes, void* stream);
 MV_API int mv_prompt_attention(const mv_attention_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Workspace bytes of the three calls above (any shape; zero-initialised, 256-byte aligned, left as they need it). */
+/* Workspace bytes of the three calls above for any shape (39.5 MB: two pieces of 256 rows for each of 148 CTAs;
+ * zero-initialised, 256-byte aligned, left as they need it). */
 MV_API size_t mv_attention_workspace_bytes(void);
 
 /* mv_block_decode without a caller workspace: no counterpart in the reference (its Triton launches take

@@ -666,8 +666,12 @@ int launch_tile(const Problem& p, const Source& src, int grid, cudaStream_t st) 
 
 int run_tile(Problem& p, const Source& src, int D, bool bf16, int grid, cudaStream_t st) {
   p.tok = 2 * (kM / p.G);
-  p.extra = 2;
-  p.min_share = 3;
+  // Short prompts are items of one to four tiles, where most of the time goes into beginning and finishing them: fewer cuts
+  // (8 prompts, 2043 tokens: 24.1 us with 5 and 6, 25.9 with 2 and 3). Elsewhere cuts are worth more (24 sequences of a few
+  // tokens over 2500 keys: 23.1 us with 2 and 3, 27.2 with 5 and 6; 9999 tokens in 5 prompts 190 and 197).
+  const bool brief = p.page_table == nullptr && src.max_keys < 512ll * p.B;
+  p.extra = brief ? 5 : 2;
+  p.min_share = brief ? 6 : 3;
   p.can_cut = src.max_keys > kBN;
   if (D == 128)
     return bf16 ? launch_tile<128, true>(p, src, grid, st) : launch_tile<128, false>(p, src, grid, st);
