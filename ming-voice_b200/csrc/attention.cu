@@ -60,7 +60,9 @@ static int make_map(CUtensorMap* m, const void* base, bool bf16, int d, int toke
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                          const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_SWIZZLE_128B,
+                         // a head's row and no more: with 128-byte rows, 256 bytes would fetch the next head's too
+                         d == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(MV_ERR_INVALID, "tensor map for %s rejected (CUresult %d)", what, static_cast<int>(r));
@@ -139,7 +141,8 @@ int run(const mv_attention_args* a, const Source& src, int D, int dtype, int Hkv
     } else {
       p.cu_k = cu_k + b0;
     }
-    rc = rows <= 32 ? run_split(p, src, D, bf16, rows, grid, st) : run_tile(p, src, D, bf16, grid, st);
+    // the few-row kernel up to 16 rows per key head, the 128-row kernel above (attn_split.cu has both sides measured)
+    rc = rows <= 16 ? run_split(p, src, D, bf16, rows, grid, st) : run_tile(p, src, D, bf16, grid, st);
     if (rc != MV_OK) return rc;
   }
   return MV_OK;

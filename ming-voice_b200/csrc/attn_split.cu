@@ -10,7 +10,8 @@
 // G = 4..8 the cache has to stream at HBM speed and the products need a few percent of the tensor pipe. Both
 // products are taken transposed, S^T = K Q^T and O^T = V^T P^T, with the keys (the head's values) in the 16-row
 // operand and the query rows in the 8-column one: 8 rows fill an instruction where the untransposed form would fill
-// half of it. The cost of that is one movmatrix per 8 x 8 block of P.
+// half of it. (Two such columns of 8 rows still pay: 16 query heads to one key head over 48 x 5000 keys 38.9 us, the 128-row
+// kernel 40.4. Four did not: 32 heads 82.2 and 40.7.) The cost of that is one movmatrix per 8 x 8 block of P.
 //
 // Split: one CTA per SM takes an equal share of all key tiles (attn_common.cuh). Producer warps keep a ring of
 // key tiles filled by TMA (a box per page and 64 values, 128-byte swizzle); each of the consumer warps takes whole
@@ -25,8 +26,8 @@ namespace {
 template <int D, int NT>
 struct Cfg {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kBN = D == 128 && NT <= 2 ? 32 : 64;  // keys of a tile
-  static constexpr int kWarps = NT <= 2 ? 8 : 4;             // consumer warps
+  static constexpr int kBN = D == 128 ? 32 : 64;             // keys of a tile
+  static constexpr int kWarps = 8;                            // consumer warps
   // producer warps, a tile each in turn: issuing a tile's copies is a chain of some 800 cycles for one warp, which
   // would hold the ring to 16 KB per 0.43 us (5.6 TB/s over the card, before anything else is in the way)
   static constexpr int kProd = 4;
@@ -499,9 +500,9 @@ int launch_split(Problem& p, const Source& src, bool bf16, int grid, cudaStream_
 
 }  // namespace
 
-// The kernel for `rows_hint` rows per (sequence, key head); any number is computed rightly (tiles of tok tokens).
+// The kernel for `rows_hint` rows (at most 16) per (sequence, key head); any number is computed rightly (tiles of tok tokens).
 int run_split(Problem& p, const Source& src, int D, bool bf16, int rows_hint, int grid, cudaStream_t st) {
-  const int nt = rows_hint <= 8 && p.G <= 8 ? 1 : rows_hint <= 16 && p.G <= 16 ? 2 : 4;
+  const int nt = rows_hint <= 8 && p.G <= 8 ? 1 : 2;
   p.tok = 8 * nt / p.G;
   // Fewer items than CTAs: cutting is what fills the card, and the less a CTA has the sooner it is done (one token over
   // 812 keys, 4 key heads: 9.3 us with 2 and 7, 10.6 with 6 and 14). More: an item counts for what it costs besides its
@@ -509,14 +510,9 @@ int run_split(Problem& p, const Source& src, int D, bool bf16, int rows_hint, in
   const bool few = static_cast<long long>(p.B) * p.Hkv < grid;
   p.extra = few ? 2 : 6;
   p.min_share = few ? 7 : 14;
-  if (D == 128) {
-    if (nt == 1) return launch_split<128, 1>(p, src, bf16, grid, st);
-    if (nt == 2) return launch_split<128, 2>(p, src, bf16, grid, st);
-    return launch_split<128, 4>(p, src, bf16, grid, st);
-  }
-  if (nt == 1) return launch_split<64, 1>(p, src, bf16, grid, st);
-  if (nt == 2) return launch_split<64, 2>(p, src, bf16, grid, st);
-  return launch_split<64, 4>(p, src, bf16, grid, st);
+  if (D == 128)
+    return nt == 1 ? launch_split<128, 1>(p, src, bf16, grid, st) : launch_split<128, 2>(p, src, bf16, grid, st);
+  return nt == 1 ? launch_split<64, 1>(p, src, bf16, grid, st) : launch_split<64, 2>(p, src, bf16, grid, st);
 }
 
 }  // namespace attn
