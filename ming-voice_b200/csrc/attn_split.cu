@@ -3,8 +3,8 @@
 // Mathematics: out = sum_j 2^(t_j - m) v_j / sum_j 2^(t_j - m), t_j = scale log2(e) q . k_j, with a running maximum m
 // and sum per row: when a key tile raises m, what has been summed is multiplied by 2^(m_old - m_new).
 //
-// Measured on a B200 (16 query / 4 key heads of 128 unless said): one token over 812 keys 9.3 us, over 130501 keys (12 / 2
-// heads) 30.1 us (134 MB, 4.4 TB/s), 61 sequences of 301061 keys together 102 us (617 MB, 6.0 TB/s, 94 % of the measured copy).
+// Measured on a B200 (16 query / 4 key heads of 128 unless said): one token over 812 keys 8.6 us, over 130501 keys (12 / 2
+// heads) 29.7 us (134 MB, 4.5 TB/s), 61 sequences of 301061 keys together 100 us (617 MB, 6.2 TB/s, 95 % of the measured copy).
 //
 // Bound: memory. A key row of 2 D values serves the G query heads of its key head (4 G D flops per 4 D bytes), so at
 // G = 4..8 the cache has to stream at HBM speed and the products need a few percent of the tensor pipe. Both
@@ -436,10 +436,11 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
 
 // Joins the pieces of the item that starts in CTA blockIdx.x's range and ends in a later one's, rows blockIdx.y NT .. + NT - 1.
 // A few rows of many pieces (74 of one long sequence) are a chain of L2 latencies for one CTA (9 us for a single CTA that
-// did it all), so every row has 8 warps: warp w joins pieces w, w + 8, .. in order, then the warps' results are joined.
+// did it all), so every row has 8 warps: warp w joins pieces w, w + 8, .. in order, then the warps' results are joined. 64
+// registers, so that four CTAs, of which most find nothing to do, fit an SM (batch of 61 sequences 101.9 -> 100.0 us).
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(256) join_kernel(const Problem p) {
-  constexpr int R = 8 * NT, kPiece = R * (D + 2), kLanes = D / 4, kAhead = 10;
+__global__ void __launch_bounds__(256, 4) join_kernel(const Problem p) {
+  constexpr int R = 8 * NT, kPiece = R * (D + 2), kLanes = D / 4, kAhead = 5;
   __shared__ float sM[8], sL[8];
   __shared__ float4 sV[8][kLanes];
   pdl_wait();

@@ -580,9 +580,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the pieces of the item that starts in CTA blockIdx.x's range and ends in a later one's: rows blockIdx.y * 32 ..
-// + 31 of its 256, a lane each, D / 8 values per warp; weights 2^(m_piece - M), pieces in CTA order.
+// + 31 of its 256, a lane each, D / 8 values per warp; weights 2^(m_piece - M), pieces in CTA order. 64 registers: most of
+// the grid's CTAs find nothing to join, and four of them fit an SM beside each other instead of two.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) combine_kernel(const Problem p) {
+__global__ void __launch_bounds__(256, 4) combine_kernel(const Problem p) {
   pdl_wait();
   const CutItem c = p.cuts[blockIdx.x];
   if (c.n <= 1) return;
@@ -592,7 +593,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const Problem p) {
   if (r >= half_tok * p.G || tok >= c.ntok) return;
   constexpr size_t kPiece = 256 * (128 + 2);
   constexpr int kVec = D / 32;                 // float4 per lane
-  constexpr int kAhead = 16 / kVec;            // pieces read at a time
+  constexpr int kAhead = 8 / kVec;             // pieces read at a time: most items have two or three
   // the first piece is CTA blockIdx.x's last (slot 1), the others are their CTAs' first (slot 0)
   auto piece = [&](int i) { return p.parts + (static_cast<size_t>(blockIdx.x + i) * 2 + (i == 0)) * kPiece; };
   float M = -INFINITY, L = 0.f;
