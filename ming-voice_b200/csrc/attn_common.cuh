@@ -23,6 +23,7 @@ namespace attn {
 
 constexpr int kMaxB = 1024;      // sequences of one launch (more: several launches)
 constexpr int kMaxCtas = 148;    // CTAs the workspace is laid out for: one per SM
+constexpr unsigned int kMaxUnits = 0x7fffffffu;  // sums of units stop here: two of them still add up in 32 bits
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLog2e = 1.442695040888963407f;
 
@@ -130,9 +131,10 @@ __device__ __forceinline__ unsigned int head_units(const Problem& p, const Seq& 
   return u;
 }
 
-// Exclusive prefix sums of the sequences' units into pre[0 .. B], by all threads of the CTA; `tmp` [32].
-template <int BN>
-__device__ __forceinline__ void build_schedule(const Problem& p, unsigned int* pre, unsigned int* tmp) {
+// Exclusive prefix sums of the sequences' units (kByItem: items) into pre[0 .. B], by all threads of the CTA; `tmp` [32].
+// Returns whether they fit 32 bits (pre[B] is 0 otherwise).
+template <int BN, bool kByItem>
+__device__ __forceinline__ bool prefix_units(const Problem& p, unsigned int* pre, unsigned int* tmp) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = (nt + 31) / 32;
   unsigned int carry = 0;
   for (int base = 0; base < p.B; base += nt) {
@@ -140,41 +142,56 @@ __device__ __forceinline__ void build_schedule(const Problem& p, unsigned int* p
     unsigned int u = 0;
     if (b < p.B) {
       const Seq s = seq_of(p, b, blockIdx.x == 0);
-      // a sequence whose share of 2^31 units is not enough (a prompt of millions of tokens) is left out and reported
-      const unsigned long long most = static_cast<unsigned long long>((s.nq + p.tok - 1) / p.tok) *
-                                      ((s.n + BN - 1) / BN + 1 + p.extra) * p.Hkv;
-      if (most < (1ull << 31) / p.B) u = head_units<BN>(p, s) * p.Hkv;
-      else if (blockIdx.x == 0) raise_error(p.ws, kErrOverflow, static_cast<unsigned int>(b));
+      const unsigned long long items = static_cast<unsigned long long>((s.nq + p.tok - 1) / p.tok) * p.Hkv;
+      const unsigned long long most = kByItem ? items : items * ((s.n + BN - 1) / BN + 1 + p.extra);
+      u = most >= kMaxUnits ? kMaxUnits : kByItem ? static_cast<unsigned int>(items) : head_units<BN>(p, s) * p.Hkv;
     }
     unsigned int x = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      if (lane >= o) x = min(x + y, kMaxUnits);
     }
     if (lane == 31) tmp[warp] = x;
     __syncthreads();
     unsigned int before = carry, all = carry;
     const int used = min(nw, (p.B - base + 31) / 32);  // warps that hold a sequence
     for (int w = 0; w < used; ++w) {
-      if (w < warp) before += tmp[w];
-      all += tmp[w];
+      if (w < warp) before = min(before + tmp[w], kMaxUnits);
+      all = min(all + tmp[w], kMaxUnits);
     }
     if (b < p.B) pre[b] = before + x - u;
     carry = all;
     if (base + nt < p.B) __syncthreads();
   }
-  if (tid == 0) pre[p.B] = carry;
+  if (tid == 0) pre[p.B] = carry < kMaxUnits ? carry : 0;
   __syncthreads();
+  return carry < kMaxUnits;
+}
+
+// The schedule into pre[0 .. B]. All sequences of a launch share 32 bits of units, whatever part of them each takes. kLong, for
+// launches whose tensors could hold more work than that (3 s and more of it): where the lengths do, an item counts as one unit, is
+// not cut, and the CTAs share the items by number. (pre[B + 1] tells; items fit, as each has query rows of its own.) Bounds that
+// do not ascend can claim rows many times over: where their sum does not fit nothing is computed, and that is reported.
+template <int BN, bool kLong>
+__device__ __forceinline__ void build_schedule(const Problem& p, unsigned int* pre, unsigned int* tmp) {
+  bool fits = prefix_units<BN, false>(p, pre, tmp);
+  if (kLong) {
+    const bool by_item = !fits;
+    if (by_item) fits = prefix_units<BN, true>(p, pre, tmp);
+    if (threadIdx.x == 0) pre[p.B + 1] = by_item;
+    __syncthreads();
+  }
+  if (!fits && threadIdx.x == 0 && blockIdx.x == 0) raise_error(p.ws, kErrOverflow, 0x701u);
 }
 
 // The CTAs' ranges [bound(c), bound(c + 1)) of the W units, bound(c) = floor(W c / ctas), before cuts move to nearby ends
 // of items.
 struct Cut {
   unsigned int W, ctas, share, rest;  // ctas: CTAs of the grid that have a range; W = share ctas + rest
-  __device__ __forceinline__ Cut(const Problem& p, unsigned int total, int grid) {
+  __device__ __forceinline__ Cut(const Problem& p, unsigned int total, bool by_item, int grid) {
     W = total;
-    ctas = min(W / p.min_share, static_cast<unsigned int>(grid));
+    ctas = min(by_item ? W : W / p.min_share, static_cast<unsigned int>(grid));
     // one sequence: its heads' items are alike, and so many cuts for each fall on their ends
     if (p.B == 1 && ctas > p.Hkv) ctas -= ctas % p.Hkv;
     if (ctas == 0) ctas = 1;
@@ -195,7 +212,7 @@ struct Cut {
 };
 
 // Walks the pieces of a CTA's range, warp by warp: every warp of the CTA walks on its own and sees the same pieces.
-template <int BN>
+template <int BN, bool kLong>
 struct Walk {
   const Problem& p;
   const unsigned int* pre;
@@ -222,7 +239,8 @@ struct Walk {
     unsigned int off = start - pre[b];
     h = static_cast<int>(off / per_head);
     off -= per_head * h;
-    const int n_t = (s.nq + p.tok - 1) / p.tok;
+    int n_t = (s.nq + p.tok - 1) / p.tok;
+    if (by_item()) n_t = 1, t = static_cast<int>(off), off = 0;
     for (int t0 = 0; n_t > 1; t0 += 32) {  // 32 token tiles at a time
       const unsigned int u = t0 + lane < n_t ? item_tiles<BN>(p, s, t0 + lane) + p.extra : 0;
       unsigned int x = u;
@@ -251,17 +269,19 @@ struct Walk {
       finish();
     }
   }
+  __device__ __forceinline__ bool by_item() const { return kLong && pre[p.B + 1] != 0; }
+  __device__ __forceinline__ unsigned int units() const { return by_item() ? 1u : tiles + p.extra; }
   // the piece's end: the item's, or the range's where that lies well inside the item
   __device__ __forceinline__ void finish() {
     i1 = tiles;
-    if (end < start + tiles + p.extra) {
+    if (end < start + units()) {
       const int o = static_cast<int>(end > start ? end - start : 0);
       if (o <= p.extra) live = false;  // the cut has moved to the item's start: the next CTA's
       else if (tiles + p.extra - o > p.extra) i1 = o - p.extra;
     }
   }
   __device__ __forceinline__ void advance() {
-    start += tiles + p.extra;
+    start += units();
     live = start < end;
     if (!live) return;
     if ((t + 1) * p.tok < s.nq) {
@@ -386,6 +406,13 @@ struct Source {
   int tokens, pages, box;
   long long max_keys;  // no sequence has more
 };
+
+// Whether the tensors could hold more units than the schedule counts: every sequence with all of its keys, token tiles of
+// `bn` keys each. (The lengths are on the device; up to this bound, the kernels without the other schedule are right for all.)
+inline bool may_be_long(const Problem& p, const Source& src, int bn) {
+  const double items = (static_cast<double>(p.T) / p.tok + p.B) * p.Hkv;
+  return items * (static_cast<double>(src.max_keys) / bn + 2 + p.extra) >= static_cast<double>(kMaxUnits);
+}
 
 // 5-D maps over keys and values [page][head][64-value part of a head][token][64 values], 128-byte swizzle, box of
 // 64 values x `box` tokens x `parts` parts: in shared memory [part][token][64 values]

@@ -110,7 +110,7 @@ __device__ __forceinline__ void join(float& M, float& L, float4& acc, float m, f
   acc.x = acc.x * a + f * v.x, acc.y = acc.y * a + f * v.y, acc.z = acc.z * a + f * v.z, acc.w = acc.w * a + f * v.w;
 }
 
-template <int D, int NT, bool BF16>
+template <int D, int NT, bool BF16, bool kLong>
 __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
     split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Problem p,
                  int box) {
@@ -140,14 +140,14 @@ __global__ void __launch_bounds__(Cfg<D, NT>::kThreads, 1)
   }
   pdl_launch_dependents();
   pdl_wait();
-  build_schedule<kBN>(p, pre, tmp);  // its barriers also publish the mbarriers
+  build_schedule<kBN, kLong>(p, pre, tmp);  // its barriers also publish the mbarriers
   const unsigned int W = pre[p.B];
   if (W == 0) {
     if (threadIdx.x == 0) p.cuts[blockIdx.x].n = 0;
     return;
   }
-  const Cut cut(p, W, gridDim.x);
-  Walk<kBN> wk(p, pre, cut, blockIdx.x);
+  const Cut cut(p, W, kLong && pre[p.B + 1], gridDim.x);
+  Walk<kBN, kLong> wk(p, pre, cut, blockIdx.x);
 
   if (warp >= NW) {
     // ---------------------------------------------------------------- producers: lane 0 issues all copies
@@ -490,7 +490,9 @@ int launch_split(Problem& p, const Source& src, bool bf16, int grid, cudaStream_
   p.can_cut = src.max_keys > C::kBN;
   const int rc = make_kv_maps(&mk, &mv_, src, p.Hkv, D, bf16, box, D / 64);
   if (rc != MV_OK) return rc;
-  auto fn = bf16 ? split_kernel<D, NT, true> : split_kernel<D, NT, false>;
+  const bool lng = may_be_long(p, src, C::kBN);
+  auto fn = bf16 ? (lng ? split_kernel<D, NT, true, true> : split_kernel<D, NT, true, false>)
+                 : (lng ? split_kernel<D, NT, false, true> : split_kernel<D, NT, false, false>);
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attention split)");
   const int rc2 = launch_pdl(fn, dim3(grid), C::kThreads, C::kSmem, st, "attention split launch", mk, mv_, p, box);

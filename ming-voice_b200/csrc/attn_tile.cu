@@ -141,7 +141,8 @@ __device__ __forceinline__ float weights(const uint32_t (&s)[4][32], float base,
 // Key tiles of a piece: [wk.i0, end), of which row tile t sees [wk.i0, end_of[t]).
 struct Tiles {
   int kend, end, end_of[2];
-  __device__ __forceinline__ Tiles(const Problem& p, const Walk<kBN>& wk, int half_tok) {
+  template <bool kLong>
+  __device__ __forceinline__ Tiles(const Problem& p, const Walk<kBN, kLong>& wk, int half_tok) {
     kend = wk.kend();
     const int ntok = wk.ntok();
     end = min(wk.i1, (kend + kBN - 1) / kBN);
@@ -150,7 +151,7 @@ struct Tiles {
   }
 };
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool kLong>
 __global__ void __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const Problem p, int box) {
@@ -215,15 +216,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_before_sync();
   pdl_launch_dependents();
   pdl_wait();
-  build_schedule<kBN>(p, pre, tmp);
+  build_schedule<kBN, kLong>(p, pre, tmp);
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   const unsigned int W = pre[p.B];
-  const Cut cut(p, W, gridDim.x);
+  const Cut cut(p, W, kLong && pre[p.B + 1], gridDim.x);
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    Walk<kBN> wk(p, pre, cut, blockIdx.x);
+    Walk<kBN, kLong> wk(p, pre, cut, blockIdx.x);
     if (warp == 0 || warp == 2) {
       // ---------------------------------------------------------------- TMA producers: lane 0 issues all copies
       const bool is_v = warp == 2;
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ------------------------------------------------------------------ softmax: tile t, a thread per row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    Walk<kBN> wk(p, pre, cut, blockIdx.x);
+    Walk<kBN, kLong> wk(p, pre, cut, blockIdx.x);
     const int t = warp >= 8, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + t * 128, tP = C::tmem_p(tmem, t) + lanes, tO = C::tmem_o(tmem, t) + lanes;
@@ -655,7 +656,7 @@ int launch_tile(const Problem& p, const Source& src, int grid, cudaStream_t st) 
   int rc = make_kv_maps(&mk, &mv_, src, p.Hkv, D, BF16, box, 1);
   if (rc == MV_OK) rc = make_q_map(&mq, p, D, BF16, p.tok / 2);
   if (rc != MV_OK) return rc;
-  auto fn = tile_kernel<D, BF16>;
+  auto fn = may_be_long(p, src, kBN) ? tile_kernel<D, BF16, true> : tile_kernel<D, BF16, false>;
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(attention tile)");
   rc = launch_pdl(fn, dim3(grid), kThreads, C::kSmem, st, "attention tile launch", mq, mk, mv_, p, box);
