@@ -49,24 +49,30 @@ class Sequences:
         return PagedKV.empty(self.num_pages, self.page_size, attn.n_kv_heads, attn.head_dim, attn.w_qkv.dtype, self.device)
 
     def extend(self, new, prompts=False):
-        """The batch of new[s] tokens for each sequence s of the dict, in its order; their pages are taken now."""
-        rows = []
+        """The batch of new[s] tokens for each sequence s of the dict, in its order; their pages are taken now. A step that is
+        refused, or fails, changes nothing."""
+        pages, taken = {}, 0  # the sequences' pages after the step, and how many of them are new
         for s, n in new.items():
             if prompts and self.lens[s]:
                 raise ValueError(f"sequence {s} has {self.lens[s]} tokens already")
             need = -(-(self.lens[s] + n) // self.page_size)
-            if need > self.max_pages or need - len(self.pages[s]) > len(self.free):
+            more = max(need - len(self.pages[s]), 0)
+            if need > self.max_pages or taken + more > len(self.free):
                 raise RuntimeError(f"no room for {n} more tokens of sequence {s}")
-            while len(self.pages[s]) < need:
-                self.pages[s].append(self.free.pop())
-            self.lens[s] += n
-            rows.append(self.pages[s] + [0] * (self.max_pages - need))
+            pages[s] = self.pages[s] + [self.free[-1 - i] for i in range(taken, taken + more)]
+            taken += more
         cu = [0]
         for n in new.values():
             cu.append(cu[-1] + n)
         i32 = dict(dtype=torch.int32, device=self.device)
-        return Batch(torch.tensor(cu, **i32), torch.tensor(rows, **i32).reshape(len(rows), self.max_pages),
-                     torch.tensor([self.lens[s] for s in new], **i32), max(new.values(), default=0), prompts)
+        rows = torch.tensor([p + [0] * (self.max_pages - len(p)) for p in pages.values()], **i32)
+        batch = Batch(torch.tensor(cu, **i32), rows.reshape(len(pages), self.max_pages),
+                      torch.tensor([self.lens[s] + n for s, n in new.items()], **i32), max(new.values(), default=0), prompts)
+        del self.free[len(self.free) - taken:]
+        for s, n in new.items():
+            self.pages[s] = pages[s]
+            self.lens[s] += n
+        return batch
 
     def release(self, s):
         """Gives back the pages of sequence s."""
