@@ -39,7 +39,7 @@ class Sequences:
 
     def __init__(self, num_pages, page_size, max_seqs, max_len, device="cuda"):
         self.num_pages, self.page_size, self.device = num_pages, page_size, torch.device(device)
-        self.max_pages = -(-max_len // page_size)
+        self.max_len, self.max_pages = max_len, -(-max_len // page_size)
         self.free = list(range(num_pages - 1, -1, -1))
         self.pages = [[] for _ in range(max_seqs)]
         self.lens = [0] * max_seqs
@@ -53,11 +53,13 @@ class Sequences:
         refused, or fails, changes nothing."""
         pages, taken = {}, 0  # the sequences' pages after the step, and how many of them are new
         for s, n in new.items():
+            if n < 0:
+                raise ValueError(f"{n} new tokens of sequence {s}")
             if prompts and self.lens[s]:
                 raise ValueError(f"sequence {s} has {self.lens[s]} tokens already")
             need = -(-(self.lens[s] + n) // self.page_size)
             more = max(need - len(self.pages[s]), 0)
-            if need > self.max_pages or taken + more > len(self.free):
+            if self.lens[s] + n > self.max_len or taken + more > len(self.free):
                 raise RuntimeError(f"no room for {n} more tokens of sequence {s}")
             pages[s] = self.pages[s] + [self.free[-1 - i] for i in range(taken, taken + more)]
             taken += more

@@ -36,3 +36,16 @@ def test_pages_in_order_and_given_back():
     assert seqs.lens == [8, 0] and sorted(seqs.free) == [0, 1, 3, 4]
     empty = seqs.extend({})
     assert empty.page_table.shape == (0, 4) and empty.cu_seqlens.tolist() == [0] and empty.max_q == 0
+
+
+@pytest.mark.parametrize("new,exc", [({0: 51}, RuntimeError), ({1: 50, 0: 51}, RuntimeError), ({0: -1}, ValueError)])
+def test_lengths_stay_within_max_len(new, exc):
+    """max_len inside a page: the page's other slots are no room (a rotation table of max_len rows has none for them)."""
+    seqs = Sequences(num_pages=9, page_size=16, max_seqs=2, max_len=50, device="cpu")
+    before = state(seqs)
+    with pytest.raises(exc):
+        seqs.extend(new)
+    assert state(seqs) == before
+    assert seqs.extend({0: 50}).kv_lens.tolist() == [50]
+    with pytest.raises(RuntimeError):
+        seqs.extend({0: 1})
