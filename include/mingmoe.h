@@ -296,6 +296,7 @@ MV_API int mv_mask_pad_rows(void* ids, int ids_dtype, int N, int NK, const int* 
  *  - All indices (cu_seqlens, lengths, page ids) are read on the device: nothing synchronises the host and a
  *    captured graph serves every length. What does not fit the tensors is clamped or skipped, never read or
  *    written out of range, and reported in the workspace's error word (4 or 5).
+ *  - As everywhere in this header, the caller makes the device of the tensors and of `stream` current.
  *
  * Paged cache: k and v [num_pages, page_size, n_kv_heads, head_dim] through strides (page, token, head), so a
  * [num_pages, n_kv_heads, page_size, head_dim] cache works as well. page_size is a power of two in 8..256.

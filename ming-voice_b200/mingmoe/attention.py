@@ -10,7 +10,8 @@ The calls read their arguments in C++ (csrc/attention_host.cpp) where these are 
 below it refuses what does not fit and copies what only needs another layout.
 
 Lengths, bounds and page ids are int32 device tensors, read on the device: no call synchronises the host, and a
-captured graph serves whatever lengths its buffers hold at the replay.
+captured graph serves whatever lengths its buffers hold at the replay. A call runs on its tensors' device, on that device's
+current stream, whichever device is current.
 """
 from __future__ import annotations
 
@@ -166,6 +167,10 @@ def kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, *, q=None, q_out=Non
     cos_sin: fp32 [max_pos, rot_dim], a position's rot_dim / 2 cosines then its sines (rotation_table); None copies
     without rotating. rot_dim is a multiple of 16 up to D. Pairs are (i, i + rot_dim / 2), or (2i, 2i + 1) when
     `interleaved`. positions: int32 [T] rows of cos_sin, if not the cache positions. q_out may be q itself."""
+    if torch._C._cuda_getDevice() != cache._key[2]:  # launches go to the current device
+        with torch.cuda.device(cache._key[2]):
+            return kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, q=q, q_out=q_out, cos_sin=cos_sin,
+                             positions=positions, interleaved=interleaved)
     r = (_module or _host()).kv_append(cache._key[0], cache._key[2], k, v, page_table, cu_seqlens, kv_lens, q, q_out,
                                        cos_sin, positions, interleaved)
     if type(r) is int:
@@ -211,6 +216,10 @@ def paged_attention(q, cache, page_table, cu_seqlens, kv_lens, *, max_q=None, sc
     (kv_append): out [T, Hq, D], and with return_lse also lse [T, Hq] fp32 (ln of the sum of exp scores; -inf for a
     row that sees no key, whose out is 0). max_q: the largest number of new tokens of a sequence, where the caller
     knows it; it only chooses the kernel. scale defaults to 1 / sqrt(D)."""
+    if torch._C._cuda_getDevice() != cache._key[2]:
+        with torch.cuda.device(cache._key[2]):
+            return paged_attention(q, cache, page_table, cu_seqlens, kv_lens, max_q=max_q, scale=scale, causal=causal,
+                                   out=out, return_lse=return_lse)
     r = (_module or _host()).paged_attention(cache._key[0], cache._key[2], q, page_table, cu_seqlens, kv_lens, max_q,
                                              scale, causal, out, return_lse)
     if type(r) is int:
@@ -235,6 +244,10 @@ def prompt_attention(q, k, v, cu_seqlens, *, cu_seqlens_k=None, max_q=None, scal
     """Attention over packed prompts: q [Tq, Hq, D], k, v [Tk, Hkv, D], sequence b's queries in rows
     cu_seqlens[b]:cu_seqlens[b + 1] and its keys in the same rows of k and v (or in cu_seqlens_k's). Causal masks
     align the ends: token i of n sees keys j <= n_keys - n + i. Returns as paged_attention."""
+    if q.get_device() >= 0 and torch._C._cuda_getDevice() != q.get_device():
+        with torch.cuda.device(q.get_device()):
+            return prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=cu_seqlens_k, max_q=max_q, scale=scale, causal=causal,
+                                    out=out, return_lse=return_lse)
     r = (_module or _host()).prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, max_q, scale, causal, out, return_lse)
     if type(r) is int:
         L.check(r, "prompt_attention")

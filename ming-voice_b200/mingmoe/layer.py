@@ -127,7 +127,8 @@ class AttentionBlock:
 
     def __call__(self, x, cache, batch):
         """x [T, H] bf16 of the batch's packed tokens -> [T, H]; their keys and values go into `cache`."""
-        return self.output(self.attend(self.project(x), cache, batch), x)
+        with torch.cuda.device(x.device):
+            return self.output(self.attend(self.project(x), cache, batch), x)
 
 
 class DecoderLayer:
@@ -137,5 +138,6 @@ class DecoderLayer:
         self.attn, self.moe, self.cache = attn, moe_block, cache
 
     def __call__(self, x, batch):
-        h = self.attn(x, self.cache, batch)
-        return self.moe.decode(h) if h.shape[0] <= moe.DECODE_MAX_M else self.moe.prefill(h)
+        with torch.cuda.device(x.device):
+            h = self.attn(x, self.cache, batch)
+            return self.moe.decode(h) if h.shape[0] <= moe.DECODE_MAX_M else self.moe.prefill(h)
