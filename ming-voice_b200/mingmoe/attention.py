@@ -66,15 +66,15 @@ class PagedKV:
 
 
 def _fit(t, name, d, dtype, device):
-    """A [T, heads, d] operand that the kernels cannot take as it is: refused, or copied where only its layout has no
-    16-byte vectors."""
+    """A [T, heads, d] operand that the kernels cannot take as it is: refused, or copied where only its layout or address
+    has no 16-byte vectors."""
     if t.ndim != 3 or t.shape[2] != d:
         raise ValueError(f"{name} must be [T, heads, {d}], got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
     if t.device != device:
         raise RuntimeError(f"{name} is on {t.device}, expected {device}")
-    return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _rows(t, name, d, dtype, device, index):

@@ -1,0 +1,30 @@
+"""GPU parity of the attention calls on arguments at the edge of what they take, against the plain 64-bit implementation."""
+import pytest
+import torch
+
+from mingmoe import attention as A
+from oracle import attention_oracle as O
+from test_gpu_attention import BF, Paged, check, cu_of, errors, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def off(t, n):
+    """The tensor's values in a contiguous tensor that begins n elements behind a 16-byte address."""
+    flat = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)
+    return flat[n:n + t.numel()].view(t.shape).copy_(t)
+
+
+@pytest.mark.parametrize("n", [1, 4])
+def test_operands_off_a_16_byte_address(cuda, n):
+    new, kv = [3, 2], [40, 2]
+    P = Paged(cuda, BF, 2, 128, 16, kv)
+    cu = cu_of(new, cuda)
+    q, k, v = (randn((5, h, 128), BF, cuda, i) for i, h in enumerate((8, 2, 2)))
+    refs = [O.attention(q[cu[b]:cu[b + 1]], P.k[b], P.v[b], True) for b in range(2)]
+    check(A.paged_attention(off(q, n), P.cache, P.table, cu, P.lens), None, refs, cu)
+    refs = [O.attention(q[cu[b]:cu[b + 1]], k[cu[b]:cu[b + 1]], v[cu[b]:cu[b + 1]], True) for b in range(2)]
+    check(A.prompt_attention(off(q, n), off(k, n), off(v, n), cu), None, refs, cu)
+    assert torch.equal(A.kv_append(P.cache, off(k, n), off(v, n), P.table, cu, P.lens, q=off(q, n)), q)
+    assert torch.equal(O.gather(P.kc, P.table[0], 40)[37:], k[:3]) and torch.equal(O.gather(P.vc, P.table[1], 2), v[3:])
+    assert errors() == []
