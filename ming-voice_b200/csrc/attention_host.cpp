@@ -11,6 +11,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -39,7 +40,9 @@ std::vector<Workspace>& workspaces() {  // under the GIL
 struct Launch {
   void *stream, *ws;
   size_t bytes;
+  // false also where another device is current: the entry points launch on the current one, and the Python code changes it
   bool find(int device) {
+    if (c10::cuda::current_device() != device) return false;
     stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
     for (const Workspace& w : workspaces())
       if (w.device == device && w.stream == stream) {

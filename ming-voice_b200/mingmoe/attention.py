@@ -167,10 +167,6 @@ def kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, *, q=None, q_out=Non
     cos_sin: fp32 [max_pos, rot_dim], a position's rot_dim / 2 cosines then its sines (rotation_table); None copies
     without rotating. rot_dim is a multiple of 16 up to D. Pairs are (i, i + rot_dim / 2), or (2i, 2i + 1) when
     `interleaved`. positions: int32 [T] rows of cos_sin, if not the cache positions. q_out may be q itself."""
-    if torch._C._cuda_getDevice() != cache._key[2]:  # launches go to the current device
-        with torch.cuda.device(cache._key[2]):
-            return kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, q=q, q_out=q_out, cos_sin=cos_sin,
-                             positions=positions, interleaved=interleaved)
     r = (_module or _host()).kv_append(cache._key[0], cache._key[2], k, v, page_table, cu_seqlens, kv_lens, q, q_out,
                                        cos_sin, positions, interleaved)
     if type(r) is int:
@@ -178,6 +174,10 @@ def kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, *, q=None, q_out=Non
     if r is not NotImplemented:
         return r
     c_ptr, dev, index, dtype, n_kv, d = cache._key
+    if torch._C._cuda_getDevice() != index:  # launches go to the current one
+        with torch.cuda.device(index):
+            return kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, q=q, q_out=q_out, cos_sin=cos_sin,
+                             positions=positions, interleaved=interleaved)
     k, T, H, k_st, k_sh, kp = _rows(k, "k", d, dtype, dev, index)
     v, Tv, Hv, v_st, v_sh, vp = _rows(v, "v", d, dtype, dev, index)
     if H != n_kv or Hv != n_kv or Tv != T:
@@ -216,10 +216,6 @@ def paged_attention(q, cache, page_table, cu_seqlens, kv_lens, *, max_q=None, sc
     (kv_append): out [T, Hq, D], and with return_lse also lse [T, Hq] fp32 (ln of the sum of exp scores; -inf for a
     row that sees no key, whose out is 0). max_q: the largest number of new tokens of a sequence, where the caller
     knows it; it only chooses the kernel. scale defaults to 1 / sqrt(D)."""
-    if torch._C._cuda_getDevice() != cache._key[2]:
-        with torch.cuda.device(cache._key[2]):
-            return paged_attention(q, cache, page_table, cu_seqlens, kv_lens, max_q=max_q, scale=scale, causal=causal,
-                                   out=out, return_lse=return_lse)
     r = (_module or _host()).paged_attention(cache._key[0], cache._key[2], q, page_table, cu_seqlens, kv_lens, max_q,
                                              scale, causal, out, return_lse)
     if type(r) is int:
@@ -227,6 +223,10 @@ def paged_attention(q, cache, page_table, cu_seqlens, kv_lens, *, max_q=None, sc
     if r is not NotImplemented:
         return r
     c_ptr, dev, index, dtype, _, d = cache._key
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return paged_attention(q, cache, page_table, cu_seqlens, kv_lens, max_q=max_q, scale=scale, causal=causal,
+                                   out=out, return_lse=return_lse)
     q, T, Hq, q_st, q_sh, qp = _rows(q, "q", d, dtype, dev, index)
     B, max_pages, pt_stride = _batch(page_table, cu_seqlens, kv_lens, dev, index)
     out, o_st, o_sh, op = _out(out, "out", q, dev)
@@ -244,10 +244,6 @@ def prompt_attention(q, k, v, cu_seqlens, *, cu_seqlens_k=None, max_q=None, scal
     """Attention over packed prompts: q [Tq, Hq, D], k, v [Tk, Hkv, D], sequence b's queries in rows
     cu_seqlens[b]:cu_seqlens[b + 1] and its keys in the same rows of k and v (or in cu_seqlens_k's). Causal masks
     align the ends: token i of n sees keys j <= n_keys - n + i. Returns as paged_attention."""
-    if q.get_device() >= 0 and torch._C._cuda_getDevice() != q.get_device():
-        with torch.cuda.device(q.get_device()):
-            return prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=cu_seqlens_k, max_q=max_q, scale=scale, causal=causal,
-                                    out=out, return_lse=return_lse)
     r = (_module or _host()).prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, max_q, scale, causal, out, return_lse)
     if type(r) is int:
         L.check(r, "prompt_attention")
@@ -256,6 +252,10 @@ def prompt_attention(q, k, v, cu_seqlens, *, cu_seqlens_k=None, max_q=None, scal
     dtype, index, dev = q.dtype, q.get_device(), q.device
     if index < 0:
         L.require_cuda(q)
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=cu_seqlens_k, max_q=max_q, scale=scale, causal=causal,
+                                    out=out, return_lse=return_lse)
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise TypeError("prompt_attention: tensors must be bf16 or f16")
     if q.ndim != 3:
