@@ -168,7 +168,7 @@ extern "C" int mv_paged_attention(const mv_attention_args* a, void* workspace, s
                 a->max_q);
   if (a->T == 0 || a->B == 0) return MV_OK;
   if (a->q == nullptr || a->out == nullptr || a->cu_seqlens == nullptr || a->kv_lens == nullptr ||
-      a->page_table == nullptr)
+      (a->page_table == nullptr && a->max_pages > 0))
     return fail(MV_ERR_INVALID, "%s: null pointer", who);
   if (a->max_pages > 1 && a->B > 1 && a->pt_stride < a->max_pages)
     return fail(MV_ERR_INVALID, "%s: page table row stride %lld shorter than max_pages=%d", who, a->pt_stride,

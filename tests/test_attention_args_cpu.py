@@ -19,3 +19,15 @@ def test_rows_that_fit_are_taken_as_they_are():
     t = torch.zeros(3, 6, 64, dtype=torch.bfloat16)[:, 2:5]
     got, T, H, st, sh, p = A._rows(t, "q", 64, torch.bfloat16, t.device, -1)
     assert got is t and p == t.data_ptr() and (T, H, st, sh) == (3, 3, 384, 64)
+
+
+def test_null_page_table_needs_no_columns():
+    """The entry point without a GPU: a table of no columns may be null, and what is checked behind it is reached."""
+    import ctypes as C
+
+    from mingmoe import _lib as L
+    from test_attention_cpu import attn, kv
+    lib, c = L.lib(), kv()
+    nws = lib.mv_attention_workspace_bytes()
+    assert lib.mv_paged_attention(C.byref(attn(c, page_table=None, max_pages=0)), 4096, nws - 1, None) == L.MV_ERR_WORKSPACE
+    assert lib.mv_paged_attention(C.byref(attn(c, page_table=None)), 4096, nws - 1, None) == L.MV_ERR_INVALID

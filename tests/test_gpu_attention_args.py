@@ -28,3 +28,18 @@ def test_operands_off_a_16_byte_address(cuda, n):
     assert torch.equal(A.kv_append(P.cache, off(k, n), off(v, n), P.table, cu, P.lens, q=off(q, n)), q)
     assert torch.equal(O.gather(P.kc, P.table[0], 40)[37:], k[:3]) and torch.equal(O.gather(P.vc, P.table[1], 2), v[3:])
     assert errors() == []
+
+
+def test_page_table_without_columns(cuda):
+    """Sequences that have no page yet: rows without a key."""
+    P = Paged(cuda, BF, 2, 128, 16, [0, 0])
+    q = randn((3, 8, 128), BF, cuda, 1)
+    for hint in (2, 1000):
+        for causal in (True, False):
+            out, lse = A.paged_attention(q, P.cache, P.table[:, :0].contiguous(), cu_of([1, 2], cuda), P.lens, max_q=hint,
+                                         causal=causal, return_lse=True)
+            assert bool((out == 0).all()) and bool((lse == -torch.inf).all())
+    assert errors() == []
+    # a length that has no page is clamped to none and reported
+    out = A.paged_attention(q, P.cache, P.table[:, :0].contiguous(), cu_of([1, 2], cuda), P.lens + 1)
+    assert bool((out == 0).all()) and errors() == [5]
