@@ -120,6 +120,13 @@ bool integer(PyObject* o, long* v) {
   return *v >= 0 && *v <= 0x7fffffff;
 }
 
+bool flag(PyObject* o, bool* v) {
+  const int t = PyObject_IsTrue(o);
+  if (t < 0) PyErr_Clear();  // the Python code meets it again and raises
+  *v = t == 1;
+  return t >= 0;
+}
+
 PyObject* wrap(const at::Tensor& out, const at::Tensor& lse) {
   PyObject* o = THPVariable_Wrap(out);
   if (!lse.defined() || o == nullptr) return o;
@@ -128,14 +135,17 @@ PyObject* wrap(const at::Tensor& out, const at::Tensor& lse) {
 }
 
 // scale, causal, return_lse, max_q of the attention calls
-bool options(PyObject* max_q, PyObject* scale, PyObject* causal, int d, mv_attention_args* a) {
+bool options(PyObject* max_q, PyObject* scale, PyObject* causal, PyObject* return_lse, int d, mv_attention_args* a,
+             bool* with_lse) {
+  bool c;
+  if (!flag(causal, &c) || !flag(return_lse, with_lse)) return false;
   long m = a->T;
   if (max_q != Py_None && !integer(max_q, &m)) return false;
   double s = 1.0 / std::sqrt(static_cast<double>(d));
   if (scale != Py_None && !number(scale, &s)) return false;
   a->max_q = static_cast<int>(m);
   a->scale = static_cast<float>(s);
-  a->causal = PyObject_IsTrue(causal) == 1;
+  a->causal = c;
   return true;
 }
 
@@ -178,7 +188,9 @@ PyObject* append_impl(PyObject* const* o) {
     if (!ints(o[10], 1, dev, &pos) || pos->size(0) != T) return plain_not();
     a.positions = iptr(pos);
   }
-  a.interleaved = PyObject_IsTrue(o[11]) == 1;
+  bool interleaved;
+  if (!flag(o[11], &interleaved)) return plain_not();
+  a.interleaved = interleaved;
   at::Tensor qo;
   if (o[7] != Py_None) {
     if (!rows(o[7], d, type, dev, &q) || q->size(0) != T || !l.find(dev) || !result(o[8], *q, &qo)) return plain_not();
@@ -205,8 +217,9 @@ PyObject* paged_impl(PyObject* const* o) {
     return plain_not();
   a.T = static_cast<int>(q->size(0)), a.Hq = static_cast<int>(q->size(1)), a.B = b.B;
   at::Tensor out, lse;
-  if (!options(o[6], o[7], o[8], d, &a) || !l.find(dev) || !result(o[9], *q, &out)) return plain_not();
-  if (PyObject_IsTrue(o[10]) == 1) lse = at::empty({a.T, a.Hq}, q->options().dtype(at::kFloat));
+  bool with_lse;
+  if (!options(o[6], o[7], o[8], o[10], d, &a, &with_lse) || !l.find(dev) || !result(o[9], *q, &out)) return plain_not();
+  if (with_lse) lse = at::empty({a.T, a.Hq}, q->options().dtype(at::kFloat));
   a.cache = c;
   a.q = q->data_ptr(), a.out = out.data_ptr();
   a.lse = lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr;
@@ -239,8 +252,9 @@ PyObject* prompt_impl(PyObject* const* o) {
   mv_attention_args a{};
   a.T = static_cast<int>(q.size(0)), a.Hq = static_cast<int>(q.size(1)), a.B = static_cast<int>(cu->size(0)) - 1;
   at::Tensor out, lse;
-  if (!options(o[5], o[6], o[7], d, &a) || !l.find(dev) || !result(o[8], q, &out)) return plain_not();
-  if (PyObject_IsTrue(o[9]) == 1) lse = at::empty({a.T, a.Hq}, q.options().dtype(at::kFloat));
+  bool with_lse;
+  if (!options(o[5], o[6], o[7], o[9], d, &a, &with_lse) || !l.find(dev) || !result(o[8], q, &out)) return plain_not();
+  if (with_lse) lse = at::empty({a.T, a.Hq}, q.options().dtype(at::kFloat));
   a.q = q.data_ptr(), a.k = k->data_ptr(), a.v = v->data_ptr(), a.out = out.data_ptr();
   a.lse = lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr;
   a.cu_seqlens = iptr(cu), a.cu_seqlens_k = cuk == nullptr ? nullptr : iptr(cuk);

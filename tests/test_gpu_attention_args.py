@@ -43,3 +43,22 @@ def test_page_table_without_columns(cuda):
     # a length that has no page is clamped to none and reported
     out = A.paged_attention(q, P.cache, P.table[:, :0].contiguous(), cu_of([1, 2], cuda), P.lens + 1)
     assert bool((out == 0).all()) and errors() == [5]
+
+
+@pytest.mark.parametrize("name", ["causal", "return_lse"])
+def test_flag_without_a_truth_value(cuda, name):
+    """A flag whose truth value raises: that error, and nothing is launched."""
+    P = Paged(cuda, BF, 2, 128, 16, [3])
+    q, cu, out = randn((1, 8, 128), BF, cuda, 1), cu_of([1], cuda), torch.full((1, 8, 128), 7.0, dtype=BF, device=cuda)
+    A.paged_attention(q, P.cache, P.table, cu, P.lens)  # the stream's workspace exists: calls go through the host module
+    for flag in (torch.ones(2), torch.ones(2, device=cuda)):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            A.paged_attention(q, P.cache, P.table, cu, P.lens, out=out, **{name: flag})
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            A.prompt_attention(q, q, q, cu, out=out, **{name: flag})
+    assert bool((out == 7).all())
+    k = randn((1, 2, 128), BF, cuda, 2)
+    before = P.kc.clone()
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        A.kv_append(P.cache, k, k, P.table, cu, P.lens, interleaved=torch.ones(2))
+    assert torch.equal(before.view(torch.int16), P.kc.view(torch.int16))
