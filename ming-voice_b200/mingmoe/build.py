@@ -89,10 +89,8 @@ HOST_OUT = os.path.join(HERE, "_attention_host.so")
 
 
 def build_host(verbose: bool = False, force: bool = False) -> str:
-    """The Python module `_attention_host`."""
-    newest = max(os.path.getmtime(p) for p in [HOST_SRC, *glob.glob(os.path.join(INCLUDE, "*.h"))])
-    if os.path.exists(HOST_OUT) and os.path.getmtime(HOST_OUT) >= newest and not force:
-        return HOST_OUT
+    """The Python module `_attention_host`. It is bound to the headers of one torch and one Python, so the command that compiled
+    it (with their versions) is kept beside the objects, and another command compiles it again."""
     import sysconfig
 
     import torch
@@ -104,12 +102,22 @@ def build_host(verbose: bool = False, force: bool = False) -> str:
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in inc], HOST_SRC, "-o",
            tmp, f"-L{os.path.join(tdir, 'lib')}", "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    made_by = f"torch {torch.__version__}, python {sys.version}: {' '.join(cmd).replace(ROOT, '.')}\n"
+    record = os.path.join(BUILD, "attention_host.cmd")
+    newest = max([os.path.getmtime(p) for p in [HOST_SRC, *glob.glob(os.path.join(INCLUDE, "*.h"))]])
+    if os.path.exists(HOST_OUT) and os.path.getmtime(HOST_OUT) >= newest and not force and os.path.exists(record):
+        with open(record) as f:
+            if f.read() == made_by:
+                return HOST_OUT
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {HOST_SRC}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, HOST_OUT)
+    os.makedirs(BUILD, exist_ok=True)
+    with open(record, "w") as f:
+        f.write(made_by)
     return HOST_OUT
 
 
