@@ -42,13 +42,23 @@ struct Problem {
   int tok;                // tokens of a tile
   int causal;
   int extra;              // units an item counts besides its key tiles
-  int min_share;          // least units worth a CTA of their own; more than 2 extra
+  int min_share;          // least units worth a CTA of their own
   bool can_cut;           // an item may have more than one tile, so that the joining kernel is needed
   float scale_log2;       // scale * log2(e): softmax in powers of two
   WsHeader* ws;
   struct CutItem* cuts;  // [kMaxCtas]
   float* parts;          // [kMaxCtas][2] pieces: slot 1 starts its item, slot 0 starts inside it
 };
+
+// The cut rule of a launch. A range is then never shorter than `extra`, so that of two cuts one at most lies within the last
+// `extra` units of an item: there it moves to the item's end, and last_cta() names the range before it. (A shorter range could
+// move two cuts to the same end. A range may still be left empty, by cuts that move to both of its ends.)
+template <int kExtra, int kMinShare>
+inline void cut_rule(Problem& p) {
+  static_assert(kMinShare >= kExtra, "two cuts could move to one end");
+  p.extra = kExtra;
+  p.min_share = kMinShare;
+}
 
 // What the joining kernel needs of a cut item, left by the CTA whose range holds its start; written by every CTA.
 struct CutItem {

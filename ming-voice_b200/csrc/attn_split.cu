@@ -511,8 +511,8 @@ int run_split(Problem& p, const Source& src, int D, bool bf16, int rows_hint, in
   // 812 keys, 4 key heads: 9.3 us with 2 and 7, 10.6 with 6 and 14). More: an item counts for what it costs besides its
   // tiles, so that CTAs with several short items get less (61 sequences of 300000 keys: 101.9 us with 6, 104.3 with 2).
   const bool few = static_cast<long long>(p.B) * p.Hkv < grid;
-  p.extra = few ? 2 : 6;
-  p.min_share = few ? 7 : 14;
+  if (few) cut_rule<2, 7>(p);
+  else cut_rule<6, 14>(p);
   if (D == 128)
     return nt == 1 ? launch_split<128, 1>(p, src, bf16, grid, st) : launch_split<128, 2>(p, src, bf16, grid, st);
   return nt == 1 ? launch_split<64, 1>(p, src, bf16, grid, st) : launch_split<64, 2>(p, src, bf16, grid, st);

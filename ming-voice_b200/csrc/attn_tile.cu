@@ -672,8 +672,8 @@ int run_tile(Problem& p, const Source& src, int D, bool bf16, int grid, cudaStre
   // (8 prompts, 2043 tokens: 24.1 us with 5 and 6, 25.9 with 2 and 3). Elsewhere cuts are worth more (24 sequences of a few
   // tokens over 2500 keys: 23.1 us with 2 and 3, 27.2 with 5 and 6; 9999 tokens in 5 prompts 190 and 197).
   const bool brief = p.page_table == nullptr && src.max_keys < 512ll * p.B;
-  p.extra = brief ? 5 : 2;
-  p.min_share = brief ? 6 : 3;
+  if (brief) cut_rule<5, 6>(p);
+  else cut_rule<2, 3>(p);
   p.can_cut = src.max_keys > kBN;
   if (D == 128)
     return bf16 ? launch_tile<128, true>(p, src, grid, st) : launch_tile<128, false>(p, src, grid, st);
