@@ -286,8 +286,9 @@ MV_API int mv_mask_pad_rows(void* ids, int ids_dtype, int N, int NK, const int* 
 
 /* ---- attention over a paged cache and over packed prompts ----
  *
- * The attention half of a decoder layer, beside the MoE block above (ming-voice leaves it to its attention
- * libraries, engine.py:234-282). Common terms:
+ * The attention half of a decoder layer, beside the MoE block above, with grouped heads (ming-voice has that form for one
+ * token of its Talker, fast_talker.py:166; its main model's own attention, engine.py:234-282, is of another kind and not
+ * here). Inference only. Common terms:
  *  - A batch of B sequences is packed: sequence b owns rows [cu_seqlens[b], cu_seqlens[b + 1]) of the token
  *    tensors (cu_seqlens [B + 1] int32, ascending; a sequence may own no row).
  *  - Heads are grouped: query head h reads key / value head h / G, G = Hq / Hkv (a whole number, 1..64).
@@ -342,11 +343,11 @@ MV_API int mv_kv_append(const mv_kv_append_args* a, void* workspace, size_t work
  * the keys cu_seqlens_k[b] .. cu_seqlens_k[b + 1] of a prompt; NULL cu_seqlens_k: cu_seqlens):
  *   s_j = scale q . k_j,  out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s),  lse = ln sum_j exp(s_j)
  * q, out [T, Hq, head_dim]; lse [T, Hq] f32 contiguous or NULL. A row without a visible key gives out 0 and
- * lse -inf. Scores, maxima, sums and outputs are held in fp32; the weights exp(s - max) are rounded to the element
- * type for their product with v (the tensor cores' operand). Values of masked or unowned slots (of any content,
- * NaN and infinities included) never reach a result, but for one case: a non-finite value row that some queries of
- * a sequence see can reach the other queries of that sequence that are computed in the same tile. max_q is the
- * caller's largest q_len (0: unknown), used to choose a kernel only: a wrong value costs time, not correctness.
+ * lse -inf; rows outside every sequence are left alone. Scores, maxima, sums and outputs are held in fp32; the
+ * weights exp(s - max) are rounded to the element type for their product with v (the tensor cores' operand). Values of
+ * masked or unowned slots (of any content, NaN and infinities included) never reach a result, but for one case: a
+ * non-finite value row that some queries of a sequence see can reach the other queries of that sequence that are
+ * computed in the same tile. max_q is the caller's largest q_len (0: unknown), used to choose a kernel only: a wrong value costs time, not correctness.
  * scale > 0. Results do not depend on the run: fixed summation order. Sequences may be of any length; from 2^31 key tiles
  * (summed over all token tiles and key heads of up to 1024 sequences) on, work is shared by token tiles of a key head, whatever
  * their lengths. cu_seqlens that does not ascend may leave everything out (error 3).

@@ -108,8 +108,10 @@ __device__ __forceinline__ int item_tiles(const Problem& p, const Seq& s, int t)
   return max((keys_seen(p, s, min(s.nq, (t + 1) * p.tok)) + BN - 1) / BN, 1);
 }
 
-// sum of floor((a i + b) / m) over 0 <= i < n (a, b >= 0), as a count of lattice points under a line: whole multiples of m
-// are taken out of a and b, then the axes are exchanged, as in Euclid's algorithm.
+// sum of floor((a i + b) / m) over 0 <= i < n (a, b >= 0): the number of lattice points (i, y), y >= 1, on or under the line
+// (a i + b) / m. Whole multiples of m in a and b are counted outright; then both are below m, and the points are counted along
+// y instead, where the line's slope is m / a: the pair (m, a) shrinks as in Euclid's algorithm. (The reciprocity of such sums:
+// Graham, Knuth, Patashnik, Concrete Mathematics, section 3.5.)
 __device__ __forceinline__ unsigned int floor_sum(unsigned int n, unsigned int m, unsigned int a, unsigned int b) {
   unsigned int sum = 0;
   while (n > 0) {

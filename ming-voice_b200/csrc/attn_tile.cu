@@ -8,9 +8,10 @@
 // multiply-adds (512 + 512 cycles at D = 128) and 16384 exponentials (1024 cycles at 16 a cycle and SM), so the two
 // have to run side by side.
 //
-// Measured on a B200: 20000 causal tokens in 2 prompts, 16 / 4 heads of 128, bf16: 850 us (1232 TFLOP/s, 73 % of the measured
-// burst; 1006 us in a long loop, where power is the bound); 2043 new tokens over 45000 cached 210 us (1082); 9999 tokens, all
-// pairs, 16 / 16 heads of 64, f16: 190 us (606; the exponential unit is busy 75 % of the time).
+// Measured on a B200, call after call: 20000 causal tokens in 2 prompts, 16 / 4 heads of 128, bf16: 998 us (1050 TFLOP/s, 62 % of
+// the measured burst and 73 % of the sustained peak: power is the bound; 855 us in a few calls after a pause); 2043 new tokens
+// over 45000 cached 249 us (913; 210); 9999 tokens, all pairs, 16 / 16 heads of 64, f16: 192 us (598; the exponential unit is
+// busy 75 % of the time).
 //
 // Layout of a CTA (one per SM): a work item is two tiles of 128 rows (row = token * G + head) of one sequence and key
 // head, which share the key and value tiles in shared memory.
@@ -108,10 +109,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// The row's weights 2^(s scale + base) of a tile into TMEM, rounded to the element type there (as operands of the second
-// product); returns their fp32 sum. Bound by the exponential unit: 8 cycles an instruction and scheduler, 1052 for the
-// 128 of a row. (Handing 2 to 8 of 16 pairs to a polynomial of degree 4 or 5 on the FMA pipe gave 1075 to 1219, and
-// longer kernels: the clamp, the rounding and the packed multiplies cost what they relieve.)
+// The row's weights 2^(s scale + base) of a tile into TMEM, rounded to the element type there; returns their fp32 sum. They are
+// rounded because the second product takes 16-bit operands: 32-bit ones (tf32) run at half the rate and would need twice the
+// TMEM columns, which are all taken. The mean relative error of the outputs against 64 bits goes from 1.6e-3 (the result's own
+// rounding) to 2.2e-3 in bf16 (20000 tokens), from 2.1e-4 to 2.9e-4 in f16 (2000 tokens, all pairs).
+// Bound by the exponential unit: 8 cycles an instruction and scheduler, 1052 for the 128 of a row. (Handing 2 to 8 of 16 pairs
+// to a polynomial of degree 4 or 5 on the FMA pipe gave 1075 to 1219, and longer kernels: the clamp, the rounding and the
+// packed multiplies cost what they relieve.)
 template <typename C, bool BF16>
 __device__ __forceinline__ float weights(const uint32_t (&s)[4][32], float base, float scale, uint32_t tP,
                                          uint64_t* half_done) {
@@ -670,7 +674,8 @@ int run_tile(Problem& p, const Source& src, int D, bool bf16, int grid, cudaStre
   p.tok = 2 * (kM / p.G);
   // Short prompts are items of one to four tiles, where most of the time goes into beginning and finishing them: fewer cuts
   // (8 prompts, 2043 tokens: 24.1 us with 5 and 6, 25.9 with 2 and 3). Elsewhere cuts are worth more (24 sequences of a few
-  // tokens over 2500 keys: 23.1 us with 2 and 3, 27.2 with 5 and 6; 9999 tokens in 5 prompts 190 and 197).
+  // tokens over 2500 keys: 23.1 us with 2 and 3, 27.2 with 5 and 6; 9999 tokens in 5 prompts 190 and 197). The host knows the
+  // mean length only, and of a paged cache not even that: a batch that it takes for the other kind is some us slower.
   const bool brief = p.page_table == nullptr && src.max_keys < 512ll * p.B;
   if (brief) cut_rule<5, 6>(p);
   else cut_rule<2, 3>(p);

@@ -4,8 +4,8 @@
 //   (a, b) -> (a cos - b sin, b cos + a sin), in fp32, rounded once to the element type; the rest is copied.
 // Bound: memory (every value is read and written once). A lane owns the same 16 values (two 16-byte vectors) of
 // several heads of one token, so a table row is read once per token and not once per head, and the vectors of all
-// its heads are in flight together. Measured on a B200: 16001 tokens of 16 / 4 heads of 128, 205 MB, 34.3 us (5.97 TB/s, 92 %
-// of the measured copy); one token 2.8 us in a graph.
+// its heads are in flight together. Measured on a B200: 16001 tokens of 16 / 4 heads of 128, 205 MB, 35.3 us call after call
+// (5.8 TB/s, 90 % of the measured copy; 34.3 us in a graph); one token 6.6 to 7.1 us as called, 2.8 us in a graph.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -11,7 +11,7 @@ below it refuses what does not fit and copies what only needs another layout.
 
 Lengths, bounds and page ids are int32 device tensors, read on the device: no call synchronises the host, and a
 captured graph serves whatever lengths its buffers hold at the replay. A call runs on its tensors' device, on that device's
-current stream, whichever device is current.
+current stream, whichever device is current. Inference only: the results of inputs that require a gradient have no history.
 """
 from __future__ import annotations
 
@@ -161,7 +161,7 @@ _ws: dict = {}  # (device, stream) -> address and size of the "attention" worksp
 def kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, *, q=None, q_out=None, cos_sin=None, positions=None,
               interleaved=False):
     """Appends k, v [T, Hkv, D] of T packed new tokens to `cache`, rotating k (and q) by their positions on the way;
-    returns the rotated q ([T, Hq, D]; None without q). kv_lens [B] are the lengths with the new tokens in them:
+    returns the rotated q ([T, Hq, D]; None without q), without a gradient. kv_lens [B] are the lengths with the new tokens in them:
     new token i of n lands at position kv_lens[b] - n + i.
 
     cos_sin: fp32 [max_pos, rot_dim], a position's rot_dim / 2 cosines then its sines (rotation_table); None copies
@@ -214,8 +214,8 @@ def paged_attention(q, cache, page_table, cu_seqlens, kv_lens, *, max_q=None, sc
                     return_lse=False):
     """Attention of the packed new tokens q [T, Hq, D] over the cache, which holds their keys and values already
     (kv_append): out [T, Hq, D], and with return_lse also lse [T, Hq] fp32 (ln of the sum of exp scores; -inf for a
-    row that sees no key, whose out is 0). max_q: the largest number of new tokens of a sequence, where the caller
-    knows it; it only chooses the kernel. scale defaults to 1 / sqrt(D)."""
+    row that sees no key, whose out is 0), without a gradient. max_q: the largest number of new tokens of a sequence,
+    where the caller knows it; it only chooses the kernel. scale defaults to 1 / sqrt(D)."""
     r = (_module or _host()).paged_attention(cache._key[0], cache._key[2], q, page_table, cu_seqlens, kv_lens, max_q,
                                              scale, causal, out, return_lse)
     if type(r) is int:
@@ -243,7 +243,7 @@ def prompt_attention(q, k, v, cu_seqlens, *, cu_seqlens_k=None, max_q=None, scal
                      return_lse=False):
     """Attention over packed prompts: q [Tq, Hq, D], k, v [Tk, Hkv, D], sequence b's queries in rows
     cu_seqlens[b]:cu_seqlens[b + 1] and its keys in the same rows of k and v (or in cu_seqlens_k's). Causal masks
-    align the ends: token i of n sees keys j <= n_keys - n + i. Returns as paged_attention."""
+    align the ends: token i of n sees keys j <= n_keys - n + i. Returns as paged_attention, without a gradient."""
     r = (_module or _host()).prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, max_q, scale, causal, out, return_lse)
     if type(r) is int:
         L.check(r, "prompt_attention")

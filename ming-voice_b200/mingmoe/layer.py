@@ -5,7 +5,7 @@
 
 The projections are the small-linear kernel (norm prologue, residual epilogue) up to 16 tokens and plain GEMMs above;
 the attention is kv_append + paged_attention for new tokens of running sequences, and kv_append + prompt_attention for
-whole prompts, which need not be read back from the cache.
+whole prompts, which need not be read back from the cache. Inference only: nothing here has a backward pass.
 
     seqs = Sequences(num_pages=4096, page_size=64, max_seqs=32, max_len=8192)
     layers = [DecoderLayer(attn, moe, seqs.cache(attn)) for attn, moe in ...]
@@ -118,7 +118,9 @@ class AttentionBlock:
         return paged_attention(q, cache, *where, max_q=batch.max_q)
 
     def output(self, o, x):
-        """x + W_o o, the residual added in fp32 and the sum rounded once."""
+        """x + W_o o. Up to 16 tokens the residual is added in fp32 and the sum rounded once; above, it is the accumulator of
+        the library GEMM, which may round partial sums to bf16 where it splits them (torch.backends.cuda.matmul.
+        allow_bf16_reduced_precision_reduction)."""
         import fastlinear
         o = o.reshape(x.shape[0], -1)
         if x.shape[0] <= moe.DECODE_MAX_M:
