@@ -347,7 +347,8 @@ MV_API int mv_kv_append(const mv_kv_append_args* a, void* workspace, size_t work
  * weights exp(s - max) are rounded to the element type for their product with v (the tensor cores' operand). Values of
  * masked or unowned slots (of any content, NaN and infinities included) never reach a result, but for one case: a
  * non-finite value row that some queries of a sequence see can reach the other queries of that sequence that are
- * computed in the same tile. max_q is the caller's largest q_len (0: unknown), used to choose a kernel only: a wrong value costs time, not correctness.
+ * computed in the same tile. max_q is the caller's largest q_len (0: unknown), used to choose a kernel only: a wrong
+ * value costs time, not correctness.
  * scale > 0. Results do not depend on the run: fixed summation order. Sequences may be of any length; from 2^31 key tiles
  * (summed over all token tiles and key heads of up to 1024 sequences) on, work is shared by token tiles of a key head, whatever
  * their lengths. cu_seqlens that does not ascend may leave everything out (error 3).

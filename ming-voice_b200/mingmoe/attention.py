@@ -161,8 +161,8 @@ _ws: dict = {}  # (device, stream) -> address and size of the "attention" worksp
 def kv_append(cache, k, v, page_table, cu_seqlens, kv_lens, *, q=None, q_out=None, cos_sin=None, positions=None,
               interleaved=False):
     """Appends k, v [T, Hkv, D] of T packed new tokens to `cache`, rotating k (and q) by their positions on the way;
-    returns the rotated q ([T, Hq, D]; None without q), without a gradient. kv_lens [B] are the lengths with the new tokens in them:
-    new token i of n lands at position kv_lens[b] - n + i.
+    returns the rotated q ([T, Hq, D]; None without q), without a gradient. kv_lens [B] are the lengths with the new tokens
+    in them: new token i of n lands at position kv_lens[b] - n + i.
 
     cos_sin: fp32 [max_pos, rot_dim], a position's rot_dim / 2 cosines then its sines (rotation_table); None copies
     without rotating. rot_dim is a multiple of 16 up to D. Pairs are (i, i + rot_dim / 2), or (2i, 2i + 1) when
