@@ -376,6 +376,116 @@ MV_API int mv_prompt_attention(const mv_attention_args* a, void* workspace, size
  * zero-initialised, 256-byte aligned, left as they need it). */
 MV_API size_t mv_attention_workspace_bytes(void);
 
+/* ---- products with 8-bit floating-point weights ----
+ *
+ * y = x W^T (+ residual) with e4m3 values and one scale for each block of 128, as fastlinear.small_linear's counterpart for
+ * weights in 8 bits (no counterpart in the reference).
+ *  x   [T, K] bf16 / f16 (any row stride x_st >= 0 and alignment). Per token and block of 128 columns (the last one may be
+ *      shorter) x is rounded to e4m3 on the way in: a = max |x|, e the smallest integer >= -126 with a <= 448 * 2^e,
+ *      q = e4m3(x * 2^-e) to nearest even, scale 2^e. Products and divisions by powers of two are exact, so q does not depend
+ *      on an order of operations. A block with a NaN or an infinity has scale NaN: the token's results are NaN.
+ *  wq  [N, K] e4m3 bytes (row stride w_st), 16-byte aligned, w_st a multiple of 16 (N = 1: any); ws [ceil(N / 128),
+ *      ceil(K / 128)] f32 (row stride ws_st): W[n, k] = wq[n, k] * ws[n / 128, k / 128].
+ *  y[t, n] = sum over blocks b of (2^e[t, b] * ws[n / 128, b]) * sum over k in b of q[t, k] wq[n, k]  (+ residual[t, n]),
+ *  all in f32, rounded once to out_dtype (bf16, f16 or f32). residual [T, N] has out_dtype or is NULL, row stride r_st; it may
+ *  be `out` itself. Results do not depend on the run: fixed summation order.
+ * scratch: mv_fp8_linear_scratch_bytes(T, N, K) bytes, 256-byte aligned, of any content, not in use by another call that
+ * may run at the same time. workspace: a zeroed header of 256 bytes (error word), which calls may share. */
+typedef struct mv_fp8_linear_args {
+  const void *x, *wq;
+  const float* ws;
+  const void* residual;
+  void* out;
+  void* scratch;
+  long long x_st, w_st, ws_st, r_st, o_st; /* row strides in elements */
+  size_t scratch_bytes;
+  int T, N, K, x_dtype, out_dtype, pad0;
+} mv_fp8_linear_args;
+
+MV_API int mv_fp8_linear(const mv_fp8_linear_args* a, void* workspace, size_t workspace_bytes, void* stream);
+MV_API size_t mv_fp8_linear_scratch_bytes(int T, int N, int K);
+
+/* The rounding of x above by itself: q [T, K] e4m3 bytes (row stride q_st, a multiple of 16 that holds ceil(K / 128) * 128
+ * values; the columns behind K are written with zeros), scale [ceil(K / 128), T] f32 (row stride s_st): a block's scales of all
+ * tokens lie side by side. x as above, or f32. */
+MV_API int mv_quantize_fp8(const void* x, int x_dtype, long long x_st, int T, int K, void* q, long long q_st, float* scale,
+                           long long s_st, void* stream);
+
+/* Weights to e4m3 with a scale for each block of 128 x 128: scale = max |w| / 448 (at least 2^-100), q = e4m3(w / scale) to
+ * nearest even, both quotients in f32; a block that is not finite gets scale NaN. w [N, K] bf16 / f16 / f32 (row stride w_st); q [N, K] (row stride q_st >= K); scale [ceil(N / 128),
+ * ceil(K / 128)] (row stride s_st). */
+MV_API int mv_quantize_fp8_weight(const void* w, int w_dtype, long long w_st, int N, int K, void* q, long long q_st,
+                                  float* scale, long long s_st, void* stream);
+
+/* ---- drawing tokens ----
+ *
+ * One token for each row of logits [B, V] bf16 / f16 / f32 (any row stride st >= 0), from given random numbers. (The reference takes the
+ * argmax, engine.py:974-985.) Tokens are ordered by logit, the larger first, equal ones by index; with
+ * w_i = exp((logit_i - max) / temperature):
+ *   top_k  keeps the first top_k of the order (<= 0, or >= V: all);
+ *   top_p  of these, keeps a token while the weights before it in the order add up to less than top_p times the weights of all
+ *          that top_k kept (>= 1: all);
+ *   min_p  keeps a token with w_i >= min_p (<= 0: all);
+ * the first of the order is always kept. The token drawn is the lowest index whose weight, added to those of all kept tokens of
+ * a lower index, exceeds u times the sum of all kept weights. temperature <= 0 draws the first of the order. NaN settings are
+ * "off" (a NaN temperature: the first of the order; a NaN u: as 0). Weights and sums are held in 64 bits.
+ * Settings are arrays of B values, or NULL: then the value beside them holds for all rows. u [B] f32 in [0, 1) (clamped).
+ * tokens [B] int64; logprob [B] f32 or NULL: ln of the drawn token's share of the kept weights. A row without a token (all
+ * logits -inf, or one NaN) gives token -1 and logprob -inf.
+ * scratch: mv_sample_scratch_bytes(B, V) bytes of any content, 256-byte aligned, as above. */
+typedef struct mv_sample_args {
+  const void* logits;
+  const float *u, *temperature, *top_p, *min_p;
+  const int* top_k;
+  long long* tokens;
+  float* logprob;
+  void* scratch;
+  long long st;
+  size_t scratch_bytes;
+  float temperature_value, top_p_value, min_p_value;
+  int top_k_value, B, V, dtype, pad0;
+} mv_sample_args;
+
+MV_API int mv_sample(const mv_sample_args* a, void* stream);
+MV_API size_t mv_sample_scratch_bytes(int B, int V);
+
+/* ---- pages of the next step, on the device ----
+ *
+ * The state of up to max_seqs sequences of a paged cache: lens [max_seqs] int32 (tokens in the cache), pages [max_seqs,
+ * max_pages] int32 (row stride pages_st; sequence s owns the first ceil(lens[s] / page_size) entries of its row) and a stack
+ * of free page ids: free_pages [num_pages], of which the first n_free[0] are free, the last of them on top.
+ *
+ * mv_plan_step: a step brings new_tokens[b] >= 0 tokens of sequence seqs[b] (NULL: B = max_seqs and sequence b, or B = 0), packed in the
+ * batch's order. The sequences, in that order, take the pages they need from the top of the stack. Written are cu_seqlens
+ * [B + 1], kv_lens [B] (lengths with the new tokens), table [B, max_pages] (row stride table_st; the sequences' pages, zeros
+ * behind them; without seqs: NULL, `pages` is the table), slots [T] int64 (page * page_size + offset of each packed token: its
+ * row of the cache as [num_pages * page_size, ...]) and positions [T] int32 (position of each token in its sequence), where
+ * rows behind the last token get slot -1 and position 0; pages gets its new entries, lens_out and n_free_out the state after
+ * the step (they may be lens and n_free, or buffers that leave those as they are), ok[0] = 1.
+ * A step that asks for a sequence outside the state or twice, a negative number of tokens, more than max_len tokens (or
+ * max_pages pages) of a sequence, more than T tokens or more pages than are free changes nothing: ok[0] = 0, cu_seqlens is 0,
+ * kv_lens are the present lengths (0 outside the state), lens_out and n_free_out the present state.
+ * B <= max_seqs <= 2^18, page_size a power of two in 8..256. scratch: int32 [B + 2].
+ *
+ * mv_release_pages: gives back all pages of B sequences, in that order, the first page of the first below the others; their
+ * lengths become 0. A sequence outside the state or twice, or more pages than free_pages has room for: ok[0] = 0, no change.
+ *
+ * All tensors int32 and contiguous but for the given strides. */
+typedef struct mv_plan_args {
+  const int *new_tokens, *seqs, *lens, *n_free;
+  int *free_pages, *pages;
+  int *lens_out, *n_free_out;
+  int *cu_seqlens, *kv_lens, *table;
+  long long* slots;
+  int *positions, *ok, *scratch;
+  long long pages_st, table_st;
+  int B, max_seqs, max_pages, page_size, max_len, num_pages, T, pad0;
+} mv_plan_args;
+
+MV_API int mv_plan_step(const mv_plan_args* a, void* stream);
+/* Uses seqs, lens, n_free, free_pages, pages, lens_out, n_free_out, ok, pages_st, B, max_seqs, max_pages, page_size, num_pages. */
+MV_API int mv_release_pages(const mv_plan_args* a, void* stream);
+
 /* mv_block_decode without a caller workspace: no counterpart in the reference (its Triton launches take
  * torch-allocated buffers). For callers that cannot allocate device memory or keep a workspace -- a C/FFI
  * host without a device allocator, or code that must not call cudaMalloc while a stream is captured.

@@ -1,0 +1,214 @@
+// Products with 8-bit floating-point weights and a scale for each block of 128 (mv_fp8_linear), and the rounding of activations
+// and weights to that form (mv_quantize_fp8, mv_quantize_fp8_weight).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "attn_common.cuh"
+#include "common.cuh"
+#include "fp8.cuh"
+
+namespace mv {
+namespace fp8 {
+namespace {
+
+// ---------------------------------------------------------------------------------------------- rounding
+
+// Activations: a half warp owns a token's block of 128 columns, 8 values a lane. VEC: values of one load (16, 8 or 4 bytes of
+// a 16-bit type), by the alignment of the rows. Bound: memory.
+template <int DT, int VEC>
+__global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ x, long long x_st, int T, int K, int blocks,
+                                                       uint8_t* __restrict__ q, long long q_st, float* __restrict__ scale,
+                                                       long long s_st) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int sub = threadIdx.x & 15;
+  const long long unit = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const bool real = unit < static_cast<long long>(T) * blocks;
+  const int t = real ? static_cast<int>(unit / blocks) : 0, b = real ? static_cast<int>(unit % blocks) : 0;
+  float v[8];
+  const int c0 = b * kBlock + sub * 8;
+  load8<DT, VEC>(x, t * x_st, c0, real ? K : 0, v);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float up, down;
+  block_scale(top, up, down);
+  if (!real) return;
+  *reinterpret_cast<uint2*>(q + t * q_st + c0) = round8(v, down);
+  if (sub == 0) scale[b * s_st + t] = up;
+}
+
+// Weights: a CTA owns a block of 128 x 128.
+template <int DT>
+__global__ void __launch_bounds__(256) quantize_weight_kernel(const void* __restrict__ w, long long w_st, int N, int K,
+                                                              uint8_t* __restrict__ q, long long q_st,
+                                                              float* __restrict__ scale, long long s_st) {
+  __shared__ float part[8];
+  const int k0 = blockIdx.x * kBlock, n0 = blockIdx.y * kBlock;
+  const int rows = min(kBlock, N - n0), cols = min(kBlock, K - k0);
+  float top = 0.f;
+  bool nan = false;
+  for (int i = threadIdx.x; i < kBlock * kBlock; i += 256) {
+    const int r = i / kBlock, c = i % kBlock;
+    if (r >= rows || c >= cols) continue;
+    const float v = fabsf(load1<DT>(w, (n0 + r) * w_st + k0 + c));
+    nan |= !(v <= 3.4e38f);
+    top = fmaxf(top, v);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+  const bool any_nan = __syncthreads_or(nan);
+  top = part[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) top = fmaxf(top, part[i]);
+  const float s = fmaxf(__fdiv_rn(top, 448.f), 7.888609052210118e-31f);  // 2^-100
+  if (threadIdx.x == 0) scale[blockIdx.y * s_st + blockIdx.x] = any_nan ? __int_as_float(0x7fc00000) : s;
+  for (int i = threadIdx.x; i < kBlock * kBlock; i += 256) {
+    const int r = i / kBlock, c = i % kBlock;
+    if (r >= rows || c >= cols) continue;
+    q[(n0 + r) * q_st + k0 + c] = static_cast<uint8_t>(e4m3x2(__fdiv_rn(load1<DT>(w, (n0 + r) * w_st + k0 + c), s), 0.f) & 0xff);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- the plain product
+
+// A 16 x 16 tile of results per CTA, a block of 128 columns at a time in shared memory.
+template <int ODT>
+__global__ void __launch_bounds__(256) product_kernel(const LinearArgs a) {
+  __shared__ float xs[16][kBlock + 1], wsm[16][kBlock + 1];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int n0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int n = n0 + tx, t = t0 + ty;
+  float acc = 0.f;
+  for (int b = 0; b < a.blocks; ++b) {
+    const int k0 = b * kBlock;
+    for (int i = threadIdx.x; i < 16 * kBlock; i += 256) {
+      const int r = i / kBlock, c = i % kBlock;
+      xs[r][c] = t0 + r < a.T ? e4m3_to_f32(a.q[(t0 + r) * a.q_st + k0 + c]) : 0.f;
+      wsm[r][c] = n0 + r < a.N && k0 + c < a.K ? e4m3_to_f32(a.w[(n0 + r) * a.w_st + k0 + c]) : 0.f;
+    }
+    __syncthreads();
+    float d = 0.f;
+    for (int k = 0; k < kBlock; ++k) d = fmaf(xs[ty][k], wsm[tx][k], d);
+    if (n < a.N && t < a.T) acc = fmaf(d, a.scale[b * a.s_st + t] * a.ws[n / kBlock * a.ws_st + b], acc);
+    __syncthreads();
+  }
+  if (n >= a.N || t >= a.T) return;
+  if (a.residual != nullptr) acc += load1<ODT>(a.residual, t * a.r_st + n);
+  store1<ODT>(a.out, t * a.o_st + n, acc);
+}
+
+template <int DT>
+int launch_quantize(const void* x, long long x_st, int T, int K, uint8_t* q, long long q_st, float* scale, long long s_st,
+                    cudaStream_t st) {
+  const int blocks = (K + kBlock - 1) / kBlock;
+  const long long ctas = (static_cast<long long>(T) * blocks + 15) / 16;
+  if (ctas > 0x7fffffffLL) return fail(MV_ERR_INVALID, "mv_quantize_fp8: T=%d x K=%d is too large", T, K);
+  const int size = DT == MV_F32 ? 4 : 2;
+  const uintptr_t step = reinterpret_cast<uintptr_t>(x) | (T > 1 ? static_cast<uintptr_t>(x_st) * size : 0);
+  auto fn = quantize_kernel<DT, 1>;
+  if (step % (8 * 2) == 0 && K % 8 == 0)
+    fn = quantize_kernel<DT, 8>;
+  else if (step % (4 * 2) == 0 && K % 4 == 0 && DT != MV_F32)
+    fn = quantize_kernel<DT, 4>;
+  return attn::launch_pdl(fn, dim3(static_cast<unsigned int>(ctas)), 256, 0, st, "mv_quantize_fp8 launch", x, x_st, T, K, blocks,
+                          q, q_st, scale, s_st);
+}
+
+int quantize(const void* x, int dtype, long long x_st, int T, int K, uint8_t* q, long long q_st, float* scale, long long s_st,
+             cudaStream_t st) {
+  if (dtype == MV_BF16) return launch_quantize<MV_BF16>(x, x_st, T, K, q, q_st, scale, s_st, st);
+  if (dtype == MV_F16) return launch_quantize<MV_F16>(x, x_st, T, K, q, q_st, scale, s_st, st);
+  return launch_quantize<MV_F32>(x, x_st, T, K, q, q_st, scale, s_st, st);
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace fp8
+}  // namespace mv
+
+using namespace mv;
+using namespace mv::fp8;
+
+extern "C" int mv_quantize_fp8(const void* x, int x_dtype, long long x_st, int T, int K, void* q, long long q_st, float* scale,
+                               long long s_st, void* stream) {
+  const char* who = "mv_quantize_fp8";
+  if (T < 0 || K < 0) return fail(MV_ERR_INVALID, "%s: bad T=%d / K=%d", who, T, K);
+  if (x_dtype != MV_BF16 && x_dtype != MV_F16 && x_dtype != MV_F32)
+    return fail(MV_ERR_UNSUPPORTED, "%s: x must be bf16, f16 or f32", who);
+  if (T == 0 || K == 0) return MV_OK;
+  if (x == nullptr || q == nullptr || scale == nullptr) return fail(MV_ERR_INVALID, "%s: null pointer", who);
+  if (reinterpret_cast<uintptr_t>(x) % (x_dtype == MV_F32 ? 4 : 2) != 0 || !aligned16(q) || q_st % 16 != 0)
+    return fail(MV_ERR_ALIGN, "%s: q must be 16-byte aligned with rows of whole 16 bytes", who);
+  if ((T > 1 && x_st < 0) || q_st < (static_cast<long long>(K) + kBlock - 1) / kBlock * kBlock || s_st < T)
+    return fail(MV_ERR_INVALID, "%s: a row stride is too short for T=%d, K=%d", who, T, K);
+  return quantize(x, x_dtype, x_st, T, K, static_cast<uint8_t*>(q), q_st, scale, s_st, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mv_quantize_fp8_weight(const void* w, int w_dtype, long long w_st, int N, int K, void* q, long long q_st,
+                                      float* scale, long long s_st, void* stream) {
+  const char* who = "mv_quantize_fp8_weight";
+  if (N < 0 || K < 0 || N > 65535 * kBlock) return fail(MV_ERR_INVALID, "%s: bad N=%d / K=%d", who, N, K);
+  if (w_dtype != MV_BF16 && w_dtype != MV_F16 && w_dtype != MV_F32)
+    return fail(MV_ERR_UNSUPPORTED, "%s: w must be bf16, f16 or f32", who);
+  if (N == 0 || K == 0) return MV_OK;
+  if (w == nullptr || q == nullptr || scale == nullptr) return fail(MV_ERR_INVALID, "%s: null pointer", who);
+  const int kb = (K + kBlock - 1) / kBlock, nb = (N + kBlock - 1) / kBlock;
+  if ((N > 1 && (w_st < K || q_st < K)) || (nb > 1 && s_st < kb))
+    return fail(MV_ERR_INVALID, "%s: a row stride is too short for N=%d, K=%d", who, N, K);
+  auto fn = w_dtype == MV_F32 ? quantize_weight_kernel<MV_F32>
+            : w_dtype == MV_F16 ? quantize_weight_kernel<MV_F16>
+                                : quantize_weight_kernel<MV_BF16>;
+  fn<<<dim3(kb, nb), 256, 0, static_cast<cudaStream_t>(stream)>>>(w, w_st, N, K, static_cast<uint8_t*>(q), q_st, scale, s_st);
+  return cuda_status(cudaGetLastError(), "mv_quantize_fp8_weight launch");
+}
+
+extern "C" size_t mv_fp8_linear_scratch_bytes(int T, int, int K) {
+  if (T <= 0 || K <= 0) return 0;
+  const size_t blocks = (static_cast<size_t>(K) + kBlock - 1) / kBlock;
+  return align256(static_cast<size_t>(T) * blocks * kBlock) + align256(blocks * scale_stride(T) * 4);
+}
+
+extern "C" int mv_fp8_linear(const mv_fp8_linear_args* x, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "mv_fp8_linear";
+  if (x == nullptr) return fail(MV_ERR_INVALID, "%s: null pointer", who);
+  const int T = x->T, N = x->N, K = x->K;
+  if (T < 0 || N < 0 || K < 1) return fail(MV_ERR_INVALID, "%s: bad T=%d / N=%d / K=%d", who, T, N, K);
+  if (x->x_dtype != MV_BF16 && x->x_dtype != MV_F16) return fail(MV_ERR_UNSUPPORTED, "%s: x must be bf16 or f16", who);
+  if (x->out_dtype != MV_BF16 && x->out_dtype != MV_F16 && x->out_dtype != MV_F32)
+    return fail(MV_ERR_UNSUPPORTED, "%s: the result must be bf16, f16 or f32", who);
+  if (T == 0 || N == 0) return MV_OK;
+  if (x->x == nullptr || x->wq == nullptr || x->ws == nullptr || x->out == nullptr)
+    return fail(MV_ERR_INVALID, "%s: null pointer", who);
+  const long long blocks = (static_cast<long long>(K) + kBlock - 1) / kBlock;
+  if ((T > 1 && (x->x_st < 0 || x->o_st < N || (x->residual != nullptr && x->r_st < 0))) || (N > 1 && x->w_st < K) ||
+      (N > kBlock && x->ws_st < blocks))
+    return fail(MV_ERR_INVALID, "%s: a row stride is too short for T=%d, N=%d, K=%d", who, T, N, K);
+  if (!aligned16(x->wq) || (N > 1 && x->w_st % 16 != 0))
+    return fail(MV_ERR_ALIGN, "%s: wq must be 16-byte aligned with rows of whole 16 bytes", who);
+  if (workspace == nullptr || workspace_bytes < kWsHeaderBytes)
+    return fail(MV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", who, kWsHeaderBytes);
+  if (x->scratch == nullptr || x->scratch_bytes < mv_fp8_linear_scratch_bytes(T, N, K) ||
+      (reinterpret_cast<uintptr_t>(x->scratch) & 255u))
+    return fail(MV_ERR_WORKSPACE, "%s: 256-byte aligned scratch of %zu bytes needed", who, mv_fp8_linear_scratch_bytes(T, N, K));
+  LinearArgs a{};
+  a.q_st = blocks * kBlock, a.s_st = scale_stride(T), a.blocks = static_cast<int>(blocks);
+  uint8_t* scratch = static_cast<uint8_t*>(x->scratch);
+  a.q = scratch, a.scale = reinterpret_cast<float*>(scratch + align256(static_cast<size_t>(T) * a.q_st));
+  a.w = static_cast<const uint8_t*>(x->wq), a.w_st = N > 1 ? x->w_st : a.q_st, a.ws = x->ws, a.ws_st = x->ws_st;
+  a.residual = x->residual, a.r_st = x->r_st, a.out = x->out, a.o_st = x->o_st;
+  a.T = T, a.N = N, a.K = K, a.header = static_cast<WsHeader*>(workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int rc = quantize(x->x, x->x_dtype, x->x_st, T, K, a.q, a.q_st, a.scale, a.s_st, st);
+  if (rc != MV_OK) return rc;
+  auto fn = x->out_dtype == MV_F32 ? product_kernel<MV_F32> : x->out_dtype == MV_F16 ? product_kernel<MV_F16> : product_kernel<MV_BF16>;
+  return attn::launch_pdl(fn, dim3((N + 15) / 16, (T + 15) / 16), 256, 0, st, "mv_fp8_linear launch", a);
+}

@@ -70,6 +70,29 @@ class AttentionArgs(C.Structure):
                 [("scale", F32), ("pad0", I32)])
 
 
+class Fp8LinearArgs(C.Structure):
+    """mirror of `mv_fp8_linear_args`"""
+    _fields_ = ([(n, P) for n in ("x", "wq", "ws", "residual", "out", "scratch")] +
+                [(n, I64) for n in ("x_st", "w_st", "ws_st", "r_st", "o_st")] + [("scratch_bytes", SZ)] +
+                [(n, I32) for n in ("T", "N", "K", "x_dtype", "out_dtype", "pad0")])
+
+
+class SampleArgs(C.Structure):
+    """mirror of `mv_sample_args`"""
+    _fields_ = ([(n, P) for n in ("logits", "u", "temperature", "top_p", "min_p", "top_k", "tokens", "logprob", "scratch")] +
+                [("st", I64), ("scratch_bytes", SZ)] +
+                [(n, F32) for n in ("temperature_value", "top_p_value", "min_p_value")] +
+                [(n, I32) for n in ("top_k_value", "B", "V", "dtype", "pad0")])
+
+
+class PlanArgs(C.Structure):
+    """mirror of `mv_plan_args`"""
+    _fields_ = ([(n, P) for n in ("new_tokens", "seqs", "lens", "n_free", "free_pages", "pages", "lens_out", "n_free_out",
+                                  "cu_seqlens", "kv_lens", "table", "slots", "positions", "ok", "scratch")] +
+                [(n, I64) for n in ("pages_st", "table_st")] +
+                [(n, I32) for n in ("B", "max_seqs", "max_pages", "page_size", "max_len", "num_pages", "T", "pad0")])
+
+
 _SIGS = {
     "mv_version": (I32, []),
     "mv_last_error": (C.c_char_p, []),
@@ -105,6 +128,14 @@ _SIGS = {
     "mv_paged_attention": (I32, [P, P, SZ, P]),
     "mv_prompt_attention": (I32, [P, P, SZ, P]),
     "mv_attention_workspace_bytes": (SZ, []),
+    "mv_fp8_linear": (I32, [P, P, SZ, P]),
+    "mv_fp8_linear_scratch_bytes": (SZ, [I32, I32, I32]),
+    "mv_quantize_fp8": (I32, [P, I32, I64, I32, I32, P, I64, P, I64, P]),
+    "mv_quantize_fp8_weight": (I32, [P, I32, I64, I32, I32, P, I64, P, I64, P]),
+    "mv_sample": (I32, [P, P]),
+    "mv_sample_scratch_bytes": (SZ, [I32, I32]),
+    "mv_plan_step": (I32, [P, P]),
+    "mv_release_pages": (I32, [P, P]),
     "mv_ep_combine": (I32, [P, I64, P, P, I32, P, I32, I32, I32, P, P]),
 }
 
