@@ -75,36 +75,6 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const void* __rest
   }
 }
 
-// ---------------------------------------------------------------------------------------------- the plain product
-
-// A 16 x 16 tile of results per CTA, a block of 128 columns at a time in shared memory.
-template <int ODT>
-__global__ void __launch_bounds__(256) product_kernel(const LinearArgs a) {
-  __shared__ float xs[16][kBlock + 1], wsm[16][kBlock + 1];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int n0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int n = n0 + tx, t = t0 + ty;
-  float acc = 0.f;
-  for (int b = 0; b < a.blocks; ++b) {
-    const int k0 = b * kBlock;
-    for (int i = threadIdx.x; i < 16 * kBlock; i += 256) {
-      const int r = i / kBlock, c = i % kBlock;
-      xs[r][c] = t0 + r < a.T ? e4m3_to_f32(a.q[(t0 + r) * a.q_st + k0 + c]) : 0.f;
-      wsm[r][c] = n0 + r < a.N && k0 + c < a.K ? e4m3_to_f32(a.w[(n0 + r) * a.w_st + k0 + c]) : 0.f;
-    }
-    __syncthreads();
-    float d = 0.f;
-    for (int k = 0; k < kBlock; ++k) d = fmaf(xs[ty][k], wsm[tx][k], d);
-    if (n < a.N && t < a.T) acc = fmaf(d, a.scale[b * a.s_st + t] * a.ws[n / kBlock * a.ws_st + b], acc);
-    __syncthreads();
-  }
-  if (n >= a.N || t >= a.T) return;
-  if (a.residual != nullptr) acc += load1<ODT>(a.residual, t * a.r_st + n);
-  store1<ODT>(a.out, t * a.o_st + n, acc);
-}
-
 template <int DT>
 int launch_quantize(const void* x, long long x_st, int T, int K, uint8_t* q, long long q_st, float* scale, long long s_st,
                     cudaStream_t st) {
@@ -209,6 +179,5 @@ extern "C" int mv_fp8_linear(const mv_fp8_linear_args* x, void* workspace, size_
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int rc = quantize(x->x, x->x_dtype, x->x_st, T, K, a.q, a.q_st, a.scale, a.s_st, st);
   if (rc != MV_OK) return rc;
-  auto fn = x->out_dtype == MV_F32 ? product_kernel<MV_F32> : x->out_dtype == MV_F16 ? product_kernel<MV_F16> : product_kernel<MV_BF16>;
-  return attn::launch_pdl(fn, dim3((N + 15) / 16, (T + 15) / 16), 256, 0, st, "mv_fp8_linear launch", a);
+  return run_product(a, x->out_dtype, st);
 }

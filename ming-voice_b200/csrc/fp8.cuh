@@ -23,6 +23,9 @@ struct LinearArgs {
   WsHeader* header;
 };
 
+// the products (fp8_gemm.cu); w is 16-byte aligned with rows of whole 16 bytes, q and scale are in the scratch
+int run_product(const LinearArgs& a, int out_dtype, cudaStream_t st);
+
 // row stride of the activations' scales: rows begin at whole 16 bytes
 inline long long scale_stride(int T) { return (static_cast<long long>(T) + 3) / 4 * 4; }
 

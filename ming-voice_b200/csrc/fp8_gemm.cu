@@ -1,0 +1,495 @@
+// The products of mv_fp8_linear on the 5th-generation tensor cores.
+//
+// y[t, n] = sum_b sx[t, b] ws[n / 128, b] * (q[t, block b] . w[n, block b]). The tensor cores give one block's product at a
+// time in TMEM (kind::f8f6f4, 128 values of K: four instructions); the epilogue warps read it while the next block runs in the
+// other buffer, and add it in fp32 registers with its factor. Two forms of the same pipeline (TMA warp, issuing warp, epilogue
+// warps; a ring of stages with one weight tile and one activation tile each):
+//   few tokens  weights are the 128-row operand and up to 128 tokens the columns, so a tile is a weight stream of 16 KB
+//               blocks; a cluster shares a tile's blocks of K where there are fewer tiles than SMs and adds the parts over
+//               distributed shared memory in rank order.
+//   many tokens 128 tokens are the rows and 256 weight rows the columns: an epilogue thread owns one token, so a block's
+//               factor is one number per thread.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "attn_common.cuh"
+#include "common.cuh"
+#include "fp8.cuh"
+#include "tc.cuh"
+
+namespace mv {
+namespace fp8 {
+namespace {
+
+// D[tmem] (+)= A[smem] * B[smem]^T, e4m3 operands, fp32 accumulation, 32 values of K; issued by one thread.
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+
+// kind::f8f6f4: fp32 accumulator (bits 4-5 = 1), both operands e4m3 (0) and K-major, N >> 3 (17-22), M >> 4 (24-28)
+constexpr uint32_t idesc_e4m3(int M, int N) {
+  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// the 16-byte aligned 1-D copy that brings a block's activation scales along with its tiles
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[N]) {
+  if constexpr (N == 16)
+    tc::tmem_ld16(addr, r);
+  else
+    tc::tmem_ld32(addr, r);
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the value at shared address `addr` of the cluster's CTA `rank`
+__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// mbar_wait with its first try inline: the call's register moves stay off the usual path
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, WsHeader* h, unsigned int info) {
+  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, h, info);
+}
+
+constexpr int kTile = 128;                     // rows of the 128-row operand
+constexpr uint32_t kTileBytes = kTile * kBlock;  // 16 KB
+
+// ------------------------------------------------------------------------------------------------ few tokens
+
+struct FewArgs {
+  const float *ws, *scale;
+  const void* residual;
+  void* out;
+  long long ws_st, s_st, r_st, o_st;
+  int T, N, blocks, n_tiles, t_tiles, split;
+  WsHeader* header;
+};
+
+// NT token columns of a tile. Stage: weight tile, activation tile, activation scales.
+template <int NT>
+struct Few {
+  static constexpr int kStages = NT <= 32 ? 9 : NT == 64 ? 8 : 6;
+  static constexpr uint32_t kXBytes = NT * kBlock;
+  static constexpr uint32_t kStageBytes = kTileBytes + kXBytes;
+  static constexpr int kHalves = NT == 128 ? 2 : 1;  // epilogue warps per 32 rows
+  static constexpr int kCols = NT / kHalves;         // columns of an epilogue thread
+  static constexpr int kThreads = 64 + 128 * kHalves;
+  static constexpr uint32_t kTmemCols = 2 * NT < 32 ? 32 : 2 * NT;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * (kStageBytes + NT * 4);
+};
+
+template <int NT, int ODT>
+__global__ void __launch_bounds__(Few<NT>::kThreads, 1)
+    few_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const FewArgs a) {
+  using F = Few<NT>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  float* scales = reinterpret_cast<float*>(smem + F::kStages * F::kStageBytes);  // [stage][NT]
+  __shared__ alignas(8) uint64_t full[F::kStages], empty[F::kStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kEpiWarps = 4 * F::kHalves;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < F::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1 + kEpiWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpiWarps);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(&tmem_base, F::kTmemCols);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int first = blockIdx.x / a.split, step = gridDim.x / a.split;
+  const int tiles = a.n_tiles * a.t_tiles;
+  // the cluster's CTAs take equal contiguous shares of the blocks of K
+  const int b0 = a.blocks * rank / a.split, b1 = a.blocks * (rank + 1) / a.split;
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (tc::elect_one()) {
+      tc::prefetch_tmap(&wmap);
+      tc::prefetch_tmap(&xmap);
+      pdl_wait();
+      const uint32_t scale_bytes = static_cast<uint32_t>(min(static_cast<long long>(NT), a.s_st)) * 4;
+      int it = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        const int n0 = tile / a.t_tiles * kTile, t0 = tile % a.t_tiles * NT;
+        const uint32_t sb = min(scale_bytes, static_cast<uint32_t>(a.s_st - t0) * 4);
+        for (int b = b0; b < b1; ++b, ++it) {
+          const int s = it % F::kStages;
+          if (it >= F::kStages && !wait(&empty[s], (it / F::kStages + 1) & 1, a.header, 0x800u)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * F::kStageBytes;
+          mbar_arrive_expect_tx(&full[s], F::kStageBytes + sb);
+          tc::tma_load_2d(st, &wmap, &full[s], b * kBlock, n0);
+          tc::tma_load_2d(st + kTileBytes, &xmap, &full[s], b * kBlock, t0);
+          bulk_load(scales + s * NT, a.scale + b * a.s_st + t0, sb, &full[s]);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    int it = 0;
+    bool ok = true;
+    for (int tile = first; tile < tiles && ok; tile += step) {
+      for (int b = b0; b < b1; ++b, ++it) {
+        const int s = it % F::kStages, buf = it & 1;
+        if (!wait(&full[s], (it / F::kStages) & 1, a.header, 0x801u) ||
+            (it >= 2 && !wait(&acc_empty[buf], (it / 2 + 1) & 1, a.header, 0x802u))) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+        if (tc::elect_one()) {
+          const uint32_t base = smem_u32(smem + s * F::kStageBytes);
+          const uint64_t ad = tc::sw128_desc(base), bd = tc::sw128_desc(base + kTileBytes);
+#pragma unroll
+          for (int k = 0; k < kBlock / 32; ++k) mma_f8(tmem + buf * NT, ad + 2 * k, bd + 2 * k, idesc_e4m3(kTile, NT), k > 0);
+          tc::mma_commit(&empty[s]);
+          tc::mma_commit(&acc_full[buf]);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    const int e = warp - 2, quarter = warp & 3, c0 = e / 4 * F::kCols;  // the warp reads TMEM lanes 32 * quarter ..
+    const int row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
+    pdl_wait();
+    int it = 0;
+    bool ok = true;
+    for (int tile = first; tile < tiles; tile += step) {
+      const int n0 = tile / a.t_tiles * kTile, t0 = tile % a.t_tiles * NT;
+      float acc[F::kCols];
+#pragma unroll
+      for (int c = 0; c < F::kCols; ++c) acc[c] = 0.f;
+      const float* ws = a.ws + n0 / kBlock * a.ws_st;
+      float w_next = b0 < b1 ? ws[b0] : 0.f;
+      for (int b = b0; b < b1 && ok; ++b, ++it) {
+        const int s = it % F::kStages, buf = it & 1;
+        const float w = w_next;
+        if (b + 1 < b1) w_next = ws[b + 1];
+        if (!wait(&acc_full[buf], (it / 2) & 1, a.header, 0x803u)) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+        constexpr int kLd = F::kCols < 32 ? 16 : 32;
+        const float4* sc = reinterpret_cast<const float4*>(scales + s * NT + c0);
+#pragma unroll
+        for (int c = 0; c < F::kCols; c += kLd) {
+          uint32_t d[kLd];
+          tmem_load<kLd>(lanes + buf * NT + c, d);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < kLd; i += 4) {
+            const float4 f = sc[(c + i) / 4];
+            acc[c + i] = fmaf(__uint_as_float(d[i]), f.x * w, acc[c + i]);
+            acc[c + i + 1] = fmaf(__uint_as_float(d[i + 1]), f.y * w, acc[c + i + 1]);
+            acc[c + i + 2] = fmaf(__uint_as_float(d[i + 2]), f.z * w, acc[c + i + 2]);
+            acc[c + i + 3] = fmaf(__uint_as_float(d[i + 3]), f.w * w, acc[c + i + 3]);
+          }
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&acc_empty[buf]);
+          mbar_arrive(&empty[s]);
+        }
+      }
+      const int n = n0 + row;
+      if (a.split == 1) {
+        if (n < a.N && ok) {
+#pragma unroll
+          for (int c = 0; c < F::kCols; ++c) {
+            const int t = t0 + c0 + c;
+            if (t >= a.T) break;
+            float v = acc[c];
+            if (a.residual != nullptr) v += load1<ODT>(a.residual, t * a.r_st + n);
+            store1<ODT>(a.out, t * a.o_st + n, v);
+          }
+        }
+      } else {
+        // the parts lie where the ring was: its copies have landed and its products are done
+        float* part = reinterpret_cast<float*>(smem);  // [NT][128]
+        named_bar(1, 128 * F::kHalves);
+#pragma unroll
+        for (int c = 0; c < F::kCols; ++c) part[(c0 + c) * kTile + row] = acc[c];
+      }
+    }
+  }
+  if (a.split > 1) {
+    __syncwarp();
+    pdl_wait();
+    cluster_sync();
+    // every CTA adds the parts of its share of the columns, in rank order
+    const int tile = first, n0 = tile / a.t_tiles * kTile, t0 = tile % a.t_tiles * NT;
+    const uint32_t part = smem_u32(smem);
+    const int cols = min(NT, a.T - t0);
+    for (int i = threadIdx.x + rank * F::kThreads; i < cols * kTile; i += F::kThreads * a.split) {
+      const int t = t0 + i / kTile, n = n0 + i % kTile;
+      if (n >= a.N) continue;
+      float v = 0.f;
+      for (int r = 0; r < a.split; ++r) v += ld_peer(part + i * 4, r);
+      if (a.residual != nullptr) v += load1<ODT>(a.residual, t * a.r_st + n);
+      store1<ODT>(a.out, t * a.o_st + n, v);
+    }
+    cluster_sync();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, F::kTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ many tokens
+
+constexpr int kManyStages = 4, kManyN = 256;
+constexpr uint32_t kManyStageBytes = kTileBytes + kManyN * kBlock;  // 48 KB
+constexpr size_t kManySmem = 1024 + kManyStages * kManyStageBytes;
+constexpr int kManyThreads = 64 + 256;
+
+template <int ODT>
+__global__ void __launch_bounds__(kManyThreads, 1)
+    many_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const FewArgs a) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ alignas(8) uint64_t full[kManyStages], empty[kManyStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kManyStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 8);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(&tmem_base, 512);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  const int tiles = a.n_tiles * a.t_tiles;
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (tc::elect_one()) {
+      tc::prefetch_tmap(&wmap);
+      tc::prefetch_tmap(&xmap);
+      pdl_wait();
+      int it = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+        const int t0 = tile % a.t_tiles * kTile, n0 = tile / a.t_tiles * kManyN;
+        for (int b = 0; b < a.blocks; ++b, ++it) {
+          const int s = it % kManyStages;
+          if (it >= kManyStages && !wait(&empty[s], (it / kManyStages + 1) & 1, a.header, 0x810u)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * kManyStageBytes;
+          mbar_arrive_expect_tx(&full[s], kManyStageBytes);
+          tc::tma_load_2d(st, &xmap, &full[s], b * kBlock, t0);
+          tc::tma_load_2d(st + kTileBytes, &wmap, &full[s], b * kBlock, n0);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    int it = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      for (int b = 0; b < a.blocks; ++b, ++it) {
+        const int s = it % kManyStages, buf = it & 1;
+        if (!wait(&full[s], (it / kManyStages) & 1, a.header, 0x811u) ||
+            (it >= 2 && !wait(&acc_empty[buf], (it / 2 + 1) & 1, a.header, 0x812u))) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+        if (tc::elect_one()) {
+          const uint32_t base = smem_u32(smem + s * kManyStageBytes);
+          const uint64_t ad = tc::sw128_desc(base), bd = tc::sw128_desc(base + kTileBytes);
+#pragma unroll
+          for (int k = 0; k < kBlock / 32; ++k)
+            mma_f8(tmem + buf * kManyN, ad + 2 * k, bd + 2 * k, idesc_e4m3(kTile, kManyN), k > 0);
+          tc::mma_commit(&empty[s]);
+          tc::mma_commit(&acc_full[buf]);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    const int half = (warp - 2) / 4, quarter = warp & 3;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+    pdl_wait();
+    int it = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      const int t = tile % a.t_tiles * kTile + quarter * 32 + lane, n0 = tile / a.t_tiles * kManyN + half * 128;
+      const float* sx = a.scale + min(t, a.T - 1);
+      const float* ws = a.ws + min(n0, a.N - 1) / kBlock * a.ws_st;
+      float acc[128];
+#pragma unroll
+      for (int c = 0; c < 128; ++c) acc[c] = 0.f;
+      float f_next = sx[0] * ws[0];
+      for (int b = 0; b < a.blocks; ++b, ++it) {
+        const int buf = it & 1;
+        const float f = f_next;
+        if (b + 1 < a.blocks) f_next = sx[(b + 1) * a.s_st] * ws[b + 1];
+        if (!wait(&acc_full[buf], (it / 2) & 1, a.header, 0x813u)) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t d[32];
+          tc::tmem_ld32(lanes + buf * kManyN + c, d);
+          tc::tmem_ld_wait();
+          if (c == 96) {
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            ffma2(acc[c + i], acc[c + i + 1], __uint_as_float(d[i]), __uint_as_float(d[i + 1]), f, f);
+        }
+      }
+      if (t >= a.T || !ok) continue;
+#pragma unroll
+      for (int c = 0; c < 128; ++c) {
+        const int n = n0 + c;
+        if (n >= a.N) break;
+        float v = acc[c];
+        if (a.residual != nullptr) v += load1<ODT>(a.residual, t * a.r_st + n);
+        store1<ODT>(a.out, t * a.o_st + n, v);
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+int byte_map(CUtensorMap* m, const void* base, int cols, int rows, long long stride, int box_rows, const char* what) {
+  static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  if (enc == nullptr) return fail(MV_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
+  const cuuint32_t box[2] = {kBlock, static_cast<cuuint32_t>(box_rows)}, estr[2] = {1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MV_ERR_INVALID, "tensor map for %s rejected (CUresult %d)", what, static_cast<int>(r));
+  return MV_OK;
+}
+
+template <typename K>
+int launch(K fn, int grid, int threads, size_t smem, int cluster, cudaStream_t st, const CUtensorMap& wm, const CUtensorMap& xm,
+           const FewArgs& a) {
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(mv_fp8_linear)");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, fn, wm, xm, a), "mv_fp8_linear launch");
+}
+
+template <int NT, int ODT>
+int run_few(const LinearArgs& x, cudaStream_t st) {
+  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, x.header};
+  a.n_tiles = (x.N + kTile - 1) / kTile;
+  a.t_tiles = (x.T + NT - 1) / NT;
+  CUtensorMap wm, xm;
+  int rc = byte_map(&wm, x.w, x.K, x.N, x.w_st, kTile, "wq");
+  if (rc == MV_OK) rc = byte_map(&xm, x.q, static_cast<int>(x.q_st), x.T, x.q_st, NT, "the activations");
+  if (rc != MV_OK) return rc;
+  const long long tiles = static_cast<long long>(a.n_tiles) * a.t_tiles;
+  if (tiles > 0x7fffffffLL) return fail(MV_ERR_INVALID, "mv_fp8_linear: T=%d x N=%d is too large", x.T, x.N);
+  const int sms = num_sms();
+  while (a.split < 8 && tiles * a.split * 2 <= sms && a.split * 2 <= a.blocks) a.split *= 2;
+  const int grid = a.split > 1 ? static_cast<int>(tiles) * a.split : static_cast<int>(tiles < sms ? tiles : sms);
+  return launch(few_kernel<NT, ODT>, grid, Few<NT>::kThreads, Few<NT>::kSmem, a.split, st, wm, xm, a);
+}
+
+template <int ODT>
+int run_typed(const LinearArgs& x, cudaStream_t st) {
+  if (x.T <= 16) return run_few<16, ODT>(x, st);
+  if (x.T <= 32) return run_few<32, ODT>(x, st);
+  if (x.T <= 64) return run_few<64, ODT>(x, st);
+  const long long tiles = static_cast<long long>((x.N + kManyN - 1) / kManyN) * ((x.T + kTile - 1) / kTile);
+  if (tiles > 0x7fffffffLL) return fail(MV_ERR_INVALID, "mv_fp8_linear: T=%d x N=%d is too large", x.T, x.N);
+  if (tiles < num_sms() / 2) return run_few<128, ODT>(x, st);
+  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, x.header};
+  a.n_tiles = (x.N + kManyN - 1) / kManyN;
+  a.t_tiles = (x.T + kTile - 1) / kTile;
+  CUtensorMap wm, xm;
+  int rc = byte_map(&wm, x.w, x.K, x.N, x.w_st, kManyN, "wq");
+  if (rc == MV_OK) rc = byte_map(&xm, x.q, static_cast<int>(x.q_st), x.T, x.q_st, kTile, "the activations");
+  if (rc != MV_OK) return rc;
+  const int sms = num_sms();
+  return launch(many_kernel<ODT>, static_cast<int>(tiles < sms ? tiles : sms), kManyThreads, kManySmem, 1, st, wm, xm, a);
+}
+
+}  // namespace
+
+int run_product(const LinearArgs& x, int out_dtype, cudaStream_t st) {
+  if (out_dtype == MV_F32) return run_typed<MV_F32>(x, st);
+  if (out_dtype == MV_F16) return run_typed<MV_F16>(x, st);
+  return run_typed<MV_BF16>(x, st);
+}
+
+}  // namespace fp8
+}  // namespace mv
