@@ -53,6 +53,16 @@ __device__ __forceinline__ float2 unpack(uint32_t w) {
   return __half22float2(h);
 }
 
+template <int DT>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  if (DT == MV_BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // Values c0 .. c0 + 7 of the row at element offset `row`; zeros from column K on. VEC (of 16-bit types): 8 and 4 load 16 and 8
 // bytes at a time, where row and K allow it; f32 with VEC 8 loads 16 bytes twice.
 template <int DT, int VEC>

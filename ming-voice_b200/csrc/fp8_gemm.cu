@@ -67,9 +67,28 @@ __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
   return v;
 }
 
-// mbar_wait with its first try inline: the call's register moves stay off the usual path
+// mbar_wait inline: a call would save the epilogue's 128 sums around it
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, WsHeader* h, unsigned int info) {
-  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, h, info);
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      raise_error(h, kErrTimeout, info);
+      return false;
+    }
+  return true;
+}
+
+// the loads into d have landed: what uses d comes behind it for the compiler too
+__device__ __forceinline__ void landed(uint32_t (&d)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]), "+r"(d[4]), "+r"(d[5]), "+r"(d[6]), "+r"(d[7]), "+r"(d[8]),
+                 "+r"(d[9]), "+r"(d[10]), "+r"(d[11]), "+r"(d[12]), "+r"(d[13]), "+r"(d[14]), "+r"(d[15]), "+r"(d[16]),
+                 "+r"(d[17]), "+r"(d[18]), "+r"(d[19]), "+r"(d[20]), "+r"(d[21]), "+r"(d[22]), "+r"(d[23]), "+r"(d[24]),
+                 "+r"(d[25]), "+r"(d[26]), "+r"(d[27]), "+r"(d[28]), "+r"(d[29])
+               :
+               : "memory");
+  asm volatile("" : "+r"(d[30]), "+r"(d[31]) : : "memory");
 }
 
 constexpr int kTile = 128;                     // rows of the 128-row operand
@@ -275,8 +294,70 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
 
 constexpr int kManyStages = 4, kManyN = 256;
 constexpr uint32_t kManyStageBytes = kTileBytes + kManyN * kBlock;  // 48 KB
-constexpr size_t kManySmem = 1024 + kManyStages * kManyStageBytes;
-constexpr int kManyThreads = 64 + 256;
+constexpr uint32_t kLineBytes = 32 * 128;                           // an epilogue warp's staging of 32 rows
+constexpr size_t kManySmem = 1024 + kManyStages * kManyStageBytes + 8 * kLineBytes;
+constexpr int kManyThreads = 128 + 256;
+
+// 16 bytes of a warp's staging: 32 rows of 128 bytes, chunk j of row r at j ^ (r & 7), so that both a row per lane and a
+// line per 8 lanes are without bank conflicts
+__device__ __forceinline__ uint4* staged(uint8_t* buf, int r, int j) {
+  return reinterpret_cast<uint4*>(buf + r * 128 + ((j ^ (r & 7)) * 16));
+}
+
+// Moves 32 rows x 128 bytes between the staging and global memory, whole lines at a time where rows start at 16-byte addresses
+// (aligned), else an element per lane. `rows` and `cols`: what lies inside the tensor.
+template <int SIZE, bool STORE>
+__device__ __forceinline__ void move_lines(uint8_t* buf, void* global, long long stride, int rows, int cols, bool aligned, int lane) {
+  constexpr int kElems = 128 / SIZE, kChunk = 16 / SIZE;
+  uint8_t* g = static_cast<uint8_t*>(global);
+  if (aligned) {
+#pragma unroll 2
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + lane / 8, j = lane % 8;
+      if (r >= rows) continue;
+      uint8_t* p = g + (r * stride) * SIZE + j * 16;
+      if ((j + 1) * kChunk <= cols) {
+        if (STORE)
+          *reinterpret_cast<uint4*>(p) = *staged(buf, r, j);
+        else
+          *staged(buf, r, j) = *reinterpret_cast<const uint4*>(p);
+      } else {
+        uint8_t* q = reinterpret_cast<uint8_t*>(staged(buf, r, j));
+        for (int c = 0; j * kChunk + c < cols && c < kChunk; ++c) {
+          if (SIZE == 4) {
+            if (STORE) reinterpret_cast<uint32_t*>(p)[c] = reinterpret_cast<uint32_t*>(q)[c];
+            else reinterpret_cast<uint32_t*>(q)[c] = reinterpret_cast<uint32_t*>(p)[c];
+          } else {
+            if (STORE) reinterpret_cast<uint16_t*>(p)[c] = reinterpret_cast<uint16_t*>(q)[c];
+            else reinterpret_cast<uint16_t*>(q)[c] = reinterpret_cast<uint16_t*>(p)[c];
+          }
+        }
+      }
+    }
+    return;
+  }
+  for (int r = 0; r < rows; ++r) {
+#pragma unroll
+    for (int c = lane; c < kElems; c += 32) {
+      if (c >= cols) continue;
+      uint8_t* p = g + (r * stride + c) * SIZE;
+      uint8_t* q = reinterpret_cast<uint8_t*>(staged(buf, r, c / kChunk)) + c % kChunk * SIZE;
+      if (SIZE == 4) {
+        if (STORE) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<uint32_t*>(q);
+        else *reinterpret_cast<uint32_t*>(q) = *reinterpret_cast<uint32_t*>(p);
+      } else {
+        if (STORE) *reinterpret_cast<uint16_t*>(p) = *reinterpret_cast<uint16_t*>(q);
+        else *reinterpret_cast<uint16_t*>(q) = *reinterpret_cast<uint16_t*>(p);
+      }
+    }
+  }
+}
+
+// 32 TMEM columns times the factor, added to acc[0..31]
+__device__ __forceinline__ void add32(const uint32_t (&d)[32], float f, float* acc) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) ffma2(acc[i], acc[i + 1], __uint_as_float(d[i]), __uint_as_float(d[i + 1]), f, f);
+}
 
 template <int ODT>
 __global__ void __launch_bounds__(kManyThreads, 1)
@@ -302,61 +383,70 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   const int tiles = a.n_tiles * a.t_tiles;
   pdl_launch_dependents();
 
-  if (warp == 0) {
-    if (tc::elect_one()) {
-      tc::prefetch_tmap(&wmap);
-      tc::prefetch_tmap(&xmap);
-      pdl_wait();
+  // 384 threads start with 168 registers each (64512); the epilogue's 256 take 224, the other 128 keep 40 (62464)
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      if (tc::elect_one()) {
+        tc::prefetch_tmap(&wmap);
+        tc::prefetch_tmap(&xmap);
+        pdl_wait();
+        int it = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+          const int t0 = tile % a.t_tiles * kTile, n0 = tile / a.t_tiles * kManyN;
+          for (int b = 0; b < a.blocks; ++b, ++it) {
+            const int s = it % kManyStages;
+            if (it >= kManyStages && !wait(&empty[s], (it / kManyStages + 1) & 1, a.header, 0x810u)) {
+              ok = false;
+              break;
+            }
+            uint8_t* st = smem + s * kManyStageBytes;
+            mbar_arrive_expect_tx(&full[s], kManyStageBytes);
+            tc::tma_load_2d(st, &xmap, &full[s], b * kBlock, t0);
+            tc::tma_load_2d(st + kTileBytes, &wmap, &full[s], b * kBlock, n0);
+          }
+        }
+      }
+    } else if (warp == 1) {
       int it = 0;
       bool ok = true;
       for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-        const int t0 = tile % a.t_tiles * kTile, n0 = tile / a.t_tiles * kManyN;
         for (int b = 0; b < a.blocks; ++b, ++it) {
-          const int s = it % kManyStages;
-          if (it >= kManyStages && !wait(&empty[s], (it / kManyStages + 1) & 1, a.header, 0x810u)) {
+          const int s = it % kManyStages, buf = it & 1;
+          if (!wait(&full[s], (it / kManyStages) & 1, a.header, 0x811u) ||
+              (it >= 2 && !wait(&acc_empty[buf], (it / 2 + 1) & 1, a.header, 0x812u))) {
             ok = false;
             break;
           }
-          uint8_t* st = smem + s * kManyStageBytes;
-          mbar_arrive_expect_tx(&full[s], kManyStageBytes);
-          tc::tma_load_2d(st, &xmap, &full[s], b * kBlock, t0);
-          tc::tma_load_2d(st + kTileBytes, &wmap, &full[s], b * kBlock, n0);
-        }
-      }
-    }
-  } else if (warp == 1) {
-    int it = 0;
-    bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-      for (int b = 0; b < a.blocks; ++b, ++it) {
-        const int s = it % kManyStages, buf = it & 1;
-        if (!wait(&full[s], (it / kManyStages) & 1, a.header, 0x811u) ||
-            (it >= 2 && !wait(&acc_empty[buf], (it / 2 + 1) & 1, a.header, 0x812u))) {
-          ok = false;
-          break;
-        }
-        tc::fence_after_sync();
-        if (tc::elect_one()) {
-          const uint32_t base = smem_u32(smem + s * kManyStageBytes);
-          const uint64_t ad = tc::sw128_desc(base), bd = tc::sw128_desc(base + kTileBytes);
+          tc::fence_after_sync();
+          if (tc::elect_one()) {
+            const uint32_t base = smem_u32(smem + s * kManyStageBytes);
+            const uint64_t ad = tc::sw128_desc(base), bd = tc::sw128_desc(base + kTileBytes);
 #pragma unroll
-          for (int k = 0; k < kBlock / 32; ++k)
-            mma_f8(tmem + buf * kManyN, ad + 2 * k, bd + 2 * k, idesc_e4m3(kTile, kManyN), k > 0);
-          tc::mma_commit(&empty[s]);
-          tc::mma_commit(&acc_full[buf]);
+            for (int k = 0; k < kBlock / 32; ++k)
+              mma_f8(tmem + buf * kManyN, ad + 2 * k, bd + 2 * k, idesc_e4m3(kTile, kManyN), k > 0);
+            tc::mma_commit(&empty[s]);
+            tc::mma_commit(&acc_full[buf]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
     }
   } else {
-    const int half = (warp - 2) / 4, quarter = warp & 3;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    constexpr int kSize = ODT == MV_F32 ? 4 : 2, kPart = 128 / kSize;  // columns that a row of the staging holds
+    const int half = (warp - 4) / 4, quarter = warp & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+    uint8_t* line = smem + kManyStages * kManyStageBytes + (warp - 4) * kLineBytes;
+    const bool out_lines = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.o_st * kSize)) & 15) == 0;
+    const bool res_lines = ((reinterpret_cast<uintptr_t>(a.residual) | static_cast<uintptr_t>(a.r_st * kSize)) & 15) == 0;
     pdl_wait();
     int it = 0;
     bool ok = true;
     for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-      const int t = tile % a.t_tiles * kTile + quarter * 32 + lane, n0 = tile / a.t_tiles * kManyN + half * 128;
-      const float* sx = a.scale + min(t, a.T - 1);
+      const int t0 = tile % a.t_tiles * kTile + quarter * 32, n0 = tile / a.t_tiles * kManyN + half * 128;
+      const float* sx = a.scale + min(t0 + lane, a.T - 1);
       const float* ws = a.ws + min(n0, a.N - 1) / kBlock * a.ws_st;
       float acc[128];
 #pragma unroll
@@ -371,29 +461,64 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           break;
         }
         tc::fence_after_sync();
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t d[32];
-          tc::tmem_ld32(lanes + buf * kManyN + c, d);
-          tc::tmem_ld_wait();
-          if (c == 96) {
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
-          }
-#pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            ffma2(acc[c + i], acc[c + i + 1], __uint_as_float(d[i]), __uint_as_float(d[i + 1]), f, f);
-        }
+        // a load of 32 columns is under way while the last 32 are added
+        uint32_t d0[32], d1[32];
+        const uint32_t src = lanes + buf * kManyN;
+        tc::tmem_ld32(src, d0);
+        landed(d0);
+        tc::tmem_ld32(src + 32, d1);
+        add32(d0, f, acc);
+        landed(d1);
+        tc::tmem_ld32(src + 64, d0);
+        add32(d1, f, acc + 32);
+        landed(d0);
+        tc::tmem_ld32(src + 96, d1);
+        add32(d0, f, acc + 64);
+        landed(d1);
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        add32(d1, f, acc + 96);
       }
-      if (t >= a.T || !ok) continue;
+      const int rows = min(32, a.T - t0);
+      if (rows <= 0 || !ok) continue;
 #pragma unroll
-      for (int c = 0; c < 128; ++c) {
-        const int n = n0 + c;
-        if (n >= a.N) break;
-        float v = acc[c];
-        if (a.residual != nullptr) v += load1<ODT>(a.residual, t * a.r_st + n);
-        store1<ODT>(a.out, t * a.o_st + n, v);
+      for (int p = 0; p < 128 / kPart; ++p) {
+        const int n = n0 + p * kPart, cols = a.N - n;
+        if (cols <= 0) break;
+        __syncwarp();
+        if (a.residual != nullptr) {
+          move_lines<kSize, false>(line, static_cast<uint8_t*>(const_cast<void*>(a.residual)) + (t0 * a.r_st + n) * kSize,
+                                   a.r_st, rows, cols, res_lines, lane);
+          __syncwarp();
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint4* slot = staged(line, lane, j);
+          const float* v = acc + p * kPart + j * (16 / kSize);
+          if constexpr (kSize == 4) {
+            float4 o = make_float4(v[0], v[1], v[2], v[3]);
+            if (a.residual != nullptr) {
+              const float4 r = *reinterpret_cast<const float4*>(slot);
+              o.x += r.x, o.y += r.y, o.z += r.z, o.w += r.w;
+            }
+            *reinterpret_cast<float4*>(slot) = o;
+          } else {
+            uint32_t w[4];
+            uint4 r = make_uint4(0u, 0u, 0u, 0u);
+            if (a.residual != nullptr) r = *slot;
+            const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 add = unpack<ODT>(rr[i]);
+              w[i] = pack<ODT>(v[2 * i] + add.x, v[2 * i + 1] + add.y);
+            }
+            *slot = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        __syncwarp();
+        move_lines<kSize, true>(line, static_cast<uint8_t*>(a.out) + (t0 * a.o_st + n) * kSize, a.o_st, rows, cols, out_lines,
+                                lane);
       }
     }
   }
