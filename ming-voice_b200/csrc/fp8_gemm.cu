@@ -69,14 +69,18 @@ __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
 
 // mbar_wait inline: a call would save the epilogue's 128 sums around it
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, WsHeader* h, unsigned int info) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity))
-    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+  uint64_t t0 = 0;
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t now = globaltimer_ns();  // (reading it takes longer than most waits)
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
       raise_error(h, kErrTimeout, info);
       return false;
     }
-  return true;
+  }
 }
 
 // the loads into d have landed: what uses d comes behind it for the compiler too
@@ -102,6 +106,7 @@ struct FewArgs {
   void* out;
   long long ws_st, s_st, r_st, o_st;
   int T, N, blocks, n_tiles, t_tiles, split;
+  bool out_lines;  // whole lines of `out` go through its tensor map
   WsHeader* header;
 };
 
@@ -291,12 +296,61 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
 }
 
 // ------------------------------------------------------------------------------------------------ many tokens
+//
+// Two CTAs of a cluster work on one tile of 256 tokens x 256 weight rows (cta_group::2): each brings 128 rows of either
+// operand, 32 KB a block instead of 48, and holds the products of its 128 tokens. One CTA with a 128 x 256 tile was bound by
+// that traffic (16001 x 5632 x 2048 without reading its products: 200 us).
 
-constexpr int kManyStages = 4, kManyN = 256;
-constexpr uint32_t kManyStageBytes = kTileBytes + kManyN * kBlock;  // 48 KB
-constexpr uint32_t kLineBytes = 32 * 128;                           // an epilogue warp's staging of 32 rows
-constexpr size_t kManySmem = 1024 + kManyStages * kManyStageBytes + 8 * kLineBytes;
+constexpr int kManyStages = 5, kManyN = 256, kManyT = 256;
+constexpr uint32_t kManyStageBytes = 2 * kTileBytes;  // 32 KB
+constexpr uint32_t kLineBytes = 32 * 128;             // 32 rows of a warp's staging, two of these per warp
+constexpr size_t kManySmem = 1024 + kManyStages * kManyStageBytes + 8 * 2 * kLineBytes;
 constexpr int kManyThreads = 128 + 256;
+
+__device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+
+// a tile into this CTA's shared memory, counted on the barrier at cluster address `bar`
+__device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+
+// arrives on `bar` in both CTAs when the products issued so far are done
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                   smem_u32(bar)),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
+}
+
+// 32 rows of 128 bytes from shared memory to (x, y) of a tensor; what lies outside it is left out
+__device__ __forceinline__ void store_lines(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(smem_u32(src))
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// all but the last N stores have been read from shared memory
+template <int N>
+__device__ __forceinline__ void stores_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
 
 // 16 bytes of a warp's staging: 32 rows of 128 bytes, chunk j of row r at j ^ (r & 7), so that both a row per lane and a
 // line per 8 lanes are without bank conflicts
@@ -353,34 +407,38 @@ __device__ __forceinline__ void move_lines(uint8_t* buf, void* global, long long
   }
 }
 
-// 32 TMEM columns times the factor, added to acc[0..31]
-__device__ __forceinline__ void add32(const uint32_t (&d)[32], float f, float* acc) {
+// 32 TMEM columns times the factor (a pair of equal halves), added to the pairs acc[0..15]
+__device__ __forceinline__ void add32(const uint32_t (&d)[32], uint64_t f, uint64_t* acc) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 2) ffma2(acc[i], acc[i + 1], __uint_as_float(d[i]), __uint_as_float(d[i + 1]), f, f);
+  for (int i = 0; i < 16; ++i)
+    asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(acc[i]) : "r"(d[2 * i]), "r"(d[2 * i + 1]), "l"(f));
 }
 
 template <int ODT>
 __global__ void __launch_bounds__(kManyThreads, 1)
-    many_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const FewArgs a) {
+    many_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
+                const __grid_constant__ CUtensorMap omap, const FewArgs a) {
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   __shared__ alignas(8) uint64_t full[kManyStages], empty[kManyStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kManyStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 8);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 16);
     fence_mbar_init();
   }
   if (warp == 1) {
-    tc::tmem_alloc(&tmem_base, 512);
-    tc::tmem_relinquish();
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc::fence_before_sync();
   __syncthreads();
+  cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_base;
-  const int tiles = a.n_tiles * a.t_tiles;
+  const int tiles = a.n_tiles * a.t_tiles, first = blockIdx.x / 2, step = gridDim.x / 2;
   pdl_launch_dependents();
 
   // 384 threads start with 168 registers each (64512); the epilogue's 256 take 224, the other 128 keep 40 (62464)
@@ -390,28 +448,31 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       if (tc::elect_one()) {
         tc::prefetch_tmap(&wmap);
         tc::prefetch_tmap(&xmap);
+        tc::prefetch_tmap(&omap);
         pdl_wait();
         int it = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-          const int t0 = tile % a.t_tiles * kTile, n0 = tile / a.t_tiles * kManyN;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+          const int t0 = tile % a.t_tiles * kManyT + rank * 128, n0 = tile / a.t_tiles * kManyN + rank * 128;
           for (int b = 0; b < a.blocks; ++b, ++it) {
             const int s = it % kManyStages;
             if (it >= kManyStages && !wait(&empty[s], (it / kManyStages + 1) & 1, a.header, 0x810u)) {
               ok = false;
               break;
             }
+            // the first CTA's barrier counts both CTAs' tiles
             uint8_t* st = smem + s * kManyStageBytes;
-            mbar_arrive_expect_tx(&full[s], kManyStageBytes);
-            tc::tma_load_2d(st, &xmap, &full[s], b * kBlock, t0);
-            tc::tma_load_2d(st + kTileBytes, &wmap, &full[s], b * kBlock, n0);
+            const uint32_t bar = peer_addr(&full[s], 0);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kManyStageBytes);
+            pair_load(st, &xmap, bar, b * kBlock, t0);
+            pair_load(st + kTileBytes, &wmap, bar, b * kBlock, n0);
           }
         }
       }
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {
       int it = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      for (int tile = first; tile < tiles && ok; tile += step) {
         for (int b = 0; b < a.blocks; ++b, ++it) {
           const int s = it % kManyStages, buf = it & 1;
           if (!wait(&full[s], (it / kManyStages) & 1, a.header, 0x811u) ||
@@ -425,9 +486,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const uint64_t ad = tc::sw128_desc(base), bd = tc::sw128_desc(base + kTileBytes);
 #pragma unroll
             for (int k = 0; k < kBlock / 32; ++k)
-              mma_f8(tmem + buf * kManyN, ad + 2 * k, bd + 2 * k, idesc_e4m3(kTile, kManyN), k > 0);
-            tc::mma_commit(&empty[s]);
-            tc::mma_commit(&acc_full[buf]);
+              pair_mma(tmem + buf * kManyN, ad + 2 * k, bd + 2 * k, idesc_e4m3(kManyT, kManyN), k > 0);
+            pair_commit(&empty[s]);
+            pair_commit(&acc_full[buf]);
           }
           __syncwarp();
         }
@@ -438,24 +499,27 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     constexpr int kSize = ODT == MV_F32 ? 4 : 2, kPart = 128 / kSize;  // columns that a row of the staging holds
     const int half = (warp - 4) / 4, quarter = warp & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
-    uint8_t* line = smem + kManyStages * kManyStageBytes + (warp - 4) * kLineBytes;
-    const bool out_lines = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.o_st * kSize)) & 15) == 0;
+    uint8_t* lines = smem + kManyStages * kManyStageBytes + (warp - 4) * 2 * kLineBytes;
+    const uint32_t freed[2] = {peer_addr(&acc_empty[0], 0), peer_addr(&acc_empty[1], 0)};
     const bool res_lines = ((reinterpret_cast<uintptr_t>(a.residual) | static_cast<uintptr_t>(a.r_st * kSize)) & 15) == 0;
     pdl_wait();
-    int it = 0;
+    int it = 0, turn = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-      const int t0 = tile % a.t_tiles * kTile + quarter * 32, n0 = tile / a.t_tiles * kManyN + half * 128;
+    for (int tile = first; tile < tiles && ok; tile += step) {
+      const int t0 = tile % a.t_tiles * kManyT + rank * 128 + quarter * 32, n0 = tile / a.t_tiles * kManyN + half * 128;
       const float* sx = a.scale + min(t0 + lane, a.T - 1);
       const float* ws = a.ws + min(n0, a.N - 1) / kBlock * a.ws_st;
-      float acc[128];
+      uint64_t acc[64];  // pairs of columns
 #pragma unroll
-      for (int c = 0; c < 128; ++c) acc[c] = 0.f;
-      float f_next = sx[0] * ws[0];
+      for (int c = 0; c < 64; ++c) acc[c] = 0;
+      // scales are read two blocks ahead, and multiplied only when their block has come: warps issue in order
+      const int last = a.blocks - 1;
+      float s_next = sx[0], w_next = ws[0], s_then = sx[min(1, last) * a.s_st], w_then = ws[min(1, last)];
       for (int b = 0; b < a.blocks; ++b, ++it) {
         const int buf = it & 1;
-        const float f = f_next;
-        if (b + 1 < a.blocks) f_next = sx[(b + 1) * a.s_st] * ws[b + 1];
+        const float s_now = s_next, w_now = w_next;
+        s_next = s_then, w_next = w_then;
+        if (b + 2 <= last) s_then = sx[(b + 2) * a.s_st], w_then = ws[b + 2];
         if (!wait(&acc_full[buf], (it / 2) & 1, a.header, 0x813u)) {
           ok = false;
           break;
@@ -463,6 +527,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         tc::fence_after_sync();
         // a load of 32 columns is under way while the last 32 are added
         uint32_t d0[32], d1[32];
+        const float f1 = s_now * w_now;
+        uint64_t f;
+        asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "f"(f1));
         const uint32_t src = lanes + buf * kManyN;
         tc::tmem_ld32(src, d0);
         landed(d0);
@@ -470,15 +537,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         add32(d0, f, acc);
         landed(d1);
         tc::tmem_ld32(src + 64, d0);
-        add32(d1, f, acc + 32);
+        add32(d1, f, acc + 16);
         landed(d0);
         tc::tmem_ld32(src + 96, d1);
-        add32(d0, f, acc + 64);
+        add32(d0, f, acc + 32);
         landed(d1);
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
-        add32(d1, f, acc + 96);
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(freed[buf]) : "memory");
+        add32(d1, f, acc + 48);
       }
       const int rows = min(32, a.T - t0);
       if (rows <= 0 || !ok) continue;
@@ -486,6 +554,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       for (int p = 0; p < 128 / kPart; ++p) {
         const int n = n0 + p * kPart, cols = a.N - n;
         if (cols <= 0) break;
+        uint8_t* line = lines + (turn++ & 1) * kLineBytes;
+        if (a.out_lines && lane == 0) stores_read<1>();  // the store before the last was from here
         __syncwarp();
         if (a.residual != nullptr) {
           move_lines<kSize, false>(line, static_cast<uint8_t*>(const_cast<void*>(a.residual)) + (t0 * a.r_st + n) * kSize,
@@ -495,7 +565,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           uint4* slot = staged(line, lane, j);
-          const float* v = acc + p * kPart + j * (16 / kSize);
+          float v[16 / kSize];
+#pragma unroll
+          for (int i = 0; i < 8 / kSize; ++i)
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(v[2 * i]), "=f"(v[2 * i + 1]) : "l"(acc[(p * kPart + j * (16 / kSize)) / 2 + i]));
           if constexpr (kSize == 4) {
             float4 o = make_float4(v[0], v[1], v[2], v[3]);
             if (a.residual != nullptr) {
@@ -516,23 +589,31 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             *slot = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        __syncwarp();
-        move_lines<kSize, true>(line, static_cast<uint8_t*>(a.out) + (t0 * a.o_st + n) * kSize, a.o_st, rows, cols, out_lines,
-                                lane);
+        if (a.out_lines) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) store_lines(&omap, line, n, t0);
+        } else {
+          __syncwarp();
+          move_lines<kSize, true>(line, static_cast<uint8_t*>(a.out) + (t0 * a.o_st + n) * kSize, a.o_st, rows, cols, false, lane);
+        }
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc::fence_before_sync();
   __syncthreads();
+  cluster_sync();
   if (warp == 1) {
     tc::fence_after_sync();
-    tc::tmem_dealloc(tmem, 512);
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
 }
 
 // ------------------------------------------------------------------------------------------------ host
 
-int byte_map(CUtensorMap* m, const void* base, int cols, int rows, long long stride, int box_rows, const char* what) {
+// a [rows, cols] tensor of `size`-byte elements (1, 2 or 4; rows of `stride` bytes) in boxes of 128 bytes x box_rows
+int row_map(CUtensorMap* m, const void* base, int size, int cols, int rows, long long stride, int box_rows, const char* what) {
   static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -544,17 +625,19 @@ int byte_map(CUtensorMap* m, const void* base, int cols, int rows, long long str
   if (enc == nullptr) return fail(MV_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
-  const cuuint32_t box[2] = {kBlock, static_cast<cuuint32_t>(box_rows)}, estr[2] = {1, 1};
-  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), static_cast<cuuint32_t>(box_rows)}, estr[2] = {1, 1};
+  const CUtensorMapDataType type = size == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_UINT32;
+  const CUresult r = enc(m, type, 2, const_cast<void*>(base), dims, strides, box, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(MV_ERR_INVALID, "tensor map for %s rejected (CUresult %d)", what, static_cast<int>(r));
   return MV_OK;
 }
 
-template <typename K>
-int launch(K fn, int grid, int threads, size_t smem, int cluster, cudaStream_t st, const CUtensorMap& wm, const CUtensorMap& xm,
-           const FewArgs& a) {
+template <typename... P, typename... A>
+int launch(void (*fn)(P...), int grid, int threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(mv_fp8_linear)");
   cudaLaunchConfig_t cfg = {};
@@ -569,17 +652,17 @@ int launch(K fn, int grid, int threads, size_t smem, int cluster, cudaStream_t s
   attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, fn, wm, xm, a), "mv_fp8_linear launch");
+  return cuda_status(cudaLaunchKernelEx(&cfg, fn, args...), "mv_fp8_linear launch");
 }
 
 template <int NT, int ODT>
 int run_few(const LinearArgs& x, cudaStream_t st) {
-  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, x.header};
+  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, false, x.header};
   a.n_tiles = (x.N + kTile - 1) / kTile;
   a.t_tiles = (x.T + NT - 1) / NT;
   CUtensorMap wm, xm;
-  int rc = byte_map(&wm, x.w, x.K, x.N, x.w_st, kTile, "wq");
-  if (rc == MV_OK) rc = byte_map(&xm, x.q, static_cast<int>(x.q_st), x.T, x.q_st, NT, "the activations");
+  int rc = row_map(&wm, x.w, 1, x.K, x.N, x.w_st, kTile, "wq");
+  if (rc == MV_OK) rc = row_map(&xm, x.q, 1, static_cast<int>(x.q_st), x.T, x.q_st, NT, "the activations");
   if (rc != MV_OK) return rc;
   const long long tiles = static_cast<long long>(a.n_tiles) * a.t_tiles;
   if (tiles > 0x7fffffffLL) return fail(MV_ERR_INVALID, "mv_fp8_linear: T=%d x N=%d is too large", x.T, x.N);
@@ -594,18 +677,23 @@ int run_typed(const LinearArgs& x, cudaStream_t st) {
   if (x.T <= 16) return run_few<16, ODT>(x, st);
   if (x.T <= 32) return run_few<32, ODT>(x, st);
   if (x.T <= 64) return run_few<64, ODT>(x, st);
-  const long long tiles = static_cast<long long>((x.N + kManyN - 1) / kManyN) * ((x.T + kTile - 1) / kTile);
+  const long long tiles = static_cast<long long>((x.N + kManyN - 1) / kManyN) * ((x.T + kManyT - 1) / kManyT);
   if (tiles > 0x7fffffffLL) return fail(MV_ERR_INVALID, "mv_fp8_linear: T=%d x N=%d is too large", x.T, x.N);
-  if (tiles < num_sms() / 2) return run_few<128, ODT>(x, st);
-  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, x.header};
+  const int pairs = num_sms() / 2;
+  if (tiles < pairs / 2) return run_few<128, ODT>(x, st);
+  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, false, x.header};
   a.n_tiles = (x.N + kManyN - 1) / kManyN;
-  a.t_tiles = (x.T + kTile - 1) / kTile;
-  CUtensorMap wm, xm;
-  int rc = byte_map(&wm, x.w, x.K, x.N, x.w_st, kManyN, "wq");
-  if (rc == MV_OK) rc = byte_map(&xm, x.q, static_cast<int>(x.q_st), x.T, x.q_st, kTile, "the activations");
+  a.t_tiles = (x.T + kManyT - 1) / kManyT;
+  const int size = ODT == MV_F32 ? 4 : 2;
+  a.out_lines = aligned16(x.out) && x.o_st * size % 16 == 0;
+  CUtensorMap wm, xm, om;
+  int rc = row_map(&wm, x.w, 1, x.K, x.N, x.w_st, 128, "wq");
+  if (rc == MV_OK) rc = row_map(&xm, x.q, 1, static_cast<int>(x.q_st), x.T, x.q_st, 128, "the activations");
+  om = xm;
+  if (rc == MV_OK && a.out_lines) rc = row_map(&om, x.out, size, x.N, x.T, x.o_st * size, 32, "out");
   if (rc != MV_OK) return rc;
-  const int sms = num_sms();
-  return launch(many_kernel<ODT>, static_cast<int>(tiles < sms ? tiles : sms), kManyThreads, kManySmem, 1, st, wm, xm, a);
+  return launch(many_kernel<ODT>, static_cast<int>(tiles < pairs ? tiles : pairs) * 2, kManyThreads, kManySmem, 2, st, wm, xm, om,
+                a);
 }
 
 }  // namespace
