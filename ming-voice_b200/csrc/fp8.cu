@@ -16,10 +16,11 @@ namespace {
 // ---------------------------------------------------------------------------------------------- rounding
 
 // Activations: a half warp owns a token's block of 128 columns, 8 values a lane. VEC: values of one load (16, 8 or 4 bytes of
-// a 16-bit type), by the alignment of the rows. Bound: memory.
-template <int DT, int VEC>
+// a 16-bit type), by the alignment of the rows. Scales as fp32 numbers, or as their exponents' bytes: a block that is not finite
+// has NaNs among its rounded values, so the products are NaN whatever its exponent says. Bound: memory.
+template <int DT, int VEC, typename S>
 __global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ x, long long x_st, int T, int K, int blocks,
-                                                       uint8_t* __restrict__ q, long long q_st, float* __restrict__ scale,
+                                                       uint8_t* __restrict__ q, long long q_st, S* __restrict__ scale,
                                                        long long s_st) {
   pdl_launch_dependents();
   pdl_wait();
@@ -39,7 +40,12 @@ __global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ 
   block_scale(top, up, down);
   if (!real) return;
   *reinterpret_cast<uint2*>(q + t * q_st + c0) = round8(v, down);
-  if (sub == 0) scale[b * s_st + t] = up;
+  if (sub == 0) {
+    if constexpr (sizeof(S) == 1)
+      scale[b * s_st + t] = static_cast<uint8_t>(__float_as_uint(up) >> 23);
+    else
+      scale[b * s_st + t] = up;
+  }
 }
 
 // Weights: a CTA owns a block of 128 x 128.
@@ -75,24 +81,25 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const void* __rest
   }
 }
 
-template <int DT>
-int launch_quantize(const void* x, long long x_st, int T, int K, uint8_t* q, long long q_st, float* scale, long long s_st,
+template <int DT, typename S>
+int launch_quantize(const void* x, long long x_st, int T, int K, uint8_t* q, long long q_st, S* scale, long long s_st,
                     cudaStream_t st) {
   const int blocks = (K + kBlock - 1) / kBlock;
   const long long ctas = (static_cast<long long>(T) * blocks + 15) / 16;
   if (ctas > 0x7fffffffLL) return fail(MV_ERR_INVALID, "mv_quantize_fp8: T=%d x K=%d is too large", T, K);
   const int size = DT == MV_F32 ? 4 : 2;
   const uintptr_t step = reinterpret_cast<uintptr_t>(x) | (T > 1 ? static_cast<uintptr_t>(x_st) * size : 0);
-  auto fn = quantize_kernel<DT, 1>;
+  auto fn = quantize_kernel<DT, 1, S>;
   if (step % (8 * 2) == 0 && K % 8 == 0)
-    fn = quantize_kernel<DT, 8>;
+    fn = quantize_kernel<DT, 8, S>;
   else if (step % (4 * 2) == 0 && K % 4 == 0 && DT != MV_F32)
-    fn = quantize_kernel<DT, 4>;
+    fn = quantize_kernel<DT, 4, S>;
   return attn::launch_pdl(fn, dim3(static_cast<unsigned int>(ctas)), 256, 0, st, "mv_quantize_fp8 launch", x, x_st, T, K, blocks,
                           q, q_st, scale, s_st);
 }
 
-int quantize(const void* x, int dtype, long long x_st, int T, int K, uint8_t* q, long long q_st, float* scale, long long s_st,
+template <typename S>
+int quantize(const void* x, int dtype, long long x_st, int T, int K, uint8_t* q, long long q_st, S* scale, long long s_st,
              cudaStream_t st) {
   if (dtype == MV_BF16) return launch_quantize<MV_BF16>(x, x_st, T, K, q, q_st, scale, s_st, st);
   if (dtype == MV_F16) return launch_quantize<MV_F16>(x, x_st, T, K, q, q_st, scale, s_st, st);
@@ -144,7 +151,7 @@ extern "C" int mv_quantize_fp8_weight(const void* w, int w_dtype, long long w_st
 extern "C" size_t mv_fp8_linear_scratch_bytes(int T, int, int K) {
   if (T <= 0 || K <= 0) return 0;
   const size_t blocks = (static_cast<size_t>(K) + kBlock - 1) / kBlock;
-  return align256(static_cast<size_t>(T) * blocks * kBlock) + align256(blocks * scale_stride(T) * 4);
+  return align256(static_cast<size_t>(T) * blocks * kBlock) + align256(blocks * scale_stride(T));
 }
 
 extern "C" int mv_fp8_linear(const mv_fp8_linear_args* x, void* workspace, size_t workspace_bytes, void* stream) {
@@ -172,7 +179,7 @@ extern "C" int mv_fp8_linear(const mv_fp8_linear_args* x, void* workspace, size_
   LinearArgs a{};
   a.q_st = blocks * kBlock, a.s_st = scale_stride(T), a.blocks = static_cast<int>(blocks);
   uint8_t* scratch = static_cast<uint8_t*>(x->scratch);
-  a.q = scratch, a.scale = reinterpret_cast<float*>(scratch + align256(static_cast<size_t>(T) * a.q_st));
+  a.q = scratch, a.scale = scratch + align256(static_cast<size_t>(T) * a.q_st);
   a.w = static_cast<const uint8_t*>(x->wq), a.w_st = N > 1 ? x->w_st : a.q_st, a.ws = x->ws, a.ws_st = x->ws_st;
   a.residual = x->residual, a.r_st = x->r_st, a.out = x->out, a.o_st = x->o_st;
   a.T = T, a.N = N, a.K = K, a.header = static_cast<WsHeader*>(workspace);

@@ -15,7 +15,7 @@ struct LinearArgs {
   const uint8_t* w;        // [N, K] e4m3
   const float* ws;         // [N / 128, K / 128]
   uint8_t* q;              // activations [T, blocks * 128] e4m3
-  float* scale;            // [blocks, T]
+  uint8_t* scale;          // [blocks, T]: the exponents of the powers of two, 127 added (an fp32 number's)
   const void* residual;
   void* out;
   long long w_st, ws_st, q_st, s_st, r_st, o_st;
@@ -27,7 +27,7 @@ struct LinearArgs {
 int run_product(const LinearArgs& a, int out_dtype, cudaStream_t st);
 
 // row stride of the activations' scales: rows begin at whole 16 bytes
-inline long long scale_stride(int T) { return (static_cast<long long>(T) + 3) / 4 * 4; }
+inline long long scale_stride(int T) { return (static_cast<long long>(T) + 15) / 16 * 16; }
 
 template <int DT>
 __device__ __forceinline__ float load1(const void* p, long long i) {

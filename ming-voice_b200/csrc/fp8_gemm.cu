@@ -42,6 +42,19 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+// 32 lanes x 64 consecutive 32-bit columns
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, "
+      "%42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr));
+}
+
+// the exponent byte `i` of `w` as a power of two
+__device__ __forceinline__ float power(uint32_t w, int i) { return __uint_as_float((w >> (8 * i) & 0xffu) << 23); }
+
 template <int N>
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[N]) {
   if constexpr (N == 16)
@@ -84,15 +97,11 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, WsHeader* h
 }
 
 // the loads into d have landed: what uses d comes behind it for the compiler too
-__device__ __forceinline__ void landed(uint32_t (&d)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]), "+r"(d[4]), "+r"(d[5]), "+r"(d[6]), "+r"(d[7]), "+r"(d[8]),
-                 "+r"(d[9]), "+r"(d[10]), "+r"(d[11]), "+r"(d[12]), "+r"(d[13]), "+r"(d[14]), "+r"(d[15]), "+r"(d[16]),
-                 "+r"(d[17]), "+r"(d[18]), "+r"(d[19]), "+r"(d[20]), "+r"(d[21]), "+r"(d[22]), "+r"(d[23]), "+r"(d[24]),
-                 "+r"(d[25]), "+r"(d[26]), "+r"(d[27]), "+r"(d[28]), "+r"(d[29])
-               :
-               : "memory");
-  asm volatile("" : "+r"(d[30]), "+r"(d[31]) : : "memory");
+__device__ __forceinline__ void landed(uint32_t (&d)[64]) {
+  tc::tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 64; i += 16)
+    asm volatile("" : "+r"(d[i + 0]), "+r"(d[i + 1]), "+r"(d[i + 2]), "+r"(d[i + 3]), "+r"(d[i + 4]), "+r"(d[i + 5]), "+r"(d[i + 6]), "+r"(d[i + 7]), "+r"(d[i + 8]), "+r"(d[i + 9]), "+r"(d[i + 10]), "+r"(d[i + 11]), "+r"(d[i + 12]), "+r"(d[i + 13]), "+r"(d[i + 14]), "+r"(d[i + 15]) : : "memory");
 }
 
 constexpr int kTile = 128;                     // rows of the 128-row operand
@@ -101,7 +110,8 @@ constexpr uint32_t kTileBytes = kTile * kBlock;  // 16 KB
 // ------------------------------------------------------------------------------------------------ few tokens
 
 struct FewArgs {
-  const float *ws, *scale;
+  const float* ws;
+  const uint8_t* scale;
   const void* residual;
   void* out;
   long long ws_st, s_st, r_st, o_st;
@@ -120,7 +130,7 @@ struct Few {
   static constexpr int kCols = NT / kHalves;         // columns of an epilogue thread
   static constexpr int kThreads = 64 + 128 * kHalves;
   static constexpr uint32_t kTmemCols = 2 * NT < 32 ? 32 : 2 * NT;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * (kStageBytes + NT * 4);
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * (kStageBytes + NT);
 };
 
 template <int NT, int ODT>
@@ -129,7 +139,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
   using F = Few<NT>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  float* scales = reinterpret_cast<float*>(smem + F::kStages * F::kStageBytes);  // [stage][NT]
+  uint8_t* scales = smem + F::kStages * F::kStageBytes;  // [stage][NT]
   __shared__ alignas(8) uint64_t full[F::kStages], empty[F::kStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -159,12 +169,11 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
       tc::prefetch_tmap(&wmap);
       tc::prefetch_tmap(&xmap);
       pdl_wait();
-      const uint32_t scale_bytes = static_cast<uint32_t>(min(static_cast<long long>(NT), a.s_st)) * 4;
       int it = 0;
       bool ok = true;
       for (int tile = first; tile < tiles && ok; tile += step) {
         const int n0 = tile / a.t_tiles * kTile, t0 = tile % a.t_tiles * NT;
-        const uint32_t sb = min(scale_bytes, static_cast<uint32_t>(a.s_st - t0) * 4);
+        const uint32_t sb = static_cast<uint32_t>(min(static_cast<long long>(NT), a.s_st - t0));
         for (int b = b0; b < b1; ++b, ++it) {
           const int s = it % F::kStages;
           if (it >= F::kStages && !wait(&empty[s], (it / F::kStages + 1) & 1, a.header, 0x800u)) {
@@ -226,7 +235,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
         }
         tc::fence_after_sync();
         constexpr int kLd = F::kCols < 32 ? 16 : 32;
-        const float4* sc = reinterpret_cast<const float4*>(scales + s * NT + c0);
+        const uint32_t* sc = reinterpret_cast<const uint32_t*>(scales + s * NT + c0);
 #pragma unroll
         for (int c = 0; c < F::kCols; c += kLd) {
           uint32_t d[kLd];
@@ -234,11 +243,9 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
           tc::tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < kLd; i += 4) {
-            const float4 f = sc[(c + i) / 4];
-            acc[c + i] = fmaf(__uint_as_float(d[i]), f.x * w, acc[c + i]);
-            acc[c + i + 1] = fmaf(__uint_as_float(d[i + 1]), f.y * w, acc[c + i + 1]);
-            acc[c + i + 2] = fmaf(__uint_as_float(d[i + 2]), f.z * w, acc[c + i + 2]);
-            acc[c + i + 3] = fmaf(__uint_as_float(d[i + 3]), f.w * w, acc[c + i + 3]);
+            const uint32_t f = sc[(c + i) / 4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[c + i + k] = fmaf(__uint_as_float(d[i + k]), power(f, k) * w, acc[c + i + k]);
           }
         }
         tc::fence_before_sync();
@@ -304,7 +311,9 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
 constexpr int kManyStages = 5, kManyN = 256, kManyT = 256;
 constexpr uint32_t kManyStageBytes = 2 * kTileBytes;  // 32 KB
 constexpr uint32_t kLineBytes = 32 * 128;             // 32 rows of a warp's staging, two of these per warp
-constexpr size_t kManySmem = 1024 + kManyStages * kManyStageBytes + 8 * 2 * kLineBytes;
+// A slot of scales is written when the products five blocks back are done, so the epilogue is done with those seven back.
+constexpr int kScaleSlots = 8;
+constexpr size_t kManySmem = 1024 + kManyStages * kManyStageBytes + 8 * 2 * kLineBytes + kScaleSlots * 128;
 constexpr int kManyThreads = 128 + 256;
 
 __device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
@@ -407,19 +416,20 @@ __device__ __forceinline__ void move_lines(uint8_t* buf, void* global, long long
   }
 }
 
-// 32 TMEM columns times the factor (a pair of equal halves), added to the pairs acc[0..15]
-__device__ __forceinline__ void add32(const uint32_t (&d)[32], uint64_t f, uint64_t* acc) {
+// 64 TMEM columns times the factor (a pair of equal halves), added to the pairs acc[0..31]
+__device__ __forceinline__ void add64(const uint32_t (&d)[64], uint64_t f, uint64_t (&acc)[32]) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+  for (int i = 0; i < 32; ++i)
     asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(acc[i]) : "r"(d[2 * i]), "r"(d[2 * i + 1]), "l"(f));
 }
 
 template <int ODT>
 __global__ void __launch_bounds__(kManyThreads, 1)
     many_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
-                const __grid_constant__ CUtensorMap omap, const FewArgs a) {
+                const __grid_constant__ CUtensorMap smap, const __grid_constant__ CUtensorMap omap, const FewArgs a) {
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* scales = smem + kManyStages * kManyStageBytes + 8 * 2 * kLineBytes;  // [slot][128]
   __shared__ alignas(8) uint64_t full[kManyStages], empty[kManyStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -448,6 +458,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       if (tc::elect_one()) {
         tc::prefetch_tmap(&wmap);
         tc::prefetch_tmap(&xmap);
+        tc::prefetch_tmap(&smap);
         tc::prefetch_tmap(&omap);
         pdl_wait();
         int it = 0;
@@ -463,8 +474,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             // the first CTA's barrier counts both CTAs' tiles
             uint8_t* st = smem + s * kManyStageBytes;
             const uint32_t bar = peer_addr(&full[s], 0);
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kManyStageBytes);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * (kManyStageBytes + 128));
             pair_load(st, &xmap, bar, b * kBlock, t0);
+            pair_load(scales + it % kScaleSlots * 128, &smap, bar, t0, b);
             pair_load(st + kTileBytes, &wmap, bar, b * kBlock, n0);
           }
         }
@@ -497,61 +509,55 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     constexpr int kSize = ODT == MV_F32 ? 4 : 2, kPart = 128 / kSize;  // columns that a row of the staging holds
-    const int half = (warp - 4) / 4, quarter = warp & 3;
+    const int half = (warp - 4) / 4, quarter = warp & 3;  // a warp has 32 tokens and half of the tile's columns
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
     uint8_t* lines = smem + kManyStages * kManyStageBytes + (warp - 4) * 2 * kLineBytes;
-    const uint32_t freed[2] = {peer_addr(&acc_empty[0], 0), peer_addr(&acc_empty[1], 0)};
+    const uint32_t freed = peer_addr(&acc_empty[0], 0);
     const bool res_lines = ((reinterpret_cast<uintptr_t>(a.residual) | static_cast<uintptr_t>(a.r_st * kSize)) & 15) == 0;
     pdl_wait();
+    // lane l's scale of the weights of block b + l
+    auto load_ws = [&](int tile, int b) {
+      const int n0 = tile / a.t_tiles * kManyN + half * 128;
+      return b + lane < a.blocks && n0 < a.N ? a.ws[n0 / kBlock * a.ws_st + b + lane] : 0.f;
+    };
     int it = 0, turn = 0;
     bool ok = true;
+    float ws_next = load_ws(first, 0);
     for (int tile = first; tile < tiles && ok; tile += step) {
       const int t0 = tile % a.t_tiles * kManyT + rank * 128 + quarter * 32, n0 = tile / a.t_tiles * kManyN + half * 128;
-      const float* sx = a.scale + min(t0 + lane, a.T - 1);
-      const float* ws = a.ws + min(n0, a.N - 1) / kBlock * a.ws_st;
-      uint64_t acc[64];  // pairs of columns
+      float ws_now = ws_next;
+      if (tile + step < tiles) ws_next = load_ws(tile + step, 0);
+      uint64_t acc[2][32];  // pairs of columns
 #pragma unroll
-      for (int c = 0; c < 64; ++c) acc[c] = 0;
-      // scales are read two blocks ahead, and multiplied only when their block has come: warps issue in order
-      const int last = a.blocks - 1;
-      float s_next = sx[0], w_next = ws[0], s_then = sx[min(1, last) * a.s_st], w_then = ws[min(1, last)];
-      for (int b = 0; b < a.blocks; ++b, ++it) {
+      for (int c = 0; c < 32; ++c) acc[0][c] = acc[1][c] = 0;
+      for (int b = 0; b < a.blocks && ok; ++b, ++it) {
         const int buf = it & 1;
-        const float s_now = s_next, w_now = w_next;
-        s_next = s_then, w_next = w_then;
-        if (b + 2 <= last) s_then = sx[(b + 2) * a.s_st], w_then = ws[b + 2];
+        if ((b & 31) == 0 && b > 0) ws_now = load_ws(tile, b);
+        const float w_now = __shfl_sync(0xffffffffu, ws_now, b & 31);
         if (!wait(&acc_full[buf], (it / 2) & 1, a.header, 0x813u)) {
           ok = false;
           break;
         }
         tc::fence_after_sync();
-        // a load of 32 columns is under way while the last 32 are added
-        uint32_t d0[32], d1[32];
-        const float f1 = s_now * w_now;
+        const float f1 = power(scales[it % kScaleSlots * 128 + quarter * 32 + lane], 0) * w_now;
         uint64_t f;
         asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "f"(f1));
-        const uint32_t src = lanes + buf * kManyN;
-        tc::tmem_ld32(src, d0);
-        landed(d0);
-        tc::tmem_ld32(src + 32, d1);
-        add32(d0, f, acc);
-        landed(d1);
-        tc::tmem_ld32(src + 64, d0);
-        add32(d1, f, acc + 16);
-        landed(d0);
-        tc::tmem_ld32(src + 96, d1);
-        add32(d0, f, acc + 32);
-        landed(d1);
+        uint32_t d[64];
+        tmem_ld64(lanes + buf * kManyN, d);
+        landed(d);
+        add64(d, f, acc[0]);
+        tmem_ld64(lanes + buf * kManyN + 64, d);
+        landed(d);
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0)
-          asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(freed[buf]) : "memory");
-        add32(d1, f, acc + 48);
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(freed + buf * 8) : "memory");
+        add64(d, f, acc[1]);
       }
       const int rows = min(32, a.T - t0);
       if (rows <= 0 || !ok) continue;
 #pragma unroll
       for (int p = 0; p < 128 / kPart; ++p) {
+        const int h = p / (64 / kPart), c = p % (64 / kPart) * kPart;
         const int n = n0 + p * kPart, cols = a.N - n;
         if (cols <= 0) break;
         uint8_t* line = lines + (turn++ & 1) * kLineBytes;
@@ -568,7 +574,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           float v[16 / kSize];
 #pragma unroll
           for (int i = 0; i < 8 / kSize; ++i)
-            asm("mov.b64 {%0, %1}, %2;" : "=f"(v[2 * i]), "=f"(v[2 * i + 1]) : "l"(acc[(p * kPart + j * (16 / kSize)) / 2 + i]));
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(v[2 * i]), "=f"(v[2 * i + 1]) : "l"(acc[h][(c + j * (16 / kSize)) / 2 + i]));
           if constexpr (kSize == 4) {
             float4 o = make_float4(v[0], v[1], v[2], v[3]);
             if (a.residual != nullptr) {
@@ -613,7 +619,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 // ------------------------------------------------------------------------------------------------ host
 
 // a [rows, cols] tensor of `size`-byte elements (1, 2 or 4; rows of `stride` bytes) in boxes of 128 bytes x box_rows
-int row_map(CUtensorMap* m, const void* base, int size, int cols, int rows, long long stride, int box_rows, const char* what) {
+int row_map(CUtensorMap* m, const void* base, int size, int cols, int rows, long long stride, int box_rows, const char* what,
+            bool swizzle = true) {
   static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -630,7 +637,7 @@ int row_map(CUtensorMap* m, const void* base, int size, int cols, int rows, long
                                    : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
                                                : CU_TENSOR_MAP_DATA_TYPE_UINT32;
   const CUresult r = enc(m, type, 2, const_cast<void*>(base), dims, strides, box, estr,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(MV_ERR_INVALID, "tensor map for %s rejected (CUresult %d)", what, static_cast<int>(r));
   return MV_OK;
@@ -686,14 +693,15 @@ int run_typed(const LinearArgs& x, cudaStream_t st) {
   a.t_tiles = (x.T + kManyT - 1) / kManyT;
   const int size = ODT == MV_F32 ? 4 : 2;
   a.out_lines = aligned16(x.out) && x.o_st * size % 16 == 0;
-  CUtensorMap wm, xm, om;
+  CUtensorMap wm, xm, sm, om;
   int rc = row_map(&wm, x.w, 1, x.K, x.N, x.w_st, 128, "wq");
   if (rc == MV_OK) rc = row_map(&xm, x.q, 1, static_cast<int>(x.q_st), x.T, x.q_st, 128, "the activations");
+  if (rc == MV_OK) rc = row_map(&sm, x.scale, 1, static_cast<int>(x.s_st), x.blocks, x.s_st, 1, "the scales", false);
   om = xm;
   if (rc == MV_OK && a.out_lines) rc = row_map(&om, x.out, size, x.N, x.T, x.o_st * size, 32, "out");
   if (rc != MV_OK) return rc;
-  return launch(many_kernel<ODT>, static_cast<int>(tiles < pairs ? tiles : pairs) * 2, kManyThreads, kManySmem, 2, st, wm, xm, om,
-                a);
+  return launch(many_kernel<ODT>, static_cast<int>(tiles < pairs ? tiles : pairs) * 2, kManyThreads, kManySmem, 2, st, wm, xm,
+                sm, om, a);
 }
 
 }  // namespace
