@@ -116,7 +116,7 @@ struct FewArgs {
   void* out;
   long long ws_st, s_st, r_st, o_st;
   int T, N, blocks, n_tiles, t_tiles, split;
-  bool out_lines;  // whole lines of `out` go through its tensor map
+  bool out_lines, res_lines;  // whole lines of `out` and `residual` go through their tensor maps
   WsHeader* header;
 };
 
@@ -426,17 +426,19 @@ __device__ __forceinline__ void add64(const uint32_t (&d)[64], uint64_t f, uint6
 template <int ODT>
 __global__ void __launch_bounds__(kManyThreads, 1)
     many_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
-                const __grid_constant__ CUtensorMap smap, const __grid_constant__ CUtensorMap omap, const FewArgs a) {
+                const __grid_constant__ CUtensorMap smap, const __grid_constant__ CUtensorMap omap,
+                const __grid_constant__ CUtensorMap rmap, const FewArgs a) {
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* scales = smem + kManyStages * kManyStageBytes + 8 * 2 * kLineBytes;  // [slot][128]
-  __shared__ alignas(8) uint64_t full[kManyStages], empty[kManyStages], acc_full[2], acc_empty[2];
+  __shared__ alignas(8) uint64_t full[kManyStages], empty[kManyStages], acc_full[2], acc_empty[2], res_full[8];
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kManyStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 16);
+    for (int i = 0; i < 8; ++i) mbar_init(&res_full[i], 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -513,18 +515,27 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
     uint8_t* lines = smem + kManyStages * kManyStageBytes + (warp - 4) * 2 * kLineBytes;
     const uint32_t freed = peer_addr(&acc_empty[0], 0);
-    const bool res_lines = ((reinterpret_cast<uintptr_t>(a.residual) | static_cast<uintptr_t>(a.r_st * kSize)) & 15) == 0;
     pdl_wait();
     // lane l's scale of the weights of block b + l
     auto load_ws = [&](int tile, int b) {
       const int n0 = tile / a.t_tiles * kManyN + half * 128;
       return b + lane < a.blocks && n0 < a.N ? a.ws[n0 / kBlock * a.ws_st + b + lane] : 0.f;
     };
-    int it = 0, turn = 0;
+    int it = 0, turn = 0, fetched = 0;
     bool ok = true;
     float ws_next = load_ws(first, 0);
     for (int tile = first; tile < tiles && ok; tile += step) {
       const int t0 = tile % a.t_tiles * kManyT + rank * 128 + quarter * 32, n0 = tile / a.t_tiles * kManyN + half * 128;
+      const int rows = min(32, a.T - t0), cols_here = a.N - n0;
+      // the residual's first two lines come while the products are made
+      const bool fetch = a.res_lines && rows > 0 && cols_here > 0;
+      if (fetch && lane == 0) {
+        stores_read<0>();
+        const int n = cols_here > kPart ? 2 : 1;
+        uint8_t* to[2] = {lines + (turn & 1) * kLineBytes, lines + ((turn + 1) & 1) * kLineBytes};
+        mbar_arrive_expect_tx(&res_full[warp - 4], n * kLineBytes);
+        for (int i = 0; i < n; ++i) tc::tma_load_2d(to[i], &rmap, &res_full[warp - 4], n0 + i * kPart, t0);
+      }
       float ws_now = ws_next;
       if (tile + step < tiles) ws_next = load_ws(tile + step, 0);
       uint64_t acc[2][32];  // pairs of columns
@@ -553,7 +564,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(freed + buf * 8) : "memory");
         add64(d, f, acc[1]);
       }
-      const int rows = min(32, a.T - t0);
+      if (fetch && !wait(&res_full[warp - 4], fetched++ & 1, a.header, 0x814u)) ok = false;
       if (rows <= 0 || !ok) continue;
 #pragma unroll
       for (int p = 0; p < 128 / kPart; ++p) {
@@ -561,11 +572,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const int n = n0 + p * kPart, cols = a.N - n;
         if (cols <= 0) break;
         uint8_t* line = lines + (turn++ & 1) * kLineBytes;
-        if (a.out_lines && lane == 0) stores_read<1>();  // the store before the last was from here
+        if (a.out_lines && lane == 0 && !(fetch && p < 2)) stores_read<1>();  // the store before the last was from here
         __syncwarp();
-        if (a.residual != nullptr) {
+        if (a.residual != nullptr && !(fetch && p < 2)) {
           move_lines<kSize, false>(line, static_cast<uint8_t*>(const_cast<void*>(a.residual)) + (t0 * a.r_st + n) * kSize,
-                                   a.r_st, rows, cols, res_lines, lane);
+                                   a.r_st, rows, cols, a.res_lines, lane);
           __syncwarp();
         }
 #pragma unroll
@@ -664,7 +675,7 @@ int launch(void (*fn)(P...), int grid, int threads, size_t smem, int cluster, cu
 
 template <int NT, int ODT>
 int run_few(const LinearArgs& x, cudaStream_t st) {
-  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, false, x.header};
+  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, false, false, x.header};
   a.n_tiles = (x.N + kTile - 1) / kTile;
   a.t_tiles = (x.T + NT - 1) / NT;
   CUtensorMap wm, xm;
@@ -688,20 +699,22 @@ int run_typed(const LinearArgs& x, cudaStream_t st) {
   if (tiles > 0x7fffffffLL) return fail(MV_ERR_INVALID, "mv_fp8_linear: T=%d x N=%d is too large", x.T, x.N);
   const int pairs = num_sms() / 2;
   if (tiles < pairs / 2) return run_few<128, ODT>(x, st);
-  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, false, x.header};
+  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, false, false, x.header};
   a.n_tiles = (x.N + kManyN - 1) / kManyN;
   a.t_tiles = (x.T + kManyT - 1) / kManyT;
   const int size = ODT == MV_F32 ? 4 : 2;
   a.out_lines = aligned16(x.out) && x.o_st * size % 16 == 0;
-  CUtensorMap wm, xm, sm, om;
+  CUtensorMap wm, xm, sm, om, rm;
   int rc = row_map(&wm, x.w, 1, x.K, x.N, x.w_st, 128, "wq");
   if (rc == MV_OK) rc = row_map(&xm, x.q, 1, static_cast<int>(x.q_st), x.T, x.q_st, 128, "the activations");
   if (rc == MV_OK) rc = row_map(&sm, x.scale, 1, static_cast<int>(x.s_st), x.blocks, x.s_st, 1, "the scales", false);
-  om = xm;
+  a.res_lines = x.residual != nullptr && aligned16(x.residual) && x.r_st * size % 16 == 0 && (x.T == 1 || x.r_st >= x.N);
+  om = rm = xm;
   if (rc == MV_OK && a.out_lines) rc = row_map(&om, x.out, size, x.N, x.T, x.o_st * size, 32, "out");
+  if (rc == MV_OK && a.res_lines) rc = row_map(&rm, x.residual, size, x.N, x.T, x.r_st * size, 32, "residual");
   if (rc != MV_OK) return rc;
   return launch(many_kernel<ODT>, static_cast<int>(tiles < pairs ? tiles : pairs) * 2, kManyThreads, kManySmem, 2, st, wm, xm,
-                sm, om, a);
+                sm, om, rm, a);
 }
 
 }  // namespace
