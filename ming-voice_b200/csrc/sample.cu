@@ -8,11 +8,15 @@
 // the same whatever the split, and a weight below 2^-shift / 2, which no 24-bit random number can draw, is 0.
 //
 // Steps, a cluster of CTAs for each row, the row in their shared memory:
-//   1. read the row once; the largest logit
-//   2. (top-k, top-p) a histogram of t: counts and weights of 2048 bins, added up in the first CTA, which finds the bin with
-//      the border; that bin's tokens are brought together there, and their ranks and weight sums by counting give the border.
-//      A bin with more tokens than the list holds (runs of equal logits) is searched bit by bit over all CTAs.
-//   3. each CTA adds up what is kept of its part; the CTA in which the sum passes u times the total finds the token.
+//   1. read the row once; the first of the order, and (top-k) a key with at least top_k logits at or above it: the least over
+//      the CTAs of the one that top_k / C of its threads' largest logits reach
+//   2. few candidates (a small top_k, or min_p without top_p): they are brought together in the first CTA, which finds the
+//      borders and draws by itself
+//   3. else the borders: a histogram of t with 2048 bins (counts for top-k; for top-p weights, as three sums of 15 bits, since
+//      32 bits are what shared memory adds), added up in the first CTA, which finds the bin with the border; that bin's tokens
+//      are brought together there. A bin with more than the list holds (runs of equal logits) is searched over all CTAs.
+//   4. each CTA adds up what is kept of its part; the CTA in which the sum passes u times the total finds the token.
+// A border among listed tokens is found bit by bit over their places.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -43,6 +47,7 @@ struct SampleArgs {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048, kList = 4096;
+constexpr int kMostMaxima = kThreads * 3 / 4;  // of a CTA's threads, in finding the key of step 1
 constexpr uint32_t kNone = 0x007fffffu;  // the key of -inf
 
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -58,16 +63,18 @@ __device__ __forceinline__ uint64_t place_of(uint32_t key, int i) {
 
 // Weights of one row as whole numbers.
 struct Weights {
-  double m, c, lim;  // largest logit, log2(e) / temperature, least t that has a weight
+  double m, c, lim;     // largest logit, log2(e) / temperature, least t that is told apart
   uint32_t top, least;  // keys: of the largest logit, and of the least that can have a weight
   int shift;
-  __device__ __forceinline__ double t_of(float l) const { return (static_cast<double>(l) - m) * c; }
-  // 2^t in units of 2^-shift, for -48 <= t <= 0 (lower ones: 0)
-  __device__ __forceinline__ uint64_t of(float l, double t) const {
+  // 0 for the largest logit itself (which may be infinite), lim for those without a weight
+  __device__ __forceinline__ double t_of(float l, uint32_t key) const {
+    const double d = key == top ? 0.0 : static_cast<double>(l) - m;
+    return key < least ? lim : fmax(d * c, lim);
+  }
+  // 2^t in units of 2^-shift, rounded: 0 at lim
+  __device__ __forceinline__ uint64_t at(double t) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: the low word of a sum with it is the number, rounded
-    if (t < lim) return 0;
     const double r = t + kRound;
-    const int n = __double2loint(r);
     const double f = t - (r - kRound);
     double p = 1.0203121063391729e-07;
     p = fma(p, f, 1.3255224878668817e-06);
@@ -79,13 +86,17 @@ struct Weights {
     p = fma(p, f, 0.2402265069581299);
     p = fma(p, f, 0.6931471805599453);
     p = fma(p, f, 1.0);
-    const double s = __hiloint2double((1023 + n + shift) << 20, 0);
+    const double s = __hiloint2double((1023 + __double2loint(r) + shift) << 20, 0);
     return static_cast<uint64_t>(__double_as_longlong(fma(p, s, 4503599627370496.0))) & 0xfffffffffffffull;  // 2^52
   }
-  __device__ __forceinline__ uint64_t of(float l) const { return of(l, t_of(l)); }
+  __device__ __forceinline__ uint64_t of(float l, uint32_t key) const { return at(t_of(l, key)); }
+  // the key that a logit needs for 2^t (rounded down: no key at or above it is missed)
+  __device__ __forceinline__ uint32_t key_at(double t) const {
+    if (top == 0xff800000u) return top;  // beside an infinite logit only its equals have a weight
+    const double l = m + t / c * 1.0000001;
+    return key_of(l > -3.4e38 ? __double2float_rd(l) : -3.4028235e38f);
+  }
 };
-
-__device__ __forceinline__ uint64_t shfl_down(uint64_t v, int o) { return __shfl_down_sync(0xffffffffu, v, o); }
 
 __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 #pragma unroll
@@ -94,16 +105,12 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 }
 
 struct Shared {
-  unsigned long long weight[kBins];
-  unsigned long long list[kList];
-  unsigned long long part[kWarps], total, border, found_weight;
-  unsigned long long bin_before;  // of the bin that is looked into: weights of the bins before it
-  unsigned int count[kBins];
-  unsigned int counts[kWarps];
-  unsigned int n_list, top, nan, bin, bin_count_before, bin_count;
-  unsigned long long need, kept, least_place, most_place;
-  unsigned int part_n;
-  int token;
+  union {
+    unsigned int bins[4][kBins];  // counts, or the weights' bits 0-14, 15-29 and 30-45
+    unsigned long long list[kList];
+  };
+  unsigned long long part[kWarps], total, border, kept, need, least_place, most_place, best, bin_before;
+  unsigned int counts[kWarps], n_list, pivot, nan, bin, bin_count_before, part_n;
 };
 
 // Sums of (w, n) over the CTA in every thread. Two barriers.
@@ -150,8 +157,64 @@ __device__ __forceinline__ void block_before(uint64_t& w, unsigned int& n, uint6
   __syncthreads();
 }
 
+// Tokens of a list in the registers of one CTA's threads.
+struct Listed {
+  static constexpr int kEach = kList / kThreads;
+  uint64_t place[kEach], w[kEach];
+
+  // sums over the tokens whose place lies before `end`
+  __device__ __forceinline__ void before(uint64_t end, uint64_t& sum, unsigned int& n, Shared& s) const {
+    sum = 0, n = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (place[i] < end) ++n, sum += w[i];
+    block_sum(sum, n, s);
+  }
+
+  // The first place, among the `count` tokens, up to which there are at least need_n tokens (by_count) or weights of at least
+  // need_w; it exists. `sum` receives the weights up to it.
+  __device__ __forceinline__ uint64_t border(bool by_count, unsigned int need_n, uint64_t need_w, unsigned int count, uint64_t& sum,
+                                             Shared& s) const {
+    uint64_t first = ~0ull, last = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (place[i] != ~0ull) first = min(first, place[i]), last = max(last, place[i]);
+    if (threadIdx.x == 0) s.least_place = ~0ull, s.most_place = 0ull;
+    __syncthreads();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+      last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+    }
+    if ((threadIdx.x & 31) == 0 && first != ~0ull) {
+      atomicMin(&s.least_place, static_cast<unsigned long long>(first));
+      atomicMax(&s.most_place, static_cast<unsigned long long>(last));
+    }
+    __syncthreads();
+    first = s.least_place, last = s.most_place;
+    int bit = first == last ? -1 : 63 - __clzll(first ^ last);
+    uint64_t low = bit < 0 ? first : first >> bit >> 1 << bit << 1;
+    unsigned int n_low = 0, n_high = count, n;  // tokens before low, and before the end of what is left
+    for (; bit >= 0 && n_high - n_low > 1; --bit) {
+      const uint64_t mid = low | 1ull << bit;
+      before(mid, sum, n, s);
+      if (by_count ? n < need_n : sum < need_w)
+        low = mid, n_low = n;
+      else
+        n_high = n;
+    }
+    // one token lies at or behind low and before the end of what is left
+    const uint64_t end = bit < 0 ? low + 1 : low + (2ull << bit);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (place[i] >= low && place[i] < end && place[i] != ~0ull) s.border = place[i];
+    before(end, sum, n, s);
+    return s.border;
+  }
+};
+
 template <int DT>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   Shared& s = *reinterpret_cast<Shared*>(raw);
   using T = typename std::conditional<DT == MV_F32, float, uint16_t>::type;
@@ -183,7 +246,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
     if constexpr (DT == MV_F32) return -INFINITY;
     else return static_cast<uint16_t>(DT == MV_BF16 ? 0xff80 : 0xfc00);
   }();
-  // f(logit, index in the part) for this thread's share of the part; behind its end -inf
+  // f(four logits, index of the first in the part) for this thread's share of the part; behind its end -inf
   auto each = [&](auto&& f) {
     for (int i = tid * 4; i < len4; i += kThreads * 4) {
       alignas(16) T v[4];
@@ -196,18 +259,24 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = i + k < len ? src[i + k] : minus_inf;
       }
+      float l[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) f(value(v[k]), i + k);
+      for (int k = 0; k < 4; ++k) l[k] = value(v[k]);
+      f(l, i);
     }
   };
 
-  // ---- 1. the row, its largest logit
-  if (tid == 0) s.top = 0u, s.nan = 0u, s.n_list = 0u, s.token = 0x7fffffff, s.border = ~0ull;
-  if (by_k || by_p)
-    for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0u, s.weight[i] = 0ull;
+  // ---- 1. the row, the first of its order
+  if (tid == 0) s.nan = 0u, s.n_list = 0u, s.best = ~0ull;
   __syncthreads();
   uint32_t top = 0u;
+  int top_at = 0;
   bool nan = false;
+  auto meet = [&](float l, int i) {  // (a thread meets its logits in the order of their indices)
+    nan |= l != l;
+    const uint32_t key = key_of(l);
+    if (key > top) top = key, top_at = i;
+  };
   if (a.in_smem) {
     constexpr int kVec = 16 / sizeof(T);
     int done = 0;
@@ -220,255 +289,327 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
         reinterpret_cast<uint4*>(held)[i] = x;
         const T* e = reinterpret_cast<const T*>(&x);
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) {
-          const float l = value(e[k]);
-          nan |= l != l;
-          top = max(top, key_of(l));
-        }
+        for (int k = 0; k < kVec; ++k) meet(value(e[k]), i * kVec + k);
       }
       done *= kVec;
     }
+#pragma unroll 4
     for (int i = done + tid; i < len4; i += kThreads) {
       const T x = i < len ? src[i] : minus_inf;
       held[i] = x;
-      const float l = value(x);
-      nan |= l != l;
-      top = max(top, key_of(l));
+      meet(value(x), i);
     }
   } else {
-    each([&](float l, int) {
-      nan |= l != l;
-      top = max(top, key_of(l));
+    each([&](const float (&l)[4], int i) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) meet(l[k], i + k);
     });
   }
-  top = __reduce_max_sync(0xffffffffu, top);
+  uint64_t best = top == 0u ? ~0ull : place_of(top, start + top_at);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
   nan = __any_sync(0xffffffffu, nan);
   if (lane == 0) {
-    atomicMax(&s.top, top);
+    if (best != ~0ull) atomicMin(&s.best, static_cast<unsigned long long>(best));
     if (nan) s.nan = 1u;
   }
+  // a key that at least `share` of this CTA's logits reach
+  const int share = by_k ? (top_k + C - 1) / C : kMostMaxima + 1;
+  if (share <= kMostMaxima) {
+    uint32_t pivot = 0u;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t mid = pivot | 1u << bit;
+      const int n = __syncthreads_count(top >= mid);
+      if (n >= share) pivot = mid;
+      if (n >= share && n <= share + share / 8) break;
+    }
+    if (tid == 0) s.pivot = pivot;
+  }
   cluster.sync();
-  top = 0u;
+  best = ~0ull;
   unsigned int any_nan = 0;
+  uint32_t pivot = 0xffffffffu;
   for (int i = 0; i < C; ++i) {
     const Shared& p = *cluster.map_shared_rank(&s, i);
-    top = max(top, p.top);
+    best = min(best, static_cast<uint64_t>(p.best));
     any_nan |= p.nan;
+    if (share <= kMostMaxima) pivot = min(pivot, p.pivot);
   }
-  if (any_nan || top <= kNone) {
+  top = best == ~0ull ? 0u : ~static_cast<uint32_t>(best >> 32);
+  const bool nothing = any_nan || top <= kNone;
+  if (nothing || greedy) {
     if (rank == 0 && tid == 0) {
-      a.tokens[r] = -1;
-      if (a.logprob != nullptr) a.logprob[r] = -INFINITY;
+      a.tokens[r] = nothing ? -1 : static_cast<int>(static_cast<uint32_t>(best));
+      if (a.logprob != nullptr) a.logprob[r] = nothing ? -INFINITY : 0.f;
     }
-    cluster.sync();
-    return;
-  }
-  if (greedy) {
-    int first = 0x7fffffff;
-    each([&](float l, int i) {
-      if (key_of(l) == top) first = min(first, i);
-    });
-    first = __reduce_min_sync(0xffffffffu, first);
-    if (lane == 0 && first != 0x7fffffff) atomicMin(&s0.token, start + first);
-    cluster.sync();
-    if (rank == 0 && tid == 0) {
-      a.tokens[r] = s.token;
-      if (a.logprob != nullptr) a.logprob[r] = 0.f;
-    }
+    cluster.sync();  // no CTA leaves while another reads its shared memory
     return;
   }
   Weights wt;
   wt.top = top, wt.shift = a.shift;
   wt.m = of_key(top), wt.c = 1.4426950408889634 / static_cast<double>(temp);
   wt.lim = -static_cast<double>(a.shift + 2);
-  // logits below `least` have no weight for certain (rounded down; where the maximum is infinite, all others have none)
-  {
-    const double l = wt.m + wt.lim / wt.c * 1.0000001;
-    float f = l > -3.4e38 ? __double2float_rd(l) : -3.4028235e38f;
-    if (top == 0xff800000u) f = INFINITY;
-    wt.least = key_of(f);
-  }
-  const uint64_t one = 1ull << a.shift;
-  // the weight of a logit whose key is at least `least`
-  auto weight = [&](float l, uint32_t key) { return key == top ? one : wt.of(l); };
+  wt.least = wt.key_at(wt.lim);
+  const double one = static_cast<double>(1ull << a.shift);
+  const uint64_t least_w = min_p > 0.f ? static_cast<uint64_t>(fmax(ceil(static_cast<double>(min_p) * one), 1.0)) : 1;
+  // logits below this are not kept whatever the other filters do
+  const uint32_t least_key = min_p > 0.f ? max(wt.least, wt.key_at(fmax(log2(static_cast<double>(min_p)) - 1e-9, wt.lim))) : wt.least;
+  auto draw = [&](uint64_t total) {  // the sum up to the token drawn is the first above this
+    const uint64_t t = static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(total));
+    return t < total ? t : total - 1;
+  };
+  auto answer = [&](int token, uint64_t w, uint64_t total) {
+    a.tokens[r] = token;
+    if (a.logprob != nullptr) a.logprob[r] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total)));
+  };
 
-  // ---- 2. the border
-  uint64_t border = ~0ull;
-  if (by_k || by_p) {
-    const double per = -static_cast<double>(kBins) / (a.shift + 4.0);
-    auto bin_of = [&](float l, uint32_t key) { return key == top ? 0 : __double2int_rz(fmax(wt.t_of(l), wt.lim) * per); };
-    each([&](float l, int) {
-      const uint32_t key = key_of(l);
-      if (key < wt.least) return;
-      const int b = bin_of(l, key);
-      atomicAdd(&s.count[b], 1u);
-      atomicAdd(&s.weight[b], static_cast<unsigned long long>(weight(l, key)));
+  // ---- 2. few candidates
+  if (share <= kMostMaxima || (!by_k && !by_p && min_p > 0.f)) {
+    const uint32_t from = max(by_k ? pivot : 0u, by_p ? wt.least : least_key);
+    each([&](const float (&l)[4], int i) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t key = key_of(l[k]);
+        if (key < from) continue;
+        const unsigned int at = atomicAdd(&s0.n_list, 1u);
+        if (at < kList) s0.list[at] = place_of(key, start + i + k);
+      }
     });
-    __syncthreads();
-    if (rank > 0)
-      for (int i = tid; i < kBins; i += kThreads)
-        if (s.count[i] != 0u) {
-          atomicAdd(&s0.count[i], s.count[i]);
-          atomicAdd(&s0.weight[i], s.weight[i]);
+    cluster.sync();
+    const unsigned int count = s0.n_list;
+    if (count <= kList) {
+      cluster.barrier_arrive();
+      if (rank > 0) return;
+      Listed list;
+#pragma unroll
+      for (int i = 0; i < Listed::kEach; ++i) {
+        const unsigned int at = tid + i * kThreads;
+        list.place[i] = ~0ull, list.w[i] = 0;
+        if (at >= count) continue;
+        list.place[i] = s.list[at];
+        const uint32_t key = ~static_cast<uint32_t>(list.place[i] >> 32);
+        list.w[i] = wt.of(of_key(key), key);
+      }
+      uint64_t border = ~0ull, sum;
+      unsigned int n;
+      if (by_k && count > static_cast<unsigned int>(top_k)) {
+        border = list.border(true, top_k, 0, count, sum, s);
+      } else if (by_p) {
+        list.before(~0ull, sum, n, s);
+      }
+      if (by_p) {
+        // the first place up to which the weights reach top_p of top-k's; its tokens before that are all top-k's
+        const uint64_t need = static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(sum)));
+        border = list.border(false, 0, need, count, sum, s);
+      }
+      // kept tokens in the order of their indices: the draw's is the first up to which the sum is above the target
+#pragma unroll
+      for (int i = 0; i < Listed::kEach; ++i) {
+        if (list.place[i] > border || list.w[i] < least_w) list.place[i] = ~0ull, list.w[i] = 0;
+        if (list.place[i] != ~0ull) list.place[i] &= 0xffffffffull;
+      }
+      uint64_t total;
+      list.before(~0ull, total, n, s);
+      const uint64_t at = list.border(false, 0, draw(total) + 1, n, sum, s);
+#pragma unroll
+      for (int i = 0; i < Listed::kEach; ++i)
+        if (list.place[i] == at) answer(static_cast<int>(at), list.w[i], total);
+      cluster.barrier_wait();
+      return;
+    }
+    cluster.sync();  // all have read the count
+  }
+
+  // ---- 3. the borders
+  uint64_t border = ~0ull;
+  const bool bins = a.slice <= (1 << 17);  // 15 bits of as many weights fit in 32
+  const double per = -static_cast<double>(kBins) / (a.shift + 4.0);
+  auto bin_of = [&](double t) { return static_cast<unsigned int>(__double2loint(fma(t, per, 6755399441055744.0))); };
+  // first top-k's border, then top-p's among what top-k keeps
+  for (int phase = by_k ? 0 : 1; phase < (by_p ? 2 : 1); ++phase) {
+    const uint32_t from = max(wt.least, ~static_cast<uint32_t>(border >> 32));
+    uint64_t need_w = ~0ull, w;  // top-p keeps a token while the weights before it are less
+    const unsigned int need_n = static_cast<unsigned int>(top_k);
+    unsigned int bin = 0xffffffffu, n;
+    if (tid == 0) s.n_list = 0u, s.bin = bin, s.least_place = ~0ull, s.most_place = 0ull;
+    if (bins) {
+      for (int i = tid; i < 4 * kBins; i += kThreads) s.bins[0][i] = 0u;
+      __syncthreads();
+      each([&](const float (&l)[4], int i) {
+        double t[4];
+        bool in[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t key = key_of(l[k]);
+          in[k] = key >= from && place_of(key, start + i + k) <= border;
+          t[k] = wt.t_of(l[k], key);
         }
-    uint64_t need = ~0ull;  // top-p keeps a token while the weights before it are less
-    unsigned int need_n = by_k ? static_cast<unsigned int>(top_k) : 0xffffffffu;
-    // first top-k's border, whose weights top-p is a share of, then top-p's
-    for (int phase = by_k ? 0 : 1; phase < (by_p ? 2 : 1); ++phase) {
+        if (phase == 0) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (in[k]) atomicAdd(&s.bins[0][bin_of(t[k])], 1u);
+        } else {
+          uint64_t x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[k] = wt.at(t[k]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (!in[k]) continue;
+            const unsigned int b = bin_of(t[k]);
+            atomicAdd(&s.bins[1][b], static_cast<unsigned int>(x[k]) & 0x7fffu);
+            atomicAdd(&s.bins[2][b], static_cast<unsigned int>(x[k] >> 15) & 0x7fffu);
+            atomicAdd(&s.bins[3][b], static_cast<unsigned int>(x[k] >> 30));
+          }
+        }
+      });
       cluster.sync();
       if (rank == 0) {
-        constexpr int kPer = kBins / kThreads;
-        uint64_t w = 0, sum;
-        unsigned int n = 0, all;
-        for (int i = 0; i < kPer; ++i) w += s.weight[tid * kPer + i], n += s.count[tid * kPer + i];
-        block_before(w, n, sum, all, s);
-        if (phase == 1) {
-          // (after top-k: of the weights that it kept)
-          const uint64_t kept = by_k ? s.kept : sum;
-          need = static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(kept)));
+        constexpr int kPer = kBins / kThreads;  // neighbouring bins of a thread: 16 bytes of each sum
+        uint64_t wb[kPer] = {}, all_w;
+        unsigned int nb[kPer] = {}, all_n;
+        for (int c = 0; c < C; ++c) {
+          const Shared& p = *cluster.map_shared_rank(&s, c);
+          if (phase == 0) {
+            const uint4 x = reinterpret_cast<const uint4*>(p.bins[0])[tid];
+            nb[0] += x.x, nb[1] += x.y, nb[2] += x.z, nb[3] += x.w;
+          } else {
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+              const uint4 x = reinterpret_cast<const uint4*>(p.bins[q + 1])[tid];
+              wb[0] += static_cast<uint64_t>(x.x) << 15 * q, wb[1] += static_cast<uint64_t>(x.y) << 15 * q;
+              wb[2] += static_cast<uint64_t>(x.z) << 15 * q, wb[3] += static_cast<uint64_t>(x.w) << 15 * q;
+            }
+          }
         }
-        __syncthreads();
-        if (tid == 0) {
-          s.bin = 0xffffffffu, s.n_list = 0u, s.border = border, s.need = need;
-          s.least_place = ~0ull, s.most_place = 0ull;
-        }
-        __syncthreads();
-        if (phase == 0 && all < need_n && tid == 0) s.kept = sum;  // all that has a weight is kept
+        w = wb[0] + wb[1] + wb[2] + wb[3], n = nb[0] + nb[1] + nb[2] + nb[3];
+        block_before(w, n, all_w, all_n, s);
+        if (phase == 1) need_w = static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(all_w)));
+        if (tid == 0) s.need = need_w;
+#pragma unroll
         for (int i = 0; i < kPer; ++i) {
-          const int b = tid * kPer + i;
-          const uint64_t wb = s.weight[b];
-          const unsigned int nb = s.count[b];
-          const bool here = phase == 0 ? n < need_n && n + nb >= need_n : w < need && w + wb >= need;
-          if (here) s.bin = b, s.bin_before = w, s.bin_count_before = n, s.bin_count = nb;
-          w += wb, n += nb;
+          if (phase == 0 ? n < need_n && n + nb[i] >= need_n : w < need_w && w + wb[i] >= need_w)
+            s.bin = tid * kPer + i, s.bin_before = w, s.bin_count_before = n;
+          w += wb[i], n += nb[i];
         }
       }
       cluster.sync();
-      const unsigned int bin = s0.bin;
-      if (bin == 0xffffffffu) continue;
-      need = s0.need;
+      bin = s0.bin, need_w = s0.need;
+      if (bin == 0xffffffffu) continue;  // top_k keeps all that has a weight
       const uint64_t w_before = s0.bin_before;
-      const unsigned int n_before = s0.bin_count_before, n_bin = s0.bin_count;
-      if (n_bin <= kList) {
-        each([&](float l, int i) {
-          const uint32_t key = key_of(l);
-          if (key < wt.least || bin_of(l, key) != static_cast<int>(bin)) return;
-          s0.list[atomicAdd(&s0.n_list, 1u)] = place_of(key, start + i);
-        });
-        cluster.sync();
+      const unsigned int n_before = s0.bin_count_before;
+      each([&](const float (&l)[4], int i) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t key = key_of(l[k]);
+          const uint64_t place = place_of(key, start + i + k);
+          if (key < from || place > border || bin_of(wt.t_of(l[k], key)) != bin) continue;
+          const unsigned int at = atomicAdd(&s0.n_list, 1u);
+          if (at < kList) s0.list[at] = place;
+        }
+      });
+      cluster.sync();
+      const unsigned int count = s0.n_list;
+      if (count <= kList) {
         if (rank == 0) {
-          // each thread has some of the list's tokens; the border is found bit by bit from the first that differs
-          constexpr int kEach = kList / kThreads;
-          uint64_t place[kEach], w[kEach], first = ~0ull, last = 0;
+          Listed list;
 #pragma unroll
-          for (int i = 0; i < kEach; ++i) {
+          for (int i = 0; i < Listed::kEach; ++i) {
             const unsigned int at = tid + i * kThreads;
-            place[i] = ~0ull, w[i] = 0;
-            if (at >= n_bin) continue;
-            place[i] = s.list[at];
-            const uint32_t key = ~static_cast<uint32_t>(place[i] >> 32);
-            w[i] = weight(of_key(key), key);
-            first = min(first, place[i]), last = max(last, place[i]);
+            list.place[i] = ~0ull, list.w[i] = 0;
+            if (at >= count) continue;
+            list.place[i] = s.list[at];
+            const uint32_t key = ~static_cast<uint32_t>(list.place[i] >> 32);
+            if (phase == 1) list.w[i] = wt.of(of_key(key), key);
           }
-          if (first != ~0ull) {
-            atomicMin(&s.least_place, static_cast<unsigned long long>(first));
-            atomicMax(&s.most_place, static_cast<unsigned long long>(last));
-          }
-          __syncthreads();
-          first = s.least_place, last = s.most_place;
-          int bit = first == last ? -1 : 63 - __clzll(first ^ last);
-          uint64_t low = bit < 0 ? first : first >> bit >> 1 << bit << 1;
-          unsigned int n_low = 0, n_high = n_bin;  // tokens before low, and before the end of what is left
-          for (; bit >= 0 && n_high - n_low > 1; --bit) {
-            const uint64_t mid = low | 1ull << bit;
-            uint64_t sum = 0;
-            unsigned int n = 0;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i)
-              if (place[i] < mid) ++n, sum += w[i];
-            block_sum(sum, n, s);
-            if (phase == 0 ? n_before + n < need_n : w_before + sum < need)
-              low = mid, n_low = n;
-            else
-              n_high = n;
-          }
-          // one token is left at or behind low, and what lies before low
-          const uint64_t end = bit < 0 ? low + 1 : low + (2ull << bit);
-          uint64_t sum = 0;
-          unsigned int n = 0;
-#pragma unroll
-          for (int i = 0; i < kEach; ++i) {
-            if (place[i] >= low && place[i] < end && place[i] != ~0ull) s.border = min(place[i], border);
-            if (place[i] < end) sum += w[i];
-          }
-          block_sum(sum, n, s);
-          if (tid == 0) s.kept = w_before + sum;
+          list.border(phase == 0, need_n - n_before, need_w - w_before, count, w, s);
         }
         cluster.sync();
-      } else {
-        // the same over all CTAs' parts
-        uint64_t first = ~0ull, last = 0;
-        each([&](float l, int i) {
-          const uint32_t key = key_of(l);
-          if (key < wt.least || bin_of(l, key) != static_cast<int>(bin)) return;
-          const uint64_t o = place_of(key, start + i);
-          first = min(first, o), last = max(last, o);
-        });
-        if (first != ~0ull) {
-          atomicMin(&s0.least_place, static_cast<unsigned long long>(first));
-          atomicMax(&s0.most_place, static_cast<unsigned long long>(last));
-        }
-        cluster.sync();
-        first = s0.least_place, last = s0.most_place;
-        // counts and weights of what lies before `end`, over all CTAs
-        auto before = [&](uint64_t end, uint64_t& w, unsigned int& n) {
-          w = 0, n = 0;
-          each([&](float l, int i) {
-            const uint32_t key = key_of(l);
-            if (key < wt.least || place_of(key, start + i) >= end) return;
-            ++n;
-            w += weight(l, key);
-          });
-          block_sum(w, n, s);
-          if (tid == 0) s.total = w, s.part_n = n;
-          cluster.sync();
-          w = 0, n = 0;
-          for (int i = 0; i < C; ++i) {
-            const Shared& p = *cluster.map_shared_rank(&s, i);
-            w += p.total, n += p.part_n;
-          }
-          cluster.sync();
-        };
-        int bit = first == last ? -1 : 63 - __clzll(first ^ last);
-        uint64_t low = bit < 0 ? first : first >> bit >> 1 << bit << 1, w;
-        unsigned int n;
-        for (; bit >= 0; --bit) {
-          before(low | 1ull << bit, w, n);
-          if (phase == 0 ? n < need_n : w < need) low |= 1ull << bit;
-        }
-        if (phase == 0) before(low + 1, w, n);
-        if (rank == 0 && tid == 0) s.border = min(low, border), s.kept = w;
-        cluster.sync();
+        border = s0.border;
+        continue;
       }
-      border = s0.border;
-      // (the next phase's first barrier comes before the first CTA changes it)
     }
+    // the same over all CTAs' parts; counts and weights of what lies before `end`
+    auto before = [&](uint64_t end) {
+      w = 0, n = 0;
+      each([&](const float (&l)[4], int i) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t key = key_of(l[k]);
+          const uint64_t place = place_of(key, start + i + k);
+          if (key < from || place > border || place >= end) continue;
+          ++n;
+          if (phase == 1) w += wt.of(l[k], key);
+        }
+      });
+      block_sum(w, n, s);
+      if (tid == 0) s.total = w, s.part_n = n;
+      cluster.sync();
+      w = 0, n = 0;
+      for (int i = 0; i < C; ++i) {
+        const Shared& p = *cluster.map_shared_rank(&s, i);
+        w += p.total, n += p.part_n;
+      }
+      cluster.sync();
+    };
+    if (!bins) {
+      before(~0ull);
+      if (phase == 0 && n < need_n) continue;
+      need_w = static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(w)));
+    }
+    uint64_t first = ~0ull, last = 0;
+    each([&](const float (&l)[4], int i) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t key = key_of(l[k]);
+        const uint64_t place = place_of(key, start + i + k);
+        if (key < from || place > border || (bins && bin_of(wt.t_of(l[k], key)) != bin)) continue;
+        first = min(first, place), last = max(last, place);
+      }
+    });
+    if (first != ~0ull) {
+      atomicMin(&s0.least_place, static_cast<unsigned long long>(first));
+      atomicMax(&s0.most_place, static_cast<unsigned long long>(last));
+    }
+    cluster.sync();
+    first = s0.least_place, last = s0.most_place;
+    int bit = first == last ? -1 : 63 - __clzll(first ^ last);
+    uint64_t low = bit < 0 ? first : first >> bit >> 1 << bit << 1;
+    for (; bit >= 0; --bit) {
+      before(low | 1ull << bit);
+      if (phase == 0 ? n < need_n : w < need_w) low |= 1ull << bit;
+    }
+    border = low;
+    cluster.sync();  // all have read the first CTA's places
   }
 
-  // ---- 3. the draw
-  const uint64_t least_w = min_p > 0.f ? static_cast<uint64_t>(fmax(ceil(static_cast<double>(min_p) * static_cast<double>(one)), 1.0)) : 1;
-  const uint32_t last_key = max(~static_cast<uint32_t>(border >> 32), wt.least);
-  auto kept = [&](float l, int i) -> uint64_t {
-    const uint32_t key = key_of(l);
-    if (key < last_key || place_of(key, start + i) > border) return 0;
-    const uint64_t w = weight(l, key);
-    return w >= least_w ? w : 0;
+  // ---- 4. the draw
+  const uint32_t last_key = max(~static_cast<uint32_t>(border >> 32), least_key);
+  auto load = [&](int i) { return value(a.in_smem ? held[i] : src[i]); };
+  // weights of four elements from i on, `step` apart, that lie before `end`; 0 for those not kept
+  auto kept = [&](int i, int step, int end, uint64_t (&w)[4]) {
+    float l[4];
+    uint32_t key[4];
+    bool any = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      l[k] = 0.f, key[k] = 0u, w[k] = 0;
+      if (i + k * step < end) l[k] = load(i + k * step), key[k] = key_of(l[k]);
+      any |= key[k] >= last_key;
+    }
+    if (!any) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t x = wt.of(l[k], key[k]);
+      if (key[k] >= last_key && place_of(key[k], start + i + k * step) <= border && x >= least_w) w[k] = x;
+    }
   };
   // warp w owns a contiguous range of the part
-  const int range = (len4 + kWarps * 4 - 1) / (kWarps * 4) * 4;
-  uint64_t mine = 0;
-  for (int i = warp * range + lane; i < min(len, (warp + 1) * range); i += 32)
-    mine += kept(value(a.in_smem ? held[i] : src[i]), i);
+  const int range = (len4 + kWarps * 4 - 1) / (kWarps * 4) * 4, range_end = min(len, (warp + 1) * range);
+  uint64_t mine = 0, w4[4];
+  for (int i = warp * range + lane; i < range_end; i += 128) {
+    kept(i, 32, range_end, w4);
+    mine += w4[0] + w4[1] + w4[2] + w4[3];
+  }
   mine = warp_sum(mine);
   if (lane == 0) s.part[warp] = mine;
   __syncthreads();
@@ -483,33 +624,32 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
     if (i < rank) before += t;
     total += t;
   }
-  // the sum up to the token is the first above this
-  uint64_t target = static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(total));
-  target = target < total ? target : total - 1;
-  const uint64_t own = s.total;
-  cluster.sync();  // no CTA leaves, or writes part[], while another reads its total
+  const uint64_t target = draw(total), own = s.total;
+  cluster.sync();  // no CTA leaves while another reads its total
   if (target < before || target >= before + own) return;
-  int w = 0;
-  while (w < kWarps - 1 && target >= before + s.part[w]) before += s.part[w++];
-  // the range's elements in order: a thread takes neighbours
-  const int i0 = w * range, n_range = min(len, i0 + range) - i0, per = (n_range + kThreads - 1) / kThreads;
-  const int lo = min(i0 + tid * per, i0 + n_range), hi = min(lo + per, i0 + n_range);
-  uint64_t mass = 0, unused_w;
-  unsigned int n = 0, unused_n;
-  for (int i = lo; i < hi; ++i) mass += kept(value(a.in_smem ? held[i] : src[i]), i);
-  const uint64_t have = mass;
+  int part = 0;
+  while (part < kWarps - 1 && target >= before + s.part[part]) before += s.part[part++];
   __syncthreads();
-  block_before(mass, n, unused_w, unused_n, s);
+  // the range's elements in order: a thread takes neighbours
+  const int i0 = part * range, i1 = min(len, i0 + range), per_thread = (i1 - i0 + kThreads - 1) / kThreads;
+  const int lo = min(i0 + tid * per_thread, i1), hi = min(lo + per_thread, i1);
+  uint64_t mass = 0, all_w;
+  unsigned int n = 0, all_n;
+  for (int i = lo; i < hi; i += 4) {
+    kept(i, 1, hi, w4);
+    mass += w4[0] + w4[1] + w4[2] + w4[3];
+  }
+  const uint64_t have = mass;
+  block_before(mass, n, all_w, all_n, s);
   uint64_t run = before + mass;
   if (target < run || target >= run + have) return;
-  for (int i = lo; i < hi; ++i) {
-    const uint64_t x = kept(value(a.in_smem ? held[i] : src[i]), i);
-    if (target < run + x) {
-      a.tokens[r] = start + i;
-      if (a.logprob != nullptr) a.logprob[r] = static_cast<float>(log(static_cast<double>(x) / static_cast<double>(total)));
-      break;
+  for (int i = lo; i < hi; i += 4) {
+    kept(i, 1, hi, w4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (target >= run && target < run + w4[k]) answer(start + i + k, w4[k], total);
+      run += w4[k];
     }
-    run += x;
   }
 }
 
@@ -518,9 +658,9 @@ int launch(SampleArgs a, int B, cudaStream_t st) {
   const int size = DT == MV_F32 ? 4 : 2;
   constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
   constexpr size_t kMost = 227 * 1024;
-  // as many CTAs a row as keep the card busy, more where the row does not fit in their shared memory
+  // as many CTAs a row as keep the card busy, and as let two of them share an SM, one of which reads while the other computes
   int C = 1;
-  while (C < 8 && (static_cast<long long>(B) * C * 2 <= num_sms() || (static_cast<size_t>(a.V) / C + 8) * size > kMost - kFixed)) C *= 2;
+  while (C < 8 && (static_cast<long long>(B) * C * 2 <= num_sms() || (static_cast<size_t>(a.V) / C + 8) * size > kMost / 2 - 1024 - kFixed)) C *= 2;
   a.slice = ((a.V + C - 1) / C + 7) / 8 * 8;
   a.in_smem = static_cast<size_t>(a.slice) * size <= kMost - kFixed;
   const size_t smem = kFixed + (a.in_smem ? static_cast<size_t>(a.slice) * size : 0);
