@@ -3,9 +3,9 @@
 // Mathematics. Tokens are ordered by (logit descending, index ascending), as one 64-bit number `place`: the logit's bits, mapped
 // so that unsigned comparison orders them, in the upper half and the index in the lower. Each filter keeps a prefix of that order,
 // so all that is kept is given by one place, the border, and a least weight. Weights 2^t, t = (logit - max) log2(e) / temperature,
-// are whole numbers of 2^-shift (shift 45 for vocabularies up to 2^17; the polynomial for 2^f, by interpolation at the Chebyshev
-// nodes of [-1/2, 1/2], is off by 2^-44 of it at most), so that sums do not depend on their order: each border and each draw comes out
-// the same whatever the split, and a weight below 2^-shift / 2, which no 24-bit random number can draw, is 0.
+// are whole numbers of 2^-shift (shift 45 for vocabularies up to 2^17; 2^f from a table of 32 values and a polynomial of degree 5
+// that interpolates 2^g at the Chebyshev nodes of [-1/64, 1/64], off by 2^-52 of it), so that sums do not depend on their order: each border and each draw comes out
+// the same whatever the split; a weight below 2^-shift / 2, which no 24-bit random number can draw, is 0.
 //
 // Steps, a cluster of CTAs for each row, the row in their shared memory:
 //   1. read the row once; the first of the order, and (top-k) a key with at least top_k logits at or above it: the least over
@@ -13,7 +13,7 @@
 //   2. few candidates (a small top_k, or min_p without top_p): they are brought together in the first CTA, which finds the
 //      borders and draws by itself
 //   3. else the borders: a histogram of t with 2048 bins (counts for top-k; for top-p weights, as three sums of 15 bits, since
-//      32 bits are what shared memory adds), added up in the first CTA, which finds the bin with the border; that bin's tokens
+//      64-bit additions in shared memory cost seven times three of 32 bits), added up in the first CTA, which finds the bin with the border; that bin's tokens
 //      are brought together there. A bin with more than the list holds (runs of equal logits) is searched over all CTAs.
 //   4. each CTA adds up what is kept of its part; the CTA in which the sum passes u times the total finds the token.
 // A border among listed tokens is found bit by bit over their places.
@@ -66,27 +66,26 @@ struct Weights {
   double m, c, lim;     // largest logit, log2(e) / temperature, least t that is told apart
   uint32_t top, least;  // keys: of the largest logit, and of the least that can have a weight
   int shift;
+  const double* table;  // 2^(j / 32)
   // 0 for the largest logit itself (which may be infinite), lim for those without a weight
   __device__ __forceinline__ double t_of(float l, uint32_t key) const {
     const double d = key == top ? 0.0 : static_cast<double>(l) - m;
-    return key < least ? lim : fmax(d * c, lim);
+    return key < least ? lim : d * c;
   }
   // 2^t in units of 2^-shift, rounded: 0 at lim
   __device__ __forceinline__ uint64_t at(double t) const {
-    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: the low word of a sum with it is the number, rounded
+    constexpr double kRound = 211106232532992.0;  // 1.5 * 2^47: the low word of a sum with it counts 32nds, rounded
     const double r = t + kRound;
-    const double f = t - (r - kRound);
-    double p = 1.0203121063391729e-07;
-    p = fma(p, f, 1.3255224878668817e-06);
-    p = fma(p, f, 1.525268684626772e-05);
-    p = fma(p, f, 0.00015403455852453838);
-    p = fma(p, f, 0.0013333558179043112);
-    p = fma(p, f, 0.009618129159402558);
-    p = fma(p, f, 0.055504108664760424);
-    p = fma(p, f, 0.2402265069581299);
-    p = fma(p, f, 0.6931471805599453);
-    p = fma(p, f, 1.0);
-    const double s = __hiloint2double((1023 + __double2loint(r) + shift) << 20, 0);
+    const double g = t - (r - kRound);
+    const int n = __double2loint(r);
+    double p = 0.0013333604694153824;
+    p = fma(p, g, 0.009618176115571158);
+    p = fma(p, g, 0.05550410866453748);
+    p = fma(p, g, 0.24022650695623157);
+    p = fma(p, g, 0.6931471805599453);
+    p = fma(p, g, 1.0);
+    const double b = table[n & 31];
+    const double s = __hiloint2double(__double2hiint(b) + (((n >> 5) + shift) << 20), __double2loint(b));
     return static_cast<uint64_t>(__double_as_longlong(fma(p, s, 4503599627370496.0))) & 0xfffffffffffffull;  // 2^52
   }
   __device__ __forceinline__ uint64_t of(float l, uint32_t key) const { return at(t_of(l, key)); }
@@ -98,10 +97,12 @@ struct Weights {
   }
 };
 
+// three additions of 27, 27 and 10 bits, which a warp does in one instruction each
 __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  const unsigned int a = __reduce_add_sync(0xffffffffu, static_cast<unsigned int>(v) & 0x7ffffffu);
+  const unsigned int b = __reduce_add_sync(0xffffffffu, static_cast<unsigned int>(v >> 27) & 0x7ffffffu);
+  const unsigned int c = __reduce_add_sync(0xffffffffu, static_cast<unsigned int>(v >> 54));
+  return a + (static_cast<uint64_t>(b) << 27) + (static_cast<uint64_t>(c) << 54);
 }
 
 struct Shared {
@@ -110,7 +111,8 @@ struct Shared {
     unsigned long long list[kList];
   };
   unsigned long long part[kWarps], total, border, kept, need, least_place, most_place, best, bin_before;
-  unsigned int counts[kWarps], n_list, pivot, nan, bin, bin_count_before, part_n;
+  double table[32];
+  unsigned int counts[kWarps], n_list, pivot, nan, bin, bin_count_before, part_n, bin_from, bin_to;
 };
 
 // Sums of (w, n) over the CTA in every thread. Two barriers.
@@ -268,6 +270,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 
   // ---- 1. the row, the first of its order
   if (tid == 0) s.nan = 0u, s.n_list = 0u, s.best = ~0ull;
+  if (warp == 1) s.table[lane] = exp2(lane / 32.0);
   __syncthreads();
   uint32_t top = 0u;
   int top_at = 0;
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     return;
   }
   Weights wt;
-  wt.top = top, wt.shift = a.shift;
+  wt.top = top, wt.shift = a.shift, wt.table = s.table;
   wt.m = of_key(top), wt.c = 1.4426950408889634 / static_cast<double>(temp);
   wt.lim = -static_cast<double>(a.shift + 2);
   wt.least = wt.key_at(wt.lim);
@@ -380,6 +383,45 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     if (count <= kList) {
       cluster.barrier_arrive();
       if (rank > 0) return;
+      if (count <= kThreads) {
+        // a thread for each: its place among them, and the weights before it, by comparing with all
+        unsigned long long *places = s.list, *weights = places + kThreads, *index = weights + kThreads, *kept = index + kThreads;
+        uint64_t place = ~0ull, w = 0, w_before = 0;
+        unsigned int n_before = 0;
+        if (tid < count) {
+          place = places[tid];
+          const uint32_t key = ~static_cast<uint32_t>(place >> 32);
+          weights[tid] = w = wt.of(of_key(key), key);
+        }
+        __syncthreads();
+        if (warp * 32 < count) {
+#pragma unroll 4
+          for (unsigned int j = 0; j < count; ++j)
+            if (places[j] < place) ++n_before, w_before += weights[j];
+        }
+        const unsigned int most = by_k ? min(count, static_cast<unsigned int>(top_k)) : count;
+        if (tid < count && n_before == most - 1) s.kept = w_before + w;
+        __syncthreads();
+        bool keep = tid < count && n_before < most && w >= least_w;
+        if (by_p) keep &= w_before < static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(s.kept)));
+        const unsigned int n_kept = __syncthreads_count(keep);
+        if (keep) {
+          index[n_before] = place & 0xffffffffull, kept[n_before] = w;
+          if (n_before == n_kept - 1) s.total = w_before + w;
+        }
+        __syncthreads();
+        if (tid < n_kept) {
+          // the weights up to a token in the order of the indices
+          const uint64_t at = index[tid], own = kept[tid], target = draw(s.total);
+          uint64_t run = 0;
+#pragma unroll 4
+          for (unsigned int j = 0; j < n_kept; ++j)
+            if (index[j] < at) run += kept[j];
+          if (target >= run && target < run + own) answer(static_cast<int>(at), own, s.total);
+        }
+        cluster.barrier_wait();
+        return;
+      }
       Listed list;
 #pragma unroll
       for (int i = 0; i < Listed::kEach; ++i) {
@@ -431,6 +473,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     uint64_t need_w = ~0ull, w;  // top-p keeps a token while the weights before it are less
     const unsigned int need_n = static_cast<unsigned int>(top_k);
     unsigned int bin = 0xffffffffu, n;
+    uint32_t bin_from = 0u, bin_to = 0xffffffffu;
     if (tid == 0) s.n_list = 0u, s.bin = bin, s.least_place = ~0ull, s.most_place = 0ull;
     if (bins) {
       for (int i = tid; i < 4 * kBins; i += kThreads) s.bins[0][i] = 0u;
@@ -491,10 +534,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             s.bin = tid * kPer + i, s.bin_before = w, s.bin_count_before = n;
           w += wb[i], n += nb[i];
         }
+        __syncthreads();
+        if (warp == 0 && s.bin != 0xffffffffu) {
+          // the bin's least and largest keys: a key's bin falls as it rises; 32 keys are tried at a time
+          const unsigned int b = s.bin;
+          auto least_of = [&](unsigned int most_bin) {  // the least key from `from` on whose bin is at most this
+            uint32_t lo = from, hi = top;               // (top's bin is 0)
+            while (lo < hi) {
+              const uint32_t part = (hi - lo) / 32 + 1;
+              const uint32_t key = min(static_cast<uint64_t>(lo) + static_cast<uint64_t>(part) * lane, static_cast<uint64_t>(hi));
+              const unsigned int in = __ballot_sync(0xffffffffu, bin_of(wt.t_of(of_key(key), key)) <= most_bin);
+              const int k = in == 0u ? 32 : __ffs(in) - 1;  // the first key tried that is in
+              const uint64_t next = static_cast<uint64_t>(lo) + static_cast<uint64_t>(part) * k;
+              if (k < 32) hi = static_cast<uint32_t>(min(next, static_cast<uint64_t>(hi)));
+              if (k > 0) lo = static_cast<uint32_t>(min(static_cast<uint64_t>(lo) + static_cast<uint64_t>(part) * (k - 1) + 1, static_cast<uint64_t>(hi)));
+              else break;
+            }
+            return hi;
+          };
+          const uint32_t k0 = least_of(b), k1 = b == 0u ? top : least_of(b - 1) - 1;
+          if (lane == 0) s.bin_from = k0, s.bin_to = k1;
+        }
       }
       cluster.sync();
       bin = s0.bin, need_w = s0.need;
       if (bin == 0xffffffffu) continue;  // top_k keeps all that has a weight
+      bin_from = s0.bin_from, bin_to = s0.bin_to;
       const uint64_t w_before = s0.bin_before;
       const unsigned int n_before = s0.bin_count_before;
       each([&](const float (&l)[4], int i) {
@@ -502,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         for (int k = 0; k < 4; ++k) {
           const uint32_t key = key_of(l[k]);
           const uint64_t place = place_of(key, start + i + k);
-          if (key < from || place > border || bin_of(wt.t_of(l[k], key)) != bin) continue;
+          if (key < bin_from || key > bin_to || place > border) continue;
           const unsigned int at = atomicAdd(&s0.n_list, 1u);
           if (at < kList) s0.list[at] = place;
         }
@@ -562,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       for (int k = 0; k < 4; ++k) {
         const uint32_t key = key_of(l[k]);
         const uint64_t place = place_of(key, start + i + k);
-        if (key < from || place > border || (bins && bin_of(wt.t_of(l[k], key)) != bin)) continue;
+        if (key < from || key < bin_from || key > bin_to || place > border) continue;
         first = min(first, place), last = max(last, place);
       }
     });
@@ -657,10 +722,13 @@ template <int DT>
 int launch(SampleArgs a, int B, cudaStream_t st) {
   const int size = DT == MV_F32 ? 4 : 2;
   constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
-  constexpr size_t kMost = 227 * 1024;
-  // as many CTAs a row as keep the card busy, and as let two of them share an SM, one of which reads while the other computes
+  constexpr size_t kMost = 227 * 1024;  // shared memory of an SM (of which a CTA takes 1 KB for itself)
+  // two CTAs share an SM, one of which reads while the other computes: at least as many a row as that leaves room for its part, and
+  // as many as run at once
+  const auto fits = [&](int c, size_t room) { return (static_cast<size_t>(a.V) / c + 8) * size <= room - kFixed; };
+  const int at_once = 2 * num_sms();
   int C = 1;
-  while (C < 8 && (static_cast<long long>(B) * C * 2 <= num_sms() || (static_cast<size_t>(a.V) / C + 8) * size > kMost / 2 - 1024 - kFixed)) C *= 2;
+  while (C < 8 && (!fits(C, kMost / 2 - 1024) || static_cast<long long>(B) * (C + 1) <= at_once)) ++C;
   a.slice = ((a.V + C - 1) / C + 7) / 8 * 8;
   a.in_smem = static_cast<size_t>(a.slice) * size <= kMost - kFixed;
   const size_t smem = kFixed + (a.in_smem ? static_cast<size_t>(a.slice) * size : 0);
