@@ -97,6 +97,22 @@ __device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
+// Cluster barrier, called by all threads of a CTA. A warp arrives as a whole, so its lanes have to come together first: where
+// they came apart from a loop, each part arrived by itself, the barrier opened early and other CTAs read unfinished sums
+// (about 3 % of the rows of mv_sample, with barrier.cluster with and without .aligned). __syncthreads brings them together.
+__device__ __forceinline__ void cluster_arrive() {
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncthreads();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // ------------------------------------------------------------------------------------------ error flag
 
 // Workspace header layout (first 256 bytes of every kernel workspace).

@@ -68,9 +68,6 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // the value at shared address `addr` of the cluster's CTA `rank`
 __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
   uint32_t a;

@@ -47,6 +47,7 @@ struct SampleArgs {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048, kList = 4096;
+constexpr unsigned int kFew = 128;  // tokens that are put in order by comparing all with all (n * n / 128 steps of some 12 instructions)
 constexpr int kMostMaxima = kThreads * 3 / 4;  // of a CTA's threads, in finding the key of step 1
 constexpr uint32_t kNone = 0x007fffffu;  // the key of -inf
 
@@ -110,9 +111,10 @@ struct Shared {
     unsigned int bins[4][kBins];  // counts, or the weights' bits 0-14, 15-29 and 30-45
     unsigned long long list[kList];
   };
-  unsigned long long part[kWarps], total, border, kept, need, least_place, most_place, best, bin_before;
+  unsigned long long part[kWarps], total, border, kept, least_place, most_place, best, bin_before;
   double table[32];
-  unsigned int counts[kWarps], n_list, pivot, nan, bin, bin_count_before, part_n, bin_from, bin_to;
+  unsigned int fine[4][kThreads], counts[kWarps], n_list, pivot, nan, bin, bin_count_before, part_n, bin_from, bin_to;
+  int bin_here;  // the bin, where this CTA has found it
 };
 
 // Sums of (w, n) over the CTA in every thread. Two barriers.
@@ -162,55 +164,89 @@ __device__ __forceinline__ void block_before(uint64_t& w, unsigned int& n, uint6
 // Tokens of a list in the registers of one CTA's threads.
 struct Listed {
   static constexpr int kEach = kList / kThreads;
-  uint64_t place[kEach], w[kEach];
+  uint64_t place[kEach], w[kEach];  // ~0 and 0 where there is no token
+  int rows;                         // of them that are in use
 
-  // sums over the tokens whose place lies before `end`
-  __device__ __forceinline__ void before(uint64_t end, uint64_t& sum, unsigned int& n, Shared& s) const {
+  // from the list; weights where they are asked for
+  __device__ __forceinline__ void load(unsigned int count, const Weights& wt, bool weights, const Shared& s) {
+    rows = (count + kThreads - 1) / kThreads;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      place[i] = ~0ull, w[i] = 0;
+      const unsigned int at = threadIdx.x + i * kThreads;
+      if (i >= rows || at >= count) continue;
+      place[i] = s.list[at];
+      const uint32_t key = ~static_cast<uint32_t>(place[i] >> 32);
+      if (weights) w[i] = wt.of(of_key(key), key);
+    }
+  }
+  // sums over all tokens up to place `last`
+  __device__ __forceinline__ void up_to(uint64_t last, uint64_t& sum, unsigned int& n, Shared& s) const {
     sum = 0, n = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
-      if (place[i] < end) ++n, sum += w[i];
+      if (i < rows && place[i] <= last && place[i] != ~0ull) ++n, sum += w[i];
     block_sum(sum, n, s);
   }
 
-  // The first place, among the `count` tokens, up to which there are at least need_n tokens (by_count) or weights of at least
-  // need_w; it exists. `sum` receives the weights up to it.
-  __device__ __forceinline__ uint64_t border(bool by_count, unsigned int need_n, uint64_t need_w, unsigned int count, uint64_t& sum,
-                                             Shared& s) const {
-    uint64_t first = ~0ull, last = 0;
+  // The first place up to which there are at least need_n tokens (by_count) or weights of at least need_w, among the `count`
+  // tokens, which lie in from .. to; it exists. Overwrites the list.
+  __device__ __forceinline__ uint64_t border(bool by_count, unsigned int need_n, uint64_t need_w, unsigned int count, uint64_t from,
+                                             uint64_t to, Shared& s) const {
+    const int tid = threadIdx.x;
+    uint64_t w_before = 0;  // of what lies before what is still looked at
+    unsigned int n_before = 0;
+    __syncthreads();
+    // a bin for each thread over the range of the places that are left, until few of them are
+    while (count > kFew) {
+      s.fine[0][tid] = 0u, s.fine[1][tid] = 0u, s.fine[2][tid] = 0u, s.fine[3][tid] = 0u;
+      __syncthreads();
+      const int shift = max(0, 64 - __clzll(to - from) - 9);  // (512 bins)
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (i >= rows || place[i] < from || place[i] > to) continue;
+        const unsigned int b = static_cast<unsigned int>((place[i] - from) >> shift);
+        atomicAdd(&s.fine[0][b], 1u);
+        if (by_count) continue;
+        atomicAdd(&s.fine[1][b], static_cast<unsigned int>(w[i]) & 0x7fffu);
+        atomicAdd(&s.fine[2][b], static_cast<unsigned int>(w[i] >> 15) & 0x7fffu);
+        atomicAdd(&s.fine[3][b], static_cast<unsigned int>(w[i] >> 30));
+      }
+      __syncthreads();
+      const unsigned int n_bin = s.fine[0][tid];
+      const uint64_t w_bin = s.fine[1][tid] + (static_cast<uint64_t>(s.fine[2][tid]) << 15) + (static_cast<uint64_t>(s.fine[3][tid]) << 30);
+      unsigned int n = n_bin, all_n;
+      uint64_t wb = w_bin, all_w;
+      block_before(wb, n, all_w, all_n, s);
+      n += n_before, wb += w_before;
+      if (by_count ? n < need_n && n + n_bin >= need_n : wb < need_w && wb + w_bin >= need_w) {
+        s.bin_before = wb, s.bin_count_before = n, s.n_list = n_bin;
+        s.least_place = from + (static_cast<uint64_t>(tid) << shift);
+        s.most_place = s.least_place + ((1ull << shift) - 1);
+      }
+      __syncthreads();
+      from = s.least_place, to = s.most_place, w_before = s.bin_before, n_before = s.bin_count_before, count = s.n_list;
+      __syncthreads();
+    }
+    // by comparing with all that are left
+    if (tid == 0) s.n_list = 0u;
+    __syncthreads();
+    unsigned long long *places = s.list, *weights = places + kFew;
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
-      if (place[i] != ~0ull) first = min(first, place[i]), last = max(last, place[i]);
-    if (threadIdx.x == 0) s.least_place = ~0ull, s.most_place = 0ull;
+      if (i < rows && place[i] >= from && place[i] <= to) {
+        const unsigned int at = atomicAdd(&s.n_list, 1u);
+        places[at] = place[i], weights[at] = w[i];
+      }
     __syncthreads();
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-      last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
-    }
-    if ((threadIdx.x & 31) == 0 && first != ~0ull) {
-      atomicMin(&s.least_place, static_cast<unsigned long long>(first));
-      atomicMax(&s.most_place, static_cast<unsigned long long>(last));
+    if (tid < count) {
+      const uint64_t mine = places[tid], own = weights[tid];
+#pragma unroll 4
+      for (unsigned int j = 0; j < count; ++j)
+        if (places[j] < mine) ++n_before, w_before += weights[j];
+      if (by_count ? n_before == need_n - 1 : w_before < need_w && w_before + own >= need_w) s.border = mine;
     }
     __syncthreads();
-    first = s.least_place, last = s.most_place;
-    int bit = first == last ? -1 : 63 - __clzll(first ^ last);
-    uint64_t low = bit < 0 ? first : first >> bit >> 1 << bit << 1;
-    unsigned int n_low = 0, n_high = count, n;  // tokens before low, and before the end of what is left
-    for (; bit >= 0 && n_high - n_low > 1; --bit) {
-      const uint64_t mid = low | 1ull << bit;
-      before(mid, sum, n, s);
-      if (by_count ? n < need_n : sum < need_w)
-        low = mid, n_low = n;
-      else
-        n_high = n;
-    }
-    // one token lies at or behind low and before the end of what is left
-    const uint64_t end = bit < 0 ? low + 1 : low + (2ull << bit);
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-      if (place[i] >= low && place[i] < end && place[i] != ~0ull) s.border = place[i];
-    before(end, sum, n, s);
     return s.border;
   }
 };
@@ -328,16 +364,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     }
     if (tid == 0) s.pivot = pivot;
   }
-  cluster.sync();
+  cluster_sync();
   best = ~0ull;
   unsigned int any_nan = 0;
   uint32_t pivot = 0xffffffffu;
-  for (int i = 0; i < C; ++i) {
-    const Shared& p = *cluster.map_shared_rank(&s, i);
-    best = min(best, static_cast<uint64_t>(p.best));
-    any_nan |= p.nan;
-    if (share <= kMostMaxima) pivot = min(pivot, p.pivot);
+  if (lane < C) {
+    const Shared& p = *cluster.map_shared_rank(&s, lane);
+    best = p.best, any_nan = p.nan;
+    if (share <= kMostMaxima) pivot = p.pivot;
   }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
+  best = __shfl_sync(0xffffffffu, best, 0);
+  any_nan = __any_sync(0xffffffffu, any_nan != 0u);
+  pivot = __reduce_min_sync(0xffffffffu, pivot);
   top = best == ~0ull ? 0u : ~static_cast<uint32_t>(best >> 32);
   const bool nothing = any_nan || top <= kNone;
   if (nothing || greedy) {
@@ -345,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       a.tokens[r] = nothing ? -1 : static_cast<int>(static_cast<uint32_t>(best));
       if (a.logprob != nullptr) a.logprob[r] = nothing ? -INFINITY : 0.f;
     }
-    cluster.sync();  // no CTA leaves while another reads its shared memory
+    cluster_sync();  // no CTA leaves while another reads its shared memory
     return;
   }
   Weights wt;
@@ -378,14 +418,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         if (at < kList) s0.list[at] = place_of(key, start + i + k);
       }
     });
-    cluster.sync();
+    cluster_sync();
     const unsigned int count = s0.n_list;
     if (count <= kList) {
-      cluster.barrier_arrive();
+      cluster_arrive();
       if (rank > 0) return;
-      if (count <= kThreads) {
+      if (count <= 2 * kFew) {
         // a thread for each: its place among them, and the weights before it, by comparing with all
-        unsigned long long *places = s.list, *weights = places + kThreads, *index = weights + kThreads, *kept = index + kThreads;
+        unsigned long long *places = s.list, *weights = places + 2 * kFew, *index = weights + 2 * kFew, *kept = index + 2 * kFew;
         uint64_t place = ~0ull, w = 0, w_before = 0;
         unsigned int n_before = 0;
         if (tid < count) {
@@ -419,30 +459,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             if (index[j] < at) run += kept[j];
           if (target >= run && target < run + own) answer(static_cast<int>(at), own, s.total);
         }
-        cluster.barrier_wait();
+        cluster_wait();
         return;
       }
       Listed list;
-#pragma unroll
-      for (int i = 0; i < Listed::kEach; ++i) {
-        const unsigned int at = tid + i * kThreads;
-        list.place[i] = ~0ull, list.w[i] = 0;
-        if (at >= count) continue;
-        list.place[i] = s.list[at];
-        const uint32_t key = ~static_cast<uint32_t>(list.place[i] >> 32);
-        list.w[i] = wt.of(of_key(key), key);
-      }
-      uint64_t border = ~0ull, sum;
+      list.load(count, wt, true, s);
+      const uint64_t first = best, last = place_of(from, -1);  // the list's places lie between these
+      uint64_t border = ~0ull - 1, sum;
       unsigned int n;
-      if (by_k && count > static_cast<unsigned int>(top_k)) {
-        border = list.border(true, top_k, 0, count, sum, s);
-      } else if (by_p) {
-        list.before(~0ull, sum, n, s);
-      }
+      if (by_k && count > static_cast<unsigned int>(top_k)) border = list.border(true, top_k, 0, count, first, last, s);
       if (by_p) {
         // the first place up to which the weights reach top_p of top-k's; its tokens before that are all top-k's
-        const uint64_t need = static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(sum)));
-        border = list.border(false, 0, need, count, sum, s);
+        list.up_to(border, sum, n, s);
+        border = list.border(false, 0, static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(sum))), count, first,
+                             last, s);
       }
       // kept tokens in the order of their indices: the draw's is the first up to which the sum is above the target
 #pragma unroll
@@ -451,15 +481,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         if (list.place[i] != ~0ull) list.place[i] &= 0xffffffffull;
       }
       uint64_t total;
-      list.before(~0ull, total, n, s);
-      const uint64_t at = list.border(false, 0, draw(total) + 1, n, sum, s);
+      list.up_to(~0ull - 1, total, n, s);
+      const uint64_t at = list.border(false, 0, draw(total) + 1, n, 0, a.V - 1, s);
 #pragma unroll
       for (int i = 0; i < Listed::kEach; ++i)
         if (list.place[i] == at) answer(static_cast<int>(at), list.w[i], total);
-      cluster.barrier_wait();
+      cluster_wait();
       return;
     }
-    cluster.sync();  // all have read the count
+    cluster_sync();  // all have read the count
   }
 
   // ---- 3. the borders
@@ -474,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const unsigned int need_n = static_cast<unsigned int>(top_k);
     unsigned int bin = 0xffffffffu, n;
     uint32_t bin_from = 0u, bin_to = 0xffffffffu;
-    if (tid == 0) s.n_list = 0u, s.bin = bin, s.least_place = ~0ull, s.most_place = 0ull;
+    if (tid == 0) s.n_list = 0u, s.bin = bin, s.bin_here = -1, s.least_place = ~0ull, s.most_place = 0ull;
     if (bins) {
       for (int i = tid; i < 4 * kBins; i += kThreads) s.bins[0][i] = 0u;
       __syncthreads();
@@ -484,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t key = key_of(l[k]);
-          in[k] = key >= from && place_of(key, start + i + k) <= border;
+          in[k] = key >= from && (border == ~0ull || place_of(key, start + i + k) <= border);
           t[k] = wt.t_of(l[k], key);
         }
         if (phase == 0) {
@@ -505,59 +535,92 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
           }
         }
       });
-      cluster.sync();
-      if (rank == 0) {
-        constexpr int kPer = kBins / kThreads;  // neighbouring bins of a thread: 16 bytes of each sum
-        uint64_t wb[kPer] = {}, all_w;
-        unsigned int nb[kPer] = {}, all_n;
-        for (int c = 0; c < C; ++c) {
-          const Shared& p = *cluster.map_shared_rank(&s, c);
-          if (phase == 0) {
-            const uint4 x = reinterpret_cast<const uint4*>(p.bins[0])[tid];
-            nb[0] += x.x, nb[1] += x.y, nb[2] += x.z, nb[3] += x.w;
-          } else {
+      cluster_sync();
+      // each CTA adds up a share of the bins over all CTAs, a few neighbours to a thread
+      constexpr int kPer = kBins / kThreads;
+      const int share_bins = (kBins + C - 1) / C, per_thread = (share_bins + kThreads - 1) / kThreads;
+      const int share_end = min(kBins, (rank + 1) * share_bins);
+      uint64_t wb[kPer] = {}, all_w;
+      unsigned int nb[kPer] = {}, all_n;
+      w = 0, n = 0;
 #pragma unroll
-            for (int q = 0; q < 3; ++q) {
-              const uint4 x = reinterpret_cast<const uint4*>(p.bins[q + 1])[tid];
-              wb[0] += static_cast<uint64_t>(x.x) << 15 * q, wb[1] += static_cast<uint64_t>(x.y) << 15 * q;
-              wb[2] += static_cast<uint64_t>(x.z) << 15 * q, wb[3] += static_cast<uint64_t>(x.w) << 15 * q;
+      for (int i = 0; i < kPer; ++i) {
+        const int b = rank * share_bins + tid * per_thread + i;
+        if (i >= per_thread || b >= share_end) continue;
+        unsigned int x[3][8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+#pragma unroll
+          for (int q = 0; q < 3; ++q) {
+            x[q][c] = 0u;
+            if (c < C && (q == 0 || phase == 1)) x[q][c] = cluster.map_shared_rank(&s, c)->bins[phase == 0 ? 0 : q + 1][b];
+          }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (phase == 0)
+            nb[i] += x[0][c];
+          else
+            wb[i] += x[0][c] + (static_cast<uint64_t>(x[1][c]) << 15) + (static_cast<uint64_t>(x[2][c]) << 30);
+        }
+        w += wb[i], n += nb[i];
+      }
+      block_before(w, n, all_w, all_n, s);
+      if (tid == 0) s.total = all_w, s.part_n = all_n;
+      cluster_sync();
+      {
+        uint64_t of_lane = 0;
+        unsigned int n_lane = 0;
+        if (lane < C) {
+          const Shared& p = *cluster.map_shared_rank(&s, lane);
+          of_lane = p.total, n_lane = p.part_n;
+        }
+        all_w = warp_sum(of_lane);
+        w += warp_sum(lane < rank ? of_lane : 0ull);
+        n += __reduce_add_sync(0xffffffffu, lane < rank ? n_lane : 0u);
+      }
+      need_w = static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(all_w)));
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (phase == 0 ? n < need_n && n + nb[i] >= need_n : w < need_w && w + wb[i] >= need_w) {
+          s0.bin = rank * share_bins + tid * per_thread + i, s0.bin_before = w, s0.bin_count_before = n;
+          s.bin_here = rank * share_bins + tid * per_thread + i;
+        }
+        w += wb[i], n += nb[i];
+      }
+      __syncthreads();
+      if (warp < 2 && s.bin_here >= 0) {
+        // the bin's least and largest keys: a key's bin falls as the key rises
+        const unsigned int b = s.bin_here;
+        const unsigned int most = warp == 0 ? b : b - 1;  // the least key with at most this bin, which the largest logit's is
+        uint32_t key = top;
+        if (b > 0u || warp == 0) {
+          // where t has half a bin left it is near; else 32 keys at a time are tried
+          const double l0 = wt.m + (most + 0.5) / per / wt.c;
+          const uint32_t guess = key_of(l0 > -3.4e38 ? static_cast<float>(l0) : -3.4e38f);
+          uint32_t lo = from, hi = top;
+          uint32_t tried = min(max(static_cast<int64_t>(guess) - 16 + lane, static_cast<int64_t>(from)), static_cast<int64_t>(top));
+          unsigned int in = __ballot_sync(0xffffffffu, bin_of(wt.t_of(of_key(tried), tried)) <= most);
+          if (in != 0u && !(in & 1u)) {
+            lo = hi = __shfl_sync(0xffffffffu, tried, __ffs(in) - 1);
+          }
+          while (lo < hi) {
+            const uint32_t part = (hi - lo) / 32 + 1;
+            tried = min(static_cast<uint64_t>(lo) + static_cast<uint64_t>(part) * lane, static_cast<uint64_t>(hi));
+            in = __ballot_sync(0xffffffffu, bin_of(wt.t_of(of_key(tried), tried)) <= most);
+            if (in == 0u) {
+              lo = __shfl_sync(0xffffffffu, tried, 31) + 1;
+            } else {
+              const int k = __ffs(in) - 1;
+              hi = __shfl_sync(0xffffffffu, tried, k);
+              lo = k == 0 ? hi : __shfl_sync(0xffffffffu, tried, k - 1) + 1;
             }
           }
+          key = warp == 0 ? hi : hi - 1;
         }
-        w = wb[0] + wb[1] + wb[2] + wb[3], n = nb[0] + nb[1] + nb[2] + nb[3];
-        block_before(w, n, all_w, all_n, s);
-        if (phase == 1) need_w = static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(all_w)));
-        if (tid == 0) s.need = need_w;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          if (phase == 0 ? n < need_n && n + nb[i] >= need_n : w < need_w && w + wb[i] >= need_w)
-            s.bin = tid * kPer + i, s.bin_before = w, s.bin_count_before = n;
-          w += wb[i], n += nb[i];
-        }
-        __syncthreads();
-        if (warp == 0 && s.bin != 0xffffffffu) {
-          // the bin's least and largest keys: a key's bin falls as it rises; 32 keys are tried at a time
-          const unsigned int b = s.bin;
-          auto least_of = [&](unsigned int most_bin) {  // the least key from `from` on whose bin is at most this
-            uint32_t lo = from, hi = top;               // (top's bin is 0)
-            while (lo < hi) {
-              const uint32_t part = (hi - lo) / 32 + 1;
-              const uint32_t key = min(static_cast<uint64_t>(lo) + static_cast<uint64_t>(part) * lane, static_cast<uint64_t>(hi));
-              const unsigned int in = __ballot_sync(0xffffffffu, bin_of(wt.t_of(of_key(key), key)) <= most_bin);
-              const int k = in == 0u ? 32 : __ffs(in) - 1;  // the first key tried that is in
-              const uint64_t next = static_cast<uint64_t>(lo) + static_cast<uint64_t>(part) * k;
-              if (k < 32) hi = static_cast<uint32_t>(min(next, static_cast<uint64_t>(hi)));
-              if (k > 0) lo = static_cast<uint32_t>(min(static_cast<uint64_t>(lo) + static_cast<uint64_t>(part) * (k - 1) + 1, static_cast<uint64_t>(hi)));
-              else break;
-            }
-            return hi;
-          };
-          const uint32_t k0 = least_of(b), k1 = b == 0u ? top : least_of(b - 1) - 1;
-          if (lane == 0) s.bin_from = k0, s.bin_to = k1;
-        }
+        if (lane == 0) (warp == 0 ? s0.bin_from : s0.bin_to) = key;
       }
-      cluster.sync();
-      bin = s0.bin, need_w = s0.need;
+      cluster_sync();
+      bin = s0.bin;
       if (bin == 0xffffffffu) continue;  // top_k keeps all that has a weight
       bin_from = s0.bin_from, bin_to = s0.bin_to;
       const uint64_t w_before = s0.bin_before;
@@ -572,23 +635,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
           if (at < kList) s0.list[at] = place;
         }
       });
-      cluster.sync();
+      cluster_sync();
       const unsigned int count = s0.n_list;
       if (count <= kList) {
         if (rank == 0) {
           Listed list;
-#pragma unroll
-          for (int i = 0; i < Listed::kEach; ++i) {
-            const unsigned int at = tid + i * kThreads;
-            list.place[i] = ~0ull, list.w[i] = 0;
-            if (at >= count) continue;
-            list.place[i] = s.list[at];
-            const uint32_t key = ~static_cast<uint32_t>(list.place[i] >> 32);
-            if (phase == 1) list.w[i] = wt.of(of_key(key), key);
-          }
-          list.border(phase == 0, need_n - n_before, need_w - w_before, count, w, s);
+          list.load(count, wt, phase == 1, s);
+          list.border(phase == 0, need_n - n_before, need_w - w_before, count, place_of(bin_to, 0), place_of(bin_from, -1), s);
         }
-        cluster.sync();
+        cluster_sync();
         border = s0.border;
         continue;
       }
@@ -608,13 +663,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       });
       block_sum(w, n, s);
       if (tid == 0) s.total = w, s.part_n = n;
-      cluster.sync();
+      cluster_sync();
       w = 0, n = 0;
-      for (int i = 0; i < C; ++i) {
-        const Shared& p = *cluster.map_shared_rank(&s, i);
-        w += p.total, n += p.part_n;
+      if (lane < C) {
+        const Shared& p = *cluster.map_shared_rank(&s, lane);
+        w = p.total, n = p.part_n;
       }
-      cluster.sync();
+      w = warp_sum(w), n = __reduce_add_sync(0xffffffffu, n);
+      cluster_sync();
     };
     if (!bins) {
       before(~0ull);
@@ -631,12 +687,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         first = min(first, place), last = max(last, place);
       }
     });
-    if (first != ~0ull) {
-      atomicMin(&s0.least_place, static_cast<unsigned long long>(first));
-      atomicMax(&s0.most_place, static_cast<unsigned long long>(last));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+      last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
     }
-    cluster.sync();
-    first = s0.least_place, last = s0.most_place;
+    if (lane == 0 && first != ~0ull) {
+      atomicMin(&s.least_place, static_cast<unsigned long long>(first));
+      atomicMax(&s.most_place, static_cast<unsigned long long>(last));
+    }
+    cluster_sync();
+    first = ~0ull, last = 0;
+    if (lane < C) {
+      const Shared& p = *cluster.map_shared_rank(&s, lane);
+      first = p.least_place, last = p.most_place;
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+      last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+    }
+    first = __shfl_sync(0xffffffffu, first, 0), last = __shfl_sync(0xffffffffu, last, 0);
     int bit = first == last ? -1 : 63 - __clzll(first ^ last);
     uint64_t low = bit < 0 ? first : first >> bit >> 1 << bit << 1;
     for (; bit >= 0; --bit) {
@@ -644,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       if (phase == 0 ? n < need_n : w < need_w) low |= 1ull << bit;
     }
     border = low;
-    cluster.sync();  // all have read the first CTA's places
+    cluster_sync();  // all have read the first CTA's places
   }
 
   // ---- 4. the draw
@@ -665,7 +736,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint64_t x = wt.of(l[k], key[k]);
-      if (key[k] >= last_key && place_of(key[k], start + i + k * step) <= border && x >= least_w) w[k] = x;
+      w[k] = key[k] >= last_key ? x : 0;
+    }
+    if (border != ~0ull || least_w > 1) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (place_of(key[k], start + i + k * step) > border || w[k] < least_w) w[k] = 0;
     }
   };
   // warp w owns a contiguous range of the part
@@ -682,15 +758,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const uint64_t all = warp_sum(lane < kWarps ? s.part[lane] : 0ull);
     if (lane == 0) s.total = all;
   }
-  cluster.sync();
-  uint64_t before = 0, total = 0;
-  for (int i = 0; i < C; ++i) {
-    const uint64_t t = cluster.map_shared_rank(&s, i)->total;
-    if (i < rank) before += t;
-    total += t;
-  }
+  cluster_sync();
+  const uint64_t of_lane = lane < C ? cluster.map_shared_rank(&s, lane)->total : 0ull;
+  const uint64_t total = warp_sum(of_lane);
+  uint64_t before = warp_sum(lane < rank ? of_lane : 0ull);
   const uint64_t target = draw(total), own = s.total;
-  cluster.sync();  // no CTA leaves while another reads its total
+  cluster_sync();  // no CTA leaves while another reads its total
   if (target < before || target >= before + own) return;
   int part = 0;
   while (part < kWarps - 1 && target >= before + s.part[part]) before += s.part[part++];

@@ -91,6 +91,17 @@ def test_equal_logits(cuda):
             check(x.to(BF), u, **s)
 
 
+def test_equal_logits_over_and_over(cuda):
+    """Borders inside runs of equal logits that are searched over all CTAs of a row: the same at each call."""
+    x = torch.zeros(3, 70001, device=cuda)
+    x[2, ::3] = -200.0
+    u = torch.tensor([0.25, 0.99, 0.5], device=cuda)
+    for s in (dict(top_p=0.75), dict(top_p=0.75, top_k=35001), dict(top_k=35000)):
+        want = [O.sample(x[r].cpu(), u[r].item(), 1.0, s.get("top_k", 0), s.get("top_p", 1.0), 0.0)[0] for r in range(3)]
+        got = torch.stack([S.sample(x, u, **s) for _ in range(100)])
+        assert got.tolist() == [want] * 100
+
+
 def test_zeros_of_both_signs_are_equal(cuda):
     x = torch.full((1, 100), -1.0, device=cuda)
     x[0, 10], x[0, 20] = -0.0, 0.0
