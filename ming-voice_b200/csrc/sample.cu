@@ -796,12 +796,13 @@ int launch(SampleArgs a, int B, cudaStream_t st) {
   const int size = DT == MV_F32 ? 4 : 2;
   constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
   constexpr size_t kMost = 227 * 1024;  // shared memory of an SM (of which a CTA takes 1 KB for itself)
-  // two CTAs share an SM, one of which reads while the other computes: at least as many a row as that leaves room for its part, and
-  // as many as run at once
+  // Two CTAs share an SM where they can, one of which reads while the other computes: at least as many a row as that leaves room
+  // for its part. More where there are few rows: up to 5/7 of the SMs, which is what clusters find together, one CTA each (16 rows of
+  // 131072, top-p, us: 6 CTAs a row 36, 7 63, 8 42), or 7/4 of them, two CTAs each (64 rows of 32000: 4 CTAs a row 31, 5 47).
   const auto fits = [&](int c, size_t room) { return (static_cast<size_t>(a.V) / c + 8) * size <= room - kFixed; };
-  const int at_once = 2 * num_sms();
+  const long long most = 4LL * B <= num_sms() * 5 / 7 ? num_sms() * 5 / 7 : num_sms() * 7 / 4;
   int C = 1;
-  while (C < 8 && (!fits(C, kMost / 2 - 1024) || static_cast<long long>(B) * (C + 1) <= at_once)) ++C;
+  while (C < 8 && (!fits(C, kMost / 2 - 1024) || static_cast<long long>(B) * (C + 1) <= most)) ++C;
   a.slice = ((a.V + C - 1) / C + 7) / 8 * 8;
   a.in_smem = static_cast<size_t>(a.slice) * size <= kMost - kFixed;
   const size_t smem = kFixed + (a.in_smem ? static_cast<size_t>(a.slice) * size : 0);

@@ -4,8 +4,9 @@
 
 Each translation unit compiles to an object under `mingmoe/_build/` (skipped when up to date), then they
 link into `mingmoe/libmingmoe.so` next to this file. The CUDA runtime is linked statically, so the library
-depends only on the driver. `csrc/attention_host.cpp`, the host side of the attention calls, becomes the Python module
-`mingmoe/_attention_host.so` beside it (g++, torch's headers; no device code).
+depends only on the driver. `csrc/attention_host.cpp` and `csrc/serving_host.cpp`, the host side of the attention calls and of the
+8-bit products, draws and plans, become the Python modules `mingmoe/_attention_host.so` and `mingmoe/_serving_host.so` beside it
+(g++, torch's headers; no device code).
 """
 from __future__ import annotations
 
@@ -86,10 +87,12 @@ def build(verbose: bool = False, force: bool = False, ptxas_v: bool = False, out
 
 HOST_SRC = os.path.join(CSRC, "attention_host.cpp")
 HOST_OUT = os.path.join(HERE, "_attention_host.so")
+SERVING_SRC = os.path.join(CSRC, "serving_host.cpp")
+SERVING_OUT = os.path.join(HERE, "_serving_host.so")
 
 
-def build_host(verbose: bool = False, force: bool = False) -> str:
-    """The Python module `_attention_host`. It is bound to the headers of one torch and one Python, so the command that compiled
+def _build_module(src: str, out: str, verbose: bool, force: bool) -> str:
+    """A Python module in C++. It is bound to the headers of one torch and one Python, so the command that compiled
     it (with their versions) is kept beside the objects, and another command compiles it again."""
     import sysconfig
 
@@ -98,29 +101,41 @@ def build_host(verbose: bool = False, force: bool = False) -> str:
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     inc = [os.path.join(tdir, "include"), os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(cuda, "include"), INCLUDE]
-    tmp = HOST_OUT + ".tmp"
+    tmp = out + ".tmp"
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in inc], HOST_SRC, "-o",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in inc], src, "-o",
            tmp, f"-L{os.path.join(tdir, 'lib')}", "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
     made_by = f"torch {torch.__version__}, python {sys.version}: {' '.join(cmd).replace(ROOT, '.')}\n"
-    record = os.path.join(BUILD, "attention_host.cmd")
-    newest = max([os.path.getmtime(p) for p in [HOST_SRC, *glob.glob(os.path.join(INCLUDE, "*.h"))]])
-    if os.path.exists(HOST_OUT) and os.path.getmtime(HOST_OUT) >= newest and not force and os.path.exists(record):
+    record = os.path.join(BUILD, os.path.splitext(os.path.basename(src))[0] + ".cmd")
+    newest = max([os.path.getmtime(p) for p in [src, *glob.glob(os.path.join(INCLUDE, "*.h")),
+                                                *glob.glob(os.path.join(CSRC, "*.hpp"))]])
+    if os.path.exists(out) and os.path.getmtime(out) >= newest and not force and os.path.exists(record):
         with open(record) as f:
             if f.read() == made_by:
-                return HOST_OUT
+                return out
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for {HOST_SRC}:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, HOST_OUT)
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, out)
     os.makedirs(BUILD, exist_ok=True)
     with open(record, "w") as f:
         f.write(made_by)
-    return HOST_OUT
+    return out
+
+
+def build_host(verbose: bool = False, force: bool = False) -> str:
+    """The Python module `_attention_host`."""
+    return _build_module(HOST_SRC, HOST_OUT, verbose, force)
+
+
+def build_serving_host(verbose: bool = False, force: bool = False) -> str:
+    """The Python module `_serving_host`."""
+    return _build_module(SERVING_SRC, SERVING_OUT, verbose, force)
 
 
 if __name__ == "__main__":
     print(build_host(verbose="-v" in sys.argv, force="--force" in sys.argv))
+    print(build_serving_host(verbose="-v" in sys.argv, force="--force" in sys.argv))
     print(build(verbose="-v" in sys.argv, force="--force" in sys.argv, ptxas_v="--ptxas" in sys.argv))

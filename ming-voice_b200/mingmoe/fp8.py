@@ -15,6 +15,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
+from . import _serving
 
 BLOCK = 128
 _DTYPES = (torch.bfloat16, torch.float16)
@@ -24,6 +25,20 @@ E4M3 = torch.float8_e4m3fn
 def _matrix(t, name):
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"{name} must be a matrix with a unit inner stride, got {tuple(t.shape)} / {t.stride()}")
+
+
+def _header(dev):
+    """The error word of a stream's calls, which the C++ module learns of too."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    index = dev.index if dev.index is not None else torch.cuda.current_device()
+    buf = _headers.get((index, stream))
+    if buf is None:
+        buf = _headers[(index, stream)] = L.workspace("fp8", 256, dev)
+        _serving.host().workspace(index, stream, buf.data_ptr(), buf.numel())
+    return buf
+
+
+_headers: dict = {}
 
 
 def quantize_fp8_weight(w):
@@ -62,6 +77,11 @@ def quantize_fp8(x):
 def fp8_linear(x, wq, ws, *, residual=None, out=None, out_dtype=None):
     """x W^T (+ residual): x [..., K] bf16 / f16, wq [N, K] e4m3 whose rows start at whole 16 bytes, ws as above. The result has
     out_dtype (bf16, f16 or f32; that of x by default), and residual [..., N] the same type. `out` may be the residual."""
+    r = (_serving._module or _serving.host()).fp8_linear(x, wq, ws, residual, out, out_dtype)
+    if type(r) is int:
+        L.check(r, "fp8_linear")
+    if r is not NotImplemented:
+        return r
     dev = x.device
     L.require_cuda(x, wq, ws, residual, out)
     if x.dtype not in _DTYPES:
@@ -103,7 +123,7 @@ def fp8_linear(x, wq, ws, *, residual=None, out=None, out_dtype=None):
         lib = L.lib()
         ws_bytes = lib.mv_fp8_linear_scratch_bytes(rows, n, k)
         scratch = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        header = L.workspace("fp8", 256, dev)
+        header = _header(dev)
         a = L.Fp8LinearArgs(x2.data_ptr(), wq.data_ptr(), ws.data_ptr(), r2.data_ptr() if r2 is not None else 0,
                             o2.data_ptr(), scratch.data_ptr(), x2.stride(0), wq.stride(0), ws.stride(0),
                             r2.stride(0) if r2 is not None else 0, o2.stride(0), ws_bytes, rows, n, k, L.dt(x.dtype),

@@ -15,6 +15,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
+from . import _serving
 from .attention import PagedKV
 
 
@@ -73,6 +74,12 @@ def plan_step(new, lens, pages, free, n_free, *, page_size, num_tokens, seqs=Non
     itself), packed into num_tokens rows. Their pages come from the top of the free stack. pages is written in place; the
     counters go to lens_out and n_free_out, or in place too. A step that does not fit (no room, a sequence unknown or twice, a
     negative count, more tokens than num_tokens or max_len) changes nothing: ok is 0 and the step has no token."""
+    r = (_serving._module or _serving.host()).plan_step(new, lens, pages, free, n_free, page_size, num_tokens, seqs, max_len,
+                                                        lens_out, n_free_out)
+    if type(r) is int:
+        L.check(r, "plan_step")
+    if r is not NotImplemented:
+        return Step(*r, max_q, prompts)
     a, dev = _state(lens, pages, free, n_free, lens_out, n_free_out, page_size)
     L.require_cuda(new, seqs)
     if new.dim() != 1:

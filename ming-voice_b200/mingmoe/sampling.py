@@ -12,6 +12,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
+from . import _serving
 
 
 def _setting(v, name, dtype, b, dev):
@@ -30,6 +31,11 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=Non
     numbers in [0, 1). temperature, top_p, min_p: numbers or fp32 [B]; top_k: a number or int32 [B]. Off: top_k 0, top_p 1,
     min_p 0. temperature 0 takes the largest logit (the lowest index of equal ones). With return_logprob also fp32 [B]: ln of the
     probability with which the token was drawn. A row with a NaN, or of -inf alone, gives -1 (and -inf)."""
+    r = (_serving._module or _serving.host()).sample(logits, u, temperature, top_k, top_p, min_p, out, return_logprob)
+    if type(r) is int:
+        L.check(r, "sample")
+    if r is not NotImplemented:
+        return r
     L.require_cuda(logits, u)
     dev = logits.device
     if logits.dim() != 2:
