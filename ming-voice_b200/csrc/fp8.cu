@@ -25,8 +25,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ 
                                                        uint8_t* __restrict__ q, long long q_st, S* __restrict__ scale,
                                                        long long s_st) {
   pdl_wait();
-  // Only now: the product's kernel reads weights before it waits for this one, and they may come from an earlier kernel.
-  pdl_launch_dependents();
+  // Only now, and only where this is a product's first half: the product's kernel reads weights before it waits for the kernel
+  // in front of it, and they may come from an earlier one, or be what this kernel writes.
+  if (sizeof(S) == 1) pdl_launch_dependents();
   const int sub = threadIdx.x & 15;
   const long long first = static_cast<long long>(blockIdx.x) * UNITS;
   const int t0 = static_cast<int>(first / blocks), b0 = static_cast<int>(first % blocks);
@@ -160,9 +161,12 @@ extern "C" int mv_quantize_fp8_weight(const void* w, int w_dtype, long long w_st
   return cuda_status(cudaGetLastError(), "mv_quantize_fp8_weight launch");
 }
 
-extern "C" size_t mv_fp8_linear_scratch_bytes(int T, int, int K) {
+extern "C" size_t mv_fp8_linear_scratch_bytes(int T, int N, int K) {
   if (T <= 0 || K <= 0) return 0;
   const size_t blocks = (static_cast<size_t>(K) + kBlock - 1) / kBlock;
+  LinearArgs a{};
+  a.T = T, a.N = N, a.K = K, a.blocks = static_cast<int>(blocks);
+  if (one_launch(a)) return 0;
   return align256(static_cast<size_t>(T) * blocks * kBlock) + align256(blocks * scale_stride(T));
 }
 
@@ -185,9 +189,10 @@ extern "C" int mv_fp8_linear(const mv_fp8_linear_args* x, void* workspace, size_
     return fail(MV_ERR_ALIGN, "%s: wq must be 16-byte aligned with rows of whole 16 bytes", who);
   if (workspace == nullptr || workspace_bytes < kWsHeaderBytes)
     return fail(MV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", who, kWsHeaderBytes);
-  if (x->scratch == nullptr || x->scratch_bytes < mv_fp8_linear_scratch_bytes(T, N, K) ||
-      (reinterpret_cast<uintptr_t>(x->scratch) & 255u))
-    return fail(MV_ERR_WORKSPACE, "%s: 256-byte aligned scratch of %zu bytes needed", who, mv_fp8_linear_scratch_bytes(T, N, K));
+  const size_t scratch_bytes = mv_fp8_linear_scratch_bytes(T, N, K);
+  if (scratch_bytes > 0 && (x->scratch == nullptr || x->scratch_bytes < scratch_bytes ||
+                            (reinterpret_cast<uintptr_t>(x->scratch) & 255u)))
+    return fail(MV_ERR_WORKSPACE, "%s: 256-byte aligned scratch of %zu bytes needed", who, scratch_bytes);
   LinearArgs a{};
   a.q_st = blocks * kBlock, a.s_st = scale_stride(T), a.blocks = static_cast<int>(blocks);
   uint8_t* scratch = static_cast<uint8_t*>(x->scratch);
@@ -195,7 +200,9 @@ extern "C" int mv_fp8_linear(const mv_fp8_linear_args* x, void* workspace, size_
   a.w = static_cast<const uint8_t*>(x->wq), a.w_st = N > 1 ? x->w_st : a.q_st, a.ws = x->ws, a.ws_st = x->ws_st;
   a.residual = x->residual, a.r_st = x->r_st, a.out = x->out, a.o_st = x->o_st;
   a.T = T, a.N = N, a.K = K, a.header = static_cast<WsHeader*>(workspace);
+  a.x = x->x, a.x_st = T > 1 ? x->x_st : 0, a.x_dtype = x->x_dtype;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (one_launch(a)) return run_product(a, x->out_dtype, st);
   const int rc = quantize(x->x, x->x_dtype, x->x_st, T, K, a.q, a.q_st, a.scale, a.s_st, st);
   if (rc != MV_OK) return rc;
   return run_product(a, x->out_dtype, st);

@@ -12,6 +12,9 @@ namespace fp8 {
 constexpr int kBlock = 128;  // columns (and rows of a weight) that share a scale
 
 struct LinearArgs {
+  const void* x;           // activations as they come
+  long long x_st;
+  int x_dtype;
   const uint8_t* w;        // [N, K] e4m3
   const float* ws;         // [N / 128, K / 128]
   uint8_t* q;              // activations [T, blocks * 128] e4m3
@@ -25,6 +28,8 @@ struct LinearArgs {
 
 // the products (fp8_gemm.cu); w is 16-byte aligned with rows of whole 16 bytes, q and scale are in the scratch
 int run_product(const LinearArgs& a, int out_dtype, cudaStream_t st);
+// whether it rounds the activations itself (of T, N, K, blocks)
+bool one_launch(const LinearArgs& a);
 
 // row stride of the activations' scales: rows begin at whole 16 bytes
 inline long long scale_stride(int T) { return (static_cast<long long>(T) + 15) / 16 * 16; }

@@ -68,12 +68,12 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-// the value at shared address `addr` of the cluster's CTA `rank`
-__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
+// four values at shared address `addr` of the cluster's CTA `rank`
+__device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
   uint32_t a;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
   return v;
 }
 
@@ -113,9 +113,33 @@ struct FewArgs {
   void* out;
   long long ws_st, s_st, r_st, o_st;
   int T, N, blocks, n_tiles, t_tiles, split;
+  bool x_bf16;                // type of the activations that the kernel rounds itself
   bool out_lines, res_lines;  // whole lines of `out` and `residual` go through their tensor maps
   WsHeader* header;
 };
+
+// Adds the parts [cols][128] of a cluster's CTAs in rank order, each CTA a share of the columns; the loads of all parts are under way
+// together (one after another they took 64 x 2048 x 2048 14.5 us).
+template <int ODT>
+__device__ __forceinline__ void join_parts(const FewArgs& a, uint32_t part, int n0, int t0, int cols, int rank, int threads) {
+  for (int i = (threadIdx.x + rank * threads) * 4; i < cols * kTile; i += threads * a.split * 4) {
+    const int t = t0 + i / kTile, n = n0 + i % kTile;
+    float4 p[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < a.split) p[r] = ld_peer(part + i * 4, r);
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < a.split) v[0] += p[r].x, v[1] += p[r].y, v[2] += p[r].z, v[3] += p[r].w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (n + k >= a.N) break;
+      if (a.residual != nullptr) v[k] += load1<ODT>(a.residual, t * a.r_st + n + k);
+      store1<ODT>(a.out, t * a.o_st + n + k, v[k]);
+    }
+  }
+}
 
 // NT token columns of a tile. Stage: weight tile, activation tile, activation scales.
 template <int NT>
@@ -126,7 +150,8 @@ struct Few {
   static constexpr int kHalves = NT == 128 ? 2 : 1;  // epilogue warps per 32 rows
   static constexpr int kCols = NT / kHalves;         // columns of an epilogue thread
   static constexpr int kThreads = 64 + 128 * kHalves;
-  static constexpr uint32_t kTmemCols = 2 * NT < 32 ? 32 : 2 * NT;
+  static constexpr int kBufs = NT == 128 ? 4 : 8;    // blocks' products in TMEM
+  static constexpr uint32_t kTmemCols = kBufs * NT;
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * (kStageBytes + NT);
 };
 
@@ -137,13 +162,13 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* scales = smem + F::kStages * F::kStageBytes;  // [stage][NT]
-  __shared__ alignas(8) uint64_t full[F::kStages], empty[F::kStages], acc_full[2], acc_empty[2];
+  __shared__ alignas(8) uint64_t full[F::kStages], empty[F::kStages], acc_full[F::kBufs], acc_empty[F::kBufs];
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kEpiWarps = 4 * F::kHalves;
   if (threadIdx.x == 0) {
     for (int i = 0; i < F::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1 + kEpiWarps);
-    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpiWarps);
+    for (int i = 0; i < F::kBufs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpiWarps);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -190,9 +215,9 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
     bool ok = true;
     for (int tile = first; tile < tiles && ok; tile += step) {
       for (int b = b0; b < b1; ++b, ++it) {
-        const int s = it % F::kStages, buf = it & 1;
+        const int s = it % F::kStages, buf = it % F::kBufs;
         if (!wait(&full[s], (it / F::kStages) & 1, a.header, 0x801u) ||
-            (it >= 2 && !wait(&acc_empty[buf], (it / 2 + 1) & 1, a.header, 0x802u))) {
+            (it >= F::kBufs && !wait(&acc_empty[buf], (it / F::kBufs + 1) & 1, a.header, 0x802u))) {
           ok = false;
           break;
         }
@@ -223,10 +248,10 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
       const float* ws = a.ws + n0 / kBlock * a.ws_st;
       float w_next = b0 < b1 ? ws[b0] : 0.f;
       for (int b = b0; b < b1 && ok; ++b, ++it) {
-        const int s = it % F::kStages, buf = it & 1;
+        const int s = it % F::kStages, buf = it % F::kBufs;
         const float w = w_next;
         if (b + 1 < b1) w_next = ws[b + 1];
-        if (!wait(&acc_full[buf], (it / 2) & 1, a.header, 0x803u)) {
+        if (!wait(&acc_full[buf], (it / F::kBufs) & 1, a.header, 0x803u)) {
           ok = false;
           break;
         }
@@ -277,18 +302,9 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
     __syncwarp();
     pdl_wait();
     cluster_sync();
-    // every CTA adds the parts of its share of the columns, in rank order
-    const int tile = first, n0 = tile / a.t_tiles * kTile, t0 = tile % a.t_tiles * NT;
-    const uint32_t part = smem_u32(smem);
-    const int cols = min(NT, a.T - t0);
-    for (int i = threadIdx.x + rank * F::kThreads; i < cols * kTile; i += F::kThreads * a.split) {
-      const int t = t0 + i / kTile, n = n0 + i % kTile;
-      if (n >= a.N) continue;
-      float v = 0.f;
-      for (int r = 0; r < a.split; ++r) v += ld_peer(part + i * 4, r);
-      if (a.residual != nullptr) v += load1<ODT>(a.residual, t * a.r_st + n);
-      store1<ODT>(a.out, t * a.o_st + n, v);
-    }
+    const int tile = first;
+    join_parts<ODT>(a, smem_u32(smem), tile / a.t_tiles * kTile, tile % a.t_tiles * NT, min(NT, a.T - tile % a.t_tiles * NT), rank,
+                    F::kThreads);
     cluster_sync();
   }
   tc::fence_before_sync();
@@ -296,6 +312,209 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
   if (warp == 1) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, F::kTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ a few tokens, few rows
+//
+// The same with the activations rounded by the epilogue warps while the first weights are on their way: one launch, and no
+// activation traffic in the ring. All blocks of a CTA's share of K lie in shared memory.
+
+constexpr int kTokenN = 16, kTokenBlocks = 32, kTokenStages = 12;
+constexpr int kTokenBufs = 8;  // blocks' products in TMEM: the issuing warp does not wait for the epilogue of the last two
+constexpr uint32_t kTokenXBytes = kTokenN * kBlock;  // of a block
+
+inline size_t token_smem(int blocks, int stages) {
+  return 1024 + static_cast<size_t>(stages) * kTileBytes + static_cast<size_t>(blocks) * (kTokenXBytes + kTokenN * 4);
+}
+
+struct TokenArgs {
+  FewArgs f;
+  const void* x;
+  long long x_st;
+  int K, stages, vec;
+};
+
+template <int XDT, int VEC>
+__device__ __forceinline__ void round_tokens(const TokenArgs& a, int b0, int b1, uint8_t* xs, float* scales, int tid) {
+  // a half warp has a token's block; eight blocks at a time are under way
+  const int sub = tid & 15, units = (b1 - b0) * a.f.T;
+  constexpr int kDeep = 4;
+  for (int u0 = tid >> 4; u0 < units + (tid >> 4); u0 += 8 * kDeep) {
+    float v[kDeep][8];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int u = u0 + 8 * i, b = u / a.f.T, t = u % a.f.T;
+      load8<XDT, VEC>(a.x, t * a.x_st, (b0 + b) * kBlock + sub * 8, u < units ? a.K : 0, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int u = u0 + 8 * i, b = u / a.f.T, t = u % a.f.T;
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[i][k]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      float up, down;
+      block_scale(top, up, down);
+      if (u >= units) continue;
+      // the 128-byte swizzle of the operand's layout: 16-byte piece j of row t at j ^ (t & 7)
+      *reinterpret_cast<uint2*>(xs + b * kTokenXBytes + t * kBlock + (((sub >> 1) ^ (t & 7)) << 4) + (sub & 1) * 8) =
+          round8(v[i], down);
+      if (sub == 0) scales[b * kTokenN + t] = up;
+    }
+  }
+}
+
+template <int ODT>
+__global__ void __launch_bounds__(192, 1) token_kernel(const __grid_constant__ CUtensorMap wmap, const TokenArgs g) {
+  const FewArgs& a = g.f;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int b0 = a.blocks * rank / a.split, b1 = a.blocks * (rank + 1) / a.split;
+  uint8_t* xs = smem + g.stages * kTileBytes;                                     // [block][token][128], swizzled
+  float* scales = reinterpret_cast<float*>(xs + (b1 - b0) * kTokenXBytes);        // [block][token]
+  __shared__ alignas(8) uint64_t full[kTokenStages], empty[kTokenStages], acc_full[kTokenBufs], acc_empty[kTokenBufs], x_full;
+  __shared__ uint32_t tmem_base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < g.stages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < kTokenBufs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 4);
+    mbar_init(&x_full, 4);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(&tmem_base, kTokenBufs * kTokenN);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  const int first = blockIdx.x / a.split, step = gridDim.x / a.split;
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (tc::elect_one()) {
+      tc::prefetch_tmap(&wmap);
+      // weights only: they do not depend on the kernel in front of this one
+      int it = 0;
+      bool ok = true;
+      for (int tile = first; tile < a.n_tiles && ok; tile += step) {
+        for (int b = b0; b < b1; ++b, ++it) {
+          const int s = it % g.stages;
+          if (it >= g.stages && !wait(&empty[s], (it / g.stages + 1) & 1, a.header, 0x820u)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[s], kTileBytes);
+          tc::tma_load_2d(smem + s * kTileBytes, &wmap, &full[s], b * kBlock, tile * kTile);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    int it = 0;
+    bool ok = wait(&x_full, 0, a.header, 0x824u);
+    for (int tile = first; tile < a.n_tiles && ok; tile += step) {
+      for (int b = b0; b < b1; ++b, ++it) {
+        const int s = it % g.stages, buf = it % kTokenBufs;
+        if (!wait(&full[s], (it / g.stages) & 1, a.header, 0x821u) ||
+            (it >= kTokenBufs && !wait(&acc_empty[buf], (it / kTokenBufs + 1) & 1, a.header, 0x822u))) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+        if (tc::elect_one()) {
+          const uint64_t ad = tc::sw128_desc(smem_u32(smem + s * kTileBytes));
+          const uint64_t bd = tc::sw128_desc(smem_u32(xs + (b - b0) * kTokenXBytes));
+#pragma unroll
+          for (int k = 0; k < kBlock / 32; ++k)
+            mma_f8(tmem + buf * kTokenN, ad + 2 * k, bd + 2 * k, idesc_e4m3(kTile, kTokenN), k > 0);
+          tc::mma_commit(&empty[s]);
+          tc::mma_commit(&acc_full[buf]);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    const int quarter = warp & 3, row = quarter * 32 + lane, tid = threadIdx.x - 64;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    pdl_wait();
+    if (g.vec == 8)
+      g.f.x_bf16 ? round_tokens<MV_BF16, 8>(g, b0, b1, xs, scales, tid) : round_tokens<MV_F16, 8>(g, b0, b1, xs, scales, tid);
+    else
+      g.f.x_bf16 ? round_tokens<MV_BF16, 1>(g, b0, b1, xs, scales, tid) : round_tokens<MV_F16, 1>(g, b0, b1, xs, scales, tid);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&x_full);
+    named_bar(1, 128);  // the scales of all four warps
+    int it = 0;
+    bool ok = true;
+    for (int tile = first; tile < a.n_tiles; tile += step) {
+      const int n0 = tile * kTile;
+      float acc[kTokenN];
+#pragma unroll
+      for (int c = 0; c < kTokenN; ++c) acc[c] = 0.f;
+      const float* ws = a.ws + n0 / kBlock * a.ws_st;
+      // lane l: the weights' scale of block b0 + l
+      const float ws_lane = b0 + lane < b1 ? ws[b0 + lane] : 0.f;
+      for (int b = b0; b < b1 && ok; ++b, ++it) {
+        const int buf = it % kTokenBufs;
+        const float w = __shfl_sync(0xffffffffu, ws_lane, b - b0);
+        if (!wait(&acc_full[buf], (it / kTokenBufs) & 1, a.header, 0x823u)) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+        uint32_t d[kTokenN];
+        tc::tmem_ld16(lanes + buf * kTokenN, d);
+        tc::tmem_ld_wait();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        const float4* sc = reinterpret_cast<const float4*>(scales + (b - b0) * kTokenN);
+#pragma unroll
+        for (int i = 0; i < kTokenN; i += 4) {
+          if (i >= a.T) break;
+          const float4 f = sc[i / 4];
+          acc[i] = fmaf(__uint_as_float(d[i]), f.x * w, acc[i]);
+          acc[i + 1] = fmaf(__uint_as_float(d[i + 1]), f.y * w, acc[i + 1]);
+          acc[i + 2] = fmaf(__uint_as_float(d[i + 2]), f.z * w, acc[i + 2]);
+          acc[i + 3] = fmaf(__uint_as_float(d[i + 3]), f.w * w, acc[i + 3]);
+        }
+      }
+      const int n = n0 + row;
+      if (a.split == 1) {
+        if (n < a.N && ok) {
+#pragma unroll
+          for (int t = 0; t < kTokenN; ++t) {
+            if (t >= a.T) break;
+            float v = acc[t];
+            if (a.residual != nullptr) v += load1<ODT>(a.residual, t * a.r_st + n);
+            store1<ODT>(a.out, t * a.o_st + n, v);
+          }
+        }
+      } else {
+        // the parts lie where the ring was: its copies have landed and its products are done
+        float* part = reinterpret_cast<float*>(smem);  // [token][128]
+        named_bar(1, 128);
+#pragma unroll
+        for (int t = 0; t < kTokenN; ++t) part[t * kTile + row] = acc[t];
+      }
+    }
+  }
+  if (a.split > 1) {
+    pdl_wait();
+    cluster_sync();
+    join_parts<ODT>(a, smem_u32(smem), first * kTile, 0, a.T, rank, 192);
+    cluster_sync();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, kTokenBufs * kTokenN);
   }
 }
 
@@ -670,9 +889,36 @@ int launch(void (*fn)(P...), int grid, int threads, size_t smem, int cluster, cu
   return cuda_status(cudaLaunchKernelEx(&cfg, fn, args...), "mv_fp8_linear launch");
 }
 
+// CTAs that share a tile's blocks of K: as many as find place at once, which clusters do on some 5/7 of the SMs (64 x 2048 x 2048, 16
+// tiles: clusters of 4 7.8 us, of 8 12.2)
+int split_of(long long tiles, int blocks) {
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= num_sms() * 5 / 7 && split * 2 <= blocks) split *= 2;
+  return split;
+}
+
+template <int ODT>
+int run_token(const LinearArgs& x, cudaStream_t st) {
+  TokenArgs g{};
+  g.f = FewArgs{x.ws, nullptr, x.residual, x.out, x.ws_st, 0, x.r_st, x.o_st, x.T, x.N, x.blocks, (x.N + kTile - 1) / kTile, 1, 1,
+                x.x_dtype == MV_BF16, false, false, x.header};
+  g.x = x.x, g.x_st = x.x_st, g.K = x.K;
+  g.vec = ((reinterpret_cast<uintptr_t>(x.x) | static_cast<uintptr_t>(x.x_st * 2)) & 15) == 0 && x.K % 8 == 0 ? 8 : 1;
+  g.f.split = split_of(g.f.n_tiles, x.blocks);
+  const int share = (x.blocks + g.f.split - 1) / g.f.split;
+  g.stages = kTokenStages;
+  while (token_smem(share, g.stages) > 226 * 1024) --g.stages;
+  CUtensorMap wm;
+  const int rc = row_map(&wm, x.w, 1, x.K, x.N, x.w_st, kTile, "wq");
+  if (rc != MV_OK) return rc;
+  const int sms = num_sms(), tiles = g.f.n_tiles;
+  const int grid = g.f.split > 1 ? tiles * g.f.split : tiles < sms ? tiles : sms;
+  return launch(token_kernel<ODT>, grid, 192, token_smem(share, g.stages), g.f.split, st, wm, g);
+}
+
 template <int NT, int ODT>
 int run_few(const LinearArgs& x, cudaStream_t st) {
-  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, false, false, x.header};
+  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, x.x_dtype == MV_BF16, false, false, x.header};
   a.n_tiles = (x.N + kTile - 1) / kTile;
   a.t_tiles = (x.T + NT - 1) / NT;
   CUtensorMap wm, xm;
@@ -682,13 +928,14 @@ int run_few(const LinearArgs& x, cudaStream_t st) {
   const long long tiles = static_cast<long long>(a.n_tiles) * a.t_tiles;
   if (tiles > 0x7fffffffLL) return fail(MV_ERR_INVALID, "mv_fp8_linear: T=%d x N=%d is too large", x.T, x.N);
   const int sms = num_sms();
-  while (a.split < 8 && tiles * a.split * 2 <= sms && a.split * 2 <= a.blocks) a.split *= 2;
+  a.split = split_of(tiles, a.blocks);
   const int grid = a.split > 1 ? static_cast<int>(tiles) * a.split : static_cast<int>(tiles < sms ? tiles : sms);
   return launch(few_kernel<NT, ODT>, grid, Few<NT>::kThreads, Few<NT>::kSmem, a.split, st, wm, xm, a);
 }
 
 template <int ODT>
 int run_typed(const LinearArgs& x, cudaStream_t st) {
+  if (one_launch(x)) return run_token<ODT>(x, st);
   if (x.T <= 16) return run_few<16, ODT>(x, st);
   if (x.T <= 32) return run_few<32, ODT>(x, st);
   if (x.T <= 64) return run_few<64, ODT>(x, st);
@@ -696,7 +943,7 @@ int run_typed(const LinearArgs& x, cudaStream_t st) {
   if (tiles > 0x7fffffffLL) return fail(MV_ERR_INVALID, "mv_fp8_linear: T=%d x N=%d is too large", x.T, x.N);
   const int pairs = num_sms() / 2;
   if (tiles < pairs / 2) return run_few<128, ODT>(x, st);
-  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, false, false, x.header};
+  FewArgs a{x.ws, x.scale, x.residual, x.out, x.ws_st, x.s_st, x.r_st, x.o_st, x.T, x.N, x.blocks, 0, 0, 1, x.x_dtype == MV_BF16, false, false, x.header};
   a.n_tiles = (x.N + kManyN - 1) / kManyN;
   a.t_tiles = (x.T + kManyT - 1) / kManyT;
   const int size = ODT == MV_F32 ? 4 : 2;
@@ -715,6 +962,15 @@ int run_typed(const LinearArgs& x, cudaStream_t st) {
 }
 
 }  // namespace
+
+// Up to four tokens over rows that do not fill the card by themselves: one launch less is 3 us as called (2560 x 2048, one token:
+// 10.7 -> 7.6; in a graph 5.6 / 5.5). 16 tokens take longer to round in each CTA than once before (7.4 us against 6.6), and over a
+// vocabulary the activations' place in shared memory is missed by the ring (131072 x 2048: 52.4 us against 50.1).
+bool one_launch(const LinearArgs& x) {
+  const int split = split_of((x.N + kTile - 1) / kTile, x.blocks);
+  if (x.T > 4 || split == 1) return false;
+  return (x.blocks + split - 1) / split <= kTokenBlocks;  // shared memory for the rounded activations
+}
 
 int run_product(const LinearArgs& x, int out_dtype, cudaStream_t st) {
   if (out_dtype == MV_F32) return run_typed<MV_F32>(x, st);
