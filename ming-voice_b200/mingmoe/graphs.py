@@ -1,4 +1,4 @@
-"""CUDA-graph replay of a block stack: the decode step and padded-bucket prefill.
+"""CUDA-graph replay of a block stack: the decode step and padded-bucket prefill; and of a whole token step.
 
 ming-voice captures its whole decode step once per attention bucket and replays it (engine.py:694-714, replay at
 :980), and captures prefill once per padded prompt length (PREFILL_BUCKETS 32 / 64 / 128, engine.py:716-757),
@@ -9,6 +9,10 @@ prompts run eagerly in chunks (:964-970). The same two patterns for a stack of M
   PrefillGraphs(blocks)      one graph per bucket; the padded rows are dropped from the expert GEMMs through a
                              device-side valid-row count (mv_mask_pad_rows), so one graph serves every length up
                              to its bucket.
+
+  TokenGraph(decoder, seqs)  one token of every running sequence: pages planned, embedding, layers, head, tokens drawn
+                             (the reference's _decode_step with its argmax, engine.py:681-685, :974-985, which goes
+                             back to the host for each token).
 
 Graphs are captured on a side stream after two eager warm-up runs (which create the workspaces: none is created
 or resized inside a capture) and replayed on the caller's current stream. Results live in static buffers that
@@ -109,3 +113,46 @@ class PrefillGraphs:
         self.n_valid.fill_(T)
         self.graphs[tb].replay()
         return self.y[:T]
+
+
+class TokenGraph:
+    """One new token of each running sequence of `seqs` (paging.DeviceSequences) in one graph, from its pages to the token drawn:
+    nothing of a step needs the host.
+
+    tokens [S] int64 are the sequences' last tokens, replaced by those drawn; new [S] int32 is 1 for a running sequence and 0 for
+    an idle one, whose token stays; u [S] and the settings temperature, top_k, top_p, min_p [S] are those of sampling.sample.
+    All are buffers that the caller fills (u anew for each step); logits [S, V], logprob [S] and ok [1] (0: no room, nothing was
+    changed but the tokens, which then mean nothing) are results of the last step."""
+
+    def __init__(self, decoder, seqs):
+        from . import sampling
+        n, dev = seqs.lens.shape[0], seqs.device
+        self.decoder, self.seqs = decoder, seqs
+        self.tokens = torch.zeros(n, dtype=torch.int64, device=dev)
+        self.new = torch.zeros(n, dtype=torch.int32, device=dev)
+        self.u, self.temperature, self.top_p = (torch.zeros(n, device=dev), torch.ones(n, device=dev), torch.ones(n, device=dev))
+        self.min_p, self.top_k = torch.zeros(n, device=dev), torch.zeros(n, dtype=torch.int32, device=dev)
+        packed = torch.zeros(n + 1, dtype=torch.int64, device=dev)
+
+        def step():
+            batch = self.seqs.extend(self.new, n, max_q=1)
+            running = self.new == 1
+            # running sequences' tokens to their rows, those of idle ones behind the last
+            packed.scatter_(0, torch.where(running, batch.cu_seqlens[:-1], n).long(), self.tokens)
+            self.logits = self.decoder(packed[:n], batch)
+            drawn, self.logprob = sampling.sample(self.logits, self.u, temperature=self.temperature, top_k=self.top_k,
+                                                  top_p=self.top_p, min_p=self.min_p, return_logprob=True)
+            self.tokens.copy_(torch.where(running, drawn, self.tokens))
+            self.ok = batch.ok
+
+        self.step = step  # (the same, eagerly)
+        s = torch.cuda.Stream(device=dev)
+        s.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(s):
+            # the warm-up runs with no sequence running, which leaves the pages as they are
+            self.graph = _capture(step, s, torch.cuda.graph_pool_handle())
+        torch.cuda.current_stream(dev).wait_stream(s)
+
+    def __call__(self):
+        self.graph.replay()
+        return self.tokens
