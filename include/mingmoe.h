@@ -388,7 +388,7 @@ MV_API size_t mv_attention_workspace_bytes(void);
  *      ceil(K / 128)] f32 (row stride ws_st): W[n, k] = wq[n, k] * ws[n / 128, k / 128].
  *  y[t, n] = sum over blocks b of (2^e[t, b] * ws[n / 128, b]) * sum over k in b of q[t, k] wq[n, k]  (+ residual[t, n]),
  *  all in f32, rounded once to out_dtype (bf16, f16 or f32). residual [T, N] has out_dtype or is NULL, row stride r_st; it may
- *  be `out` itself. Results do not depend on the run: fixed summation order.
+ *  be `out` itself; no other overlap with `out` is taken, and none of x. Results do not depend on the run: fixed summation order.
  * scratch: mv_fp8_linear_scratch_bytes(T, N, K) bytes, 256-byte aligned, of any content, not in use by another call that
  * may run at the same time. workspace: a zeroed header of 256 bytes (error word), which calls may share. */
 typedef struct mv_fp8_linear_args {

@@ -119,6 +119,16 @@ int quantize(const void* x, int dtype, long long x_st, int T, int K, uint8_t* q,
   return launch_quantize<MV_F32>(x, x_st, T, K, q, q_st, scale, s_st, st);
 }
 
+// whether two [rows, cols] tensors (row strides and widths in bytes) have a byte in common; columns of one buffer side by side
+// have none
+bool overlap(const void* p, long long p_st, long long p_w, const void* q, long long q_st, long long q_w, int rows) {
+  const long long a = static_cast<long long>(reinterpret_cast<uintptr_t>(p)), b = static_cast<long long>(reinterpret_cast<uintptr_t>(q));
+  if (a + (rows - 1) * p_st + p_w <= b || b + (rows - 1) * q_st + q_w <= a) return false;
+  if (rows < 2 || p_st != q_st || p_st <= 0) return true;
+  const long long d = ((b - a) % p_st + p_st) % p_st;
+  return d < p_w || d + q_w > p_st;
+}
+
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
@@ -187,6 +197,12 @@ extern "C" int mv_fp8_linear(const mv_fp8_linear_args* x, void* workspace, size_
     return fail(MV_ERR_INVALID, "%s: a row stride is too short for T=%d, N=%d, K=%d", who, T, N, K);
   if (!aligned16(x->wq) || (N > 1 && x->w_st % 16 != 0))
     return fail(MV_ERR_ALIGN, "%s: wq must be 16-byte aligned with rows of whole 16 bytes", who);
+  const int size = elem_size(x->out_dtype);
+  if (overlap(x->out, x->o_st * size, static_cast<long long>(N) * size, x->x, x->x_st * 2, K * 2LL, T))
+    return fail(MV_ERR_INVALID, "%s: out overlaps x", who);
+  if (x->residual != nullptr && !(x->residual == x->out && (T == 1 || x->r_st == x->o_st)) &&
+      overlap(x->out, x->o_st * size, static_cast<long long>(N) * size, x->residual, x->r_st * size, static_cast<long long>(N) * size, T))
+    return fail(MV_ERR_INVALID, "%s: residual overlaps out without being it", who);
   if (workspace == nullptr || workspace_bytes < kWsHeaderBytes)
     return fail(MV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", who, kWsHeaderBytes);
   const size_t scratch_bytes = mv_fp8_linear_scratch_bytes(T, N, K);

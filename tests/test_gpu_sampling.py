@@ -59,6 +59,14 @@ def test_vocabularies(cuda, v):
             check(x, u, **s)
 
 
+@pytest.mark.parametrize("v,dtype", [(300007, F32), (600011, BF), (800021, F32), (1300021, BF), (2100001, F32)])
+def test_rows_that_shared_memory_does_not_hold(cuda, v, dtype):
+    x, u = logits_of(cuda, 3, v, 40, dtype), uniform(cuda, 3, 41)
+    for s in (dict(), dict(top_k=60, top_p=0.9), dict(top_k=9000), dict(top_p=0.9), dict(top_k=200000, top_p=0.7), dict(min_p=0.01),
+              dict(temperature=0.0)):
+        check(x, u, **s)
+
+
 @pytest.mark.parametrize("b", [1, 2, 5, 18, 19, 37, 60, 148, 149, 300])
 def test_batches(cuda, b):
     x, u = logits_of(cuda, b, 3001, 5, BF), uniform(cuda, b, 6)

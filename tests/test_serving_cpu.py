@@ -13,7 +13,7 @@ P16 = 4096  # an address that is never read
 
 
 def linear(**kw):
-    a = L.Fp8LinearArgs(P16, P16, P16, 0, P16, P16, 256, 256, 2, 0, 300, 1 << 20, 40, 300, 256, L.MV_BF16, L.MV_F32, 0)
+    a = L.Fp8LinearArgs(P16, P16, P16, 0, 1 << 24, P16, 256, 256, 2, 0, 300, 1 << 20, 40, 300, 256, L.MV_BF16, L.MV_F32, 0)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -25,6 +25,8 @@ def linear(**kw):
     (dict(out_dtype=L.MV_I8), L.MV_ERR_UNSUPPORTED), (dict(x=0), L.MV_ERR_INVALID), (dict(wq=0), L.MV_ERR_INVALID),
     (dict(ws=0), L.MV_ERR_INVALID), (dict(out=0), L.MV_ERR_INVALID), (dict(x_st=-1), L.MV_ERR_INVALID),
     (dict(o_st=299), L.MV_ERR_INVALID), (dict(w_st=240), L.MV_ERR_INVALID), (dict(ws_st=1), L.MV_ERR_INVALID),
+    (dict(out=P16), L.MV_ERR_INVALID), (dict(out=P16 + 256 * 2 * 39), L.MV_ERR_INVALID),  # x and out overlap
+    (dict(residual=(1 << 24) + 4, r_st=300), L.MV_ERR_INVALID), (dict(residual=1 << 24, r_st=299), L.MV_ERR_INVALID),
     (dict(wq=P16 + 8), L.MV_ERR_ALIGN), (dict(w_st=264), L.MV_ERR_ALIGN), (dict(scratch=0), L.MV_ERR_WORKSPACE),
     (dict(scratch=P16 + 16), L.MV_ERR_WORKSPACE), (dict(scratch_bytes=100), L.MV_ERR_WORKSPACE)])
 def test_linear_refusals(kw, code):
@@ -40,6 +42,14 @@ def test_linear_workspace_and_nothing_to_do():
         assert lib.mv_fp8_linear(C.byref(linear(x=0, out=0, **kw)), None, 0, None) == L.MV_OK
     assert lib.mv_fp8_linear_scratch_bytes(0, 10, 10) == 0
     assert lib.mv_fp8_linear_scratch_bytes(100, 10, 200) >= 100 * 256 + 2 * 100
+
+
+def test_columns_of_one_buffer_do_not_overlap():
+    """x in the first 512 bytes of rows of 2048, the result behind it: taken (and refused for its workspace only)."""
+    kw = dict(x=P16, x_st=1024, out=P16 + 512, o_st=512, out_dtype=L.MV_F32)
+    assert L.lib().mv_fp8_linear(C.byref(linear(**kw)), None, 0, None) == L.MV_ERR_WORKSPACE
+    kw["out"] = P16 + 508
+    assert L.lib().mv_fp8_linear(C.byref(linear(**kw)), None, 0, None) == L.MV_ERR_INVALID
 
 
 def test_quantize_refusals():
