@@ -147,7 +147,7 @@ struct Few {
   static constexpr int kStages = NT <= 32 ? 9 : NT == 64 ? 8 : 6;
   static constexpr uint32_t kXBytes = NT * kBlock;
   static constexpr uint32_t kStageBytes = kTileBytes + kXBytes;
-  static constexpr int kHalves = NT == 128 ? 2 : 1;  // epilogue warps per 32 rows
+  static constexpr int kHalves = NT >= 64 ? 2 : 1;  // epilogue warps per 32 rows
   static constexpr int kCols = NT / kHalves;         // columns of an epilogue thread
   static constexpr int kThreads = 64 + 128 * kHalves;
   static constexpr int kBufs = NT == 128 ? 4 : 8;    // blocks' products in TMEM

@@ -62,20 +62,15 @@ __device__ __forceinline__ uint64_t place_of(uint32_t key, int i) {
   return static_cast<uint64_t>(~key) << 32 | static_cast<uint32_t>(i);
 }
 
-// Weights of one row as whole numbers.
+// Weights of one row as whole numbers. Logits are compared as fp32 numbers (an integer operation costs twice as much).
 struct Weights {
-  double m, c, lim;     // largest logit, log2(e) / temperature, least t that is told apart
-  uint32_t top, least;  // keys: of the largest logit, and of the least that can have a weight
-  int shift;
-  const double* table;  // 2^(j / 32)
-  // 0 for the largest logit itself (which may be infinite), lim for those without a weight
-  __device__ __forceinline__ double t_of(float l, uint32_t key) const {
-    const double d = key == top ? 0.0 : static_cast<double>(l) - m;
-    return key < least ? lim : d * c;
-  }
-  // 2^t in units of 2^-shift, rounded: 0 at lim
-  __device__ __forceinline__ uint64_t at(double t) const {
+  double m, c;          // largest logit, log2(e) / temperature
+  float top, least;     // the largest logit, and the least that can have a weight
+  const double* table;  // 2^(j / 32 + shift)
+  // 2^t in units of 2^-shift, rounded, for a logit from `least` on; of others what comes out
+  __device__ __forceinline__ uint64_t of(float l) const {
     constexpr double kRound = 211106232532992.0;  // 1.5 * 2^47: the low word of a sum with it counts 32nds, rounded
+    const double t = l == top ? 0.0 : (static_cast<double>(l) - m) * c;  // (the largest logit may be infinite)
     const double r = t + kRound;
     const double g = t - (r - kRound);
     const int n = __double2loint(r);
@@ -86,15 +81,14 @@ struct Weights {
     p = fma(p, g, 0.6931471805599453);
     p = fma(p, g, 1.0);
     const double b = table[n & 31];
-    const double s = __hiloint2double(__double2hiint(b) + (((n >> 5) + shift) << 20), __double2loint(b));
+    const double s = __hiloint2double(__double2hiint(b) + (n & ~31) * 32768, __double2loint(b));  // 20 - 5 bits up
     return static_cast<uint64_t>(__double_as_longlong(fma(p, s, 4503599627370496.0))) & 0xfffffffffffffull;  // 2^52
   }
-  __device__ __forceinline__ uint64_t of(float l, uint32_t key) const { return at(t_of(l, key)); }
-  // the key that a logit needs for 2^t (rounded down: no key at or above it is missed)
-  __device__ __forceinline__ uint32_t key_at(double t) const {
-    if (top == 0xff800000u) return top;  // beside an infinite logit only its equals have a weight
+  // the logit whose weight is 2^t (rounded down: no logit that heavy is missed)
+  __device__ __forceinline__ float logit_at(double t) const {
+    if (isinf(top)) return top;  // beside an infinite logit only its equals have a weight
     const double l = m + t / c * 1.0000001;
-    return key_of(l > -3.4e38 ? __double2float_rd(l) : -3.4028235e38f);
+    return l > -3.4e38 ? __double2float_rd(l) : -3.4028235e38f;
   }
 };
 
@@ -177,7 +171,7 @@ struct Listed {
       if (i >= rows || at >= count) continue;
       place[i] = s.list[at];
       const uint32_t key = ~static_cast<uint32_t>(place[i] >> 32);
-      if (weights) w[i] = wt.of(of_key(key), key);
+      if (weights) w[i] = wt.of(of_key(key));
     }
   }
   // sums over all tokens up to place `last`
@@ -306,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 
   // ---- 1. the row, the first of its order
   if (tid == 0) s.nan = 0u, s.n_list = 0u, s.best = ~0ull;
-  if (warp == 1) s.table[lane] = exp2(lane / 32.0);
+  if (warp == 1) s.table[lane] = exp2(lane / 32.0 + a.shift);
   __syncthreads();
   uint32_t top = 0u;
   int top_at = 0;
@@ -389,14 +383,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     return;
   }
   Weights wt;
-  wt.top = top, wt.shift = a.shift, wt.table = s.table;
-  wt.m = of_key(top), wt.c = 1.4426950408889634 / static_cast<double>(temp);
-  wt.lim = -static_cast<double>(a.shift + 2);
-  wt.least = wt.key_at(wt.lim);
+  wt.top = of_key(top), wt.table = s.table;
+  wt.m = wt.top, wt.c = 1.4426950408889634 / static_cast<double>(temp);
+  const double lim = -static_cast<double>(a.shift + 2);
+  wt.least = wt.logit_at(lim);
   const double one = static_cast<double>(1ull << a.shift);
   const uint64_t least_w = min_p > 0.f ? static_cast<uint64_t>(fmax(ceil(static_cast<double>(min_p) * one), 1.0)) : 1;
   // logits below this are not kept whatever the other filters do
-  const uint32_t least_key = min_p > 0.f ? max(wt.least, wt.key_at(fmax(log2(static_cast<double>(min_p)) - 1e-9, wt.lim))) : wt.least;
+  const float least_logit = min_p > 0.f ? fmaxf(wt.least, wt.logit_at(fmax(log2(static_cast<double>(min_p)) - 1e-9, lim))) : wt.least;
   auto draw = [&](uint64_t total) {  // the sum up to the token drawn is the first above this
     const uint64_t t = static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(total));
     return t < total ? t : total - 1;
@@ -408,14 +402,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 
   // ---- 2. few candidates
   if (share <= kMostMaxima || (!by_k && !by_p && min_p > 0.f)) {
-    const uint32_t from = max(by_k ? pivot : 0u, by_p ? wt.least : least_key);
+    const float from = fmaxf(by_k ? of_key(pivot) : -INFINITY, by_p ? wt.least : least_logit);
     each([&](const float (&l)[4], int i) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t key = key_of(l[k]);
-        if (key < from) continue;
+        if (!(l[k] >= from)) continue;
         const unsigned int at = atomicAdd(&s0.n_list, 1u);
-        if (at < kList) s0.list[at] = place_of(key, start + i + k);
+        if (at < kList) s0.list[at] = place_of(key_of(l[k]), start + i + k);
       }
     });
     cluster_sync();
@@ -431,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         if (tid < count) {
           place = places[tid];
           const uint32_t key = ~static_cast<uint32_t>(place >> 32);
-          weights[tid] = w = wt.of(of_key(key), key);
+          weights[tid] = w = wt.of(of_key(key));
         }
         __syncthreads();
         if (warp * 32 < count) {
@@ -464,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       }
       Listed list;
       list.load(count, wt, true, s);
-      const uint64_t first = best, last = place_of(from, -1);  // the list's places lie between these
+      const uint64_t first = best, last = place_of(key_of(from), -1);  // the list's places lie between these
       uint64_t border = ~0ull - 1, sum;
       unsigned int n;
       if (by_k && count > static_cast<unsigned int>(top_k)) border = list.border(true, top_k, 0, count, first, last, s);
@@ -495,11 +488,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   // ---- 3. the borders
   uint64_t border = ~0ull;
   const bool bins = a.slice <= (1 << 17);  // 15 bits of as many weights fit in 32
-  const double per = -static_cast<double>(kBins) / (a.shift + 4.0);
-  auto bin_of = [&](double t) { return static_cast<unsigned int>(__double2loint(fma(t, per, 6755399441055744.0))); };
+  // the bin of a logit with a weight: how far it lies below the largest, in fp32, whose roundings keep the order
+  const float per = static_cast<float>(static_cast<double>(kBins) / (a.shift + 4.0) * wt.c);
+  auto bin_of = [&](float l) -> unsigned int {
+    return l == wt.top ? 0u : __float_as_uint((wt.top - l) * per + 8388608.0f) & (kBins * 2 - 1);  // 2^23
+  };
   // first top-k's border, then top-p's among what top-k keeps
   for (int phase = by_k ? 0 : 1; phase < (by_p ? 2 : 1); ++phase) {
-    const uint32_t from = max(wt.least, ~static_cast<uint32_t>(border >> 32));
+    // what the last phase kept: logits above `from`, and equal ones up to an index
+    const uint32_t from_key = max(key_of(wt.least), ~static_cast<uint32_t>(border >> 32));
+    const float from = of_key(from_key);
+    const unsigned int from_last = from_key == ~static_cast<uint32_t>(border >> 32) ? static_cast<uint32_t>(border) : 0xffffffffu;
+    auto is_in = [&](float l, int i) { return l > from || (l == from && static_cast<unsigned int>(start + i) <= from_last); };
     uint64_t need_w = ~0ull, w;  // top-p keeps a token while the weights before it are less
     const unsigned int need_n = static_cast<unsigned int>(top_k);
     unsigned int bin = 0xffffffffu, n;
@@ -509,28 +509,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       for (int i = tid; i < 4 * kBins; i += kThreads) s.bins[0][i] = 0u;
       __syncthreads();
       each([&](const float (&l)[4], int i) {
-        double t[4];
-        bool in[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t key = key_of(l[k]);
-          in[k] = key >= from && (border == ~0ull || place_of(key, start + i + k) <= border);
-          t[k] = wt.t_of(l[k], key);
-        }
         if (phase == 0) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (in[k]) atomicAdd(&s.bins[0][bin_of(t[k])], 1u);
+            if (is_in(l[k], i + k)) atomicAdd(&s.bins[0][bin_of(l[k])], 1u);
         } else {
           uint64_t x[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = wt.at(t[k]);
+          for (int k = 0; k < 4; ++k) x[k] = wt.of(l[k]);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            if (!in[k]) continue;
-            const unsigned int b = bin_of(t[k]);
+            if (!is_in(l[k], i + k)) continue;
+            const unsigned int b = bin_of(l[k]);
             atomicAdd(&s.bins[1][b], static_cast<unsigned int>(x[k]) & 0x7fffu);
-            atomicAdd(&s.bins[2][b], static_cast<unsigned int>(x[k] >> 15) & 0x7fffu);
+            atomicAdd(&s.bins[2][b], static_cast<unsigned int>(x[k]) >> 15 & 0x7fffu);
             atomicAdd(&s.bins[3][b], static_cast<unsigned int>(x[k] >> 30));
           }
         }
@@ -594,19 +586,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         const unsigned int most = warp == 0 ? b : b - 1;  // the least key with at most this bin, which the largest logit's is
         uint32_t key = top;
         if (b > 0u || warp == 0) {
-          // where t has half a bin left it is near; else 32 keys at a time are tried
-          const double l0 = wt.m + (most + 0.5) / per / wt.c;
+          // where the rounding to the bin turns it is near; else 32 keys at a time are tried
+          const double l0 = wt.m - (most + 0.5) / static_cast<double>(per);
           const uint32_t guess = key_of(l0 > -3.4e38 ? static_cast<float>(l0) : -3.4e38f);
-          uint32_t lo = from, hi = top;
-          uint32_t tried = min(max(static_cast<int64_t>(guess) - 16 + lane, static_cast<int64_t>(from)), static_cast<int64_t>(top));
-          unsigned int in = __ballot_sync(0xffffffffu, bin_of(wt.t_of(of_key(tried), tried)) <= most);
+          uint32_t lo = from_key, hi = top;
+          uint32_t tried = min(max(static_cast<int64_t>(guess) - 16 + lane, static_cast<int64_t>(from_key)), static_cast<int64_t>(top));
+          unsigned int in = __ballot_sync(0xffffffffu, bin_of(of_key(tried)) <= most);
           if (in != 0u && !(in & 1u)) {
             lo = hi = __shfl_sync(0xffffffffu, tried, __ffs(in) - 1);
           }
           while (lo < hi) {
             const uint32_t part = (hi - lo) / 32 + 1;
             tried = min(static_cast<uint64_t>(lo) + static_cast<uint64_t>(part) * lane, static_cast<uint64_t>(hi));
-            in = __ballot_sync(0xffffffffu, bin_of(wt.t_of(of_key(tried), tried)) <= most);
+            in = __ballot_sync(0xffffffffu, bin_of(of_key(tried)) <= most);
             if (in == 0u) {
               lo = __shfl_sync(0xffffffffu, tried, 31) + 1;
             } else {
@@ -625,14 +617,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       bin_from = s0.bin_from, bin_to = s0.bin_to;
       const uint64_t w_before = s0.bin_before;
       const unsigned int n_before = s0.bin_count_before;
+      const float bin_least = of_key(bin_from), bin_most = of_key(bin_to);
       each([&](const float (&l)[4], int i) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t key = key_of(l[k]);
-          const uint64_t place = place_of(key, start + i + k);
-          if (key < bin_from || key > bin_to || place > border) continue;
+          if (!(l[k] >= bin_least && l[k] <= bin_most && is_in(l[k], i + k))) continue;
           const unsigned int at = atomicAdd(&s0.n_list, 1u);
-          if (at < kList) s0.list[at] = place;
+          if (at < kList) s0.list[at] = place_of(key_of(l[k]), start + i + k);
         }
       });
       cluster_sync();
@@ -654,11 +645,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       each([&](const float (&l)[4], int i) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t key = key_of(l[k]);
-          const uint64_t place = place_of(key, start + i + k);
-          if (key < from || place > border || place >= end) continue;
+          if (!is_in(l[k], i + k) || place_of(key_of(l[k]), start + i + k) >= end) continue;
           ++n;
-          if (phase == 1) w += wt.of(l[k], key);
+          if (phase == 1) w += wt.of(l[k]);
         }
       });
       block_sum(w, n, s);
@@ -683,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       for (int k = 0; k < 4; ++k) {
         const uint32_t key = key_of(l[k]);
         const uint64_t place = place_of(key, start + i + k);
-        if (key < from || key < bin_from || key > bin_to || place > border) continue;
+        if (!is_in(l[k], i + k) || key < bin_from || key > bin_to) continue;
         first = min(first, place), last = max(last, place);
       }
     });
@@ -719,29 +708,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   }
 
   // ---- 4. the draw
-  const uint32_t last_key = max(~static_cast<uint32_t>(border >> 32), least_key);
+  const uint32_t last_key = max(~static_cast<uint32_t>(border >> 32), key_of(least_logit));
+  const float last_logit = of_key(last_key);
+  const unsigned int last_index = last_key == ~static_cast<uint32_t>(border >> 32) ? static_cast<uint32_t>(border) : 0xffffffffu;
   auto load = [&](int i) { return value(a.in_smem ? held[i] : src[i]); };
   // weights of four elements from i on, `step` apart, that lie before `end`; 0 for those not kept
   auto kept = [&](int i, int step, int end, uint64_t (&w)[4]) {
     float l[4];
-    uint32_t key[4];
     bool any = false;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      l[k] = 0.f, key[k] = 0u, w[k] = 0;
-      if (i + k * step < end) l[k] = load(i + k * step), key[k] = key_of(l[k]);
-      any |= key[k] >= last_key;
+      l[k] = -INFINITY, w[k] = 0;
+      if (i + k * step < end) l[k] = load(i + k * step);
+      any |= l[k] >= last_logit;
     }
     if (!any) return;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint64_t x = wt.of(l[k], key[k]);
-      w[k] = key[k] >= last_key ? x : 0;
+      const uint64_t x = wt.of(l[k]);
+      if (l[k] > last_logit || (l[k] == last_logit && static_cast<unsigned int>(start + i + k * step) <= last_index)) w[k] = x;
     }
-    if (border != ~0ull || least_w > 1) {
+    if (least_w > 1) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (place_of(key[k], start + i + k * step) > border || w[k] < least_w) w[k] = 0;
+        if (w[k] < least_w) w[k] = 0;
     }
   };
   // warp w owns a contiguous range of the part

@@ -8,6 +8,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -66,6 +67,8 @@ bool rows_of(const at::Tensor& t, int64_t* rows, int64_t* stride) {
 }
 
 PyObject* guarded(PyObject* (*f)(PyObject* const*), PyObject* const* args) {
+  // results are new tensors, or views of those, without a history: no dispatch through the layers that keep one
+  at::AutoDispatchBelowADInplaceOrView guard;
   try {
     return f(args);
   } catch (const std::exception&) {  // an allocation that failed: the Python code meets it again and raises torch's error
