@@ -45,10 +45,16 @@ struct SampleArgs {
   bool vectors;  // rows start at 16-byte addresses
 };
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 2048, kList = 4096;
+// A CTA's threads and what goes by them: 512 for few rows, else 256, four of which share an SM (launch_rows).
+template <int kThreads>
+struct Cta {
+  static constexpr int kWarps = kThreads / 32;
+  static constexpr int kBins = 4 * kThreads, kList = 8 * kThreads;
+  static constexpr int kFine = kThreads == 256 ? 8 : 9;   // log2 of the finer bins, one for each thread
+  static constexpr int kMostMaxima = kThreads * 3 / 4;    // of the threads, in finding the key of step 1
+  static_assert(1 << kFine == kThreads, "a finer bin for each thread");
+};
 constexpr unsigned int kFew = 128;  // tokens that are put in order by comparing all with all (n * n / 128 steps of some 12 instructions)
-constexpr int kMostMaxima = kThreads * 3 / 4;  // of a CTA's threads, in finding the key of step 1
 constexpr uint32_t kNone = 0x007fffffu;  // the key of -inf
 
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -100,19 +106,23 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
   return a + (static_cast<uint64_t>(b) << 27) + (static_cast<uint64_t>(c) << 54);
 }
 
-struct Shared {
+template <int kThreads>
+struct Shared : Cta<kThreads> {
+  using C = Cta<kThreads>;
   union {
-    unsigned int bins[4][kBins];  // counts, or the weights' bits 0-14, 15-29 and 30-45
-    unsigned long long list[kList];
+    unsigned int bins[4][C::kBins];  // counts, or the weights' bits 0-14, 15-29 and 30-45
+    unsigned long long list[C::kList];
   };
-  unsigned long long part[kWarps], total, border, kept, least_place, most_place, best, bin_before;
+  unsigned long long part[C::kWarps], total, border, kept, least_place, most_place, best, bin_before;
   double table[32];
-  unsigned int fine[4][kThreads], counts[kWarps], n_list, pivot, nan, bin, bin_count_before, part_n, bin_from, bin_to;
+  unsigned int fine[4][kThreads], counts[C::kWarps], n_list, pivot, nan, bin, bin_count_before, part_n, bin_from, bin_to;
   int bin_here;  // the bin, where this CTA has found it
 };
 
 // Sums of (w, n) over the CTA in every thread. Two barriers.
-__device__ __forceinline__ void block_sum(uint64_t& w, unsigned int& n, Shared& s) {
+template <int kThreads>
+__device__ __forceinline__ void block_sum(uint64_t& w, unsigned int& n, Shared<kThreads>& s) {
+  constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   w = warp_sum(w);
   n = __reduce_add_sync(0xffffffffu, n);
@@ -126,7 +136,10 @@ __device__ __forceinline__ void block_sum(uint64_t& w, unsigned int& n, Shared& 
 }
 
 // Sums of (w, n) over the threads before this one, in thread order, and over all. Two barriers.
-__device__ __forceinline__ void block_before(uint64_t& w, unsigned int& n, uint64_t& total_w, unsigned int& total_n, Shared& s) {
+template <int kThreads>
+__device__ __forceinline__ void block_before(uint64_t& w, unsigned int& n, uint64_t& total_w, unsigned int& total_n,
+                                             Shared<kThreads>& s) {
+  constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t w0 = w;
   const unsigned int n0 = n;
@@ -156,8 +169,10 @@ __device__ __forceinline__ void block_before(uint64_t& w, unsigned int& n, uint6
 }
 
 // Tokens of a list in the registers of one CTA's threads.
+template <int kThreads>
 struct Listed {
-  static constexpr int kEach = kList / kThreads;
+  using Shared = Shared<kThreads>;
+  static constexpr int kEach = Cta<kThreads>::kList / kThreads, kFine = Cta<kThreads>::kFine;
   uint64_t place[kEach], w[kEach];  // ~0 and 0 where there is no token
   int rows;                         // of them that are in use
 
@@ -195,7 +210,7 @@ struct Listed {
     while (count > kFew) {
       s.fine[0][tid] = 0u, s.fine[1][tid] = 0u, s.fine[2][tid] = 0u, s.fine[3][tid] = 0u;
       __syncthreads();
-      const int shift = max(0, 64 - __clzll(to - from) - 9);  // (512 bins)
+      const int shift = max(0, 64 - __clzll(to - from) - kFine);
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         if (i >= rows || place[i] < from || place[i] > to) continue;
@@ -245,8 +260,10 @@ struct Listed {
   }
 };
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
+template <int DT, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const SampleArgs a) {
+  using Shared = Shared<kThreads>;
+  constexpr int kWarps = Shared::kWarps, kBins = Shared::kBins, kList = Shared::kList, kMostMaxima = Shared::kMostMaxima;
   extern __shared__ __align__(16) uint8_t raw[];
   Shared& s = *reinterpret_cast<Shared*>(raw);
   using T = typename std::conditional<DT == MV_F32, float, uint16_t>::type;
@@ -455,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         cluster_wait();
         return;
       }
-      Listed list;
+      Listed<kThreads> list;
       list.load(count, wt, true, s);
       const uint64_t first = best, last = place_of(key_of(from), -1);  // the list's places lie between these
       uint64_t border = ~0ull - 1, sum;
@@ -469,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       }
       // kept tokens in the order of their indices: the draw's is the first up to which the sum is above the target
 #pragma unroll
-      for (int i = 0; i < Listed::kEach; ++i) {
+      for (int i = 0; i < Listed<kThreads>::kEach; ++i) {
         if (list.place[i] > border || list.w[i] < least_w) list.place[i] = ~0ull, list.w[i] = 0;
         if (list.place[i] != ~0ull) list.place[i] &= 0xffffffffull;
       }
@@ -477,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       list.up_to(~0ull - 1, total, n, s);
       const uint64_t at = list.border(false, 0, draw(total) + 1, n, 0, a.V - 1, s);
 #pragma unroll
-      for (int i = 0; i < Listed::kEach; ++i)
+      for (int i = 0; i < Listed<kThreads>::kEach; ++i)
         if (list.place[i] == at) answer(static_cast<int>(at), list.w[i], total);
       cluster_wait();
       return;
@@ -630,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       const unsigned int count = s0.n_list;
       if (count <= kList) {
         if (rank == 0) {
-          Listed list;
+          Listed<kThreads> list;
           list.load(count, wt, phase == 1, s);
           list.border(phase == 0, need_n - n_before, need_w - w_before, count, place_of(bin_to, 0), place_of(bin_from, -1), s);
         }
@@ -781,22 +798,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   }
 }
 
-template <int DT>
-int launch(SampleArgs a, int B, cudaStream_t st) {
+constexpr size_t kSm = 227 * 1024;  // shared memory of an SM, of which a CTA takes 1 KB for itself
+
+template <int kThreads>
+constexpr size_t fixed_smem() {
+  return (sizeof(Shared<kThreads>) + 15) / 16 * 16;
+}
+
+template <int DT, int kThreads>
+int launch(SampleArgs a, int B, int C, cudaStream_t st) {
   const int size = DT == MV_F32 ? 4 : 2;
-  constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
-  constexpr size_t kMost = 227 * 1024;  // shared memory of an SM (of which a CTA takes 1 KB for itself)
-  // Two CTAs share an SM where they can, one of which reads while the other computes: at least as many a row as that leaves room
-  // for its part. More where there are few rows: up to 5/7 of the SMs, which is what clusters find together, one CTA each (16 rows of
-  // 131072, top-p, us: 6 CTAs a row 36, 7 63, 8 42), or 7/4 of them, two CTAs each (64 rows of 32000: 4 CTAs a row 31, 5 47).
-  const auto fits = [&](int c, size_t room) { return (static_cast<size_t>(a.V) / c + 8) * size <= room - kFixed; };
-  const long long most = 4LL * B <= num_sms() * 5 / 7 ? num_sms() * 5 / 7 : num_sms() * 7 / 4;
-  int C = 1;
-  while (C < 8 && (!fits(C, kMost / 2 - 1024) || static_cast<long long>(B) * (C + 1) <= most)) ++C;
   a.slice = ((a.V + C - 1) / C + 7) / 8 * 8;
-  a.in_smem = static_cast<size_t>(a.slice) * size <= kMost - kFixed;
-  const size_t smem = kFixed + (a.in_smem ? static_cast<size_t>(a.slice) * size : 0);
-  auto fn = sample_kernel<DT>;
+  a.in_smem = static_cast<size_t>(a.slice) * size <= kSm - fixed_smem<kThreads>();
+  const size_t smem = fixed_smem<kThreads>() + (a.in_smem ? static_cast<size_t>(a.slice) * size : 0);
+  auto fn = sample_kernel<DT, kThreads>;
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(mv_sample)");
   cudaLaunchConfig_t cfg = {};
@@ -812,6 +827,23 @@ int launch(SampleArgs a, int B, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = C > 1 ? 2 : 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, fn, a), "mv_sample launch");
+}
+
+// CTAs of a row. Few rows: CTAs of 512 threads, as many a row as fill 5/7 of the SMs, which is what clusters find together (16 rows of
+// 131072, top-p, us: 6 CTAs a row 36, 7 63, 8 42; one row: 28, and 34 with 256 threads). More rows: four CTAs of 256 share an SM, some of
+// which read or wait while others compute (48 rows of 100277, top-p, us: 45; two CTAs of 512 65): at least as many a row as that
+// leaves room for its part, and more up to 7/8 of the places.
+template <int DT>
+int launch_rows(const SampleArgs& a, int B, cudaStream_t st) {
+  const int size = DT == MV_F32 ? 4 : 2, sms = num_sms();
+  if (4LL * B <= sms * 5 / 7) {
+    const int C = sms * 5 / 7 / B;
+    return launch<DT, 512>(a, B, C < 8 ? C : 8, st);
+  }
+  const auto fits = [&](int c) { return (static_cast<size_t>(a.V) / c + 8) * size <= kSm / 4 - 1024 - fixed_smem<256>(); };
+  int C = 1;
+  while (C < 8 && (!fits(C) || static_cast<long long>(B) * (C + 1) <= sms * 7 / 2)) ++C;
+  return launch<DT, 256>(a, B, C, st);
 }
 
 }  // namespace
@@ -843,6 +875,6 @@ extern "C" int mv_sample(const mv_sample_args* x, void* stream) {
   if (a.shift > 45) a.shift = 45;
   a.vectors = aligned16(x->logits) && a.st * size % 16 == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (x->dtype == MV_F32) return launch<MV_F32>(a, x->B, st);
-  return x->dtype == MV_BF16 ? launch<MV_BF16>(a, x->B, st) : launch<MV_F16>(a, x->B, st);
+  if (x->dtype == MV_F32) return launch_rows<MV_F32>(a, x->B, st);
+  return x->dtype == MV_BF16 ? launch_rows<MV_BF16>(a, x->B, st) : launch_rows<MV_F16>(a, x->B, st);
 }
