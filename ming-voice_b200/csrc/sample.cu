@@ -832,7 +832,8 @@ int launch(SampleArgs a, int B, int C, cudaStream_t st) {
 // CTAs of a row. Few rows: CTAs of 512 threads, as many a row as fill 5/7 of the SMs, which is what clusters find together (16 rows of
 // 131072, top-p, us: 6 CTAs a row 36, 7 63, 8 42; one row: 28, and 34 with 256 threads). More rows: four CTAs of 256 share an SM, some of
 // which read or wait while others compute (48 rows of 100277, top-p, us: 45; two CTAs of 512 65): at least as many a row as that
-// leaves room for its part, and more up to 7/8 of the places.
+// leaves room for its part, and more up to 7/8 of the places. Parts of eight CTAs that are too long for that: two of 512 again (192 rows of
+// 131072 in f32, min_p: 61 us; with 256 threads 65).
 template <int DT>
 int launch_rows(const SampleArgs& a, int B, cudaStream_t st) {
   const int size = DT == MV_F32 ? 4 : 2, sms = num_sms();
@@ -840,9 +841,14 @@ int launch_rows(const SampleArgs& a, int B, cudaStream_t st) {
     const int C = sms * 5 / 7 / B;
     return launch<DT, 512>(a, B, C < 8 ? C : 8, st);
   }
-  const auto fits = [&](int c) { return (static_cast<size_t>(a.V) / c + 8) * size <= kSm / 4 - 1024 - fixed_smem<256>(); };
+  // whether n CTAs' parts, c of them a row, find room on an SM
+  const auto fits = [&](int c, int n, size_t fixed) { return (static_cast<size_t>(a.V) / c + 8) * size <= kSm / n - 1024 - fixed; };
   int C = 1;
-  while (C < 8 && (!fits(C) || static_cast<long long>(B) * (C + 1) <= sms * 7 / 2)) ++C;
+  if (!fits(8, 4, fixed_smem<256>())) {
+    while (C < 8 && !fits(C, 2, fixed_smem<512>())) ++C;
+    return launch<DT, 512>(a, B, C, st);
+  }
+  while (C < 8 && (!fits(C, 4, fixed_smem<256>()) || static_cast<long long>(B) * (C + 1) <= sms * 7 / 2)) ++C;
   return launch<DT, 256>(a, B, C, st);
 }
 
