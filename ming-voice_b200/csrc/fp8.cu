@@ -1,5 +1,9 @@
-// Products with 8-bit floating-point weights and a scale for each block of 128 (mv_fp8_linear), and the rounding of activations
-// and weights to that form (mv_quantize_fp8, mv_quantize_fp8_weight).
+// Products with 8-bit floating-point weights and a scale for each block of 128 (mv_fp8_linear; the products are in fp8_gemm.cu), and
+// the rounding of activations and weights to that form (mv_quantize_fp8, mv_quantize_fp8_weight).
+//
+// An activation block's scale is a power of two: x / scale is exact, so the rounded values do not depend on how the quotient is
+// taken, and an e4m3 number has as many significant bits at any power of two (down to 2^-6 of 448). Bound: memory; 16001 x 2048 in 19.6
+// us, 5.0 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -7,8 +7,12 @@
 //   few tokens  weights are the 128-row operand and up to 128 tokens the columns, so a tile is a weight stream of 16 KB
 //               blocks; a cluster shares a tile's blocks of K where there are fewer tiles than SMs and adds the parts over
 //               distributed shared memory in rank order.
-//   many tokens 128 tokens are the rows and 256 weight rows the columns: an epilogue thread owns one token, so a block's
-//               factor is one number per thread.
+//   many tokens 256 tokens are the rows and 256 weight rows the columns of a pair of CTAs: an epilogue thread owns one token, so
+//               a block's factor is one number per thread.
+// Bound and measured (B200; graph replays): few tokens by the weights' bytes, 131072 x 2048 for one token 50 us (5.4 TB/s, 83 % of the
+// measured copy; the rest is the start of 4 us and the last wave of tiles), for 64 tokens 65 us; many tokens by the tensor pipe
+// and the hand-over of each block between it and the epilogue, 16001 x 5632 x 2048 197 us with the activations' rounding (1.87
+// PFLOP/s), 4096 x 5632 x 8192 180 us (2.1); products added up in TMEM instead, which one scale a row would allow, take 148.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -521,8 +525,10 @@ __global__ void __launch_bounds__(192, 1) token_kernel(const __grid_constant__ C
 // ------------------------------------------------------------------------------------------------ many tokens
 //
 // Two CTAs of a cluster work on one tile of 256 tokens x 256 weight rows (cta_group::2): each brings 128 rows of either
-// operand, 32 KB a block instead of 48, and holds the products of its 128 tokens. One CTA with a 128 x 256 tile was bound by
-// that traffic (16001 x 5632 x 2048 without reading its products: 200 us).
+// operand, 32 KB a block instead of 48, and holds the products of its 128 tokens (16001 x 5632 x 2048: 222 us with one CTA's tiles of 128 x
+// 256, 195 with pairs). The products of a block's 256 columns are handed over together: halves of 128, four buffers instead
+// of two, took 253 us, since a hand-over costs more than the reads behind it. The pair's epilogue frees a buffer by a plain arrive
+// on the first CTA's barrier: with .release.cluster, which waits for all earlier memory operations, it took 394 us.
 
 constexpr int kManyStages = 5, kManyN = 256, kManyT = 256;
 constexpr uint32_t kManyStageBytes = 2 * kTileBytes;  // 32 KB

@@ -4,7 +4,9 @@
 // its place on the free stack; all else is a copy. Bound: latency (a step of a few hundred sequences moves some kilobytes).
 // One CTA checks the step, sums and writes the counters; what grows with the tokens and the page table's width is written by a
 // second kernel over the whole card, which takes page ids from the state as it was before the step, so that nothing in it
-// depends on the order of its threads.
+// depends on the order of its threads. Measured on a B200: one token of each of 61 sequences 9.6 us as called (4.8 in a graph, one
+// launch), 16001 tokens of 9 prompts 12.8 (7.8), 2000 tokens of 1000 sequences with their rows of 516 pages gathered 12.9 (12.3); the
+// host side of a call is 8 to 9 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
 

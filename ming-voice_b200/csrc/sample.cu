@@ -16,7 +16,13 @@
 //      64-bit additions in shared memory cost seven times three of 32 bits), added up in the first CTA, which finds the bin with the border; that bin's tokens
 //      are brought together there. A bin with more than the list holds (runs of equal logits) is searched over all CTAs.
 //   4. each CTA adds up what is kept of its part; the CTA in which the sum passes u times the total finds the token.
-// A border among listed tokens is found bit by bit over their places.
+// A border among listed tokens is found over their places, by finer and finer bins and by comparing the last few with one another.
+//
+// Bound: many rows by the weights (a 64-bit exponential is some 60 cycles of a quarter SM for 32 logits; every logit has one where top-p
+// or nothing is asked for) and by the steps of a row that wait for one another; one row by those steps alone (a cluster barrier and the
+// reads behind it are 1 us, and there are 4 to 12). Measured on a B200, call after call: one row of 131072 f32 with all filters 10.9 us,
+// 192 rows of 131072 bf16 with min_p 43 (a copy of them 7.8), 48 rows of 100277 f32 with top-p over a flat distribution 50, 128 rows of
+// 50257 bf16 with settings of their own 46.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -830,10 +836,10 @@ int launch(SampleArgs a, int B, int C, cudaStream_t st) {
 }
 
 // CTAs of a row. Few rows: CTAs of 512 threads, as many a row as fill 5/7 of the SMs, which is what clusters find together (16 rows of
-// 131072, top-p, us: 6 CTAs a row 36, 7 63, 8 42; one row: 28, and 34 with 256 threads). More rows: four CTAs of 256 share an SM, some of
-// which read or wait while others compute (48 rows of 100277, top-p, us: 45; two CTAs of 512 65): at least as many a row as that
-// leaves room for its part, and more up to 7/8 of the places. Parts of eight CTAs that are too long for that: two of 512 again (192 rows of
-// 131072 in f32, min_p: 61 us; with 256 threads 65).
+// 131072, top-p, us: 6 CTAs a row 36, 7 63, 8 42; one row: 28, and 34 with 256 threads). More rows: up to four CTAs of 256 share an SM,
+// some of which read or wait while others compute (48 rows of 100277, three on an SM, top-p, us: 45; two of 512 65): at least as many a
+// row as leaves room for four, or eight, and more up to 7/8 of the places. Where three of eight CTAs' parts find no room on an SM, two of
+// 512 threads (192 rows of 131072 in f32, min_p: 61 us; two of 256 65).
 template <int DT>
 int launch_rows(const SampleArgs& a, int B, cudaStream_t st) {
   const int size = DT == MV_F32 ? 4 : 2, sms = num_sms();
@@ -844,7 +850,7 @@ int launch_rows(const SampleArgs& a, int B, cudaStream_t st) {
   // whether n CTAs' parts, c of them a row, find room on an SM
   const auto fits = [&](int c, int n, size_t fixed) { return (static_cast<size_t>(a.V) / c + 8) * size <= kSm / n - 1024 - fixed; };
   int C = 1;
-  if (!fits(8, 4, fixed_smem<256>())) {
+  if (!fits(8, 3, fixed_smem<256>())) {
     while (C < 8 && !fits(C, 2, fixed_smem<512>())) ++C;
     return launch<DT, 512>(a, B, C, st);
   }
