@@ -3,7 +3,7 @@
 // Mathematics. Tokens are ordered by (logit descending, index ascending), as one 64-bit number `place`: the logit's bits, mapped
 // so that unsigned comparison orders them, in the upper half and the index in the lower. Each filter keeps a prefix of that order,
 // so all that is kept is given by one place, the border, and a least weight. Weights 2^t, t = (logit - max) log2(e) / temperature,
-// are whole numbers of 2^-shift (shift 45 for vocabularies up to 2^17; 2^f from a table of 32 values and a polynomial of degree 5
+// are whole numbers of 2^-shift (shift 45 for vocabularies of 2^17, more for smaller ones up to 51; 2^f from a table of 32 values and a polynomial of degree 5
 // that interpolates 2^g at the Chebyshev nodes of [-1/64, 1/64], off by 2^-52 of it), so that sums do not depend on their order: each border and each draw comes out
 // the same whatever the split; a weight below 2^-shift / 2, which no 24-bit random number can draw, is 0.
 //
@@ -82,9 +82,10 @@ struct Weights {
   // 2^t in units of 2^-shift, rounded, for a logit from `least` on; of others what comes out
   __device__ __forceinline__ uint64_t of(float l) const {
     constexpr double kRound = 211106232532992.0;  // 1.5 * 2^47: the low word of a sum with it counts 32nds, rounded
-    const double t = l == top ? 0.0 : (static_cast<double>(l) - m) * c;  // (the largest logit may be infinite)
-    const double r = t + kRound;
-    const double g = t - (r - kRound);
+    // (the largest logit may be infinite; roundings are spelled out, so that each use of this gives the same weight)
+    const double t = l == top ? 0.0 : __dmul_rn(__dsub_rn(static_cast<double>(l), m), c);
+    const double r = __dadd_rn(t, kRound);
+    const double g = __dsub_rn(t, __dsub_rn(r, kRound));
     const int n = __double2loint(r);
     double p = 0.0013333604694153824;
     p = fma(p, g, 0.009618176115571158);
@@ -116,7 +117,7 @@ template <int kThreads>
 struct Shared : Cta<kThreads> {
   using C = Cta<kThreads>;
   union {
-    unsigned int bins[4][C::kBins];  // counts, or the weights' bits 0-14, 15-29 and 30-45
+    unsigned int bins[4][C::kBins];  // counts, or the weights' bits 0-14, 15-29 and 30-51
     unsigned long long list[C::kList];
   };
   unsigned long long part[C::kWarps], total, border, kept, least_place, most_place, best, bin_before;
@@ -215,6 +216,7 @@ struct Listed {
     // a bin for each thread over the range of the places that are left, until few of them are
     while (count > kFew) {
       s.fine[0][tid] = 0u, s.fine[1][tid] = 0u, s.fine[2][tid] = 0u, s.fine[3][tid] = 0u;
+      if (tid == 0) s.n_list = 0u;
       __syncthreads();
       const int shift = max(0, 64 - __clzll(to - from) - kFine);
 #pragma unroll
@@ -242,9 +244,10 @@ struct Listed {
       __syncthreads();
       from = s.least_place, to = s.most_place, w_before = s.bin_before, n_before = s.bin_count_before, count = s.n_list;
       __syncthreads();
+      if (count == 0u) return to;  // (no place has what is asked for: it does not happen, and must not hold the loop)
     }
     // by comparing with all that are left
-    if (tid == 0) s.n_list = 0u;
+    if (tid == 0) s.n_list = 0u, s.border = to;
     __syncthreads();
     unsigned long long *places = s.list, *weights = places + kFew;
 #pragma unroll
@@ -514,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   // the bin of a logit with a weight: how far it lies below the largest, in fp32, whose roundings keep the order
   const float per = static_cast<float>(static_cast<double>(kBins) / (a.shift + 4.0) * wt.c);
   auto bin_of = [&](float l) -> unsigned int {
-    return l == wt.top ? 0u : __float_as_uint((wt.top - l) * per + 8388608.0f) & (kBins * 2 - 1);  // 2^23
+    return l == wt.top ? 0u : __float_as_uint(fmaf(wt.top - l, per, 8388608.0f)) & (kBins * 2 - 1);  // 2^23
   };
   // first top-k's border, then top-p's among what top-k keeps
   for (int phase = by_k ? 0 : 1; phase < (by_p ? 2 : 1); ++phase) {
@@ -816,6 +819,8 @@ int launch(SampleArgs a, int B, int C, cudaStream_t st) {
   const int size = DT == MV_F32 ? 4 : 2;
   a.slice = ((a.V + C - 1) / C + 7) / 8 * 8;
   a.in_smem = static_cast<size_t>(a.slice) * size <= kSm - fixed_smem<kThreads>();
+  // a CTA's sums of the weights' upper bits stay within 32: its part times 2^(shift - 30)
+  if (C == 1 && a.shift + attn::log2_of(a.V > 1 ? a.V : 2) > 61) --a.shift;
   const size_t smem = fixed_smem<kThreads>() + (a.in_smem ? static_cast<size_t>(a.slice) * size : 0);
   auto fn = sample_kernel<DT, kThreads>;
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
@@ -882,9 +887,9 @@ extern "C" int mv_sample(const mv_sample_args* x, void* stream) {
   a.top_k = x->top_k, a.tokens = x->tokens, a.logprob = x->logprob, a.st = x->B > 1 ? x->st : 0;
   a.temperature_value = x->temperature_value, a.top_p_value = x->top_p_value, a.min_p_value = x->min_p_value;
   a.top_k_value = x->top_k_value, a.V = x->V;
-  // sums of V weights stay below 2^62, weights below 2^52
+  // sums of V weights stay within 2^62, and weights below 2^52
   a.shift = 62 - attn::log2_of(x->V > 1 ? x->V : 2);
-  if (a.shift > 45) a.shift = 45;
+  if (a.shift > 51) a.shift = 51;
   a.vectors = aligned16(x->logits) && a.st * size % 16 == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (x->dtype == MV_F32) return launch_rows<MV_F32>(a, x->B, st);
