@@ -828,13 +828,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             *slot = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        if (a.out_lines) {
+        // a tensor store writes whole 16 bytes: a line that ends inside them would reach into what lies behind it
+        if (a.out_lines && cols >= kPart) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) store_lines(&omap, line, n, t0);
         } else {
           __syncwarp();
-          move_lines<kSize, true>(line, static_cast<uint8_t*>(a.out) + (t0 * a.o_st + n) * kSize, a.o_st, rows, cols, false, lane);
+          move_lines<kSize, true>(line, static_cast<uint8_t*>(a.out) + (t0 * a.o_st + n) * kSize, a.o_st, rows, cols, a.out_lines, lane);
+          if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");  // (an empty one, for stores_read's count)
         }
       }
     }

@@ -182,6 +182,36 @@ def test_strides(cuda):
             assert torch.equal(out[:, 3:259], y) and bool((out[:, :3] == 0).all()) and bool((out[:, 259:] == 0).all())
 
 
+@pytest.mark.parametrize("ot", [BF, FP, F32])
+@pytest.mark.parametrize("t,n", [(3, 131), (40, 1001), (130, 2095), (700, 2095), (700, 5803), (600, 2944), (2100, 1191)])
+def test_columns_beside_the_result_stay(cuda, ot, t, n):
+    """Results with a ragged end inside rows of whole 16 bytes, at addresses of whole 16 bytes."""
+    x, r = randn(cuda, (t, 200), 60, BF), randn(cuda, (t, n), 61, ot)
+    wq, ws = weight(cuda, n, 200, 62)
+    buf = torch.full((t + 2, (n + 31) // 16 * 16), 7.0, dtype=ot, device=cuda)
+    for at in (0, 8, 16):
+        for res in (None, r):
+            buf.fill_(7)
+            out = buf[1:t + 1, at:at + n]
+            if out.shape[1] < n:
+                continue
+            F.fp8_linear(x, wq, ws, residual=res, out=out, out_dtype=ot)
+            check(out, x, wq, ws, res)
+            out.fill_(7)
+            assert bool((buf == 7).all())
+
+
+@pytest.mark.parametrize("k", [1, 7, 100, 130, 1001])
+def test_bytes_behind_a_row_of_weights_do_not_count(cuda, k):
+    """Weights whose rows lie in wider ones, with NaNs right behind them."""
+    wide = torch.full((5000, (k + 47) // 16 * 16), 0x7f, dtype=torch.uint8, device=cuda).view(F.E4M3)
+    good, ws = weight(cuda, 5000, k, 63)
+    wide[:, :k] = good
+    for t in (2, 9, 100, 600):
+        x = randn(cuda, (t, k), 64, BF)
+        check(F.fp8_linear(x, wide[:, :k], ws, out_dtype=F32), x, good, ws)
+
+
 def test_in_place_residual(cuda):
     for t in (2, 200):
         x, r = randn(cuda, (t, 384), 23, BF), randn(cuda, (t, 500), 24, BF)
