@@ -421,7 +421,7 @@ MV_API int mv_quantize_fp8_weight(const void* w, int w_dtype, long long w_st, in
  *
  * One token for each row of logits [B, V] bf16 / f16 / f32 (any row stride st >= 0), from given random numbers. (The reference takes the
  * argmax, engine.py:974-985.) Tokens are ordered by logit, the larger first, equal ones by index; with
- * w_i = exp((logit_i - max) / temperature):
+ * w_i = exp((logit_i - max) / temperature), 1 for those equal to an infinite max, 0 infinitely far below max whatever the temperature:
  *   top_k  keeps the first top_k of the order (<= 0, or >= V: all);
  *   top_p  of these, keeps a token while the weights before it in the order add up to less than top_p times the weights of all
  *          that top_k kept (>= 1: all);

@@ -97,11 +97,12 @@ struct Weights {
     const double s = __hiloint2double(__double2hiint(b) + (n & ~31) * 32768, __double2loint(b));  // 20 - 5 bits up
     return static_cast<uint64_t>(__double_as_longlong(fma(p, s, 4503599627370496.0))) & 0xfffffffffffffull;  // 2^52
   }
-  // the logit whose weight is 2^t (rounded down: no logit that heavy is missed)
+  // The least logit whose weight is 2^t or more. Rounded up, so that it is no lighter either, however far apart the numbers of its
+  // size lie: lighter ones have no bin, and their powers of two leave the exponent's range.
   __device__ __forceinline__ float logit_at(double t) const {
     if (isinf(top)) return top;  // beside an infinite logit only its equals have a weight
     const double l = m + t / c * 1.0000001;
-    return l > -3.4e38 ? __double2float_rd(l) : -3.4028235e38f;
+    return l > -3.4e38 ? __double2float_ru(l) : -3.4028235e38f;
   }
 };
 
@@ -514,10 +515,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   // ---- 3. the borders
   uint64_t border = ~0ull;
   const bool bins = a.slice <= (1 << 17);  // 15 bits of as many weights fit in 32
-  // the bin of a logit with a weight: how far it lies below the largest, in fp32, whose roundings keep the order
-  const float per = static_cast<float>(static_cast<double>(kBins) / (a.shift + 4.0) * wt.c);
+  // the bin of a logit with a weight: how far it lies below the largest, in fp32, whose roundings keep the order (both factors are
+  // held finite: distances of logits at the type's two ends, temperatures below 2^-122)
+  const float per = static_cast<float>(fmin(static_cast<double>(kBins) / (a.shift + 4.0) * wt.c, 3.4e38));
   auto bin_of = [&](float l) -> unsigned int {
-    return l == wt.top ? 0u : __float_as_uint(fmaf(wt.top - l, per, 8388608.0f)) & (kBins * 2 - 1);  // 2^23
+    return l == wt.top ? 0u : __float_as_uint(fmaf(fminf(wt.top - l, 3.4e38f), per, 8388608.0f)) & (kBins * 2 - 1);  // 2^23
   };
   // first top-k's border, then top-p's among what top-k keeps
   for (int phase = by_k ? 0 : 1; phase < (by_p ? 2 : 1); ++phase) {

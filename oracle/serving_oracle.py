@@ -75,7 +75,8 @@ def sample(logits, u, temperature, top_k, top_p, min_p):
     m = l[order[0]]
     if not temperature > 0:
         return int(order[0]), 0.0
-    z = torch.where(l == m, 0.0, (l - m) / temperature)
+    # infinitely far below the first of the order is no weight, at an infinite temperature too (inf / inf has no value)
+    z = torch.where(l == m, 0.0, torch.where((l - m).isinf(), -math.inf, (l - m) / temperature))
     w = torch.exp(z)[order]
     n = min(V, top_k) if top_k > 0 else V
     if top_p < 1:

@@ -149,6 +149,34 @@ def test_extreme_numbers(cuda):
         check(x * scale, v, **s)
 
 
+@pytest.mark.parametrize("temperature", [0.001, 1.0, 50.0, 200.0])
+def test_logits_that_lie_far_apart_for_the_temperature(cuda, temperature):
+    """Neighbouring numbers of the logits' size are further apart than weights reach: the least logit of weight has none below it."""
+    for step, size in ((64.0, 1e9), (0.0625, 1e6), (2.0 ** -19, 12.0)):
+        t = temperature * step / 64
+        g = torch.Generator(device=cuda).manual_seed(50)
+        for lowest in (2, 4000):
+            x = size - step * torch.randint(0, lowest, (5, 9001), generator=g, device=cuda).float()
+            x[3:] = size - step  # one at the top, all others next to it
+            x[3, 4444] = size
+            x[4, 17] = size
+            for s in (dict(), dict(top_p=0.9), dict(top_k=3000), dict(top_k=3000, top_p=0.6), dict(top_k=40, top_p=0.8), dict(min_p=0.02)):
+                check(x, uniform(cuda, 5, 51), temperature=t, **s)
+
+
+def test_numbers_at_the_ends_of_the_type(cuda):
+    """Distances that pass the largest number, temperatures below the least normal one and infinite ones."""
+    top = torch.finfo(F32).max
+    x = logits_of(cuda, 4, 9001, 52)
+    x[0, ::2], x[0, 1::2] = top, -top
+    x[1] *= 1e38
+    x[2] = x[2].clamp(-1, 1) * top
+    x[3, 5:] *= 1e-42
+    for t in (1e-45, 1e-40, 1e-38, 1.0, 1e38, top, INF):
+        for s in (dict(), dict(top_p=0.9), dict(top_k=3000), dict(top_k=3000, top_p=0.6), dict(top_k=40, top_p=0.8), dict(min_p=0.02)):
+            check(x, uniform(cuda, 4, 53), temperature=t, **s)
+
+
 def test_strides_and_out(cuda):
     big = logits_of(cuda, 9, 4100, 16, BF)
     u = uniform(cuda, 4, 17)
