@@ -837,6 +837,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           __syncwarp();
           move_lines<kSize, true>(line, static_cast<uint8_t*>(a.out) + (t0 * a.o_st + n) * kSize, a.o_st, rows, cols, a.out_lines, lane);
           if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");  // (an empty one, for stores_read's count)
+          // all lanes have read the line before the next residual's copy may come into it
+          fence_proxy_async_smem();
+          __syncwarp();
         }
       }
     }

@@ -201,6 +201,22 @@ def test_columns_beside_the_result_stay(cuda, ot, t, n):
             assert bool((buf == 7).all())
 
 
+@pytest.mark.parametrize("ot", [BF, FP, F32])
+def test_a_ragged_result_of_several_tiles_a_pair(cuda, ot):
+    """Lines that are written by elements lie where the next tile's residual goes: the same as from rows that have no such copies."""
+    t, n = 9001, 1201
+    x = randn(cuda, (t, 384), 65, BF)
+    wq, ws = weight(cuda, n, 384, 66)
+    wide = randn(cuda, (t, 1216), 67, ot)
+    want = F.fp8_linear(x, wq, ws, residual=wide[:, :n].contiguous(), out_dtype=ot)
+    check(want[:200], x[:200], wq, ws, wide[:200, :n])
+    out = torch.empty_like(wide)[:, :n]
+    for _ in range(5):
+        out.fill_(7)
+        F.fp8_linear(x, wq, ws, residual=wide[:, :n], out=out, out_dtype=ot)
+        assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("k", [1, 7, 100, 130, 1001])
 def test_bytes_behind_a_row_of_weights_do_not_count(cuda, k):
     """Weights whose rows lie in wider ones, with NaNs right behind them."""
