@@ -173,7 +173,9 @@ class Decoder:
 
     def __call__(self, tokens, batch):
         """tokens [T] (packed, any integer type) -> logits [B, V], fp32 from an 8-bit head and bf16 from a plain one. A sequence
-        without a token in the batch gets logits of another one's."""
+        without a token in the batch gets logits of another one's; a batch without any token is refused."""
+        if tokens.dim() != 1 or tokens.shape[0] == 0:
+            raise ValueError(f"tokens must be [T] with T > 0, got {list(tokens.shape)}")
         import fastlinear
         import fused_ops  # the drop-in modules (same directory on sys.path)
         with torch.cuda.device(self.embedding.device):

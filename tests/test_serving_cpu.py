@@ -132,3 +132,10 @@ def test_weights_that_do_not_fit():
         AttentionBlock((wq, None), torch.zeros(100, 512), torch.ones(100), 8, 2, 64, None)
     with pytest.raises(ValueError):
         Decoder(torch.zeros(10, 96), [], torch.ones(96), (wq, None))
+
+
+def test_a_decoder_needs_a_token():
+    decoder = Decoder(torch.zeros(10, 96), [], torch.ones(96), torch.zeros(10, 96))
+    for tokens in (torch.zeros(0, dtype=torch.int64), torch.zeros(1, 2, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="tokens"):
+            decoder(tokens, None)
