@@ -21,7 +21,7 @@
 // Bound: many rows by the weights (a 64-bit exponential is some 60 cycles of a quarter SM for 32 logits; every logit has one where top-p
 // or nothing is asked for) and by the steps of a row that wait for one another; one row by those steps alone (a cluster barrier and the
 // reads behind it are 1 us, and there are 4 to 12). Measured on a B200, call after call: one row of 131072 f32 with all filters 10.9 us,
-// 192 rows of 131072 bf16 with min_p 43 (a copy of them 7.8), 48 rows of 100277 f32 with top-p over a flat distribution 50, 128 rows of
+// 192 rows of 131072 bf16 with min_p 40 (a copy of them 7.8), 48 rows of 100277 f32 with top-p over a flat distribution 50, 128 rows of
 // 50257 bf16 with settings of their own 46.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
