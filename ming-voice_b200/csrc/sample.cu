@@ -3,7 +3,7 @@
 // Mathematics. Tokens are ordered by (logit descending, index ascending), as one 64-bit number `place`: the logit's bits, mapped
 // so that unsigned comparison orders them, in the upper half and the index in the lower. Each filter keeps a prefix of that order,
 // so all that is kept is given by one place, the border, and a least weight. Weights 2^t, t = (logit - max) log2(e) / temperature,
-// are whole numbers of 2^-shift (shift 45 for vocabularies of 2^17, more for smaller ones up to 51; 2^f from a table of 32 values and a polynomial of degree 5
+// are whole numbers of 2^-shift (shift 44 for vocabularies of 2^17, more for smaller ones up to 51; 2^f from a table of 32 values and a polynomial of degree 5
 // that interpolates 2^g at the Chebyshev nodes of [-1/64, 1/64], off by 2^-52 of it), so that sums do not depend on their order: each border and each draw comes out
 // the same whatever the split; a weight below 2^-shift / 2, which no 24-bit random number can draw, is 0.
 //
@@ -245,11 +245,12 @@ struct Listed {
       __syncthreads();
       from = s.least_place, to = s.most_place, w_before = s.bin_before, n_before = s.bin_count_before, count = s.n_list;
       __syncthreads();
-      if (count == 0u) return to;  // (no place has what is asked for: it does not happen, and must not hold the loop)
+      if (count == 0u) break;  // (no place has what is asked for: it does not happen, and must not hold the loop)
     }
     // by comparing with all that are left
     if (tid == 0) s.n_list = 0u, s.border = to;
     __syncthreads();
+    if (count == 0u) return to;
     unsigned long long *places = s.list, *weights = places + kFew;
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
@@ -821,8 +822,6 @@ int launch(SampleArgs a, int B, int C, cudaStream_t st) {
   const int size = DT == MV_F32 ? 4 : 2;
   a.slice = ((a.V + C - 1) / C + 7) / 8 * 8;
   a.in_smem = static_cast<size_t>(a.slice) * size <= kSm - fixed_smem<kThreads>();
-  // a CTA's sums of the weights' upper bits stay within 32: its part times 2^(shift - 30)
-  if (C == 1 && a.shift + attn::log2_of(a.V > 1 ? a.V : 2) > 61) --a.shift;
   const size_t smem = fixed_smem<kThreads>() + (a.in_smem ? static_cast<size_t>(a.slice) * size : 0);
   auto fn = sample_kernel<DT, kThreads>;
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
@@ -889,8 +888,9 @@ extern "C" int mv_sample(const mv_sample_args* x, void* stream) {
   a.top_k = x->top_k, a.tokens = x->tokens, a.logprob = x->logprob, a.st = x->B > 1 ? x->st : 0;
   a.temperature_value = x->temperature_value, a.top_p_value = x->top_p_value, a.min_p_value = x->min_p_value;
   a.top_k_value = x->top_k_value, a.V = x->V;
-  // sums of V weights stay within 2^62, and weights below 2^52
-  a.shift = 62 - attn::log2_of(x->V > 1 ? x->V : 2);
+  // Weights stay below 2^52, and sums of V of them within 2^61: those of their bits from 30 on (2^31) fit in 32, for a list that holds
+  // the whole row too. It goes by V alone, so that a row's weights do not depend on the batch or the split.
+  a.shift = 61 - attn::log2_of(x->V > 1 ? x->V : 2);
   if (a.shift > 51) a.shift = 51;
   a.vectors = aligned16(x->logits) && a.st * size % 16 == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -1,0 +1,52 @@
+"""GPU parity of drawing tokens where rows fill the lists and histograms, in each of the launch's shapes: batches of up to 26 rows (CTAs of
+512 threads), of more (256 threads, one to eight CTAs a row), and of rows too long for three of those on an SM."""
+import math
+
+import pytest
+import torch
+
+from mingmoe import sampling as S
+from oracle import serving_oracle as O
+
+pytestmark = pytest.mark.gpu
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def expected(row, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    f32 = lambda v: torch.tensor(v, dtype=F32).item()
+    return O.sample(row, u, f32(temperature), top_k, f32(top_p), f32(min_p))
+
+
+def unit(v):
+    """The number whose multiples weights of v tokens are."""
+    return 2.0 ** -min(51, 61 - max(1, math.ceil(math.log2(v))))
+
+
+@pytest.mark.parametrize("b", [1, 26, 27, 60, 300])
+@pytest.mark.parametrize("v", [2047, 2048, 2049, 4095, 4096, 4097])
+def test_equal_logits_that_fill_a_list(cuda, b, v):
+    """All logits equal: the whole row is one bin of the histogram and of each finer one, up to the list's last place."""
+    x = torch.zeros(b, v, device=cuda)
+    u = (torch.arange(b, device=cuda) * 0.6180339887) % 1.0
+    for s in (dict(top_p=0.9), dict(top_p=0.25), dict(top_k=50, top_p=0.9), dict(top_k=v - 1, top_p=0.75), dict(top_k=v // 2),
+              dict(min_p=0.5), dict(top_p=0.5, min_p=0.5)):
+        want = [expected(x[0].cpu(), n, **s) for n in u.tolist()]
+        tokens, logprob = S.sample(x, u, return_logprob=True, **s)
+        assert tokens.tolist() == [t for t, _ in want], s
+        assert all(abs(got - p) <= 2.0 ** -24 * abs(p) + 1e-9 for got, (_, p) in zip(logprob.tolist(), want)), s
+
+
+@pytest.mark.parametrize("v", [1500, 2048, 17000, 70001])
+def test_the_unit_of_weights_goes_by_the_vocabulary_alone(cuda, v):
+    """u = 0 draws the first token with a weight: one of 0.6 units has one and one of 0.4 has none, whatever the batch."""
+    f = [0.4, 0.45, 0.55, 0.6, 0.9]
+    x = torch.full((len(f), v), -1.0, device=cuda)
+    x[:, 0] = torch.tensor([math.log(n * unit(v)) for n in f])
+    x[:, 1] = 0.0
+    u = torch.zeros(len(f), device=cuda)
+    results = []
+    for copies in (1, 6, 12, 60):
+        tokens, logprob = S.sample(x.repeat(copies, 1), u.repeat(copies), return_logprob=True)
+        assert tokens.tolist() == [int(n < 0.5) for n in f] * copies
+        results.append(logprob.view(copies, len(f)))
+    assert all(torch.equal(r, results[0].expand_as(r)) for r in results)
