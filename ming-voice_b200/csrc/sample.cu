@@ -123,7 +123,7 @@ struct Shared : Cta<kThreads> {
   };
   unsigned long long part[C::kWarps], total, border, kept, least_place, most_place, best, bin_before;
   double table[32];
-  unsigned int fine[4][kThreads], counts[C::kWarps], n_list, pivot, nan, bin, bin_count_before, part_n, bin_from, bin_to;
+  unsigned int fine[4][kThreads], counts[C::kWarps], n_list, n_left, pivot, nan, bin, bin_count_before, part_n, bin_from, bin_to;
   int bin_here;  // the bin, where this CTA has found it
 };
 
@@ -211,13 +211,14 @@ struct Listed {
   __device__ __forceinline__ uint64_t border(bool by_count, unsigned int need_n, uint64_t need_w, unsigned int count, uint64_t from,
                                              uint64_t to, Shared& s) const {
     const int tid = threadIdx.x;
+    // (n_left, not n_list: other CTAs may still be reading how long the list was)
     uint64_t w_before = 0;  // of what lies before what is still looked at
     unsigned int n_before = 0;
     __syncthreads();
     // a bin for each thread over the range of the places that are left, until few of them are
     while (count > kFew) {
       s.fine[0][tid] = 0u, s.fine[1][tid] = 0u, s.fine[2][tid] = 0u, s.fine[3][tid] = 0u;
-      if (tid == 0) s.n_list = 0u;
+      if (tid == 0) s.n_left = 0u;
       __syncthreads();
       const int shift = max(0, 64 - __clzll(to - from) - kFine);
 #pragma unroll
@@ -238,24 +239,24 @@ struct Listed {
       block_before(wb, n, all_w, all_n, s);
       n += n_before, wb += w_before;
       if (by_count ? n < need_n && n + n_bin >= need_n : wb < need_w && wb + w_bin >= need_w) {
-        s.bin_before = wb, s.bin_count_before = n, s.n_list = n_bin;
+        s.bin_before = wb, s.bin_count_before = n, s.n_left = n_bin;
         s.least_place = from + (static_cast<uint64_t>(tid) << shift);
         s.most_place = s.least_place + ((1ull << shift) - 1);
       }
       __syncthreads();
-      from = s.least_place, to = s.most_place, w_before = s.bin_before, n_before = s.bin_count_before, count = s.n_list;
+      from = s.least_place, to = s.most_place, w_before = s.bin_before, n_before = s.bin_count_before, count = s.n_left;
       __syncthreads();
       if (count == 0u) break;  // (no place has what is asked for: it does not happen, and must not hold the loop)
     }
     // by comparing with all that are left
-    if (tid == 0) s.n_list = 0u, s.border = to;
+    if (tid == 0) s.n_left = 0u, s.border = to;
     __syncthreads();
     if (count == 0u) return to;
     unsigned long long *places = s.list, *weights = places + kFew;
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
       if (i < rows && place[i] >= from && place[i] <= to) {
-        const unsigned int at = atomicAdd(&s.n_list, 1u);
+        const unsigned int at = atomicAdd(&s.n_left, 1u);
         places[at] = place[i], weights[at] = w[i];
       }
     __syncthreads();

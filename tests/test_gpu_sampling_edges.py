@@ -17,6 +17,22 @@ def expected(row, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     return O.sample(row, u, f32(temperature), top_k, f32(top_p), f32(min_p))
 
 
+def check_copies(x, u, b, **s):
+    """The rows of x over and over, b in all, each against the plain draw."""
+    n = x.shape[0]
+    at = torch.arange(b, device=x.device) % n
+    tokens, logprob = S.sample(x[at], u[at], return_logprob=True, **s)
+    want = [expected(row, v, **s) for row, v in zip(x.cpu(), u.tolist())]
+    assert tokens.tolist() == [want[i % n][0] for i in range(b)], s
+    for r, got in enumerate(logprob.tolist()):
+        p = want[r % n][1]
+        assert got == p or abs(got - p) <= 2.0 ** -24 * abs(p) + 1e-9, (r, got, p, s)
+
+
+# rows and vocabularies of the three launch shapes
+SHAPES = [(3, 9001, F32), (40, 9001, F32), (300, 9001, F32), (40, 70001, BF), (30, 131072, F32)]
+
+
 def unit(v):
     """The number whose multiples weights of v tokens are."""
     return 2.0 ** -min(51, 61 - max(1, math.ceil(math.log2(v))))
@@ -50,3 +66,16 @@ def test_the_unit_of_weights_goes_by_the_vocabulary_alone(cuda, v):
         assert tokens.tolist() == [int(n < 0.5) for n in f] * copies
         results.append(logprob.view(copies, len(f)))
     assert all(torch.equal(r, results[0].expand_as(r)) for r in results)
+
+
+@pytest.mark.parametrize("b,v,dtype", SHAPES)
+@pytest.mark.parametrize("n", [1, 2, 127, 128, 129, 255, 256, 257, 511, 513, 2047, 2048, 2049, 4095, 4096, 4097, 9000])
+def test_lists_of_every_length(cuda, b, v, dtype, n):
+    """n candidates that min_p leaves, or that top-k and top-p choose from."""
+    g = torch.Generator(device=cuda).manual_seed(n)
+    x = torch.full((5, v), -30.0, device=cuda)
+    for r in range(5):
+        x[r, torch.randperm(v, generator=g, device=cuda)[:n]] = torch.randn(n, generator=g, device=cuda).clamp(-3, 3)
+    x, u = x.to(dtype), torch.rand(5, generator=g, device=cuda)
+    for s in (dict(min_p=0.0005), dict(top_k=n), dict(top_k=n, top_p=0.8), dict(top_k=max(1, n - 1), min_p=0.01), dict(top_p=0.7)):
+        check_copies(x, u, b, **s)
