@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
   constexpr int kEpiWarps = 4 * F::kHalves;
   if (threadIdx.x == 0) {
     for (int i = 0; i < F::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1 + kEpiWarps);
-    for (int i = 0; i < F::kBufs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpiWarps);
+    for (int i = 0; i < F::kBufs; ++i) mbar_init(&acc_full[i], 2), mbar_init(&acc_empty[i], kEpiWarps);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -233,6 +233,9 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
           for (int k = 0; k < kBlock / 32; ++k) mma_f8(tmem + buf * NT, ad + 2 * k, bd + 2 * k, idesc_e4m3(kTile, NT), k > 0);
           tc::mma_commit(&empty[s]);
           tc::mma_commit(&acc_full[buf]);
+          // The epilogue reads the stage's scales, and a commit hands on nothing but its products: this thread, which has waited for
+          // the copies, arrives too (a wait of each epilogue warp for the copies took 61 x 100277 x 1500 3 us).
+          mbar_arrive(&acc_full[buf]);
         }
         __syncwarp();
       }
@@ -653,14 +656,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* scales = smem + kManyStages * kManyStageBytes + 8 * 2 * kLineBytes;  // [slot][128]
-  __shared__ alignas(8) uint64_t full[kManyStages], empty[kManyStages], acc_full[2], acc_empty[2], res_full[8];
+  __shared__ alignas(8) uint64_t full[kManyStages], empty[kManyStages], acc_full[2], acc_empty[2], res_full[8], scale_full[kScaleSlots];
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kManyStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 16);
+    for (int i = 0; i < 2; ++i) mbar_init(&acc_full[i], 2), mbar_init(&acc_empty[i], 16);
     for (int i = 0; i < 8; ++i) mbar_init(&res_full[i], 1);
+    for (int i = 0; i < kScaleSlots; ++i) mbar_init(&scale_full[i], 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -698,9 +702,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             // the first CTA's barrier counts both CTAs' tiles
             uint8_t* st = smem + s * kManyStageBytes;
             const uint32_t bar = peer_addr(&full[s], 0);
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * (kManyStageBytes + 128));
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kManyStageBytes);
             pair_load(st, &xmap, bar, b * kBlock, t0);
-            pair_load(scales + it % kScaleSlots * 128, &smap, bar, t0, b);
+            mbar_arrive_expect_tx(&scale_full[it % kScaleSlots], 128);
+            tc::tma_load_2d(scales + it % kScaleSlots * 128, &smap, &scale_full[it % kScaleSlots], t0, b);
             pair_load(st + kTileBytes, &wmap, bar, b * kBlock, n0);
           }
         }
@@ -727,6 +732,24 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             pair_commit(&acc_full[buf]);
           }
           __syncwarp();
+        }
+      }
+    } else if (warp == 2) {
+      // The scales' hand-over: a commit, the other CTA's on top of it, hands on nothing but its products, so a block's products are there
+      // for the epilogue once its scales are too. (A wait of each epilogue warp for the scales took 16001 x 5632 x 2048 8 to 14 us.)
+      if (tc::elect_one()) {
+        int it = 0;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+          for (int b = 0; b < a.blocks; ++b, ++it) {
+            // (an arrival ahead of the block two back would end that one's phase)
+            if ((it >= 2 && !wait(&acc_full[it & 1], (it / 2 + 1) & 1, a.header, 0x815u)) ||
+                !wait(&scale_full[it % kScaleSlots], (it / kScaleSlots) & 1, a.header, 0x816u)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive(&acc_full[it & 1]);
+          }
         }
       }
     }
