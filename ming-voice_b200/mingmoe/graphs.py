@@ -121,8 +121,9 @@ class TokenGraph:
 
     tokens [S] int64 are the sequences' last tokens, replaced by those drawn; new [S] int32 is 1 for a running sequence and 0 for
     an idle one, whose token stays; u [S] and the settings temperature, top_k, top_p, min_p [S] are those of sampling.sample.
-    All are buffers that the caller fills (u anew for each step); logits [S, V], logprob [S] and ok [1] (0: no room, nothing was
-    changed but the tokens, which then mean nothing) are results of the last step."""
+    All are buffers that the caller fills (u anew for each step); logits [S, V], logprob [S] and ok [1] are results of the last step.
+    ok 0: no room, nothing was changed, the tokens neither, and logits and logprob mean nothing: release pages, or let sequences idle, and
+    replay."""
 
     def __init__(self, decoder, seqs):
         from . import sampling
@@ -142,7 +143,7 @@ class TokenGraph:
             self.logits = self.decoder(packed[:n], batch)
             drawn, self.logprob = sampling.sample(self.logits, self.u, temperature=self.temperature, top_k=self.top_k,
                                                   top_p=self.top_p, min_p=self.min_p, return_logprob=True)
-            self.tokens.copy_(torch.where(running, drawn, self.tokens))
+            self.tokens.copy_(torch.where(running & (batch.ok == 1), drawn, self.tokens))
             self.ok = batch.ok
 
         self.step = step  # (the same, eagerly)
