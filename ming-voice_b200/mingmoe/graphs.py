@@ -120,7 +120,8 @@ class TokenGraph:
     nothing of a step needs the host.
 
     tokens [S] int64 are the sequences' last tokens, replaced by those drawn; new [S] int32 is 1 for a running sequence and 0 for
-    an idle one, whose token stays; u [S] and the settings temperature, top_k, top_p, min_p [S] are those of sampling.sample.
+    an idle one, whose token stays; a sequence whose token is negative idles too (-1 was drawn: a row of logits without a token), until the
+    caller puts a token there; u [S] and the settings temperature, top_k, top_p, min_p [S] are those of sampling.sample.
     All are buffers that the caller fills (u anew for each step); logits [S, V], logprob [S] and ok [1] are results of the last step.
     ok 0: no room, nothing was changed, the tokens neither, and logits and logprob mean nothing: release pages, or let sequences idle, and
     replay."""
@@ -136,8 +137,8 @@ class TokenGraph:
         packed = torch.zeros(n + 1, dtype=torch.int64, device=dev)
 
         def step():
-            batch = self.seqs.extend(self.new, n, max_q=1)
-            running = self.new == 1
+            running = (self.new == 1) & (self.tokens >= 0)
+            batch = self.seqs.extend(running.int(), n, max_q=1)
             # running sequences' tokens to their rows, those of idle ones behind the last
             packed.scatter_(0, torch.where(running, batch.cu_seqlens[:-1], n).long(), self.tokens)
             self.logits = self.decoder(packed[:n], batch)

@@ -74,3 +74,31 @@ def test_a_step_without_room_keeps_the_tokens(cuda):
         assert tight.seqs.lens.tolist() == wide.seqs.lens.tolist() == host.lens
     assert refused == [1] and tight.tokens.tolist() != [11, 12, 13]
     assert not L.all_workspace_errors()
+
+
+def test_a_sequence_without_a_token_stops(cuda):
+    """A row whose logits hold no token gives -1, which is no token of the next step: the sequence idles until the caller puts one there."""
+    seqs = DeviceSequences(20, 8, 3, 64, device=cuda)
+    inner = make(cuda, seqs)
+    grammar = torch.full((V,), False, device=cuda)
+    grammar[7] = True  # nothing may follow token 7
+
+    def decoder(tokens, batch):
+        last = tokens[(batch.cu_seqlens[1:] - 1).clamp(min=0)]
+        return inner(tokens, batch).masked_fill(grammar[last][:, None], -float("inf"))
+
+    loop = TokenGraph(decoder, seqs)
+    inner(torch.arange(9, device=cuda), seqs.extend(ints([3, 2, 4], cuda), 9, max_q=4, prompts=True))
+    loop.tokens.copy_(torch.tensor([1, 7, 2]))
+    loop.new.fill_(1)
+    loop.temperature.zero_()
+    loop()
+    assert loop.tokens[1].item() == -1 and loop.logprob[1].item() == -float("inf") and seqs.lens.tolist() == [4, 3, 5]
+    others = loop.tokens[[0, 2]]
+    assert bool((others >= 0).all()) and not bool((others == 7).any())
+    loop()
+    assert loop.ok.item() == 1 and loop.tokens[1].item() == -1 and seqs.lens.tolist() == [5, 3, 6]
+    loop.tokens[1] = 9
+    loop()
+    assert loop.tokens[1].item() >= 0 and seqs.lens.tolist() == [6, 4, 7]
+    assert not L.all_workspace_errors()
