@@ -463,8 +463,10 @@ MV_API size_t mv_sample_scratch_bytes(int B, int V);
  * row of the cache as [num_pages * page_size, ...]) and positions [T] int32 (position of each token in its sequence), where
  * rows behind the last token get slot -1 and position 0; pages gets its new entries, lens_out and n_free_out the state after
  * the step (they may be lens and n_free, or buffers that leave those as they are), ok[0] = 1.
+ * prompts: not 0 where the step's tokens are to be whole prompts, which attend to one another alone.
  * A step that asks for a sequence outside the state or twice, a negative number of tokens, more than max_len tokens (or
- * max_pages pages) of a sequence, more than T tokens or more pages than are free changes nothing: ok[0] = 0, cu_seqlens is 0,
+ * max_pages pages) of a sequence, with `prompts` tokens of a sequence that has some already, more than T tokens or more pages than are
+ * free changes nothing: ok[0] = 0, cu_seqlens is 0,
  * kv_lens are the present lengths (0 outside the state), lens_out and n_free_out the present state.
  * B <= max_seqs <= 2^18, page_size a power of two in 8..256. scratch: int32 [B + 2].
  *
@@ -480,7 +482,7 @@ typedef struct mv_plan_args {
   long long* slots;
   int *positions, *ok, *scratch;
   long long pages_st, table_st;
-  int B, max_seqs, max_pages, page_size, max_len, num_pages, T, pad0;
+  int B, max_seqs, max_pages, page_size, max_len, num_pages, T, prompts;
 } mv_plan_args;
 
 MV_API int mv_plan_step(const mv_plan_args* a, void* stream);

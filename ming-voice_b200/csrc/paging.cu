@@ -26,6 +26,7 @@ struct PlanArgs {
   int *positions, *ok, *scratch;  // scratch: the batch's first pages on the stack [B + 1], then the stack's height before the step
   long long pages_st, table_st;
   int B, max_seqs, max_pages, page_shift, max_len, num_pages, T;
+  bool prompts;  // tokens only for sequences that have none
 };
 
 __device__ __forceinline__ int pages_of(int tokens, int shift) {
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const PlanArgs a, bool a
     }
     if (a.seqs != nullptr && (atomicOr(&seen[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u)) bad = true;
     const int old = a.lens[s];
-    if (old < 0 || n > limit - min(old, limit)) {
+    if (old < 0 || n > limit - min(old, limit) || (a.prompts && n > 0 && old > 0)) {
       bad = true;
       continue;
     }
@@ -286,7 +287,7 @@ PlanArgs state_of(const mv_plan_args* x) {
   a.cu = x->cu_seqlens, a.kv_lens = x->kv_lens, a.table = x->table, a.slots = x->slots, a.positions = x->positions;
   a.ok = x->ok, a.scratch = x->scratch, a.pages_st = x->pages_st, a.table_st = x->table_st;
   a.B = x->B, a.max_seqs = x->max_seqs, a.max_pages = x->max_pages, a.page_shift = attn::log2_of(x->page_size);
-  a.max_len = x->max_len, a.num_pages = x->num_pages, a.T = x->T;
+  a.max_len = x->max_len, a.num_pages = x->num_pages, a.T = x->T, a.prompts = x->prompts != 0;
   return a;
 }
 

@@ -214,7 +214,7 @@ bool ints(PyObject* o, int64_t size, int dev, const at::Tensor** out) {
          (t->size(0) <= 1 || t->stride(0) == 1);
 }
 
-// plan_step(new, lens, pages, free, n_free, page_size, num_tokens, seqs, max_len, lens_out, n_free_out):
+// plan_step(new, lens, pages, free, n_free, page_size, num_tokens, seqs, max_len, lens_out, n_free_out, prompts):
 // (cu_seqlens, kv_lens, page_table, slots, positions, ok)
 PyObject* plan_impl(PyObject* const* o) {
   const at::Tensor *fresh, *lens, *pages = tensor(o[2]), *free_pages, *n_free, *seqs = nullptr, *lens_out, *n_free_out;
@@ -235,6 +235,11 @@ PyObject* plan_impl(PyObject* const* o) {
   if (o[8] != Py_None) max_len = PyLong_AsLongLong(o[8]);
   if (PyErr_Occurred()) {
     PyErr_Clear();
+    return plain_not();
+  }
+  const int prompts = PyObject_IsTrue(o[11]);
+  if (prompts < 0) {
+    PyErr_Clear();  // the Python code meets it again and raises
     return plain_not();
   }
   if (page < 0 || page > 0x7fffffff || tokens < 0 || tokens > 0x7fffffff - 3 * b - 4 || max_len < 0) return plain_not();
@@ -260,7 +265,7 @@ PyObject* plan_impl(PyObject* const* o) {
   a.pages_st = pages->stride(0), a.B = static_cast<int>(b), a.max_seqs = static_cast<int>(s);
   a.max_pages = static_cast<int>(p), a.page_size = static_cast<int>(page);
   a.max_len = static_cast<int>(max_len < 0x7fffffff ? max_len : 0x7fffffff);
-  a.num_pages = static_cast<int>(free_pages->size(0)), a.T = static_cast<int>(tokens);
+  a.num_pages = static_cast<int>(free_pages->size(0)), a.T = static_cast<int>(tokens), a.prompts = prompts;
   const int rc = g_plan(&a, stream_of(dev));
   if (rc != MV_OK) return PyLong_FromLong(rc);
   if (seqs == nullptr) Py_INCREF(o[2]);
@@ -270,7 +275,7 @@ PyObject* plan_impl(PyObject* const* o) {
 
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) { return n == 6 ? guarded(linear_impl, a) : plain_not(); }
 PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) { return n == 8 ? guarded(sample_impl, a) : plain_not(); }
-PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) { return n == 11 ? guarded(plan_impl, a) : plain_not(); }
+PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) { return n == 12 ? guarded(plan_impl, a) : plain_not(); }
 
 // bind(addresses of mv_fp8_linear, mv_fp8_linear_scratch_bytes, mv_sample, mv_sample_scratch_bytes, mv_plan_step)
 PyObject* bind(PyObject*, PyObject* args) {

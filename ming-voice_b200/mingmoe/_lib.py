@@ -90,7 +90,7 @@ class PlanArgs(C.Structure):
     _fields_ = ([(n, P) for n in ("new_tokens", "seqs", "lens", "n_free", "free_pages", "pages", "lens_out", "n_free_out",
                                   "cu_seqlens", "kv_lens", "table", "slots", "positions", "ok", "scratch")] +
                 [(n, I64) for n in ("pages_st", "table_st")] +
-                [(n, I32) for n in ("B", "max_seqs", "max_pages", "page_size", "max_len", "num_pages", "T", "pad0")])
+                [(n, I32) for n in ("B", "max_seqs", "max_pages", "page_size", "max_len", "num_pages", "T", "prompts")])
 
 
 _SIGS = {

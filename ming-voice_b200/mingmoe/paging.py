@@ -73,9 +73,9 @@ def plan_step(new, lens, pages, free, n_free, *, page_size, num_tokens, seqs=Non
     """The Step of new[b] more tokens for each sequence seqs[b] (None: for sequence b, new [S], and the page table is `pages`
     itself), packed into num_tokens rows. Their pages come from the top of the free stack. pages is written in place; the
     counters go to lens_out and n_free_out, or in place too. A step that does not fit (no room, a sequence unknown or twice, a
-    negative count, more tokens than num_tokens or max_len) changes nothing: ok is 0 and the step has no token."""
+    negative count, more tokens than num_tokens or max_len, with `prompts` tokens of a sequence that has some already) changes nothing: ok is 0 and the step has no token."""
     r = (_serving._module or _serving.host()).plan_step(new, lens, pages, free, n_free, page_size, num_tokens, seqs, max_len,
-                                                        lens_out, n_free_out)
+                                                        lens_out, n_free_out, prompts)
     if type(r) is int:
         L.check(r, "plan_step")
     if r is not NotImplemented:
@@ -100,6 +100,7 @@ def plan_step(new, lens, pages, free, n_free, *, page_size, num_tokens, seqs=Non
     a.new_tokens, a.cu_seqlens, a.kv_lens = new.data_ptr(), cu.data_ptr(), kv_lens.data_ptr()
     a.slots, a.positions, a.ok, a.scratch = slots.data_ptr(), positions.data_ptr(), ok.data_ptr(), scratch.data_ptr()
     a.B, a.T, a.max_len = b, num_tokens, min(p * page_size if max_len is None else max_len, 0x7fffffff)
+    a.prompts = int(bool(prompts))
     with torch.cuda.device(dev):
         L.check(L.lib().mv_plan_step(C.byref(a), L.stream_ptr(dev)), "plan_step")
     return Step(cu, kv_lens, table, slots, positions, ok, max_q, prompts)
@@ -139,7 +140,7 @@ class DeviceSequences:
 
     def extend(self, new, num_tokens, seqs=None, *, max_q=None, prompts=False):
         """plan_step on this state. num_tokens: rows of the step's packed tokens (max_q: at most so many of one sequence), both
-        known to the host. prompts: every sequence of the step begins here."""
+        known to the host. prompts: every sequence that gets tokens begins here, and a step in which one has tokens already is refused."""
         return plan_step(new, self.lens, self.pages, self.free, self.n_free, page_size=self.page_size,
                          num_tokens=num_tokens, seqs=seqs, max_len=self.max_len, max_q=max_q, prompts=prompts)
 
