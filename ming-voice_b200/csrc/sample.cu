@@ -424,10 +424,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     const uint64_t t = static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(total));
     return t < total ? t : total - 1;
   };
-  auto answer = [&](int token, uint64_t w, uint64_t total) {
+  auto answer = [&](int token, float l, uint64_t total) {
     a.tokens[r] = token;
-    if (a.logprob != nullptr) a.logprob[r] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total)));
+    // from the logit: its weight of few units would be off by half of one
+    const double z = l == wt.top ? 0.0 : (static_cast<double>(l) - wt.m) / static_cast<double>(temp);
+    if (a.logprob != nullptr) a.logprob[r] = static_cast<float>(z - log(static_cast<double>(total) / one));
   };
+
+  // a place with its halves exchanged: kept tokens in the order of their indices
+  auto by_index = [](uint64_t place) { return place << 32 | place >> 32; };
+  auto logit_of = [](uint64_t at) { return of_key(~static_cast<uint32_t>(at)); };
 
   // ---- 2. few candidates
   if (share <= kMostMaxima || (!by_k && !by_p && min_p > 0.f)) {
@@ -468,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
         if (by_p) keep &= w_before < static_cast<uint64_t>(ceil(static_cast<double>(top_p) * static_cast<double>(s.kept)));
         const unsigned int n_kept = __syncthreads_count(keep);
         if (keep) {
-          index[n_before] = place & 0xffffffffull, kept[n_before] = w;
+          index[n_before] = by_index(place), kept[n_before] = w;
           if (n_before == n_kept - 1) s.total = w_before + w;
         }
         __syncthreads();
@@ -479,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 #pragma unroll 4
           for (unsigned int j = 0; j < n_kept; ++j)
             if (index[j] < at) run += kept[j];
-          if (target >= run && target < run + own) answer(static_cast<int>(at), own, s.total);
+          if (target >= run && target < run + own) answer(static_cast<int>(at >> 32), logit_of(at), s.total);
         }
         cluster_wait();
         return;
@@ -500,14 +506,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 #pragma unroll
       for (int i = 0; i < Listed<kThreads>::kEach; ++i) {
         if (list.place[i] > border || list.w[i] < least_w) list.place[i] = ~0ull, list.w[i] = 0;
-        if (list.place[i] != ~0ull) list.place[i] &= 0xffffffffull;
+        if (list.place[i] != ~0ull) list.place[i] = by_index(list.place[i]);
       }
       uint64_t total;
       list.up_to(~0ull - 1, total, n, s);
-      const uint64_t at = list.border(false, 0, draw(total) + 1, n, 0, a.V - 1, s);
-#pragma unroll
-      for (int i = 0; i < Listed<kThreads>::kEach; ++i)
-        if (list.place[i] == at) answer(static_cast<int>(at), list.w[i], total);
+      const uint64_t at = list.border(false, 0, draw(total) + 1, n, 0, (static_cast<uint64_t>(a.V) << 32) - 1, s);
+      if (tid == 0) answer(static_cast<int>(at >> 32), logit_of(at), total);
       cluster_wait();
       return;
     }
@@ -805,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     kept(i, 1, hi, w4);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (target >= run && target < run + w4[k]) answer(start + i + k, w4[k], total);
+      if (target >= run && target < run + w4[k]) answer(start + i + k, load(i + k), total);
       run += w4[k];
     }
   }

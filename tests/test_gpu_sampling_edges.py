@@ -79,3 +79,24 @@ def test_lists_of_every_length(cuda, b, v, dtype, n):
     x, u = x.to(dtype), torch.rand(5, generator=g, device=cuda)
     for s in (dict(min_p=0.0005), dict(top_k=n), dict(top_k=n, top_p=0.8), dict(top_k=max(1, n - 1), min_p=0.01), dict(top_p=0.7)):
         check_copies(x, u, b, **s)
+
+
+@pytest.mark.parametrize("b,v,dtype", [*SHAPES, (3, 131072, F32), (2, 800021, F32)])
+def test_log_probabilities_of_unlikely_tokens(cuda, b, v, dtype):
+    """u = 0 draws the first kept token, whose weight is only some thousand units: its log-probability is off by its rounding to fp32
+    and by what the rounded weights, half a unit each, make of their sum."""
+    g = torch.Generator(device=cuda).manual_seed(1)
+    for n, settings in ((120, (dict(), dict(top_k=150), dict(min_p=1e-12), dict(top_k=150, temperature=1.25))),
+                        (1500, (dict(), dict(top_k=1600), dict(min_p=1e-12), dict(temperature=0.75)))):
+        x = torch.full((5, v), -60.0, device=cuda)
+        for r in range(5):
+            x[r, torch.randperm(v, generator=g, device=cuda)[:n]] = -2.0 - 16.0 * torch.rand(n, generator=g, device=cuda)
+            x[r, 0], x[r, 7] = -18.0 - r, 0.0
+        x, u = x.to(dtype), torch.zeros(b, device=cuda)
+        for s in settings:
+            tokens, logprob = S.sample(x[torch.arange(b, device=cuda) % 5], u, return_logprob=True, **s)
+            want = [expected(row, 0.0, **s) for row in x.cpu()]
+            assert [t for t, _ in want] == [0] * 5 and tokens.tolist() == [0] * b
+            for i, got in enumerate(logprob.tolist()):
+                p = want[i % 5][1]
+                assert abs(got - p) <= 2.0 ** -24 * abs(p) + v * unit(v) / 2, (i, got, p, s)
