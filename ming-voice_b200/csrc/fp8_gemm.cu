@@ -105,6 +105,7 @@ __device__ __forceinline__ void landed(uint32_t (&d)[64]) {
     asm volatile("" : "+r"(d[i + 0]), "+r"(d[i + 1]), "+r"(d[i + 2]), "+r"(d[i + 3]), "+r"(d[i + 4]), "+r"(d[i + 5]), "+r"(d[i + 6]), "+r"(d[i + 7]), "+r"(d[i + 8]), "+r"(d[i + 9]), "+r"(d[i + 10]), "+r"(d[i + 11]), "+r"(d[i + 12]), "+r"(d[i + 13]), "+r"(d[i + 14]), "+r"(d[i + 15]) : : "memory");
 }
 
+constexpr size_t kMostSmem = 226 * 1024;       // dynamic shared memory of a CTA, beside the barriers
 constexpr int kTile = 128;                     // rows of the 128-row operand
 constexpr uint32_t kTileBytes = kTile * kBlock;  // 16 KB
 
@@ -906,7 +907,8 @@ int row_map(CUtensorMap* m, const void* base, int size, int cols, int rows, long
 
 template <typename... P, typename... A>
 int launch(void (*fn)(P...), int grid, int threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // the most that any call takes: the limit is the kernel's, not the launch's, and another thread may be about to launch
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostSmem));
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(mv_fp8_linear)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -941,7 +943,7 @@ int run_token(const LinearArgs& x, cudaStream_t st) {
   g.f.split = split_of(g.f.n_tiles, x.blocks);
   const int share = (x.blocks + g.f.split - 1) / g.f.split;
   g.stages = kTokenStages;
-  while (token_smem(share, g.stages) > 226 * 1024) --g.stages;
+  while (token_smem(share, g.stages) > kMostSmem) --g.stages;
   CUtensorMap wm;
   const int rc = row_map(&wm, x.w, 1, x.K, x.N, x.w_st, kTile, "wq");
   if (rc != MV_OK) return rc;

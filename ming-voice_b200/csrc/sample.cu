@@ -829,7 +829,8 @@ int launch(SampleArgs a, int B, int C, cudaStream_t st) {
   a.in_smem = static_cast<size_t>(a.slice) * size <= kSm - fixed_smem<kThreads>();
   const size_t smem = fixed_smem<kThreads>() + (a.in_smem ? static_cast<size_t>(a.slice) * size : 0);
   auto fn = sample_kernel<DT, kThreads>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // the most that any call takes: the limit is the kernel's, not the launch's, and another thread may be about to launch
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSm));
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(mv_sample)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned int>(B) * C);
