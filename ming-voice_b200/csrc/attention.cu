@@ -58,12 +58,14 @@ static int make_map(CUtensorMap* m, const void* base, bool bf16, int d, int toke
                                  static_cast<cuuint64_t>(pages > 1 ? sp : d) * 2};
   const cuuint32_t boxes[5] = {64, static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(parts), 1, 1};
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
-                         const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B,
-                         // a head's row and no more: with 128-byte rows, 256 bytes would fetch the next head's too
-                         d == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const auto encode = [&] {
+    return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides,
+               boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               // a head's row and no more: with 128-byte rows, 256 bytes would fetch the next head's too
+               d == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT && bind_context()) r = encode();
   if (r != CUDA_SUCCESS)
     return fail(MV_ERR_INVALID, "tensor map for %s rejected (CUresult %d)", what, static_cast<int>(r));
   return MV_OK;
@@ -83,10 +85,13 @@ int make_q_map(CUtensorMap* m, const Problem& p, int d, bool bf16, int tok) {
                                  static_cast<cuuint64_t>(p.T > 1 ? p.q_st : d) * 2};
   const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(p.G), static_cast<cuuint32_t>(tok)};
   const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                         const_cast<uint16_t*>(p.q), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const auto encode = [&] {
+    return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<uint16_t*>(p.q), dims,
+               strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT && bind_context()) r = encode();
   if (r != CUDA_SUCCESS) return fail(MV_ERR_INVALID, "tensor map for q rejected (CUresult %d)", static_cast<int>(r));
   return MV_OK;
 }

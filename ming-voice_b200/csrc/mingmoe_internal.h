@@ -47,4 +47,11 @@ inline int elem_size(int dtype) {
 
 int num_sms();
 
+// Makes the current device's context current in this thread, as runtime calls do by themselves. Driver calls do not: the first of a new
+// thread answers CUDA_ERROR_INVALID_CONTEXT.
+inline bool bind_context() {
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess;
+}
+
 }  // namespace mv
