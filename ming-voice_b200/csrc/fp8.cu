@@ -7,6 +7,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "attn_common.cuh"
@@ -77,7 +78,7 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const void* __rest
     const int r = i / kBlock, c = i % kBlock;
     if (r >= rows || c >= cols) continue;
     const float v = fabsf(load1<DT>(w, (n0 + r) * w_st + k0 + c));
-    nan |= !(v <= 3.4e38f);
+    nan |= !(v <= FLT_MAX);
     top = fmaxf(top, v);
   }
 #pragma unroll
