@@ -429,7 +429,10 @@ MV_API int mv_quantize_fp8_weight(const void* w, int w_dtype, long long w_st, in
  * the first of the order is always kept. The token drawn is the lowest index whose weight, added to those of all kept tokens of
  * a lower index, exceeds u times the sum of all kept weights. temperature <= 0 draws the first of the order. NaN settings are
  * "off" (a NaN temperature: the first of the order; a NaN u: as 0). Weights are computed in f64 and held as whole numbers of 2^-51
- * (2^-(61 - log2 V), log2 V rounded up, above 1024 tokens: 2^-44 for 2^17), sums in 64 bits.
+ * (2^-(61 - log2 V), log2 V rounded up, above 1024 tokens: 2^-44 for 2^17), to nearest, and summed in 64 bits without rounding. So a
+ * sum is off by at most V / 2 such units, 2^-28 of the largest weight for 2^17 tokens, 2^-24 for 2^19, 2^-18 for 2^22: a border, or
+ * u times the total, that lies within that of a token's end may fall to its neighbour. A weight below half a unit is 0: u = 0 draws the
+ * first kept token of at least that weight.
  * Settings are arrays of B values, or NULL: then the value beside them holds for all rows. u [B] f32 in [0, 1) (clamped).
  * tokens [B] int64; logprob [B] f32 or NULL: ln of the drawn token's share of the kept weights. A row without a token (all
  * logits -inf, or one NaN) gives token -1 and logprob -inf.

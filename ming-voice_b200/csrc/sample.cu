@@ -5,7 +5,8 @@
 // so all that is kept is given by one place, the border, and a least weight. Weights 2^t, t = (logit - max) log2(e) / temperature,
 // are whole numbers of 2^-shift (shift 44 for vocabularies of 2^17, more for smaller ones up to 51; 2^f from a table of 32 values and a polynomial of degree 5
 // that interpolates 2^g at the Chebyshev nodes of [-1/64, 1/64], off by 2^-52 of it), so that sums do not depend on their order: each border and each draw comes out
-// the same whatever the split; a weight below 2^-shift / 2, which no 24-bit random number can draw, is 0.
+// the same whatever the split. A weight is off by half a unit at most (below that it is 0), so a sum of V by V 2^-(shift + 1) of the
+// largest weight: 2^-28 for 2^17 tokens; from 2^19 on (2^-24) a random number of 24 bits may resolve it.
 //
 // Steps, a cluster of CTAs for each row, the row in their shared memory:
 //   1. read the row once; the first of the order, and (top-k) a key with at least top_k logits at or above it: the least over

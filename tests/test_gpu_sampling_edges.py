@@ -100,3 +100,24 @@ def test_log_probabilities_of_unlikely_tokens(cuda, b, v, dtype):
             for i, got in enumerate(logprob.tolist()):
                 p = want[i % 5][1]
                 assert abs(got - p) <= 2.0 ** -24 * abs(p) + v * unit(v) / 2, (i, got, p, s)
+
+
+@pytest.mark.parametrize("v", [1 << 17, 1 << 19, (1 << 22) - 5])
+@pytest.mark.parametrize("units", [0.45, 0.55, 1.45])
+def test_tails_of_about_a_unit(cuda, v, units):
+    """Weights are rounded to whole units, so a running sum is off by half a unit a token: the token drawn is the definition's but for
+    that, whatever the tail adds up to."""
+    at = v // 3
+    x = torch.full((1, v), math.log(units * unit(v)), device=cuda)
+    x[0, at] = 0.0
+    run = torch.cumsum(torch.exp(x[0].double()), 0)
+    total, off = run[-1].item(), v * unit(v) / 2
+    for u in (0.0, 1e-7, 2.0 ** -24, 0.5, 1.0 - 2.0 ** -23, 1.0 - 2.0 ** -24):
+        t = S.sample(x, torch.tensor([u], device=cuda))[0].item()
+        f = torch.tensor(u, dtype=F32).item()
+        assert run[t].item() > f * total - off * (1 + f)
+        assert t == 0 or run[t - 1].item() <= f * total + off * (1 + f)
+        if units < 0.5:
+            assert t == at  # the tail has no weight
+        if u == 0.0:
+            assert t == (at if units < 0.5 else 0)
