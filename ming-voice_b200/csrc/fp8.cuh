@@ -134,11 +134,5 @@ __device__ __forceinline__ uint2 round8(const float (&v)[8], float down) {
   return o;
 }
 
-__device__ __forceinline__ float e4m3_to_f32(uint8_t b) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(b)));
-  return __half2float(__ushort_as_half(static_cast<uint16_t>(h & 0xffffu)));
-}
-
 }  // namespace fp8
 }  // namespace mv

@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(Few<NT>::kThreads, 1)
 // ------------------------------------------------------------------------------------------------ a few tokens, few rows
 //
 // The same with the activations rounded by the epilogue warps while the first weights are on their way: one launch, and no
-// activation traffic in the ring. All blocks of a CTA's share of K lie in shared memory.
+// activation traffic in the ring. All blocks of a CTA's share of K lie in shared memory; a cluster has one tile (one_launch).
 
 constexpr int kTokenN = 16, kTokenBlocks = 32, kTokenStages = 12;
 constexpr int kTokenBufs = 8;  // blocks' products in TMEM: the issuing warp does not wait for the epilogue of the last two
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(192, 1) token_kernel(const __grid_constant__ C
   const FewArgs& a = g.f;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int rank = static_cast<int>(cluster_rank());
   const int b0 = a.blocks * rank / a.split, b1 = a.blocks * (rank + 1) / a.split;
   uint8_t* xs = smem + g.stages * kTileBytes;                                     // [block][token][128], swizzled
   float* scales = reinterpret_cast<float*>(xs + (b1 - b0) * kTokenXBytes);        // [block][token]
@@ -400,50 +400,38 @@ __global__ void __launch_bounds__(192, 1) token_kernel(const __grid_constant__ C
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_base;
-  const int first = blockIdx.x / a.split, step = gridDim.x / a.split;
+  const int tile = blockIdx.x / a.split;
   pdl_launch_dependents();
 
   if (warp == 0) {
     if (tc::elect_one()) {
       tc::prefetch_tmap(&wmap);
       // weights only: they do not depend on the kernel in front of this one
-      int it = 0;
-      bool ok = true;
-      for (int tile = first; tile < a.n_tiles && ok; tile += step) {
-        for (int b = b0; b < b1; ++b, ++it) {
-          const int s = it % g.stages;
-          if (it >= g.stages && !wait(&empty[s], (it / g.stages + 1) & 1, a.header, 0x820u)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&full[s], kTileBytes);
-          tc::tma_load_2d(smem + s * kTileBytes, &wmap, &full[s], b * kBlock, tile * kTile);
-        }
+      for (int b = b0, it = 0; b < b1; ++b, ++it) {
+        const int s = it % g.stages;
+        if (it >= g.stages && !wait(&empty[s], (it / g.stages + 1) & 1, a.header, 0x820u)) break;
+        mbar_arrive_expect_tx(&full[s], kTileBytes);
+        tc::tma_load_2d(smem + s * kTileBytes, &wmap, &full[s], b * kBlock, tile * kTile);
       }
     }
   } else if (warp == 1) {
-    int it = 0;
-    bool ok = wait(&x_full, 0, a.header, 0x824u);
-    for (int tile = first; tile < a.n_tiles && ok; tile += step) {
-      for (int b = b0; b < b1; ++b, ++it) {
-        const int s = it % g.stages, buf = it % kTokenBufs;
-        if (!wait(&full[s], (it / g.stages) & 1, a.header, 0x821u) ||
-            (it >= kTokenBufs && !wait(&acc_empty[buf], (it / kTokenBufs + 1) & 1, a.header, 0x822u))) {
-          ok = false;
-          break;
-        }
-        tc::fence_after_sync();
-        if (tc::elect_one()) {
-          const uint64_t ad = tc::sw128_desc(smem_u32(smem + s * kTileBytes));
-          const uint64_t bd = tc::sw128_desc(smem_u32(xs + (b - b0) * kTokenXBytes));
+    const bool rounded = wait(&x_full, 0, a.header, 0x824u);
+    for (int b = b0, it = 0; b < b1 && rounded; ++b, ++it) {
+      const int s = it % g.stages, buf = it % kTokenBufs;
+      if (!wait(&full[s], (it / g.stages) & 1, a.header, 0x821u) ||
+          (it >= kTokenBufs && !wait(&acc_empty[buf], (it / kTokenBufs + 1) & 1, a.header, 0x822u)))
+        break;
+      tc::fence_after_sync();
+      if (tc::elect_one()) {
+        const uint64_t ad = tc::sw128_desc(smem_u32(smem + s * kTileBytes));
+        const uint64_t bd = tc::sw128_desc(smem_u32(xs + (b - b0) * kTokenXBytes));
 #pragma unroll
-          for (int k = 0; k < kBlock / 32; ++k)
-            mma_f8(tmem + buf * kTokenN, ad + 2 * k, bd + 2 * k, idesc_e4m3(kTile, kTokenN), k > 0);
-          tc::mma_commit(&empty[s]);
-          tc::mma_commit(&acc_full[buf]);
-        }
-        __syncwarp();
+        for (int k = 0; k < kBlock / 32; ++k)
+          mma_f8(tmem + buf * kTokenN, ad + 2 * k, bd + 2 * k, idesc_e4m3(kTile, kTokenN), k > 0);
+        tc::mma_commit(&empty[s]);
+        tc::mma_commit(&acc_full[buf]);
       }
+      __syncwarp();
     }
   } else {
     const int quarter = warp & 3, row = quarter * 32 + lane, tid = threadIdx.x - 64;
@@ -457,67 +445,43 @@ __global__ void __launch_bounds__(192, 1) token_kernel(const __grid_constant__ C
     __syncwarp();
     if (lane == 0) mbar_arrive(&x_full);
     named_bar(1, 128);  // the scales of all four warps
-    int it = 0;
-    bool ok = true;
-    for (int tile = first; tile < a.n_tiles; tile += step) {
-      const int n0 = tile * kTile;
-      float acc[kTokenN];
+    float acc[kTokenN];
 #pragma unroll
-      for (int c = 0; c < kTokenN; ++c) acc[c] = 0.f;
-      const float* ws = a.ws + n0 / kBlock * a.ws_st;
-      // lane l: the weights' scale of block b0 + l
-      const float ws_lane = b0 + lane < b1 ? ws[b0 + lane] : 0.f;
-      for (int b = b0; b < b1 && ok; ++b, ++it) {
-        const int buf = it % kTokenBufs;
-        const float w = __shfl_sync(0xffffffffu, ws_lane, b - b0);
-        if (!wait(&acc_full[buf], (it / kTokenBufs) & 1, a.header, 0x823u)) {
-          ok = false;
-          break;
-        }
-        tc::fence_after_sync();
-        uint32_t d[kTokenN];
-        tc::tmem_ld16(lanes + buf * kTokenN, d);
-        tc::tmem_ld_wait();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
-        const float4* sc = reinterpret_cast<const float4*>(scales + (b - b0) * kTokenN);
+    for (int c = 0; c < kTokenN; ++c) acc[c] = 0.f;
+    // lane l: the weights' scale of block b0 + l
+    const float ws_lane = b0 + lane < b1 ? a.ws[tile * a.ws_st + b0 + lane] : 0.f;
+    for (int b = b0, it = 0; b < b1; ++b, ++it) {
+      const int buf = it % kTokenBufs;
+      const float w = __shfl_sync(0xffffffffu, ws_lane, b - b0);
+      if (!wait(&acc_full[buf], (it / kTokenBufs) & 1, a.header, 0x823u)) break;
+      tc::fence_after_sync();
+      uint32_t d[kTokenN];
+      tc::tmem_ld16(lanes + buf * kTokenN, d);
+      tc::tmem_ld_wait();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      const float4* sc = reinterpret_cast<const float4*>(scales + (b - b0) * kTokenN);
 #pragma unroll
-        for (int i = 0; i < kTokenN; i += 4) {
-          if (i >= a.T) break;
-          const float4 f = sc[i / 4];
-          acc[i] = fmaf(__uint_as_float(d[i]), f.x * w, acc[i]);
-          acc[i + 1] = fmaf(__uint_as_float(d[i + 1]), f.y * w, acc[i + 1]);
-          acc[i + 2] = fmaf(__uint_as_float(d[i + 2]), f.z * w, acc[i + 2]);
-          acc[i + 3] = fmaf(__uint_as_float(d[i + 3]), f.w * w, acc[i + 3]);
-        }
-      }
-      const int n = n0 + row;
-      if (a.split == 1) {
-        if (n < a.N && ok) {
-#pragma unroll
-          for (int t = 0; t < kTokenN; ++t) {
-            if (t >= a.T) break;
-            float v = acc[t];
-            if (a.residual != nullptr) v += load1<ODT>(a.residual, t * a.r_st + n);
-            store1<ODT>(a.out, t * a.o_st + n, v);
-          }
-        }
-      } else {
-        // the parts lie where the ring was: its copies have landed and its products are done
-        float* part = reinterpret_cast<float*>(smem);  // [token][128]
-        named_bar(1, 128);
-#pragma unroll
-        for (int t = 0; t < kTokenN; ++t) part[t * kTile + row] = acc[t];
+      for (int i = 0; i < kTokenN; i += 4) {
+        if (i >= a.T) break;
+        const float4 f = sc[i / 4];
+        acc[i] = fmaf(__uint_as_float(d[i]), f.x * w, acc[i]);
+        acc[i + 1] = fmaf(__uint_as_float(d[i + 1]), f.y * w, acc[i + 1]);
+        acc[i + 2] = fmaf(__uint_as_float(d[i + 2]), f.z * w, acc[i + 2]);
+        acc[i + 3] = fmaf(__uint_as_float(d[i + 3]), f.w * w, acc[i + 3]);
       }
     }
+    // the parts lie where the ring was: its copies have landed and its products are done
+    float* part = reinterpret_cast<float*>(smem);  // [token][128]
+    named_bar(1, 128);
+#pragma unroll
+    for (int t = 0; t < kTokenN; ++t) part[t * kTile + row] = acc[t];
   }
-  if (a.split > 1) {
-    pdl_wait();
-    cluster_sync();
-    join_parts<ODT>(a, smem_u32(smem), first * kTile, 0, a.T, rank, 192);
-    cluster_sync();
-  }
+  pdl_wait();
+  cluster_sync();
+  join_parts<ODT>(a, smem_u32(smem), tile * kTile, 0, a.T, rank, 192);
+  cluster_sync();
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 1) {
@@ -951,9 +915,7 @@ int run_token(const LinearArgs& x, cudaStream_t st) {
   CUtensorMap wm;
   const int rc = row_map(&wm, x.w, 1, x.K, x.N, x.w_st, kTile, "wq");
   if (rc != MV_OK) return rc;
-  const int sms = num_sms(), tiles = g.f.n_tiles;
-  const int grid = g.f.split > 1 ? tiles * g.f.split : tiles < sms ? tiles : sms;
-  return launch(token_kernel<ODT>, grid, 192, token_smem(share, g.stages), g.f.split, st, wm, g);
+  return launch(token_kernel<ODT>, g.f.n_tiles * g.f.split, 192, token_smem(share, g.stages), g.f.split, st, wm, g);
 }
 
 template <int NT, int ODT>

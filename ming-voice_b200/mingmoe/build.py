@@ -107,8 +107,7 @@ def _build_module(src: str, out: str, verbose: bool, force: bool) -> str:
            tmp, f"-L{os.path.join(tdir, 'lib')}", "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
     made_by = f"torch {torch.__version__}, python {sys.version}: {' '.join(cmd).replace(ROOT, '.')}\n"
     record = os.path.join(BUILD, os.path.splitext(os.path.basename(src))[0] + ".cmd")
-    newest = max([os.path.getmtime(p) for p in [src, *glob.glob(os.path.join(INCLUDE, "*.h")),
-                                                *glob.glob(os.path.join(CSRC, "*.hpp"))]])
+    newest = max([os.path.getmtime(p) for p in [src, *glob.glob(os.path.join(INCLUDE, "*.h"))]])
     if os.path.exists(out) and os.path.getmtime(out) >= newest and not force and os.path.exists(record):
         with open(record) as f:
             if f.read() == made_by:
