@@ -436,7 +436,7 @@ MV_API int mv_quantize_fp8_weight(const void* w, int w_dtype, long long w_st, in
  * Settings are arrays of B values, or NULL: then the value beside them holds for all rows. u [B] f32 in [0, 1) (clamped).
  * tokens [B] int64; logprob [B] f32 or NULL: ln of the drawn token's share of the kept weights. A row without a token (all
  * logits -inf, or one NaN) gives token -1 and logprob -inf.
- * scratch: mv_sample_scratch_bytes(B, V) bytes of any content, 256-byte aligned, as above. */
+ * scratch is not used, and mv_sample_scratch_bytes is 0: a draw needs no memory but its results. */
 typedef struct mv_sample_args {
   const void* logits;
   const float *u, *temperature, *top_p, *min_p;

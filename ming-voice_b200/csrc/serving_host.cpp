@@ -24,7 +24,6 @@ namespace {
 int (*g_linear)(const mv_fp8_linear_args*, void*, size_t, void*) = nullptr;
 size_t (*g_linear_scratch)(int, int, int) = nullptr;
 int (*g_sample)(const mv_sample_args*, void*) = nullptr;
-size_t (*g_sample_scratch)(int, int) = nullptr;
 int (*g_plan)(const mv_plan_args*, void*) = nullptr;
 
 struct Workspace {
@@ -174,7 +173,7 @@ PyObject* sample_impl(PyObject* const* o) {
     PyErr_Clear();  // the Python code meets it again and raises
     return plain_not();
   }
-  at::Tensor out, logprob, scratch;
+  at::Tensor out, logprob;
   if (o[6] == Py_None) {
     out = at::empty({b}, l->options().dtype(at::kLong));
   } else {
@@ -186,16 +185,11 @@ PyObject* sample_impl(PyObject* const* o) {
   }
   if (with) logprob = at::empty({b}, l->options().dtype(at::kFloat));
   mv_sample_args a{};
-  const size_t bytes = g_sample_scratch(static_cast<int>(b), static_cast<int>(v));
-  if (bytes > 0) {
-    scratch = at::empty({static_cast<int64_t>(bytes)}, l->options().dtype(at::kByte));
-    a.scratch = scratch.data_ptr();
-  }
   a.logits = l->data_ptr(), a.u = static_cast<const float*>(pu), a.temperature = static_cast<const float*>(pt);
   a.top_p = static_cast<const float*>(pp), a.min_p = static_cast<const float*>(pm), a.top_k = static_cast<const int*>(pk);
   a.tokens = static_cast<long long*>(out.data_ptr());
   a.logprob = with ? static_cast<float*>(logprob.data_ptr()) : nullptr;
-  a.st = l->stride(0), a.scratch_bytes = bytes;
+  a.st = l->stride(0);
   a.temperature_value = static_cast<float>(t), a.top_p_value = static_cast<float>(p), a.min_p_value = static_cast<float>(m);
   a.top_k_value = static_cast<int>(k), a.B = static_cast<int>(b), a.V = static_cast<int>(v), a.dtype = code(l->scalar_type());
   const int rc = g_sample(&a, stream_of(dev));
@@ -277,15 +271,14 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) { return n == 6 ? 
 PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) { return n == 8 ? guarded(sample_impl, a) : plain_not(); }
 PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) { return n == 12 ? guarded(plan_impl, a) : plain_not(); }
 
-// bind(addresses of mv_fp8_linear, mv_fp8_linear_scratch_bytes, mv_sample, mv_sample_scratch_bytes, mv_plan_step)
+// bind(addresses of mv_fp8_linear, mv_fp8_linear_scratch_bytes, mv_sample, mv_plan_step)
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long f[5];
-  if (!PyArg_ParseTuple(args, "KKKKK", &f[0], &f[1], &f[2], &f[3], &f[4])) return nullptr;
+  unsigned long long f[4];
+  if (!PyArg_ParseTuple(args, "KKKK", &f[0], &f[1], &f[2], &f[3])) return nullptr;
   g_linear = reinterpret_cast<decltype(g_linear)>(f[0]);
   g_linear_scratch = reinterpret_cast<decltype(g_linear_scratch)>(f[1]);
   g_sample = reinterpret_cast<decltype(g_sample)>(f[2]);
-  g_sample_scratch = reinterpret_cast<decltype(g_sample_scratch)>(f[3]);
-  g_plan = reinterpret_cast<decltype(g_plan)>(f[4]);
+  g_plan = reinterpret_cast<decltype(g_plan)>(f[3]);
   Py_RETURN_NONE;
 }
 

@@ -18,6 +18,6 @@ def host():
                               "`python ming-voice_b200/mingmoe/build.py` (or __graft_entry__.build())") from e
         lib = L.lib()
         m.bind(*(C.cast(f, C.c_void_p).value for f in (lib.mv_fp8_linear, lib.mv_fp8_linear_scratch_bytes, lib.mv_sample,
-                                                       lib.mv_sample_scratch_bytes, lib.mv_plan_step)))
+                                                       lib.mv_plan_step)))
         _module = m
     return _module

@@ -61,11 +61,8 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=Non
     u = u.contiguous()
     logprob = torch.empty(b, dtype=f32, device=dev) if return_logprob else None
     with torch.cuda.device(dev):
-        lib = L.lib()
-        nbytes = lib.mv_sample_scratch_bytes(b, v)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         a = L.SampleArgs(logits.data_ptr(), u.data_ptr(), *(x.data_ptr() if x is not None else 0 for x in (t, p, m, k)),
-                         out.data_ptr(), logprob.data_ptr() if return_logprob else 0, scratch.data_ptr(), logits.stride(0),
-                         nbytes, tv, pv, mv, min(max(int(kv), 0), 0x7fffffff), b, v, L.dt(logits), 0)
-        L.check(lib.mv_sample(C.byref(a), L.stream_ptr(dev)), "sample")
+                         out.data_ptr(), logprob.data_ptr() if return_logprob else 0, 0, logits.stride(0),
+                         0, tv, pv, mv, min(max(int(kv), 0), 0x7fffffff), b, v, L.dt(logits), 0)
+        L.check(L.lib().mv_sample(C.byref(a), L.stream_ptr(dev)), "sample")
     return (out, logprob) if return_logprob else out
