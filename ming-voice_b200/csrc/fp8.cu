@@ -30,8 +30,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ 
                                                        uint8_t* __restrict__ q, long long q_st, S* __restrict__ scale,
                                                        long long s_st) {
   pdl_wait();
-  // Only now, and only where this is a product's first half: the product's kernel reads weights before it waits for the kernel
-  // in front of it, and they may come from an earlier one, or be what this kernel writes.
+  // where this is a product's first half, its second may be scheduled
   if (sizeof(S) == 1) pdl_launch_dependents();
   const int sub = threadIdx.x & 15;
   const long long first = static_cast<long long>(blockIdx.x) * UNITS;
