@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ 
   }
 }
 
-// Weights: a CTA owns a block of 128 x 128.
+// Weights: a CTA owns a block of 128 x 128. Done once for a model, so by single elements: 131072 x 2048 bf16 in 521 us, 1.5 TB/s.
 template <int DT>
 __global__ void __launch_bounds__(256) quantize_weight_kernel(const void* __restrict__ w, long long w_st, int N, int K,
                                                               uint8_t* __restrict__ q, long long q_st,

@@ -11,8 +11,9 @@
 //               a block's factor is one number per thread.
 // Bound and measured (B200; graph replays): few tokens by the weights' bytes, 131072 x 2048 for one token 50 us (5.4 TB/s, 83 % of the
 // measured copy; the rest is the start of 4 us and the last wave of tiles), for 64 tokens 65 us; many tokens by the tensor pipe
-// and the hand-over of each block between it and the epilogue, 16001 x 5632 x 2048 197 us with the activations' rounding (1.87
-// PFLOP/s), 4096 x 5632 x 8192 180 us (2.1); products added up in TMEM instead, which one scale a row would allow, take 148.
+// and the hand-over of each block between it and the epilogue, 16001 x 5632 x 2048 195 to 203 us by card with the
+// activations' rounding (1.82 to 1.89 PFLOP/s), 4096 x 5632 x 8192 178 to 185 (2.0 to 2.1; products added up in TMEM instead, which one
+// scale a row would allow, take 148).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
