@@ -153,8 +153,10 @@ class TokenGraph:
         with torch.cuda.stream(s):
             # the warm-up runs with no sequence running, which leaves the pages as they are
             self.graph = _capture(step, s, torch.cuda.graph_pool_handle())
+        self._results = self.logits, self.logprob, self.ok  # the graph's buffers: an eager step has others
         torch.cuda.current_stream(dev).wait_stream(s)
 
     def __call__(self):
         self.graph.replay()
+        self.logits, self.logprob, self.ok = self._results
         return self.tokens

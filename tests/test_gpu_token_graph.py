@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from mingmoe import _lib as L
-from mingmoe import fp8
+from mingmoe import fp8, sampling
 from mingmoe.attention import rotation_table
 from mingmoe.block import MoeBlock
 from mingmoe.graphs import TokenGraph
@@ -102,3 +102,23 @@ def test_a_sequence_without_a_token_stops(cuda):
     loop()
     assert loop.tokens[1].item() >= 0 and seqs.lens.tolist() == [6, 4, 7]
     assert not L.all_workspace_errors()
+
+
+def test_results_are_the_last_steps_whether_captured_or_not(cuda):
+    """Steps one by one between replays: logits, logprob and ok are those of the step that came last."""
+    seqs = DeviceSequences(3, 8, 2, 64, device=cuda)
+    loop = TokenGraph(make(cuda, seqs), seqs)
+    loop.decoder(torch.arange(10, device=cuda), seqs.extend(ints([6, 4], cuda), 10, max_q=6, prompts=True))
+    loop.new.fill_(1)
+    for i, step in enumerate([loop, loop.step, loop, loop, loop.step, loop, loop.step, loop]):
+        loop.u.copy_(torch.rand(2, generator=torch.Generator(device=cuda).manual_seed(i), device=cuda))
+        before = seqs.lens.tolist()
+        step()
+        fits = sum(-(-(n + 1) // 8) for n in before) <= 3
+        assert loop.ok.item() == fits
+        if fits:
+            drawn, logprob = sampling.sample(loop.logits, loop.u, return_logprob=True)
+            assert torch.equal(drawn, loop.tokens) and torch.equal(logprob, loop.logprob)
+        else:
+            assert seqs.lens.tolist() == before
+    assert not fits
